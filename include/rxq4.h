@@ -60,6 +60,13 @@ extern "C" {
 #define RXQ4_GGML_TYPE_Q5_K 13
 #define RXQ4_GGML_TYPE_Q6_K 14
 #define RXQ4_MAX_K 65536
+/* Limits of the serving entry points (rxq4_qk_norm_rope, rxq4_attention_paged_f16,
+ * rxq4_sample_f32). */
+#define RXQ4_MAX_SEQS 65536
+#define RXQ4_MAX_TOKENS 1048576
+#define RXQ4_MAX_POSITIONS 16777216
+#define RXQ4_MAX_HEADS 1024
+#define RXQ4_MAX_VOCAB 4194304
 
 /* Element types for the typed GEMM entry point. */
 #define RXQ4_DTYPE_F32 0
@@ -187,6 +194,111 @@ int rxq4_attention_prefill_f16(void *out, const void *q, const void *k_cache,
                                const void *v_cache, int n_heads, int n_kv_heads, int head_dim,
                                int N, int start_pos, float scale, int kv_int8,
                                const float *k_scales, const float *v_scales, void *stream);
+
+/* NEW.  A paged KV cache of one layer, shared by the sequences of a batch.
+ * Page p holds page_size consecutive positions of one sequence as
+ * [slot][n_kv_heads][head_dim], page_stride elements after page p - 1 (0: dense;
+ * e.g. K and V pages alternating in one allocation have twice the dense
+ * stride).  fp16, or int8 with per-(position, KV head) fp32 scales
+ * [n_pages][page_size][n_kv_heads] (NULL: 1, for reading only).  Row i of
+ * page_table names the pages of sequence i in order; NULL: one sequence whose
+ * page j is page j, i.e. a contiguous cache [pos][n_kv_heads][head_dim].  An
+ * entry outside [0, n_pages) is a hole: its positions are never read or
+ * written, and no token attends to them.  Pages may be shared by sequences as
+ * long as no call writes to a shared slot.  page_size: a power of two, 1 to
+ * 1024; head_dim and alignment as the attention entry points above; n_pages *
+ * page_size below 2^31. */
+typedef struct rxq4_paged_kv {
+    void *k, *v;
+    float *k_scales, *v_scales;
+    const int32_t *page_table;   /* device, [n_seqs][table_stride] */
+    int64_t page_stride;         /* elements from page to page, 0: dense */
+    int table_stride;            /* entries per sequence */
+    int n_pages;
+    int page_size;
+    int n_kv_heads;
+    int head_dim;
+    int kv_int8;
+} rxq4_paged_kv;
+
+/* NEW.  The new tokens of a batch of sequences: those of sequence i are the rows
+ * [q_starts[i], q_starts[i + 1]) of q and the like, and the last of its
+ * seq_lens[i] positions (its cached positions and the new ones).  Both arrays
+ * are in device memory, so a captured launch can be replayed with other
+ * lengths as long as the limits below hold.  Rows before q_starts[0] and from
+ * q_starts[n_seqs] on (a padded batch) are left as they are.  A token whose
+ * position would be negative (seq_lens[i] below the new tokens) attends to
+ * nothing. */
+typedef struct rxq4_seq_batch {
+    const int32_t *q_starts;   /* device, [n_seqs + 1], ascending */
+    const int32_t *seq_lens;   /* device, [n_seqs] */
+    int n_seqs;
+    int n_tokens;   /* rows of q: a limit of every q_starts value */
+    int max_new;    /* no sequence has more new tokens (those past it are not computed) */
+    int max_len;    /* no seq_lens value is larger (positions past it are not seen) */
+} rxq4_seq_batch;
+
+/* NEW.  The step between a layer's Q/K/V projection and its attention, in one
+ * pass: RMS norm of every query and key head (q_weight, k_weight: fp32
+ * [head_dim], NULL: none), rotation of the first n_rot dims of queries and keys
+ * by position * inv_freq[i] (fp32 [n_rot / 2], device; the product in 64 bits)
+ * in pairs (i, i + n_rot / 2), or (2 i, 2 i + 1) where `interleaved`, and the
+ * store of keys and values into the cache's slots of their positions.
+ *   q_out   fp16 [n_tokens][n_heads][head_dim]; may be q itself where that is
+ *           fp16 with the same stride, and overlap it in no other way
+ *   q, k, v x_dtype (F16, BF16, F32), 16-byte aligned, rows q_stride / kv_stride
+ *           elements apart (multiples of 8): slices of one fused output, or
+ *           three arrays
+ * Everything is computed in fp32 and rounded once.  int8 caches get scale =
+ * max |row| / 127 and rint(row / scale) per position and head, both scale arrays
+ * given; a row with a NaN gets a NaN scale, one with an infinity an infinite
+ * one (either reads as NaN).  Tokens at negative positions get a zero query
+ * row; keys and values whose position is negative, in a hole or past the table
+ * are not stored.  Two rows for one slot (a page shared by sequences) race.
+ * No counterpart in the reference, whose KernelSupport names rope, rmsnorm and
+ * kv_convert and leaves them to its caller. */
+int rxq4_qk_norm_rope(void *q_out, const void *q, const void *k, const void *v, int x_dtype,
+                      int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_weight,
+                      const float *k_weight, float eps, const float *inv_freq, int n_rot,
+                      int interleaved, const rxq4_seq_batch *batch, const rxq4_paged_kv *cache,
+                      void *stream);
+
+/* NEW.  Attention of each sequence's new tokens over its pages: a token at
+ * position p attends to positions [0, p] (causal), holes left out; fp32
+ * softmax, fp16 out [n_tokens][n_heads][head_dim].  A batch may mix decoding
+ * sequences (one new token), drafts and prompt chunks.  A token that sees
+ * nothing gets zeros.  What the cache holds at positions a token does not see
+ * does not reach its row, infinities and NaN included.  Few tokens on long
+ * contexts split over the stream's workspace described above (a graph captured
+ * with such a call uses the capturing stream's, also where it is replayed on
+ * another).
+ * No counterpart in the reference, whose KernelSupport names
+ * paged_decode_attention. */
+int rxq4_attention_paged_f16(void *out, const void *q, int n_heads, float scale,
+                             const rxq4_seq_batch *batch, const rxq4_paged_kv *cache,
+                             void *stream);
+
+/* NEW.  The next token of each row of logits [n_rows][n_vocab] (fp32, rows
+ * row_stride elements apart), from u[row] in [0, 1) (clamped to it; NaN: 0).
+ * Every array but logits has one value per row in device memory; a NULL
+ * parameter array leaves that parameter out.
+ *   weights  w_i = exp((l_i - max l) / temperature), 64-bit; a NaN logit counts as
+ *            -infinity; +infinities share the row.  temperature 0 or below (or
+ *            NaN): the largest logit, lowest index, whatever else is given
+ *   order    logits descending, equal ones by index ascending
+ *   top_k    the first top_k of the order (0 or below: all)
+ *   top_p    of those the shortest prefix whose weight is top_p of theirs (1 or
+ *            above, NaN: all; the first always stays)
+ *   min_p    of those the ones with w_i >= min_p (the first always stays)
+ *   ids      the first of the kept whose weight and the weights before it come to
+ *            more than u times the weight of all kept; -1 where every logit is
+ *            -infinity or NaN
+ * Results do not depend on scheduling.  Up to 48 MiB of the stream's workspace
+ * (above) hold what a row's workgroups hand on.
+ * No counterpart in the reference, which stops at the logits. */
+int rxq4_sample_f32(int32_t *ids, const float *logits, int64_t row_stride, int n_rows,
+                    int n_vocab, const float *temperature, const int32_t *top_k,
+                    const float *top_p, const float *min_p, const float *u, void *stream);
 
 /* The reference's host GEMV (gemv_quant_cpu, q4_gemm.cu:1742-1854, with its
  * callers' output rounding: fp16 at 1898, fp32 at 2016, the residual's

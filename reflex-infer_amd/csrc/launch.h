@@ -182,6 +182,40 @@ hipError_t launch_prefill_attention(uint16_t *out, const uint16_t *q, const void
                                     int head_dim, int n_tok, int start, float scale, int kv_int8,
                                     const PrefillPlan &plan, hipStream_t stream);
 
+// The serving operators over a paged cache (rxq4_paged_kv, rxq4_seq_batch), their
+// arguments checked.
+struct PagedCache {
+    uint8_t *k, *v;
+    float *ks, *vs;          // int8 only
+    const int32_t *table;    // null: identity
+    int64_t page_bytes;      // K or V bytes from page to page
+    int width;               // table entries per sequence
+    int n_pages, shift;      // page_size = 1 << shift
+    int n_kv, hd;
+};
+struct SeqBatch {
+    const int32_t *starts, *lens;
+    int n_seqs, n_tokens, max_new, max_len;
+};
+hipError_t launch_qk_norm_rope(uint16_t *q_out, const void *q, const void *k, const void *v, int x_dtype,
+                               int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_weight,
+                               const float *k_weight, float eps, const float *inv_freq, int n_rot,
+                               int interleaved, const SeqBatch &batch, const PagedCache &cache, int kv_int8,
+                               hipStream_t stream);
+hipError_t launch_attention_paged(uint16_t *out, const uint16_t *q, int n_heads, float scale,
+                                  const SeqBatch &batch, const PagedCache &cache, int kv_int8,
+                                  hipStream_t stream);
+
+struct SampleRows {
+    int32_t *ids;
+    const float *logits;
+    int64_t stride;
+    int n_vocab;
+    const float *temperature, *top_p, *min_p, *u;
+    const int32_t *top_k;
+};
+hipError_t launch_sample(const SampleRows &rows, int n_rows, hipStream_t stream);
+
 // fp32 rows -> Q4_K blocks (min/max quantiser).
 hipError_t launch_quantize(uint8_t *dst, const float *src, int64_t n_blocks,
                            hipStream_t stream);

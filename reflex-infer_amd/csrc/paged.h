@@ -1,0 +1,56 @@
+// paged.h -- where the tokens of a batch and the positions of a paged cache lie:
+// device helpers shared by the serving kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "launch.h"
+
+namespace rxq4 {
+
+// One sequence of a batch: rows [row0, row0 + n) of q, the first at position
+// pos0 (negative where seq_lens is below the new tokens).  Whatever the device
+// arrays hold, the rows lie within [0, n_tokens).
+struct SeqSpan {
+    int row0, n, pos0;
+};
+__device__ __forceinline__ SeqSpan seq_span(const SeqBatch &b, int s) {
+    const int a = min(max(b.starts[s], 0), b.n_tokens);
+    const int e = min(max(b.starts[s + 1], a), b.n_tokens);
+    return SeqSpan{a, e - a, b.lens[s] - (e - a)};
+}
+
+// The sequence that row t belongs to (n_seqs: none), the same for a whole wave:
+// the number of sequences that end at or before t.
+__device__ __forceinline__ int seq_of_row(const SeqBatch &b, int t) {
+    const int lane = threadIdx.x & 63;
+    int seq = 0;
+    for (int i = 0; i < b.n_seqs; i += 64) {
+        const bool ends = i + lane < b.n_seqs && b.starts[i + lane + 1] <= t;
+        const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(ends));
+        seq += n;
+        if (n < 64) break;
+    }
+    return __builtin_amdgcn_readfirstlane(seq);
+}
+
+// Positions that the batch's tokens may see or store: below the table's end.
+__device__ __forceinline__ int position_limit(const SeqBatch &b, const PagedCache &c) {
+    return (int)min((int64_t)b.max_len, (int64_t)c.width << c.shift);
+}
+
+// The slot (page * page_size + place) of position pos < position_limit of
+// sequence s, -1 in a hole.  Slots are below 2^31.
+__device__ __forceinline__ int slot_of(const PagedCache &c, int s, int pos) {
+    const int i = pos >> c.shift;
+    const int page = c.table ? c.table[(int64_t)s * c.width + i] : i;
+    return (unsigned)page < (unsigned)c.n_pages ? (page << c.shift) + (pos & ((1 << c.shift) - 1)) : -1;
+}
+
+// Bytes from the cache's base to a slot's row of `row_bytes`.
+__device__ __forceinline__ int64_t slot_bytes(const PagedCache &c, int slot, int row_bytes) {
+    return (int64_t)(slot >> c.shift) * c.page_bytes + (int64_t)(slot & ((1 << c.shift) - 1)) * row_bytes;
+}
+
+}  // namespace rxq4

@@ -1,0 +1,219 @@
+// qk_rope.hip -- between a layer's Q/K/V projection and its attention: RMS norm of
+// each query and key head, rotation by position, and the store of the new keys
+// and values into a paged cache (fp16, or int8 with a scale per position and
+// head), in one pass over the projection's output.
+//
+//   norm      x w / sqrt(mean x^2 + eps)
+//   rotation  (a, b) -> (a cos - b sin, b cos + a sin) of the pairs (i, i + n_rot / 2)
+//             or (2 i, 2 i + 1), the angle position * inv_freq[i]: its product and
+//             its remainder to whole turns in 64 bits (in 32 the angle of position
+//             100000 would be off by 2^-8 of a turn), sine and cosine of the
+//             remainder in 32
+//   int8      scale = max |x| / 127, rint(x / scale), both divisions IEEE, so that
+//             the bytes follow from the 32-bit row alone
+// A workgroup takes one token and up to kWaves * kPasses * (heads a wave) of its
+// heads: its threads form the token's sines and cosines once, in LDS; then each
+// head belongs to L lanes of a wave, 8 dims a lane (16-byte loads and stores),
+// the sums over the L lanes by lane swaps and the pair's other half through the
+// wave's own LDS.
+#include <math.h>
+
+#include "launch.h"
+#include "mfma_util.h"
+#include "paged.h"
+#include "q4k_device.h"
+
+namespace rxq4 {
+namespace {
+
+constexpr int kWaves = 4;
+
+struct RopeParams {
+    uint16_t *q_out;
+    const void *q, *k, *v;
+    int64_t q_stride, kv_stride;
+    const float *qw, *kw, *inv_freq;
+    float eps;
+    int n_heads, n_rot, interleaved;
+    int heads_wg;  // heads (queries, keys, values in order) of a workgroup
+    SeqBatch b;
+    PagedCache c;
+};
+
+template <int DT>
+__device__ __forceinline__ void load8(const void *base, int64_t at, float *x) {
+    if constexpr (DT == RXQ4_DTYPE_F32) {
+        const f32x4 *s = reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + at);
+        const f32x4 a = s[0], b = s[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = a[i];
+            x[4 + i] = b[i];
+        }
+    } else {
+        const u32x4 a = load16(static_cast<const uint16_t *>(base) + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = DT == RXQ4_DTYPE_F16 ? f16_bits_to_f32(a[i] & 0xFFFFu) : bf16_bits_to_f32(a[i] & 0xFFFFu);
+            x[2 * i + 1] = DT == RXQ4_DTYPE_F16 ? f16_bits_to_f32(a[i] >> 16) : bf16_bits_to_f32(a[i] >> 16);
+        }
+    }
+}
+
+// A wave's LDS accesses stay in order between its lanes.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// DT: type of q, k, v; L: lanes a head (8 L >= head_dim).
+template <int DT, int L, bool I8>
+__global__ __launch_bounds__(64 * kWaves) void qk_rope_kernel(RopeParams p) {
+    constexpr int HPW = 64 / L;  // heads of a wave at a time
+    __shared__ float cs[128], sn[128];
+    __shared__ __attribute__((aligned(16))) float xl[kWaves][64 * 8];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int t = blockIdx.x;
+    const int seq = seq_of_row(p.b, t);
+    if (seq >= p.b.n_seqs) return;  // uniform
+    const SeqSpan span = seq_span(p.b, seq);
+    if (t < span.row0 || t - span.row0 >= min(span.n, p.b.max_new)) return;
+    const int pos = span.pos0 + (t - span.row0);
+    const int hd = p.c.hd, half = p.n_rot >> 1;
+    const int slot = pos >= 0 && pos < position_limit(p.b, p.c) ? slot_of(p.c, seq, pos) : -1;
+    if (tid < half) {
+        const double turns = (double)pos * (double)p.inv_freq[tid] * 0.15915494309189533577;
+        float s, c;
+        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+        cs[tid] = c;
+        sn[tid] = s;
+    }
+    __syncthreads();
+    const int sub = lane % L;
+    const bool dims = 8 * sub < hd;
+    const int n_all = p.n_heads + 2 * p.c.n_kv;
+    const int h_end = min(n_all, ((int)blockIdx.y + 1) * p.heads_wg);
+    float *const mine = xl[w] + lane * 8;
+    float *const head = xl[w] + (lane - sub) * 8;
+    for (int h0 = blockIdx.y * p.heads_wg + w * HPW; h0 < h_end; h0 += kWaves * HPW) {
+        const int h = min(h0 + lane / L, h_end - 1);  // (lanes past the last head repeat it)
+        const bool live = h0 + lane / L < h_end && dims;
+        const bool is_q = h < p.n_heads, is_v = h >= p.n_heads + p.c.n_kv;
+        const int hk = is_q ? h : is_v ? h - p.n_heads - p.c.n_kv : h - p.n_heads;
+        const void *src = is_q ? p.q : is_v ? p.v : p.k;
+        const int d0 = dims ? 8 * sub : 0;
+        float x[8];
+        load8<DT>(src, (int64_t)t * (is_q ? p.q_stride : p.kv_stride) + (int64_t)hk * hd + d0, x);
+        const float *wt = is_q ? p.qw : is_v ? nullptr : p.kw;
+        if (p.qw || p.kw) {  // uniform; lanes whose head has no weight leave theirs
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += dims ? x[i] * x[i] : 0.0f;
+            ss = group_sum<L>(ss);
+            if (wt) {
+                const float r = 1.0f / sqrtf(ss / (float)hd + p.eps);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = x[i] * r * wt[d0 + i];
+            }
+        }
+        if (half > 0) {  // uniform
+            if (p.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = 4 * sub + i;
+                    if (!is_v && j < half) {
+                        const float a = x[2 * i], b = x[2 * i + 1];
+                        x[2 * i] = a * cs[j] - b * sn[j];
+                        x[2 * i + 1] = b * cs[j] + a * sn[j];
+                    }
+                }
+            } else {
+                wave_lds_fence();  // the reads of the heads before are done
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mine[i] = x[i];
+                wave_lds_fence();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int d = 8 * sub + i;
+                    if (!is_v && d < p.n_rot) {
+                        const bool first = d < half;
+                        const int j = first ? d : d - half;
+                        const float y = head[first ? d + half : d - half];
+                        x[i] = first ? x[i] * cs[j] - y * sn[j] : x[i] * cs[j] + y * sn[j];
+                    }
+                }
+            }
+        }
+        if (is_q) {
+            const bool none = pos < 0;
+            u32x4 r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = none ? 0u : pack2<RXQ4_DTYPE_F16>(x[2 * i], x[2 * i + 1]);
+            if (live) *reinterpret_cast<u32x4 *>(p.q_out + ((int64_t)t * p.n_heads + h) * hd + d0) = r;
+        } else if constexpr (!I8) {
+            u32x4 r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = pack2<RXQ4_DTYPE_F16>(x[2 * i], x[2 * i + 1]);
+            uint8_t *dst = (is_v ? p.c.v : p.c.k) + slot_bytes(p.c, max(slot, 0), p.c.n_kv * hd * 2) + (hk * hd + d0) * 2;
+            if (live && slot >= 0) *reinterpret_cast<u32x4 *>(dst) = r;
+        }
+        if constexpr (I8) {
+            // the largest |x| as bits: an infinity or NaN is larger than any number
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (dims) top = max(top, __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu);
+#pragma unroll
+            for (int off = L / 2; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+            const float scale = __builtin_bit_cast(float, top) / 127.0f;
+            uint32_t b[2] = {0u, 0u};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = scale > 0.0f && scale < INFINITY ? rintf(x[i] / scale) : 0.0f;
+                const int n = (int)fminf(fmaxf(y, -127.0f), 127.0f);
+                b[i >> 2] |= ((uint32_t)n & 0xFFu) << (8 * (i & 3));
+            }
+            if (!is_q && live && slot >= 0) {
+                uint8_t *dst = (is_v ? p.c.v : p.c.k) + slot_bytes(p.c, slot, p.c.n_kv * hd) + hk * hd + d0;
+                *reinterpret_cast<u32x2 *>(dst) = u32x2{b[0], b[1]};
+                if (sub == 0) (is_v ? p.c.vs : p.c.ks)[(int64_t)slot * p.c.n_kv + hk] = scale;
+            }
+        }
+    }
+}
+
+template <int DT, int L>
+void launch_l(const RopeParams &p, dim3 grid, int i8, hipStream_t st) {
+    if (i8) qk_rope_kernel<DT, L, true><<<grid, 64 * kWaves, 0, st>>>(p);
+    else qk_rope_kernel<DT, L, false><<<grid, 64 * kWaves, 0, st>>>(p);
+}
+
+template <int DT>
+void launch_dt(RopeParams &p, int i8, hipStream_t st) {
+    const int L = p.c.hd <= 64 ? 8 : p.c.hd <= 128 ? 16 : 32;
+    const int n_all = p.n_heads + 2 * p.c.n_kv, at_once = kWaves * (64 / L);
+    p.heads_wg = n_all;
+    const dim3 grid(p.b.n_tokens, (n_all + p.heads_wg - 1) / p.heads_wg);
+    (void)at_once;
+    if (L == 8) launch_l<DT, 8>(p, grid, i8, st);
+    else if (L == 16) launch_l<DT, 16>(p, grid, i8, st);
+    else launch_l<DT, 32>(p, grid, i8, st);
+}
+
+}  // namespace
+
+hipError_t launch_qk_norm_rope(uint16_t *q_out, const void *q, const void *k, const void *v, int x_dtype,
+                               int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_weight,
+                               const float *k_weight, float eps, const float *inv_freq, int n_rot,
+                               int interleaved, const SeqBatch &batch, const PagedCache &cache, int kv_int8,
+                               hipStream_t st) {
+    RopeParams p{q_out, q, k, v, q_stride, kv_stride, q_weight, k_weight, inv_freq, eps,
+                 n_heads, n_rot, interleaved, 0, batch, cache};
+    if (x_dtype == RXQ4_DTYPE_F32) launch_dt<RXQ4_DTYPE_F32>(p, kv_int8, st);
+    else if (x_dtype == RXQ4_DTYPE_F16) launch_dt<RXQ4_DTYPE_F16>(p, kv_int8, st);
+    else launch_dt<RXQ4_DTYPE_BF16>(p, kv_int8, st);
+    return hipGetLastError();
+}
+
+}  // namespace rxq4

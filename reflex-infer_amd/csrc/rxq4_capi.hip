@@ -456,6 +456,165 @@ int rxq4_attention_prefill_f16(void *out, const void *q, const void *k_cache,
                      head_dim, N, start_pos + 1, scale, kv_int8, k_scales, v_scales, stream);
 }
 
+}  // extern "C"
+
+namespace {
+
+// Checks of the serving entry points' shared arguments; n_heads is checked with
+// the cache's heads.
+int check_batch(const char *fn, const rxq4_seq_batch *b) {
+    if (!b) return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: null batch", fn);
+    if (b->n_seqs < 0 || b->n_tokens < 0 || b->max_new < 0 || b->max_len < 0)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT,
+                         "%s: n_seqs=%d n_tokens=%d max_new=%d max_len=%d", fn, b->n_seqs,
+                         b->n_tokens, b->max_new, b->max_len);
+    if (b->n_seqs > 0 && (!b->q_starts || !b->seq_lens))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: null q_starts or seq_lens", fn);
+    if (b->n_seqs > RXQ4_MAX_SEQS || b->n_tokens > RXQ4_MAX_TOKENS || b->max_len > RXQ4_MAX_POSITIONS)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT,
+                         "%s: n_seqs=%d (at most %d), n_tokens=%d (%d) or max_len=%d (%d)", fn,
+                         b->n_seqs, RXQ4_MAX_SEQS, b->n_tokens, RXQ4_MAX_TOKENS, b->max_len,
+                         RXQ4_MAX_POSITIONS);
+    return RXQ4_STATUS_SUCCESS;
+}
+
+int check_cache(const char *fn, const rxq4_paged_kv *c, int n_heads, int n_seqs) {
+    if (!c) return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: null cache", fn);
+    if (n_heads <= 0 || c->n_kv_heads <= 0 || n_heads % c->n_kv_heads != 0 || n_heads > RXQ4_MAX_HEADS)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT,
+                         "%s: n_heads=%d must be a positive multiple of n_kv_heads=%d, at most %d",
+                         fn, n_heads, c->n_kv_heads, RXQ4_MAX_HEADS);
+    const int align = c->kv_int8 ? 16 : 8;
+    if (c->head_dim <= 0 || c->head_dim > 256 || c->head_dim % align != 0)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT,
+                         "%s: head_dim=%d must be a multiple of %d and <= 256", fn, c->head_dim, align);
+    if (c->page_size <= 0 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)) != 0)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT,
+                         "%s: page_size=%d must be a power of two, 1 to 1024", fn, c->page_size);
+    if (c->n_pages < 0 || (int64_t)c->n_pages * c->page_size > 0x7FFFFFFF)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: n_pages=%d of %d positions", fn,
+                         c->n_pages, c->page_size);
+    const int64_t dense = (int64_t)c->page_size * c->n_kv_heads * c->head_dim;
+    if (c->page_stride != 0 && (c->page_stride < dense || c->page_stride % align != 0 ||
+                                c->page_stride > (int64_t(1) << 40)))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT,
+                         "%s: page_stride=%lld must be 0 or a multiple of %d and >= %lld", fn,
+                         (long long)c->page_stride, align, (long long)dense);
+    if (c->n_pages > 0 && (!c->k || !c->v || !aligned16(c->k) || !aligned16(c->v)))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: k/v null or not 16-byte aligned", fn);
+    if (!c->page_table && n_seqs > 1)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: null page_table with %d sequences", fn, n_seqs);
+    if (c->page_table && c->table_stride < 0)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: table_stride=%d", fn, c->table_stride);
+    return RXQ4_STATUS_SUCCESS;
+}
+
+rxq4::PagedCache device_cache(const rxq4_paged_kv &c) {
+    rxq4::PagedCache p{};
+    const int64_t dense = (int64_t)c.page_size * c.n_kv_heads * c.head_dim;
+    p.k = static_cast<uint8_t *>(c.k);
+    p.v = static_cast<uint8_t *>(c.v);
+    p.ks = c.kv_int8 ? c.k_scales : nullptr;
+    p.vs = c.kv_int8 ? c.v_scales : nullptr;
+    p.table = c.page_table;
+    p.page_bytes = (c.page_stride ? c.page_stride : dense) * (c.kv_int8 ? 1 : 2);
+    p.width = c.page_table ? c.table_stride : c.n_pages;
+    p.n_pages = c.n_pages;
+    p.shift = __builtin_ctz((unsigned)c.page_size);
+    p.n_kv = c.n_kv_heads;
+    p.hd = c.head_dim;
+    return p;
+}
+
+rxq4::SeqBatch device_batch(const rxq4_seq_batch &b) {
+    return rxq4::SeqBatch{b.q_starts, b.seq_lens, b.n_seqs, b.n_tokens, b.max_new, b.max_len};
+}
+
+}  // namespace
+
+extern "C" {
+
+int rxq4_qk_norm_rope(void *q_out, const void *q, const void *k, const void *v, int x_dtype,
+                      int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_weight,
+                      const float *k_weight, float eps, const float *inv_freq, int n_rot,
+                      int interleaved, const rxq4_seq_batch *batch, const rxq4_paged_kv *cache,
+                      void *stream) {
+    const char *fn = "rxq4_qk_norm_rope";
+    int s = check_batch(fn, batch);
+    if (s != RXQ4_STATUS_SUCCESS) return s;
+    if ((s = check_cache(fn, cache, n_heads, batch->n_seqs)) != RXQ4_STATUS_SUCCESS) return s;
+    if (x_dtype != RXQ4_DTYPE_F16 && x_dtype != RXQ4_DTYPE_BF16 && x_dtype != RXQ4_DTYPE_F32)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: x_dtype=%d", fn, x_dtype);
+    const int64_t q_row = (int64_t)n_heads * cache->head_dim, kv_row = (int64_t)cache->n_kv_heads * cache->head_dim;
+    if (q_stride < q_row || kv_stride < kv_row || q_stride % 8 != 0 || kv_stride % 8 != 0 ||
+        q_stride > (int64_t(1) << 32) || kv_stride > (int64_t(1) << 32))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT,
+                         "%s: q_stride=%lld, kv_stride=%lld must be multiples of 8 and hold %lld, %lld", fn,
+                         (long long)q_stride, (long long)kv_stride, (long long)q_row, (long long)kv_row);
+    if (n_rot < 0 || n_rot > cache->head_dim || n_rot % 2 != 0)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: n_rot=%d must be even, at most head_dim=%d", fn,
+                         n_rot, cache->head_dim);
+    if ((q_weight || k_weight) && !(eps >= 0.0f))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: eps=%g", fn, eps);
+    if (batch->n_seqs == 0 || batch->n_tokens == 0) return ok();
+    if (!q_out || !q || !k || !v || !aligned16(q_out) || !aligned16(q) || !aligned16(k) || !aligned16(v))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: q_out/q/k/v null or not 16-byte aligned", fn);
+    if (n_rot > 0 && !inv_freq)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: null inv_freq", fn);
+    if (cache->kv_int8 && (!cache->k_scales || !cache->v_scales))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: an int8 cache needs both scale arrays", fn);
+    const int64_t esz = x_dtype == RXQ4_DTYPE_F32 ? 4 : 2;
+    const uintptr_t o0 = reinterpret_cast<uintptr_t>(q_out), o1 = o0 + (uintptr_t)(batch->n_tokens * q_row * 2);
+    const uintptr_t i0 = reinterpret_cast<uintptr_t>(q),
+                    i1 = i0 + (uintptr_t)(((batch->n_tokens - 1) * q_stride + q_row) * esz);
+    if (o0 < i1 && i0 < o1 && !(o0 == i0 && x_dtype == RXQ4_DTYPE_F16 && q_stride == q_row))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT,
+                         "%s: q_out overlaps q (it may be q itself, fp16 and without gaps)", fn);
+    if ((s = check_device(fn)) != RXQ4_STATUS_SUCCESS) return s;
+    return from_hip(rxq4::launch_qk_norm_rope(static_cast<uint16_t *>(q_out), q, k, v, x_dtype, q_stride,
+                                              kv_stride, n_heads, q_weight, k_weight, eps, inv_freq, n_rot,
+                                              interleaved ? 1 : 0, device_batch(*batch), device_cache(*cache),
+                                              cache->kv_int8 ? 1 : 0, static_cast<hipStream_t>(stream)),
+                    fn);
+}
+
+int rxq4_attention_paged_f16(void *out, const void *q, int n_heads, float scale,
+                             const rxq4_seq_batch *batch, const rxq4_paged_kv *cache,
+                             void *stream) {
+    const char *fn = "rxq4_attention_paged_f16";
+    int s = check_batch(fn, batch);
+    if (s != RXQ4_STATUS_SUCCESS) return s;
+    if ((s = check_cache(fn, cache, n_heads, batch->n_seqs)) != RXQ4_STATUS_SUCCESS) return s;
+    if (!(scale - scale == 0.0f)) return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: scale=%g", fn, scale);
+    if (batch->n_seqs == 0 || batch->n_tokens == 0 || batch->max_new == 0) return ok();
+    if (!out || !q || !aligned16(out) || !aligned16(q))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: q/out null or not 16-byte aligned", fn);
+    if ((s = check_device(fn)) != RXQ4_STATUS_SUCCESS) return s;
+    return from_hip(rxq4::launch_attention_paged(static_cast<uint16_t *>(out), static_cast<const uint16_t *>(q),
+                                                 n_heads, scale, device_batch(*batch), device_cache(*cache),
+                                                 cache->kv_int8 ? 1 : 0, static_cast<hipStream_t>(stream)),
+                    fn);
+}
+
+int rxq4_sample_f32(int32_t *ids, const float *logits, int64_t row_stride, int n_rows,
+                    int n_vocab, const float *temperature, const int32_t *top_k,
+                    const float *top_p, const float *min_p, const float *u, void *stream) {
+    const char *fn = "rxq4_sample_f32";
+    if (n_rows < 0 || n_vocab <= 0 || n_vocab > RXQ4_MAX_VOCAB || row_stride < n_vocab)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: n_rows=%d n_vocab=%d (1 to %d) row_stride=%lld", fn,
+                         n_rows, n_vocab, RXQ4_MAX_VOCAB, (long long)row_stride);
+    if (n_rows == 0) return ok();
+    if (!ids || !logits || !u) return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: null ids, logits or u", fn);
+    const int s = check_device(fn);
+    if (s != RXQ4_STATUS_SUCCESS) return s;
+    const rxq4::SampleRows rows{ids, logits, row_stride, n_vocab, temperature, top_p, min_p, u, top_k};
+    return from_hip(rxq4::launch_sample(rows, n_rows, static_cast<hipStream_t>(stream)), fn);
+}
+
+}  // extern "C"
+
+extern "C" {
+
 const void *rxq4_resolve_weights(const void *w, const void *w_device) {
     if (w_device) return w_device;
     if (!w) return nullptr;

@@ -20,6 +20,19 @@ class Rows(ctypes.Structure):
     _fields_ = [("y", c_void_p), ("w", c_void_p), ("ggml_type", c_int), ("M", c_int)]
 
 
+class PagedKVStruct(ctypes.Structure):
+    """rxq4_paged_kv: a paged KV cache."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scales", c_void_p), ("v_scales", c_void_p),
+                ("page_table", c_void_p), ("page_stride", c_int64), ("table_stride", c_int), ("n_pages", c_int),
+                ("page_size", c_int), ("n_kv_heads", c_int), ("head_dim", c_int), ("kv_int8", c_int)]
+
+
+class SeqBatchStruct(ctypes.Structure):
+    """rxq4_seq_batch: the new tokens of a batch of sequences."""
+    _fields_ = [("q_starts", c_void_p), ("seq_lens", c_void_p), ("n_seqs", c_int), ("n_tokens", c_int),
+                ("max_new", c_int), ("max_len", c_int)]
+
+
 # name -> (restype, argtypes); every name is declared in include/rxq4.h.
 SIGNATURES = {
     "rxq4_gemv_f16": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p]),
@@ -44,6 +57,13 @@ SIGNATURES = {
     "rxq4_attention_prefill_f16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                            c_int, c_int, c_int, ctypes.c_float, c_int, c_void_p,
                                            c_void_p, c_void_p]),
+    "rxq4_qk_norm_rope": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p,
+                                  c_void_p, ctypes.c_float, c_void_p, c_int, c_int,
+                                  ctypes.POINTER(SeqBatchStruct), ctypes.POINTER(PagedKVStruct), c_void_p]),
+    "rxq4_attention_paged_f16": (c_int, [c_void_p, c_void_p, c_int, ctypes.c_float, ctypes.POINTER(SeqBatchStruct),
+                                         ctypes.POINTER(PagedKVStruct), c_void_p]),
+    "rxq4_sample_f32": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                c_void_p, c_void_p]),
     "rxq4_host_gemv": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int,
                                c_int]),
     "rxq4_host_gemv_calls": (ctypes.c_longlong, []),
@@ -203,6 +223,142 @@ def attention_prefill_f16(out, q, k, v, n_heads, n_kv_heads, head_dim, N, start_
         _ptr(out), _ptr(q), _ptr(k), _ptr(v), n_heads, n_kv_heads, head_dim, N, start_pos, scale,
         int(kv_int8), _ptr(k_scales), _ptr(v_scales), _stream(stream)),
         "rxq4_attention_prefill_f16")
+
+
+def _int32(t, what):
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor")
+    return t
+
+
+def _same_device(name, first, *others):
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError(f"{name}: tensors on {device} and {t.device}")
+
+
+def _on_current_device(name, t):
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name}: tensors on {t.device}, which is not the current GPU")
+
+
+class PagedKV:
+    """A layer's paged KV cache, built once beside its tensors: k, v
+    [n_pages, page_size, n_kv_heads, head_dim] fp16 or int8 (the pages may lie
+    apart in memory, each dense in itself), int8 scales [n_pages, page_size,
+    n_kv_heads] fp32, page_table int32 [n_seqs, pages] (None: one sequence whose
+    pages are in order).  Holds the tensors."""
+
+    def __init__(self, k, v, page_table=None, k_scales=None, v_scales=None):
+        n_pages, page_size, n_kv, hd = k.shape
+        if v.shape != k.shape or v.dtype != k.dtype or k.dtype not in (torch.float16, torch.int8):
+            raise ValueError("PagedKV: k and v must be alike, fp16 or int8")
+        stride = k.stride(0) if n_pages > 1 else page_size * n_kv * hd
+        for t in (k, v):
+            if t.stride()[1:] != (n_kv * hd, hd, 1) or (n_pages > 1 and t.stride(0) != stride):
+                raise ValueError("PagedKV: a page must be dense, and K and V pages lie alike")
+        for t in (k_scales, v_scales):
+            if t is not None and (t.dtype != torch.float32 or t.shape != k.shape[:3] or not t.is_contiguous()):
+                raise ValueError("PagedKV: scales must be contiguous fp32 [n_pages, page_size, n_kv_heads]")
+        if page_table is not None and (page_table.dim() != 2 or page_table.dtype != torch.int32 or
+                                       (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
+            raise ValueError("PagedKV: page_table must be int32 [n_seqs, pages], its rows dense")
+        _same_device("PagedKV", k, v, page_table, k_scales, v_scales)
+        self.tensors = (k, v, page_table, k_scales, v_scales)
+        self.n_seqs = 1 if page_table is None else page_table.shape[0]
+        self.n_kv_heads, self.head_dim = n_kv, hd
+        pages = 0 if page_table is None else page_table.shape[1]
+        if pages > 0 and self.n_seqs > 1 and page_table.stride(0) != pages:
+            raise ValueError("PagedKV: page_table must be dense")
+        self.struct = PagedKVStruct(_ptr(k), _ptr(v), _ptr(k_scales), _ptr(v_scales), _ptr(page_table), stride, pages,
+                                    n_pages, page_size, n_kv, hd, int(k.dtype == torch.int8))
+        self.ref = ctypes.byref(self.struct)
+
+
+class SeqBatch:
+    """The new tokens of a batch (rxq4_seq_batch): q_starts int32 [n_seqs + 1],
+    seq_lens int32 [n_seqs] on the device, and their limits.  Holds the tensors,
+    whose values may change between calls (and replays) within the limits."""
+
+    def __init__(self, q_starts, seq_lens, n_tokens, max_new, max_len):
+        self.tensors = (_int32(q_starts, "q_starts"), _int32(seq_lens, "seq_lens"))
+        self.n_seqs, self.n_tokens = seq_lens.numel(), n_tokens
+        if q_starts.numel() != self.n_seqs + 1:
+            raise ValueError("SeqBatch: q_starts must have one value more than seq_lens")
+        _same_device("SeqBatch", q_starts, seq_lens)
+        self.struct = SeqBatchStruct(_ptr(q_starts), _ptr(seq_lens), self.n_seqs, n_tokens, max_new, max_len)
+        self.ref = ctypes.byref(self.struct)
+
+
+def _fits(name, batch, cache):
+    if batch.n_seqs > cache.n_seqs:
+        raise ValueError(f"{name}: {batch.n_seqs} sequences, page_table has {cache.n_seqs}")
+    _same_device(name, batch.tensors[0], cache.tensors[0])
+
+
+def qk_norm_rope(q_out, q, k, v, batch, cache, inv_freq, q_weight=None, k_weight=None, eps=1e-6, interleaved=False,
+                 stream=None):
+    """q [n_tokens, n_heads, head_dim] and k, v [n_tokens, n_kv_heads, head_dim]
+    (fp16, bf16 or fp32, e.g. slices of one fused projection): head norms,
+    rotation by position * inv_freq, queries to q_out, keys and values into the
+    cache's pages."""
+    _fits("qk_norm_rope", batch, cache)
+    n, heads, hd = q.shape
+    want = (batch.n_tokens, cache.n_kv_heads, cache.head_dim)
+    if (n, hd) != (want[0], want[2]) or k.shape != want or v.shape != want or q_out.shape != q.shape:
+        raise ValueError(f"qk_norm_rope: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, q_out "
+                         f"{tuple(q_out.shape)} for {want[0]} tokens, {want[1]} KV heads of {want[2]}")
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    if sq[1:] != (hd, 1) or sk[1:] != (hd, 1) or sv[1:] != (hd, 1) or (sk[0] != sv[0] and n > 1) or \
+            q.dtype != k.dtype or q.dtype != v.dtype or q_out.dtype != torch.float16 or not q_out.is_contiguous():
+        raise ValueError("qk_norm_rope: rows must be dense, k and v rows equally far apart, q, k, v of one type, "
+                         "q_out contiguous fp16")
+    for t in (inv_freq, q_weight, k_weight):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous()):
+            raise ValueError("qk_norm_rope: inv_freq and weights must be contiguous fp32")
+    for t in (q_weight, k_weight):
+        if t is not None and t.numel() != hd:
+            raise ValueError(f"qk_norm_rope: weights must have head_dim={hd} values")
+    _same_device("qk_norm_rope", cache.tensors[0], q_out, q, k, v, inv_freq, q_weight, k_weight)
+    _on_current_device("qk_norm_rope", q)
+    return _check(lib().rxq4_qk_norm_rope(
+        _ptr(q_out), _ptr(q), _ptr(k), _ptr(v), _dtype_code(q), sq[0] if n > 1 else heads * hd,
+        sk[0] if n > 1 else want[1] * hd, heads, _ptr(q_weight), _ptr(k_weight), eps, _ptr(inv_freq),
+        0 if inv_freq is None else 2 * inv_freq.numel(), int(interleaved), batch.ref, cache.ref, _stream(stream)),
+        "rxq4_qk_norm_rope")
+
+
+def attention_paged_f16(out, q, batch, cache, scale, stream=None):
+    """out, q fp16 [n_tokens, n_heads, head_dim]: each sequence's new tokens over
+    its pages, causal."""
+    _fits("attention_paged_f16", batch, cache)
+    if q.dim() != 3 or q.shape[0] != batch.n_tokens or q.shape[2] != cache.head_dim or out.shape != q.shape or \
+            q.dtype != torch.float16 or out.dtype != torch.float16 or not q.is_contiguous() or not out.is_contiguous():
+        raise ValueError(f"attention_paged_f16: q and out must be contiguous fp16 [{batch.n_tokens}, n_heads, "
+                         f"{cache.head_dim}]")
+    _same_device("attention_paged_f16", cache.tensors[0], out, q)
+    _on_current_device("attention_paged_f16", q)
+    return _check(lib().rxq4_attention_paged_f16(_ptr(out), _ptr(q), q.shape[1], scale, batch.ref, cache.ref,
+                                                 _stream(stream)), "rxq4_attention_paged_f16")
+
+
+def sample_f32(ids, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
+    """ids int32 [n] = the next token of each row of logits fp32 [n, vocab] from u
+    fp32 [n] in [0, 1); the parameters are per-row tensors or None."""
+    n, vocab = logits.shape
+    for t, dtype in ((ids, torch.int32), (u, torch.float32), (temperature, torch.float32), (top_k, torch.int32),
+                     (top_p, torch.float32), (min_p, torch.float32)):
+        if t is not None and (t.dtype != dtype or t.numel() != n or not t.is_contiguous()):
+            raise ValueError(f"sample_f32: every parameter must have one value for each of {n} rows (fp32; ids and "
+                             "top_k int32)")
+    if logits.dtype != torch.float32 or (vocab > 1 and logits.stride(1) != 1):
+        raise ValueError("sample_f32: logits must be fp32 with dense rows")
+    _same_device("sample_f32", logits, ids, u, temperature, top_k, top_p, min_p)
+    _on_current_device("sample_f32", logits)
+    return _check(lib().rxq4_sample_f32(_ptr(ids), _ptr(logits), logits.stride(0) if n > 1 else vocab, n, vocab,
+                                        _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(u),
+                                        _stream(stream)), "rxq4_sample_f32")
 
 
 def host_gemv(w, x, M: int, K: int, ggml_type: int = GGML_TYPE_Q4_K, out: str = "f32",

@@ -1,0 +1,181 @@
+"""GPU sampling (rxq4_sample_f32) against the walk of the order in 64 bits
+(serving_reference.sample): the tokens are equal.  A draw within the sums' error of
+a border could go either way; sums are off by 2^-30 of the total at most here, and
+no drawn number below lies that near a border."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import rxq4  # noqa: F401
+from rxq4 import capi
+from tests import serving_reference as ref
+
+pytestmark = pytest.mark.gpu
+F, I = torch.float32, torch.int32
+
+
+def logits_of(seed, n, vocab, kind):
+    r = np.random.default_rng(seed)
+    if kind == "model":  # a bulk and a few raised tokens
+        l = r.standard_normal((n, vocab)) * 2
+        for row in l:
+            row[r.integers(0, vocab, 64)] += r.random(64) * 10
+    elif kind == "flat":
+        l = r.standard_normal((n, vocab)) * 0.01
+    elif kind == "equal":
+        l = np.full((n, vocab), 1.5)
+    elif kind == "few":  # many ties
+        l = r.integers(-3, 4, (n, vocab)) * 0.5
+    else:  # wide
+        l = r.standard_normal((n, vocab)) * 300
+    return l.astype(np.float32)
+
+
+def run(l, u, stride=None, **params):
+    n, vocab = l.shape
+    dev = torch.from_numpy(l).cuda()
+    if stride:
+        wide = torch.full((n, stride), 1e30, dtype=F, device="cuda")
+        wide[:, :vocab] = dev
+        dev = wide[:, :vocab]
+    ids = torch.full((n,), -7, dtype=I, device="cuda")
+    t = {k: None if v is None else torch.as_tensor(np.asarray(v), dtype=I if k == "top_k" else F).cuda()
+         for k, v in params.items()}
+    capi.sample_f32(ids, dev, torch.as_tensor(u, dtype=F).cuda(), **t)
+    return ids.cpu().numpy()
+
+
+def check(l, u, stride=None, **params):
+    got = run(l, u, stride, **params)
+    f32 = lambda k, v: int(v) if k == "top_k" else np.float32(v)  # noqa: E731
+    want = [ref.sample(l[i], np.float32(u[i]), **{k: f32(k, v[i]) for k, v in params.items() if v is not None})
+            for i in range(len(l))]
+    assert got.tolist() == want
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 63, 64, 255, 1000, 1025, 8191, 8192, 8193, 32000, 151936, 300001])
+@pytest.mark.parametrize("kind", ["model", "flat", "few"])
+def test_sizes(vocab, kind):
+    print(f"sample vocab={vocab} {kind}", flush=True)
+    n = 4
+    l = logits_of(vocab, n, vocab, kind) if vocab > 64 or kind != "model" else logits_of(vocab, n, vocab, "wide")
+    u = np.random.default_rng(vocab + 1).random(n).astype(np.float32)
+    check(l, u)
+    check(l, u, temperature=[0.7] * n, top_k=[50] * n, top_p=[0.9] * n, min_p=[0.02] * n)
+
+
+@pytest.mark.parametrize("kind", ["model", "flat", "equal", "few", "wide"])
+def test_parameters(kind):
+    """Every parameter alone, and mixtures of them row by row."""
+    n, vocab = 24, 20011
+    l = logits_of(3, n, vocab, kind)
+    r = np.random.default_rng(4)
+    u = r.random(n).astype(np.float32)
+    pick = lambda values: r.choice(values, n)  # noqa: E731
+    temperature, top_k = pick([0.0, 0.3, 0.7, 1.0, 2.5, -1.0]), pick([0, 1, 2, 40, 1000, 20011, 30000, -5])
+    top_p, min_p = pick([0.0, 0.1, 0.5, 0.95, 0.9999, 1.0, 1.5]), pick([0.0, 1e-4, 0.05, 0.5, 1.0, 2.0, -1.0])
+    check(l, u, temperature=temperature)
+    check(l, u, top_k=top_k)
+    check(l, u, top_p=top_p)
+    check(l, u, min_p=min_p)
+    check(l, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+
+
+def test_the_ends_of_u():
+    l = logits_of(5, 8, 5000, "few")
+    u = [0.0, -1.0, 1.0, 2.0, float("nan"), np.nextafter(np.float32(1), np.float32(0)), 0.5, 1e-30]
+    check(l, u, top_k=[100] * 8)
+    check(l, u)
+
+
+def test_equal_logits_follow_the_index():
+    """All weights equal: token floor(u n), exactly."""
+    n, vocab = 64, 4096
+    l = np.zeros((n, vocab), np.float32)
+    u = (np.arange(n) / n).astype(np.float32)
+    assert run(l, u).tolist() == [vocab // n * i for i in range(n)]
+    got = run(l, u, top_k=np.full(n, 64))
+    assert got.tolist() == list(range(n))
+
+
+def test_infinities_nan_and_the_lowest_number():
+    low, inf, nan = float(np.finfo(np.float32).min), float("inf"), float("nan")
+    vocab = 3000
+    l = logits_of(6, 9, vocab, "model")
+    l[0] = -inf                       # nothing: -1
+    l[1] = nan                        # nothing: -1
+    l[2] = low                        # all equal
+    l[3, :2990] = -inf
+    l[4, 5:2000] = low
+    l[5, 17] = nan
+    l[6, [40, 400, 1400]] = inf       # they share the row
+    l[7], l[7, 1234] = -inf, -5.0     # one
+    l[8] = -l[8] * 0 - 0.0            # zeros of both signs are equal
+    l[8, ::2] = 0.0
+    u = np.linspace(0.05, 0.95, 9).astype(np.float32)
+    got = run(l, u)
+    assert got[0] == -1 and got[1] == -1 and got[7] == 1234 and got[6] in (40, 400, 1400)
+    check(l, u)
+    check(l, u, temperature=[0.5] * 9, top_p=[0.9] * 9)
+    check(l, u, temperature=[1e-30] * 9)
+    check(l, u, temperature=[0.0] * 9)
+    check(l, u, temperature=[nan] * 9)
+    check(l, u, temperature=[inf] * 9, top_k=[7] * 9)
+
+
+def test_rows_far_apart_and_odd():
+    l = logits_of(7, 5, 1003, "model")
+    check(l, [0.1, 0.3, 0.5, 0.7, 0.9], stride=1011, top_k=[10] * 5)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 128, 300, 1000])
+def test_many_rows(rows):
+    l = logits_of(8, rows, 1777, "model")
+    u = np.random.default_rng(9).random(rows).astype(np.float32)
+    check(l, u, temperature=[0.8] * rows, top_p=[0.95] * rows)
+
+
+def test_more_rows_than_a_workspace_holds():
+    """The library's large vocabulary, and rows enough for several launches."""
+    n, vocab = 200, 151936
+    g = torch.Generator(device="cuda").manual_seed(10)
+    dev = torch.randn((n, vocab), generator=g, device="cuda") * 3
+    u = torch.rand(n, generator=g, device="cuda")
+    ids = torch.empty(n, dtype=I, device="cuda")
+    p = torch.full((n,), 0.9, device="cuda")
+    capi.sample_f32(ids, dev, u, top_p=p)
+    for i in list(range(0, n, 23)) + [n - 1]:
+        assert ids[i].item() == ref.sample(dev[i].cpu().numpy(), np.float32(u[i].item()), top_p=np.float32(0.9))
+    one = torch.empty(1, dtype=I, device="cuda")
+    for i in (0, 77, 199):  # a row does not depend on the others
+        capi.sample_f32(one, dev[i:i + 1], u[i:i + 1], top_p=p[:1])
+        assert one.item() == ids[i].item()
+
+
+def test_repeats_and_replays():
+    n, vocab = 6, 40000
+    l = torch.from_numpy(logits_of(11, n, vocab, "model")).cuda()
+    u = torch.rand(n, device="cuda")
+    ids = torch.empty(n, dtype=I, device="cuda")
+    k = torch.full((n,), 30, dtype=I, device="cuda")
+    s = torch.cuda.Stream()
+    capi.sample_f32(ids, l, u, top_k=k, stream=s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        capi.sample_f32(ids, l, u, top_k=k, stream=s)
+    for step in range(5):
+        u.uniform_()
+        l.add_(torch.randn_like(l) * 0.1)
+        k.fill_(5 + 10 * step)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            graph.replay()
+        torch.cuda.synchronize()
+        eager = torch.empty_like(ids)
+        capi.sample_f32(eager, l, u, top_k=k)
+        assert torch.equal(eager, ids)
+        host = l.cpu().numpy()
+        assert ids.tolist() == [ref.sample(host[i], np.float32(u[i].item()), top_k=5 + 10 * step) for i in range(n)]
