@@ -1,89 +1,445 @@
-// attn_paged.hip -- attention of a batch's new tokens over a paged KV cache.
+// attn_paged.hip -- attention of a batch's new tokens over a paged KV cache, on
+// the gfx950 matrix cores.
 //
 // Token at position p, head h: out = sum_j e^(s_j) v_j / sum_j e^(s_j) over the
 // positions j <= p whose page is in the pool, s_j = scale q.k_j, KV head h /
 // group; the sums relative to a running maximum, in fp32.
 //
-// A wave per token and head: a lane's score per position, 64 positions a step,
-// then a lane's dims of the output.
+// Query rows.  The rows of a sequence and KV head are numbered t * group + j (new
+// token t, j-th head of the group).  A workgroup takes 16 of them, the columns of
+// a 16 x 16 MFMA tile, and one chunk of positions: each K and V row is read once
+// for all of them, which is what bounds decoding (one to a few new tokens).
 #include <math.h>
 
+#include <algorithm>
+
 #include "launch.h"
+#include "mfma_util.h"
 #include "paged.h"
 #include "q4k_device.h"
 
 namespace rxq4 {
 namespace {
 
+typedef short v4i16 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTile = 64;       // positions per tile
+constexpr int kMaxChunks = 64;  // chunks of positions per sequence
+// P holds 2^kShift times the probabilities relative to the running maximum: the
+// low half of the fp16 pair that carries one ends at 2^-24, 2^-35 of it.
+constexpr float kShift = 11.0f;
+// V scales below 2^kMinScale count as that where the reference point is chosen
+// (what they weigh is 0 in an fp16 output) and those above 2^kMaxScale as that.
+constexpr float kMinScale = -40.0f, kMaxScale = 127.0f;
+
 struct PagedParams {
     uint16_t *out;
     const uint16_t *q;
+    float *part, *stats;  // [unit][chunk][row]: HD floats; (maximum in log2 units, sum)
     SeqBatch b;
     PagedCache c;
     int n_heads, group;
-    float scale;
+    float sl2;            // scale * log2(e)
+    int n_rb;             // blocks of 16 rows per sequence and KV head
+    int rows_blk;         // rows of a block that the partials hold
+    int chunk, n_chunks;  // positions per chunk; chunks per unit
 };
 
-template <bool I8>
-__global__ __launch_bounds__(64) void attn_paged_row_kernel(PagedParams p) {
-    constexpr int esz = I8 ? 1 : 2;
-    __shared__ float qs[256];
-    const int lane = threadIdx.x;
-    const int t = blockIdx.x / p.n_heads, h = blockIdx.x % p.n_heads;
-    const int s = seq_of_row(p.b, t);
-    if (s >= p.b.n_seqs) return;
-    const SeqSpan q = seq_span(p.b, s);
-    if (t < q.row0 || t - q.row0 >= min(q.n, p.b.max_new)) return;
-    const int hd = p.c.hd, kvh = h / p.group;
-    const int row_bytes = p.c.n_kv * hd * esz;
-    const int end = min(q.pos0 + (t - q.row0) + 1, position_limit(p.b, p.c));
-    const uint16_t *qrow = p.q + ((int64_t)t * p.n_heads + h) * hd;
-    for (int i = lane; i < hd; i += 64) qs[i] = f16_bits_to_f32(qrow[i]);
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p0 = 0; p0 < end; p0 += 64) {
-        const int pos = p0 + lane;
-        const int slot = pos < end ? slot_of(p.c, s, pos) : -1;
-        float sc = -INFINITY;
-        if (slot >= 0) {
-            const uint8_t *k = p.c.k + slot_bytes(p.c, slot, row_bytes) + (int64_t)kvh * hd * esz;
-            float d = 0.0f;
-            for (int i = 0; i < hd; ++i)
-                d += qs[i] * (I8 ? (float)reinterpret_cast<const int8_t *>(k)[i]
-                                 : f16_bits_to_f32(reinterpret_cast<const uint16_t *>(k)[i]));
-            if (I8 && p.c.ks) d *= p.c.ks[(int64_t)slot * p.c.n_kv + kvh];
-            sc = d * p.scale;
-        }
-        const uint64_t seen = __builtin_amdgcn_ballot_w64(slot >= 0);
-        if (seen == 0) continue;
-        const float m_new = fmaxf(m, butterfly_max<64>(sc));
-        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-        const float corr = expf(m - m_use);
-        const float e = slot >= 0 ? expf(sc - m_use) : 0.0f;
-        l = l * corr + butterfly_sum<64>(e);
-        m = m_new;
+__device__ __forceinline__ float log2_scale(float vs) {
+    return fminf(fmaxf(__builtin_amdgcn_logf(fabsf(vs)), kMinScale), kMaxScale);
+}
+
+// lo = RNE_f16(e - f32(hi)) for a pair: the difference is exact in fp32.  (Not in
+// inline asm: an MFMA may read a VALU result two wait states later at the earliest,
+// which the compiler keeps only for instructions that it knows.)
+__device__ __forceinline__ uint32_t low_halves(float e0, float e1, uint32_t hi) {
+    return pack2<RXQ4_DTYPE_F16>(e0 - f16_bits_to_f32(hi & 0xFFFFu), e1 - f16_bits_to_f32(hi >> 16));
+}
+
+// Infinities and NaN among N x 8 fp16: whether there are any (times 0 they are
+// NaN), and zeros in their place (a half with all exponent bits set carries into
+// its top bit).
+template <int N>
+__device__ __forceinline__ bool not_finite16(const u32x4 *x) {
+    f16x2 sum[4] = {};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] *= corr;
-        const float ve = I8 && p.c.vs && slot >= 0 ? p.c.vs[(int64_t)slot * p.c.n_kv + kvh] : 1.0f;
-        for (int j = 0; j < 64; ++j) {
-            if (!((seen >> j) & 1)) continue;  // uniform
-            const uint8_t *v = p.c.v + slot_bytes(p.c, __shfl(slot, j, 64), row_bytes) + (int64_t)kvh * hd * esz;
-            const float w = __shfl(e, j, 64), x = __shfl(ve, j, 64);
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t v = x[j][i];
+            sum[i] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, v), f16x2{0, 0}, sum[i]);
+        }
+    const f16x2 all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    return !(all.x == 0) || !(all.y == 0);
+}
+template <int N>
+__device__ __forceinline__ void zero_not_finite16(u32x4 *x) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t all = (((x[j][i] & 0x7C007C00u) + 0x04000400u) >> 15) & 0x00010001u;
+            x[j][i] &= ~(all * 0xFFFFu);
+        }
+}
+
+// 8 int8 (bytes of .x, .y) as 8 fp16 (exact).
+__device__ __forceinline__ u32x4 i8_to_f16(u32x2 v) {
+    uint32_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t wd = e < 2 ? v.x : v.y;
+        const int sh = 16 * (e & 1);
+        o[e] = pack2<RXQ4_DTYPE_F16>((float)(int8_t)(uint8_t)(wd >> sh), (float)(int8_t)(uint8_t)(wd >> (sh + 8)));
+    }
+    return u32x4{o[0], o[1], o[2], o[3]};
+}
+
+// Wave w takes positions 16 w .. + 15 of every 64-position tile of the chunk with
+// its own online softmax; the four waves merge at the end.  Per tile, lane l =
+// 16 g + r:
+//   S^T = K . Q^T    v_mfma_f32_16x16x32_f16, src0 = 16 positions x 32 dims of K
+//                    straight from memory (16 bytes a lane), src1 = Q^T; the lane
+//                    gets positions 4 g + i of row r;
+//   O^T += V^T P^T   v_mfma_f32_16x16x16_f16, src0 = 16 dims x 16 positions of V^T
+//                    (ds_read_tr16_b64 of the wave's V rows in LDS), src1 = P^T as
+//                    the score registers hold it, in fp16 hi + lo parts (22 bits).
+// Lane r looks up the page of position r once; the V chunks' lanes get the row's
+// offset from it.  int8: P holds the V scales, so the reference point of the
+// exponentials follows the maximum of score + log2 |scale|, and neither end of
+// fp16 is met whatever the scales.
+// The loads of NB tiles go out before their arithmetic, the table entries of the
+// next ones with them.
+template <int HD, bool I8>
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel(PagedParams p) {
+    constexpr int KS = HD / 32, DT = HD / 16, VROW = HD + 16, CH = HD / 8, NV = 16 * CH / 64;
+    constexpr int NB = HD <= 128 ? 4 : 2;
+    constexpr int esz = I8 ? 1 : 2;
+    constexpr int NM = DT * 4 + 2;  // merge values per lane: O, m, l
+    __shared__ __attribute__((aligned(16))) uint16_t vl[4][16 * VROW];
+    __shared__ float mg[4][NM][64];
+
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int n_u = p.n_chunks * p.b.n_seqs * p.c.n_kv;
+    const int rb = blockIdx.x / n_u, u = blockIdx.x % n_u;
+    const int kvh = u % p.c.n_kv, s = u / p.c.n_kv % p.b.n_seqs, c = u / (p.c.n_kv * p.b.n_seqs);
+    const int beg = c * p.chunk;
+    const int limit = position_limit(p.b, p.c);
+    if (beg >= limit && c > 0) return;
+
+    // Table entries of the first tiles, before the sequence's length is known.
+    const int32_t *const table = p.c.table ? p.c.table + (int64_t)s * p.c.width : nullptr;
+    auto entry = [&](int pos) {
+        const int i = pos >> p.c.shift;
+        return pos < limit ? (table ? table[i] : i) : -1;
+    };
+    int ent[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) ent[b] = entry(beg + kTile * b + 16 * w + r);
+    const SeqSpan span = seq_span(p.b, s);
+    const int rows = min(span.n, p.b.max_new) * p.group;
+    const int row0 = rb * 16;
+    if (row0 >= rows) return;
+    const int last_tok = (min(rows, row0 + 16) - 1) / p.group;
+    const int end_blk = min(span.pos0 + last_tok + 1, limit);
+    const int end = min(end_blk, beg + p.chunk);
+    const int row = min(row0 + r, rows - 1);  // (columns past the last row repeat it)
+    const int tok = row / p.group, head = kvh * p.group + row % p.group;
+    const bool row_ok = row0 + r < rows;
+    const int hd = p.c.hd, n_ch = hd >> 3;
+    const int64_t orow = ((int64_t)(span.row0 + tok) * p.n_heads + head) * hd;
+    if (end <= beg) {  // uniform
+        if (c == 0 && w == 0 && row_ok)  // the block sees nothing
+            for (int ch = g; ch < n_ch; ch += 4) *reinterpret_cast<u32x4 *>(p.out + orow + 8 * ch) = u32x4{0u, 0u, 0u, 0u};
+        return;
+    }
+    const int qpos = span.pos0 + tok;
+    const int row_bytes = p.c.n_kv * hd * esz;
+    const uint8_t *kb = p.c.k + (int64_t)kvh * hd * esz, *vb = p.c.v + (int64_t)kvh * hd * esz;
+
+    u32x4 qf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+        qf[ks] = 4 * ks + g < n_ch ? load16(p.q + orow + 8 * (4 * ks + g)) : u32x4{0u, 0u, 0u, 0u};
+
+    f32x4 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    bool bad = false;  // some V is not finite
+    const int n_tiles = (end - beg + kTile - 1) / kTile;
+
+    for (int j0 = 0; j0 < n_tiles; j0 += NB) {
+        u32x4 kf[NB][KS], vr[NB][NV];
+        float ksc[NB], vsc[NB];
+        uint32_t seen[NB];  // which of the wave's 16 positions there are
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int pos = beg + kTile * (j0 + b) + 16 * w + r;
+            const bool ok = pos < end && (unsigned)ent[b] < (unsigned)p.c.n_pages;
+            const int slot = ok ? (ent[b] << p.c.shift) + (pos & ((1 << p.c.shift) - 1)) : -1;
+            seen[b] = (uint32_t)__builtin_amdgcn_ballot_w64(ok) & 0xFFFFu;
+            const int64_t off = ok ? slot_bytes(p.c, slot, row_bytes) : -1;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                kf[b][ks] = u32x4{0u, 0u, 0u, 0u};
+                if (ok && 4 * ks + g < n_ch) {
+                    const uint8_t *src = kb + off + 8 * esz * (4 * ks + g);
+                    if constexpr (I8) kf[b][ks] = u32x4{reinterpret_cast<const uint32_t *>(src)[0], reinterpret_cast<const uint32_t *>(src)[1], 0u, 0u};
+                    else kf[b][ks] = load16(src);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int id = lane + 64 * j;
+                const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)off, id / CH, 64);
+                const int hi = __shfl((int)(off >> 32), id / CH, 64);
+                vr[b][j] = u32x4{0u, 0u, 0u, 0u};
+                if (hi >= 0 && id % CH < n_ch) {
+                    const uint8_t *src = vb + (((int64_t)hi << 32) | lo) + 8 * esz * (id % CH);
+                    if constexpr (I8) vr[b][j] = u32x4{reinterpret_cast<const uint32_t *>(src)[0], reinterpret_cast<const uint32_t *>(src)[1], 0u, 0u};
+                    else vr[b][j] = load16(src);
+                }
+            }
+            if constexpr (I8) {
+                const int64_t at = (int64_t)max(slot, 0) * p.c.n_kv + kvh;
+                ksc[b] = p.c.ks ? p.c.ks[at] : 1.0f;
+                vsc[b] = p.c.vs ? p.c.vs[at] : 1.0f;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) ent[b] = entry(beg + kTile * (j0 + NB + b) + 16 * w + r);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (j0 + b >= n_tiles) break;  // uniform
+            const int p0 = beg + kTile * (j0 + b) + 16 * w;
+            if (seen[b] == 0) continue;    // uniform
+            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const u32x4 k = I8 ? i8_to_f16(u32x2{kf[b][ks].x, kf[b][ks].y}) : kf[b][ks];
+                acc = mfma<RXQ4_DTYPE_F16>(k, qf[ks], acc);
+            }
+            float sv[4], vx[4], lg[4];
+            bool vis[4];
+            float mx = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int d = lane + 64 * i;
-                if (d < hd)
-                    o[i] += w * (I8 ? x * (float)reinterpret_cast<const int8_t *>(v)[d]
-                                    : f16_bits_to_f32(reinterpret_cast<const uint16_t *>(v)[d]));
+                vis[i] = ((seen[b] >> (4 * g + i)) & 1) && p0 + 4 * g + i <= qpos;
+                float x = acc[i] * p.sl2;
+                vx[i] = 1.0f;
+                lg[i] = 0.0f;
+                if constexpr (I8) {
+                    x *= __shfl(ksc[b], 4 * g + i, 64);
+                    vx[i] = __shfl(vsc[b], 4 * g + i, 64);
+                    lg[i] = log2_scale(vx[i]);
+                }
+                sv[i] = vis[i] ? x : -INFINITY;
+                mx = fmaxf(mx, sv[i] + lg[i]);
+            }
+            mx = max_xor_rows<16>(mx);
+            mx = max_xor_rows<32>(mx);
+            const float m_new = fmaxf(m, mx);
+            const bool any = m_new != -INFINITY;
+            const float corr = any ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
+            const float m_use = any ? m_new - kShift : 0.0f;
+            float e[4], sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                e[i] = __builtin_amdgcn_exp2f(sv[i] - m_use);
+                sum += e[i];
+                if (I8) e[i] = vis[i] ? e[i] * vx[i] : 0.0f;
+            }
+            l = l * corr + sum;  // this lane's positions
+            m = m_new;
+            const uint32_t h01 = pack2<RXQ4_DTYPE_F16>(e[0], e[1]), h23 = pack2<RXQ4_DTYPE_F16>(e[2], e[3]);
+            const f16x4 ph = __builtin_bit_cast(f16x4, u32x2{h01, h23});
+            const f16x4 pl = __builtin_bit_cast(f16x4, u32x2{low_halves(e[0], e[1], h01), low_halves(e[2], e[3], h23)});
+            // An infinity or NaN in V would reach the rows that do not see it as 0 times
+            // it, and the others through the low half of P: such values are staged as
+            // zeros, and the rows that see them get them at the end.
+            if constexpr (!I8) {
+                if (__builtin_amdgcn_ballot_w64(not_finite16<NV>(vr[b])) != 0) {
+                    zero_not_finite16<NV>(vr[b]);
+                    bad = true;
+                }
+            }
+            // (the wave's own earlier reads of its rows are ahead in its LDS queue)
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int id = lane + 64 * j;
+                *reinterpret_cast<u32x4 *>(&vl[w][(id / CH) * VROW + 8 * (id % CH)]) =
+                    I8 ? i8_to_f16(u32x2{vr[b][j].x, vr[b][j].y}) : vr[b][j];
+            }
+            // lane r of group g supplies dims 16 dt + 4 (r & 3) .. + 3 of position
+            // 4 g + r / 4 and receives dim 16 dt + r of positions 4 g .. + 3
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const f16x4 a = __builtin_bit_cast(
+                    f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16 *)
+                                                                   &vl[w][(4 * g + (r >> 2)) * VROW + 16 * dt + 4 * (r & 3)]));
+                o[dt] *= corr;
+                o[dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(a, ph, o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(a, pl, o[dt], 0, 0, 0);
             }
         }
     }
-    const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // (NaN stays)
+    if (bad) {  // uniform, rare: the wave's positions again
+        for (int pos = beg; pos < end; ++pos) {
+            if (((pos - beg) >> 4 & 3) != w || pos > qpos) continue;
+            const int slot = slot_of(p.c, s, pos);
+            if (slot < 0) continue;
+            const uint16_t *v = reinterpret_cast<const uint16_t *>(vb + slot_bytes(p.c, slot, row_bytes));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int d = lane + 64 * i;
-        if (d < hd) p.out[((int64_t)t * p.n_heads + h) * hd + d] = f32_to_f16_bits(o[i] * inv);
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int d = 16 * dt + 4 * g + i;
+                    const float x = d < hd ? f16_bits_to_f32(v[d]) : 0.0f;
+                    if (!(fabsf(x) < INFINITY)) o[dt][i] += x;
+                }
+        }
     }
+    l = sum_xor_rows<16>(l);
+    l = sum_xor_rows<32>(l);
+
+    // Merge: lane l of every wave holds row r, dims 16 dt + 4 g + i; wave w merges
+    // the dims of tiles dt = w, w + 4, ...
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mg[w][4 * dt + i][lane] = o[dt][i];
+    mg[w][NM - 2][lane] = m;
+    mg[w][NM - 1][lane] = l;
+    __syncthreads();
+    float mw[4], M = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        mw[v] = mg[v][NM - 2][lane];
+        M = fmaxf(M, mw[v]);
+    }
+    float cw[4], L = 0.0f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        cw[v] = M != -INFINITY ? __builtin_amdgcn_exp2f(mw[v] - M) : 0.0f;
+        L += mg[v][NM - 1][lane] * cw[v];
+    }
+    if (!row_ok) return;
+    const bool whole = end_blk <= p.chunk;  // the block has one chunk: no partials
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    const int64_t at = (((int64_t)(s * p.c.n_kv + kvh) * p.n_rb + rb) * p.n_chunks + c) * p.rows_blk + r;
+#pragma unroll
+    for (int dt = w; dt < DT; dt += 4) {
+        f32x4 ov;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) x += mg[v][4 * dt + i][lane] * cw[v];
+            ov[i] = x;
+        }
+        const int d = 16 * dt + 4 * g;
+        if (!whole) *reinterpret_cast<f32x4 *>(p.part + at * HD + d) = ov;
+        else if (d < hd)
+            *reinterpret_cast<u32x2 *>(p.out + orow + d) = u32x2{pack2<RXQ4_DTYPE_F16>(ov[0] * inv, ov[1] * inv),
+                                                                 pack2<RXQ4_DTYPE_F16>(ov[2] * inv, ov[3] * inv)};
+    }
+    if (!whole && w == 0 && g == 0) {
+        p.stats[2 * at] = M;
+        p.stats[2 * at + 1] = L;
+    }
+}
+
+// out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over a row's chunks in a fixed
+// order.  Workgroup: a row and 64 of its dims; wave v sums the chunks v, v + 4, ..,
+// the waves add up in order.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedParams p) {
+    constexpr int NS = (HD + 63) / 64;
+    __shared__ float part[4][64];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int d = blockIdx.x % NS * 64 + lane;
+    const int r = blockIdx.x / NS % p.rows_blk, u = blockIdx.x / NS / p.rows_blk;
+    const int rb = u % p.n_rb, sk = u / p.n_rb, kvh = sk % p.c.n_kv, s = sk / p.c.n_kv;
+    const int64_t at = (int64_t)u * p.n_chunks * p.rows_blk + r;
+    const float *st = p.stats + 2 * at, *src = p.part + at * HD + min(d, HD - 1);
+    const int64_t step = p.rows_blk;
+    // (the first loads before the sequence's length: what is past it is not used)
+    const int cl = min(lane, p.n_chunks - 1);
+    float mc = st[2 * cl * step], lc = st[2 * cl * step + 1];
+    constexpr int U = 4;
+    float x[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) x[i] = src[(int64_t)min(w + 4 * i, p.n_chunks - 1) * step * HD];
+    const SeqSpan span = seq_span(p.b, s);
+    const int rows = min(span.n, p.b.max_new) * p.group;
+    const int row = rb * 16 + r;
+    if (row >= rows) return;  // uniform
+    const int last_tok = (min(rows, rb * 16 + 16) - 1) / p.group;
+    const int end = min(span.pos0 + last_tok + 1, position_limit(p.b, p.c));
+    const int n_c = (max(end, 0) + p.chunk - 1) / p.chunk;
+    if (n_c <= 1) return;  // written already
+    if (lane >= n_c) {
+        mc = -INFINITY;
+        lc = 0.0f;
+    }
+    const float M = butterfly_max<64>(mc);
+    const float e = M != -INFINITY && lane < n_c ? __builtin_amdgcn_exp2f(mc - M) : 0.0f;
+    const float L = butterfly_sum<64>(e * lc);
+    float acc = 0.0f;
+    for (int c0 = 0; c0 < n_c; c0 += 4 * U) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int c = c0 + w + 4 * i;
+            const float ec = __shfl(e, min(c, 63), 64);
+            if (c < n_c && ec != 0.0f) acc += ec * x[i];
+        }
+        if (c0 + 4 * U < n_c)
+#pragma unroll
+            for (int i = 0; i < U; ++i) x[i] = src[(int64_t)min(c0 + 4 * U + w + 4 * i, n_c - 1) * step * HD];
+    }
+    part[w][lane] = acc;
+    __syncthreads();
+    if (w == 0 && d < p.c.hd) {
+        const float sum = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+        const int tok = row / p.group, head = kvh * p.group + row % p.group;
+        p.out[((int64_t)(span.row0 + tok) * p.n_heads + head) * p.c.hd + d] =
+            f32_to_f16_bits(L == 0.0f ? 0.0f : sum * (1.0f / L));
+    }
+}
+
+template <int HD>
+hipError_t launch_hd(PagedParams &p, int i8, hipStream_t st) {
+    const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
+    const int64_t rows = (int64_t)std::min(p.b.max_new, p.b.n_tokens) * p.group;
+    p.n_rb = (int)((rows + 15) / 16);
+    p.rows_blk = (int)std::min<int64_t>(rows, 16);
+    const int64_t units = (int64_t)p.b.n_seqs * p.c.n_kv * p.n_rb;
+    const int64_t len = std::max<int64_t>(1, std::min<int64_t>(p.b.max_len, (int64_t)p.c.width << p.c.shift));
+    int64_t want = std::max((4 * cus + units - 1) / units, (len + 1023) / 1024);
+    want = std::min<int64_t>({want, kMaxChunks, (len + 2 * kTile - 1) / (2 * kTile)});
+    // the partials' room
+    const size_t per = (size_t)units * p.rows_blk * (HD + 2) * 4;
+    want = std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)(kWorkspaceBytes / per)));
+    if (tuning().attn_split) want = std::min<int64_t>(want, tuning().attn_split);
+    p.chunk = (int)(((len + want - 1) / want + kTile - 1) / kTile * kTile);
+    p.n_chunks = (int)((len + p.chunk - 1) / p.chunk);
+    if (units * p.n_chunks > 0x7FFFFF) return hipErrorInvalidValue;
+    if (p.n_chunks > 1) {
+        float *ws = nullptr;
+        const hipError_t e = Scratch{}.get(st, per * p.n_chunks, &ws);
+        if (e != hipSuccess) return e;
+        p.part = ws;
+        p.stats = ws + (size_t)units * p.n_chunks * p.rows_blk * HD;
+    }
+    const unsigned grid = (unsigned)(units * p.n_chunks);
+    if (i8) attn_paged_rows_kernel<HD, true><<<grid, 256, 0, st>>>(p);
+    else attn_paged_rows_kernel<HD, false><<<grid, 256, 0, st>>>(p);
+    if (p.n_chunks > 1)
+        attn_paged_combine_kernel<HD><<<(unsigned)(units * p.rows_blk * ((HD + 63) / 64)), 256, 0, st>>>(p);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -91,11 +447,18 @@ __global__ __launch_bounds__(64) void attn_paged_row_kernel(PagedParams p) {
 hipError_t launch_attention_paged(uint16_t *out, const uint16_t *q, int n_heads, float scale,
                                   const SeqBatch &batch, const PagedCache &cache, int kv_int8,
                                   hipStream_t st) {
-    const PagedParams p{out, q, batch, cache, n_heads, n_heads / cache.n_kv, scale};
-    const unsigned grid = (unsigned)batch.n_tokens * (unsigned)n_heads;
-    if (kv_int8) attn_paged_row_kernel<true><<<grid, 64, 0, st>>>(p);
-    else attn_paged_row_kernel<false><<<grid, 64, 0, st>>>(p);
-    return hipGetLastError();
+    PagedParams p{};
+    p.out = out;
+    p.q = q;
+    p.b = batch;
+    p.c = cache;
+    p.n_heads = n_heads;
+    p.group = n_heads / cache.n_kv;
+    p.sl2 = scale * 1.4426950408889634f;
+    if (cache.hd <= 64) return launch_hd<64>(p, kv_int8, st);
+    if (cache.hd <= 96) return launch_hd<96>(p, kv_int8, st);
+    if (cache.hd <= 128) return launch_hd<128>(p, kv_int8, st);
+    return launch_hd<256>(p, kv_int8, st);
 }
 
 }  // namespace rxq4
