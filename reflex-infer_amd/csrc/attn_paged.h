@@ -1,0 +1,38 @@
+// attn_paged.h -- the arguments of the paged attention kernels: 16 query rows a
+// workgroup (attn_paged.hip) and 128 (attn_paged_block.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "launch.h"
+
+namespace rxq4 {
+
+struct PagedParams {
+    uint16_t *out;
+    const uint16_t *q;
+    float *part, *stats;  // partials: O pieces; (maximum in log2 units, sum)
+    SeqBatch b;
+    PagedCache c;
+    int n_heads, group;
+    float sl2;            // scale * log2(e)
+    int rows_limit;       // sequences of at most this many rows are the 16-row kernel's (0: none)
+    int rows_blk;         // 16 rows: rows of a sequence that the partials hold
+    int n_blocks;         // 128 rows: at most this many blocks, over the sequences
+    int chunk, n_chunks;  // positions per chunk (a multiple of 64); chunks per block at most
+};
+
+// Query rows of a workgroup of the smaller and of the larger kernel.
+constexpr int kPagedRows = 16, kPagedBlock = 128;
+
+// Sequences of more than rows_limit rows (new tokens x group), 128 rows a
+// workgroup; partials within `room` bytes at `ws` (null: no split).
+struct PagedBlockPlan {
+    int chunk, n_chunks;
+    size_t bytes;  // of partials
+};
+PagedBlockPlan plan_paged_blocks(const PagedParams &p, size_t room);
+hipError_t launch_paged_blocks(PagedParams p, const PagedBlockPlan &plan, float *ws, int kv_int8, hipStream_t st);
+
+}  // namespace rxq4

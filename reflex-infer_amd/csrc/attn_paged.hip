@@ -13,6 +13,8 @@
 
 #include <algorithm>
 
+#include "attn_paged.h"
+#include "attn_tile.h"
 #include "launch.h"
 #include "mfma_util.h"
 #include "paged.h"
@@ -21,67 +23,11 @@
 namespace rxq4 {
 namespace {
 
-typedef short v4i16 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTile = 64;       // positions per tile
 constexpr int kMaxChunks = 64;  // chunks of positions per sequence
-// P holds 2^kShift times the probabilities relative to the running maximum: the
-// low half of the fp16 pair that carries one ends at 2^-24, 2^-35 of it.
-constexpr float kShift = 11.0f;
-// V scales below 2^kMinScale count as that where the reference point is chosen
-// (what they weigh is 0 in an fp16 output) and those above 2^kMaxScale as that.
-constexpr float kMinScale = -40.0f, kMaxScale = 127.0f;
-
-struct PagedParams {
-    uint16_t *out;
-    const uint16_t *q;
-    float *part, *stats;  // [unit][chunk][row]: HD floats; (maximum in log2 units, sum)
-    SeqBatch b;
-    PagedCache c;
-    int n_heads, group;
-    float sl2;            // scale * log2(e)
-    int n_rb;             // blocks of 16 rows per sequence and KV head
-    int rows_blk;         // rows of a block that the partials hold
-    int chunk, n_chunks;  // positions per chunk; chunks per unit
-};
-
 __device__ __forceinline__ float log2_scale(float vs) {
     return fminf(fmaxf(__builtin_amdgcn_logf(fabsf(vs)), kMinScale), kMaxScale);
-}
-
-// lo = RNE_f16(e - f32(hi)) for a pair: the difference is exact in fp32.  (Not in
-// inline asm: an MFMA may read a VALU result two wait states later at the earliest,
-// which the compiler keeps only for instructions that it knows.)
-__device__ __forceinline__ uint32_t low_halves(float e0, float e1, uint32_t hi) {
-    return pack2<RXQ4_DTYPE_F16>(e0 - f16_bits_to_f32(hi & 0xFFFFu), e1 - f16_bits_to_f32(hi >> 16));
-}
-
-// Infinities and NaN among N x 8 fp16: whether there are any (times 0 they are
-// NaN), and zeros in their place (a half with all exponent bits set carries into
-// its top bit).
-template <int N>
-__device__ __forceinline__ bool not_finite16(const u32x4 *x) {
-    f16x2 sum[4] = {};
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t v = x[j][i];
-            sum[i] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, v), f16x2{0, 0}, sum[i]);
-        }
-    const f16x2 all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    return !(all.x == 0) || !(all.y == 0);
-}
-template <int N>
-__device__ __forceinline__ void zero_not_finite16(u32x4 *x) {
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t all = (((x[j][i] & 0x7C007C00u) + 0x04000400u) >> 15) & 0x00010001u;
-            x[j][i] &= ~(all * 0xFFFFu);
-        }
 }
 
 // 8 int8 (bytes of .x, .y) as 8 fp16 (exact).
@@ -122,9 +68,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel
 
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
-    const int n_u = p.n_chunks * p.b.n_seqs * p.c.n_kv;
-    const int rb = blockIdx.x / n_u, u = blockIdx.x % n_u;
-    const int kvh = u % p.c.n_kv, s = u / p.c.n_kv % p.b.n_seqs, c = u / (p.c.n_kv * p.b.n_seqs);
+    const int kvh = blockIdx.x % p.c.n_kv, u = blockIdx.x / p.c.n_kv;
+    const int s = u % p.b.n_seqs, c = u / p.b.n_seqs;
     const int beg = c * p.chunk;
     const int limit = position_limit(p.b, p.c);
     if (beg >= limit && c > 0) return;
@@ -140,18 +85,16 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel
     for (int b = 0; b < NB; ++b) ent[b] = entry(beg + kTile * b + 16 * w + r);
     const SeqSpan span = seq_span(p.b, s);
     const int rows = min(span.n, p.b.max_new) * p.group;
-    const int row0 = rb * 16;
-    if (row0 >= rows) return;
-    const int last_tok = (min(rows, row0 + 16) - 1) / p.group;
-    const int end_blk = min(span.pos0 + last_tok + 1, limit);
-    const int end = min(end_blk, beg + p.chunk);
-    const int row = min(row0 + r, rows - 1);  // (columns past the last row repeat it)
+    if (rows == 0 || rows > kPagedRows) return;
+    const int end_seq = min(span.pos0 + (rows - 1) / p.group + 1, limit);
+    const int end = min(end_seq, beg + p.chunk);
+    const int row = min(r, rows - 1);  // (columns past the last row repeat it)
     const int tok = row / p.group, head = kvh * p.group + row % p.group;
-    const bool row_ok = row0 + r < rows;
+    const bool row_ok = r < rows;
     const int hd = p.c.hd, n_ch = hd >> 3;
     const int64_t orow = ((int64_t)(span.row0 + tok) * p.n_heads + head) * hd;
     if (end <= beg) {  // uniform
-        if (c == 0 && w == 0 && row_ok)  // the block sees nothing
+        if (c == 0 && w == 0 && row_ok)  // the tokens see nothing
             for (int ch = g; ch < n_ch; ch += 4) *reinterpret_cast<u32x4 *>(p.out + orow + 8 * ch) = u32x4{0u, 0u, 0u, 0u};
         return;
     }
@@ -327,9 +270,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel
         L += mg[v][NM - 1][lane] * cw[v];
     }
     if (!row_ok) return;
-    const bool whole = end_blk <= p.chunk;  // the block has one chunk: no partials
+    const bool whole = end_seq <= p.chunk;  // one chunk: no partials
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    const int64_t at = (((int64_t)(s * p.c.n_kv + kvh) * p.n_rb + rb) * p.n_chunks + c) * p.rows_blk + r;
+    const int64_t at = ((int64_t)(s * p.c.n_kv + kvh) * p.n_chunks + c) * p.rows_blk + r;
 #pragma unroll
     for (int dt = w; dt < DT; dt += 4) {
         f32x4 ov;
@@ -362,7 +305,7 @@ __global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedParams p) 
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int d = blockIdx.x % NS * 64 + lane;
     const int r = blockIdx.x / NS % p.rows_blk, u = blockIdx.x / NS / p.rows_blk;
-    const int rb = u % p.n_rb, sk = u / p.n_rb, kvh = sk % p.c.n_kv, s = sk / p.c.n_kv;
+    const int kvh = u % p.c.n_kv, s = u / p.c.n_kv;
     const int64_t at = (int64_t)u * p.n_chunks * p.rows_blk + r;
     const float *st = p.stats + 2 * at, *src = p.part + at * HD + min(d, HD - 1);
     const int64_t step = p.rows_blk;
@@ -375,10 +318,8 @@ __global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedParams p) 
     for (int i = 0; i < U; ++i) x[i] = src[(int64_t)min(w + 4 * i, p.n_chunks - 1) * step * HD];
     const SeqSpan span = seq_span(p.b, s);
     const int rows = min(span.n, p.b.max_new) * p.group;
-    const int row = rb * 16 + r;
-    if (row >= rows) return;  // uniform
-    const int last_tok = (min(rows, rb * 16 + 16) - 1) / p.group;
-    const int end = min(span.pos0 + last_tok + 1, position_limit(p.b, p.c));
+    if (r >= rows || rows > kPagedRows) return;  // uniform
+    const int end = min(span.pos0 + (rows - 1) / p.group + 1, position_limit(p.b, p.c));
     const int n_c = (max(end, 0) + p.chunk - 1) / p.chunk;
     if (n_c <= 1) return;  // written already
     if (lane >= n_c) {
@@ -404,41 +345,43 @@ __global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedParams p) 
     __syncthreads();
     if (w == 0 && d < p.c.hd) {
         const float sum = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
-        const int tok = row / p.group, head = kvh * p.group + row % p.group;
+        const int tok = r / p.group, head = kvh * p.group + r % p.group;
         p.out[((int64_t)(span.row0 + tok) * p.n_heads + head) * p.c.hd + d] =
             f32_to_f16_bits(L == 0.0f ? 0.0f : sum * (1.0f / L));
     }
 }
 
-template <int HD>
-hipError_t launch_hd(PagedParams &p, int i8, hipStream_t st) {
+// The 16-row launch's split: its partials within `room` bytes.
+struct RowsPlan {
+    int64_t units;
+    size_t bytes;
+};
+RowsPlan plan_rows(PagedParams &p, size_t room) {
     const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
-    const int64_t rows = (int64_t)std::min(p.b.max_new, p.b.n_tokens) * p.group;
-    p.n_rb = (int)((rows + 15) / 16);
-    p.rows_blk = (int)std::min<int64_t>(rows, 16);
-    const int64_t units = (int64_t)p.b.n_seqs * p.c.n_kv * p.n_rb;
+    const int pad = p.c.hd <= 64 ? 64 : p.c.hd <= 96 ? 96 : p.c.hd <= 128 ? 128 : 256;
+    p.rows_blk = (int)std::min<int64_t>((int64_t)std::min(p.b.max_new, p.b.n_tokens) * p.group, kPagedRows);
+    const int64_t units = (int64_t)p.b.n_seqs * p.c.n_kv;
     const int64_t len = std::max<int64_t>(1, std::min<int64_t>(p.b.max_len, (int64_t)p.c.width << p.c.shift));
     int64_t want = std::max((4 * cus + units - 1) / units, (len + 1023) / 1024);
     want = std::min<int64_t>({want, kMaxChunks, (len + 2 * kTile - 1) / (2 * kTile)});
-    // the partials' room
-    const size_t per = (size_t)units * p.rows_blk * (HD + 2) * 4;
-    want = std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)(kWorkspaceBytes / per)));
+    const size_t per = (size_t)units * p.rows_blk * (pad + 2) * 4;
+    want = std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)(room / per)));
     if (tuning().attn_split) want = std::min<int64_t>(want, tuning().attn_split);
     p.chunk = (int)(((len + want - 1) / want + kTile - 1) / kTile * kTile);
     p.n_chunks = (int)((len + p.chunk - 1) / p.chunk);
-    if (units * p.n_chunks > 0x7FFFFF) return hipErrorInvalidValue;
-    if (p.n_chunks > 1) {
-        float *ws = nullptr;
-        const hipError_t e = Scratch{}.get(st, per * p.n_chunks, &ws);
-        if (e != hipSuccess) return e;
-        p.part = ws;
-        p.stats = ws + (size_t)units * p.n_chunks * p.rows_blk * HD;
-    }
-    const unsigned grid = (unsigned)(units * p.n_chunks);
+    return RowsPlan{units, p.n_chunks > 1 ? (per * p.n_chunks + 255) / 256 * 256 : 0};
+}
+
+template <int HD>
+hipError_t launch_rows(PagedParams &p, const RowsPlan &plan, float *ws, int i8, hipStream_t st) {
+    if (plan.units * p.n_chunks > 0x7FFFFF) return hipErrorInvalidValue;
+    p.part = ws;
+    p.stats = ws + (size_t)plan.units * p.n_chunks * p.rows_blk * HD;
+    const unsigned grid = (unsigned)(plan.units * p.n_chunks);
     if (i8) attn_paged_rows_kernel<HD, true><<<grid, 256, 0, st>>>(p);
     else attn_paged_rows_kernel<HD, false><<<grid, 256, 0, st>>>(p);
     if (p.n_chunks > 1)
-        attn_paged_combine_kernel<HD><<<(unsigned)(units * p.rows_blk * ((HD + 63) / 64)), 256, 0, st>>>(p);
+        attn_paged_combine_kernel<HD><<<(unsigned)(plan.units * p.rows_blk * ((HD + 63) / 64)), 256, 0, st>>>(p);
     return hipGetLastError();
 }
 
@@ -455,10 +398,29 @@ hipError_t launch_attention_paged(uint16_t *out, const uint16_t *q, int n_heads,
     p.n_heads = n_heads;
     p.group = n_heads / cache.n_kv;
     p.sl2 = scale * 1.4426950408889634f;
-    if (cache.hd <= 64) return launch_hd<64>(p, kv_int8, st);
-    if (cache.hd <= 96) return launch_hd<96>(p, kv_int8, st);
-    if (cache.hd <= 128) return launch_hd<128>(p, kv_int8, st);
-    return launch_hd<256>(p, kv_int8, st);
+    // Sequences of up to 16 rows take the 16-row kernel; where the others of the batch
+    // have more, on average half the most any has, the 128-row kernel takes them all.
+    const int64_t most = (int64_t)std::min(batch.max_new, batch.n_tokens) * p.group;
+    const bool blocks = most > kPagedRows;
+    const bool rows = !blocks || (batch.n_seqs > 1 && (int64_t)batch.n_tokens * 2 < (int64_t)batch.n_seqs * batch.max_new);
+    p.rows_limit = rows ? kPagedRows : 0;
+    PagedParams pr = p;
+    RowsPlan rp{};
+    PagedBlockPlan bp{};
+    if (rows) rp = plan_rows(pr, (blocks ? kWorkspaceBytes / 2 : kWorkspaceBytes) - 256);
+    if (blocks) bp = plan_paged_blocks(p, kWorkspaceBytes - rp.bytes);
+    float *ws = nullptr;
+    if (rp.bytes + bp.bytes > 0) {
+        const hipError_t e = Scratch{}.get(st, rp.bytes + bp.bytes, &ws);
+        if (e != hipSuccess) return e;
+    }
+    hipError_t e = hipSuccess;
+    if (blocks) e = launch_paged_blocks(p, bp, ws ? ws + rp.bytes / 4 : nullptr, kv_int8, st);
+    if (e != hipSuccess || !rows) return e;
+    if (cache.hd <= 64) return launch_rows<64>(pr, rp, ws, kv_int8, st);
+    if (cache.hd <= 96) return launch_rows<96>(pr, rp, ws, kv_int8, st);
+    if (cache.hd <= 128) return launch_rows<128>(pr, rp, ws, kv_int8, st);
+    return launch_rows<256>(pr, rp, ws, kv_int8, st);
 }
 
 }  // namespace rxq4

@@ -1,0 +1,644 @@
+// attn_paged_block.hip -- attention of prompt chunks over a paged KV cache: 128 query
+// rows a workgroup, on the gfx950 matrix cores.
+//
+// The rows of a sequence and KV head are numbered t * group + j (new token t, j-th
+// head of the group), cut into blocks of 128, the positions into tiles of 64 and
+// those into chunks where there are few blocks.  The walk over the tiles, the
+// products, the softmax, the LDS layout and the bounds are those of
+// attn_prefill.hip; what is its own:
+//   blocks   the batch's lengths are in device memory: a workgroup finds its
+//            sequence and block by a sum over the sequences' block counts, a lane a
+//            sequence;
+//   pages    lane i of a wave looks up row i of the next tile (its page's table
+//            entry is loaded a tile earlier) and hands its offset to the lanes that
+//            load the row's chunks; rows in holes or past the block's sight are
+//            zeros, and their scores -infinity;
+//   splits   a workgroup leaves (O, m, l) per query row; attn_paged_block_combine
+//            adds a row's chunks in order.
+#include <math.h>
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "attn_paged.h"
+#include "attn_tile.h"
+#include "launch.h"
+#include "mfma_util.h"
+#include "paged.h"
+#include "q4k_device.h"
+
+namespace rxq4 {
+namespace {
+
+constexpr int kMaxChunks = 64;  // chunks per block
+// An int8 tile's floats in LDS: K scales, V scales, log2 |V scale|.
+constexpr int kScl = 3 * kTile;
+
+typedef const float __attribute__((address_space(1))) *GlobalFloat;
+__device__ const float g_one = 1.0f;  // int8 caches without scales: read with stride 0
+
+// Bytes of one K or V tile and of a wave group's LDS (two buffers of K, V).
+template <int HD>
+constexpr int tile_bytes() { return kTile * HD * 2; }
+template <int HD, int G>
+constexpr int block_lds() {
+    return G * 4 * tile_bytes<HD>()      // K, V x 2 buffers
+           + G * 2 * kScl * 4            // int8 scales
+           + 2 * 256 * 4                 // (m, l) of the second group
+           + G * 4 * 4;                  // a wave's flag: V not finite
+}
+
+// Blocks of sequence s.
+__device__ __forceinline__ int seq_blocks(const PagedParams &p, int s) {
+    const int rows = min(seq_span(p.b, s).n, p.b.max_new) * p.group;
+    return rows > p.rows_limit ? (rows + kPagedBlock - 1) / kPagedBlock : 0;
+}
+
+// The sequence and block of the idx-th block of the batch, the same for a whole
+// wave; false past the last one.
+__device__ __forceinline__ bool find_block(const PagedParams &p, int idx, int &seq, int &block) {
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0; s0 < p.b.n_seqs; s0 += 64) {
+        const int n = s0 + lane < p.b.n_seqs ? seq_blocks(p, s0 + lane) : 0;
+        int upto = n;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int x = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += x;
+        }
+        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > idx);
+        if (past != 0) {
+            const int at = __builtin_ctzll(past);
+            seq = s0 + at;
+            const int mine = __builtin_amdgcn_readlane(n, at);
+            block = mine - 1 - (idx - (__builtin_amdgcn_readlane(upto, at) - mine));
+            return true;
+        }
+        idx -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
+// Tiles that a block seeing positions [0, pos_end) walks (one where it sees
+// nothing: its rows are zeros).
+__device__ __forceinline__ int block_tiles(int pos_end) { return (max(pos_end, 1) + kTile - 1) / kTile; }
+
+template <int HD, bool I8, int G>
+__global__ __launch_bounds__(256 * G) void attn_paged_block_kernel(PagedParams p) {
+    constexpr int KS = HD / 16;             // k-steps of the scores
+    constexpr int DT = HD / 32;             // 32-dim tiles of O
+    constexpr int TB = tile_bytes<HD>();
+    constexpr int CH = HD / 8;              // 16-byte chunks per row
+    constexpr int NC = kTile * CH / 256;    // 8-dim chunks per thread and tile (K, V each)
+    constexpr int esz = I8 ? 1 : 2;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+
+    const int gq = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int tid = threadIdx.x & 255, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r32 = lane & 31, h = lane >> 5;
+    uint8_t *const lds = smem + gq * 4 * TB;  // buffer b: K at 2 b TB, V at (2 b + 1) TB
+    float *const scl = reinterpret_cast<float *>(smem + G * 4 * TB) + gq * 2 * kScl;
+    float *const mgl = reinterpret_cast<float *>(smem + G * 4 * TB + G * 8 * kScl);
+    int *const bad_v = reinterpret_cast<int *>(mgl + 512) + gq * 4;
+
+    // Unit: a sequence's latest tokens first.
+    const int kvh = blockIdx.x % p.c.n_kv;
+    const int v0 = blockIdx.x / p.c.n_kv;
+    const int chunk = v0 / p.n_blocks;
+    int seq, block;
+    if (!find_block(p, v0 % p.n_blocks, seq, block)) return;  // uniform
+    const SeqSpan span = seq_span(p.b, seq);
+    const int hd = p.c.hd;
+    const int n_rows = min(span.n, p.b.max_new) * p.group;
+    const int blk_last = min(n_rows, (block + 1) * kPagedBlock) - 1;
+    const int limit = position_limit(p.b, p.c);
+    const int pos_end = min(span.pos0 + blk_last / p.group + 1, limit);  // positions the block sees
+    const int chunk_tiles = p.chunk / kTile;
+    const int n_tiles = block_tiles(pos_end);
+    const int t_beg = chunk * chunk_tiles;
+    const int t_end = min(n_tiles, t_beg + chunk_tiles);
+    if (t_beg >= t_end) return;  // uniform
+
+    // The lane's query row.
+    const int row0 = block * kPagedBlock + 32 * w;
+    const bool live_wave = row0 < n_rows;
+    const RowMap rm = row_map(min(row0, n_rows - 1), p.group);
+    int tok, hj, tok_last, unused;
+    rm.at(min(r32, max(0, n_rows - 1 - row0)), tok, hj);
+    rm.at(min(31, max(0, n_rows - 1 - row0)), tok_last, unused);
+    const int qpos = span.pos0 + tok;  // last visible position
+    const int wave_first = span.pos0 + rm.tok0;
+    const int wave_end = live_wave ? span.pos0 + __builtin_amdgcn_readfirstlane(tok_last) + 1 : 0;
+    const int row_bytes = p.c.n_kv * hd * esz;
+    const uint8_t *kb = p.c.k + (int64_t)kvh * hd * esz;
+    const uint8_t *vb = p.c.v + (int64_t)kvh * hd * esz;
+    // (global pointers: a generic load would be waited for with the LDS reads)
+    const GlobalFloat ksp = p.c.ks ? (GlobalFloat)(p.c.ks + kvh) : (GlobalFloat)&g_one;
+    const GlobalFloat vsp = p.c.vs ? (GlobalFloat)(p.c.vs + kvh) : (GlobalFloat)&g_one;
+    const int s_stride = p.c.ks ? p.c.n_kv : 0, v_stride = p.c.vs ? p.c.n_kv : 0;
+    const int n_ch = hd >> 3;
+    const bool negate = p.sl2 < 0.0f;
+    // (a tiny positive scale for 0, so that masked scores stay -inf)
+    const float sl2 = fmaxf(fabsf(p.sl2), 1e-30f);
+
+    // Q^T fragments: dims 16 ks + 8 h .. + 7 of the row (zeros past hd).
+    u32x4 qf[KS];
+    {
+        const uint16_t *qrow = p.q + ((int64_t)(span.row0 + tok) * p.n_heads + kvh * p.group + hj) * hd;
+        const uint32_t flip = negate ? 0x80008000u : 0u;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int c = 2 * ks + h;
+            u32x4 x = *reinterpret_cast<const u32x4 *>(qrow + 8 * min(c, n_ch - 1));
+            x = u32x4{x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip};
+            qf[ks] = c < n_ch ? x : u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+
+    // The thread's chunks of a tile: row, place in the row, LDS offsets.  Where a row
+    // divides the 256 chunks, chunk j is kRows rows down and the places in a K row
+    // repeat every kPerK chunks: only what differs is kept.
+    constexpr bool kEven = 256 % CH == 0;
+    constexpr int kRows = 256 / CH, kPer = kEven ? 1 : NC, kPerK = kEven && kRows % 16 ? 16 / kRows : kPer;
+    static_assert(!kEven || kRows % 4 == 0, "the places in a V row repeat");
+    int ik[kPerK], iv[kPer];
+#pragma unroll
+    for (int j = 0; j < kPerK; ++j) {
+        const int id = tid + 256 * j, pr = id / CH, c = id % CH;
+        ik[j] = pr * HD * 2 + 16 * k_pos<HD>(pr, c);
+        if (j < kPer) iv[j] = pr * HD * 2 + 16 * v_pos<HD>(pr, c);
+    }
+    auto chunk_row = [&](int j) { return kEven ? tid / CH + j * kRows : (tid + 256 * j) / CH; };
+    auto chunk_col = [&](int j) { return kEven ? tid % CH : (tid + 256 * j) % CH; };
+    auto chunk_k = [&](int j) { return ik[j % kPerK] + (kEven ? j / kPerK * kPerK * kRows * HD * 2 : 0); };
+    auto chunk_v = [&](int j) { return kEven ? iv[0] + j * kRows * HD * 2 : iv[j % kPer]; };
+    using Chunk = typename std::conditional<I8, u32x2, u32x4>::type;
+    struct Raw {
+        Chunk c[NC];
+        float s;
+    };
+    // Lane i of a wave looks up row i of a tile: the page's table entry one tile
+    // before the tile's loads, then the row's offset, which the lanes of its chunks
+    // get from it.
+    const int32_t *const table = p.c.table ? p.c.table + (int64_t)seq * p.c.width : nullptr;
+    auto entry = [&](int t) {
+        const int i = min(t * kTile + lane, limit - 1) >> p.c.shift;
+        return limit <= 0 ? -1 : table ? table[i] : i;
+    };
+    int ent = 0;
+    uint64_t there = 0;  // the tile's positions in the block's sight and in the pool
+    Raw K, V;
+    auto load_tile = [&](int t) {
+        const int pos = t * kTile + lane;
+        const bool ok = pos < pos_end && (unsigned)ent < (unsigned)p.c.n_pages;
+        there = __builtin_amdgcn_ballot_w64(ok);
+        const int slot = ok ? (ent << p.c.shift) + (pos & ((1 << p.c.shift) - 1)) : 0;
+        const int64_t off = ok ? slot_bytes(p.c, slot, row_bytes) : -1;
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)off, chunk_row(j), 64);
+            const int hi = __shfl((int)(off >> 32), chunk_row(j), 64);
+            const int64_t at = (((int64_t)hi << 32) | lo) + 8 * esz * chunk_col(j);
+            K.c[j] = Chunk{};
+            V.c[j] = Chunk{};
+            if (hi >= 0 && chunk_col(j) < n_ch) {
+                K.c[j] = *reinterpret_cast<const Chunk *>(kb + at);
+                V.c[j] = *reinterpret_cast<const Chunk *>(vb + at);
+            }
+        }
+        if (I8) {
+            K.s = ksp[(int64_t)slot * s_stride];
+            V.s = vsp[(int64_t)slot * v_stride];
+            if (!ok) K.s = V.s = 0.0f;
+        }
+        ent = entry(t + G);
+    };
+    auto widen = [](Chunk c) {
+        if constexpr (I8) {
+            const u32x2 a = i8x4_to_f16(c.x), b = i8x4_to_f16(c.y);
+            return u32x4{a.x, a.y, b.x, b.y};
+        } else {
+            return c;
+        }
+    };
+    auto store_raw = [&](const Raw &R, int off, auto place, int s_off) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) *reinterpret_cast<u32x4 *>(lds + off + place(j)) = widen(R.c[j]);
+        if (I8 && tid < kTile) scl[s_off + tid] = R.s;
+    };
+    // log2 |V scale| of the tile's positions, clamped, and a bound of theirs that
+    // seldom moves (a maximum over the lanes for every tile costs 3%).  None for
+    // the first tile, where the row's maximum is taken exactly in any case.
+    float most_log = kMaxScale;
+    auto store_log = [&](float vs, int s_off, bool first) {
+        if constexpr (I8) {
+            const float lg = fminf(fmaxf(__builtin_amdgcn_logf(fabsf(vs)), kMinScale), kMaxScale);
+            if (!first && (__builtin_amdgcn_ballot_w64(lg > most_log) != 0 || most_log >= kMaxScale))
+                most_log = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(
+                               int, butterfly_max<64>(lg) + 0.125f)));
+            if (tid < kTile) scl[s_off + tid] = lg;
+        }
+    };
+
+    // An infinity or NaN in V would reach the rows that do not see it as 0 times it, and
+    // the others through the low half of P: such values (int8: V scales) are staged
+    // again as zeros, and the rows that see them get them at the end.
+    if (lane == 0) bad_v[w] = 0;  // the wave's flag: some of its staging
+    auto look_over = [&](Raw &R, int off, int s_off) {
+        if constexpr (I8) {
+            const bool bad = !(fabsf(R.s) < INFINITY);
+            if (__builtin_amdgcn_ballot_w64(bad) == 0) return;
+            if (bad && tid < kTile) scl[s_off + tid] = 0.0f;
+        } else {
+            if (__builtin_amdgcn_ballot_w64(not_finite16<NC>(R.c)) == 0) return;
+            Raw Z = R;  // (copies: head_dim 80, 775 tokens, 20.2 us with the loaded registers changed in place, 19.5)
+#pragma unroll
+            for (int j = 0; j < NC; ++j) asm volatile("" : "+v"(Z.c[j]));
+            zero_not_finite16<NC>(Z.c);
+            store_raw(Z, off, chunk_v, s_off);
+        }
+        if (lane == 0) bad_v[w] = 1;
+    };
+
+    // Lane parts of the fragment addresses: K row 32 pt + r32, chunk
+    // 2 ks + h; V row 16 kk + 8 x + 4 h + (r16 / 4), dims 32 dt + 16 (l / 16 % 2)
+    // + 4 (r16 % 4) (the transposing read hands the lane dim 32 dt + r32).
+    const int r16 = lane & 15;
+    int ka[KS], va[DT];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) ka[ks] = r32 * HD * 2 + 16 * k_pos<HD>(r32, 2 * ks + h);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+        const int vr = 4 * h + (r16 >> 2), d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (r16 & 3);
+        va[dt] = vr * HD * 2 + 16 * v_pos<HD>(vr, d >> 3) + 2 * (d & 7);
+    }
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
+    float m = -INFINITY, l = 0.0f;  // l: this lane's positions only
+
+    u32x4 ph[4], pl[4];  // P^T hi / lo operands per 16-position k step
+    auto softmax = [&](int t, int b, uint64_t in) {
+        const int p0 = t * kTile;
+        const uint8_t *kt = lds + b * 2 * TB;
+        f32x16 s[2];
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt) {
+            s[pt] = f32x16{};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                s[pt] = mfma32h(*reinterpret_cast<const u32x4 *>(kt + ka[ks] + pt * 64 * HD), qf[ks], s[pt]);
+        }
+        if constexpr (I8) {
+            const float *sk = scl + b * kScl;
+#pragma unroll
+            for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(sk + 32 * pt + 8 * j + 4 * h);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[pt][4 * j + i] *= x[i];
+                }
+        }
+        if (p0 + kTile - 1 > wave_first || in != ~0ull) {  // uniform: the diagonal's tiles, holes
+            const uint32_t in_h[2] = {(uint32_t)in >> (4 * h), (uint32_t)(in >> 32) >> (4 * h)};
+#pragma unroll
+            for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (p0 + 32 * pt + 8 * (i >> 2) + 4 * h + (i & 3) > qpos ||
+                        !((in_h[pt] >> (8 * (i >> 2) + (i & 3))) & 1u))
+                        s[pt][i] = -INFINITY;
+        }
+        // the row's largest P in log2 units: the score, with V scales score +
+        // log2 |scale|, at most the largest of each together
+        float mx = -INFINITY;
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[pt][i]);
+        mx = max_xor_rows<32>(mx) * sl2;
+        if constexpr (I8) {
+            const float *sg = scl + b * kScl + 2 * kTile;
+            if (__builtin_amdgcn_ballot_w64(mx + most_log > m + kLazy) != 0) {  // m may have to move: exactly
+                mx = -INFINITY;
+#pragma unroll
+                for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const f32x4 x = *reinterpret_cast<const f32x4 *>(sg + 32 * pt + 8 * j + 4 * h);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            mx = fmaxf(mx, __builtin_fmaf(s[pt][4 * j + i], sl2, x[i]));
+                    }
+                mx = max_xor_rows<32>(mx);
+            } else {
+                mx = -INFINITY;
+            }
+        }
+        // m moves when the row's maximum has outgrown it by 2^kLazy (always
+        // at a row's first visible position): |P| <= 2^(kLazy + kShift), and O
+        // and l stay relative to the same m
+        if (__builtin_amdgcn_ballot_w64(mx > m + kLazy) != 0) {
+            // (each row's by its own rule: no row depends on what others see)
+            const float m_new = mx > m + kLazy ? mx : m;
+            const float corr = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
+            l *= corr;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[dt][i] *= corr;
+        }
+        const float m_use = m == -INFINITY ? 0.0f : m - kShift;  // rows with nothing visible yet: e = 0
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            f32x4 x0, x1;
+            if constexpr (I8) {
+                const float *sv = scl + b * kScl + kTile;
+                x0 = *reinterpret_cast<const f32x4 *>(sv + 16 * kk + 4 * h);
+                x1 = *reinterpret_cast<const f32x4 *>(sv + 16 * kk + 8 + 4 * h);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const int i = 8 * (kk & 1) + e;  // register of k = e
+                float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kk >> 1][i], sl2, -m_use));
+                float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kk >> 1][i + 1], sl2, -m_use));
+                l += e0;
+                l += e1;
+                if constexpr (I8) {
+                    e0 *= e < 4 ? x0[e] : x1[e - 4];
+                    e1 *= e < 4 ? x0[e + 1] : x1[e - 3];
+                }
+                const uint32_t hi = pack2<RXQ4_DTYPE_F16>(e0, e1);
+                ph[kk][e >> 1] = hi;
+                pl[kk][e >> 1] = low_halves(e0, e1, hi);
+            }
+        }
+    };
+    auto weigh = [&](int b) {
+        const uint8_t *vt = lds + (b * 2 + 1) * TB;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const uint8_t *vp = vt + va[dt] + kk * 32 * HD;
+                const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                               (__attribute__((address_space(3))) v4i16 *)vp));
+                const u32x2 v1 = __builtin_bit_cast(
+                    u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                               (__attribute__((address_space(3))) v4i16 *)(vp + 16 * HD)));
+                const u32x4 a = u32x4{v0.x, v0.y, v1.x, v1.y};
+                o[dt] = mfma32h(a, ph[kk], o[dt]);
+                o[dt] = mfma32h(a, pl[kk], o[dt]);
+            }
+    };
+
+    // Tiles t_beg + gq, + G, ...: tile j of the group is in buffer j & 1
+    // during iteration j, and tile j + 1 is written to the other one, which
+    // every wave has left at the barrier.  A tile past the wave's visible
+    // positions changes nothing and is skipped.
+    const int n_j = (t_end - t_beg - gq + G - 1) / G;  // this group's tiles
+    const int n_it = (t_end - t_beg + G - 1) / G;      // every group's iterations
+    const int t_first = t_beg + gq;
+    auto store_tile = [&](int t, int b, bool first) {
+        store_raw(K, b * 2 * TB, chunk_k, b * kScl);
+        store_raw(V, (b * 2 + 1) * TB, chunk_v, b * kScl + kTile);
+        store_log(V.s, b * kScl + 2 * kTile, first);
+        look_over(V, (b * 2 + 1) * TB, b * kScl + kTile);
+    };
+    uint64_t in = 0;
+    if (n_j > 0) {
+        ent = entry(t_first);
+        load_tile(t_first);
+        in = there;
+        store_tile(t_first, 0, true);
+    }
+    for (int j = 0; j < n_it; ++j) {
+        wait_lgkmcnt0();
+        lds_barrier();
+        const int t = t_first + G * j;
+        const bool next = j + 1 < n_j;
+        const bool live = j < n_j && t * kTile < wave_end;  // uniform
+        if (next) load_tile(t + G);
+        if (live) softmax(t, j & 1, in);
+        if (next) store_tile(t + G, (j + 1) & 1, false);
+        if (live) weigh(j & 1);
+        in = there;
+    }
+    wait_lgkmcnt0();
+    lds_barrier();
+    if (__builtin_amdgcn_readfirstlane(bad_v[0] | bad_v[1] | bad_v[2] | bad_v[3]) != 0) {
+        for (int t = t_beg; t < t_end; ++t) {
+            if ((t - t_beg) % G != gq) continue;
+            for (int pos = t * kTile; pos < min(wave_end, t * kTile + kTile); ++pos) {
+                const int slot = pos < limit ? slot_of(p.c, seq, pos) : -1;
+                if (slot < 0) continue;  // uniform
+                const uint8_t *row = vb + slot_bytes(p.c, slot, row_bytes) + 4 * esz * h;
+                const float vs = I8 ? vsp[(int64_t)slot * v_stride] : 1.0f;
+                if (pos > qpos || (I8 && fabsf(vs) < INFINITY)) continue;
+                int n = n_ch;
+                asm volatile("" : "+s"(n));  // (compared here, not kept as CH conditions)
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    if (c >= n) continue;  // uniform
+                    const u32x2 x = I8 ? u32x2{*reinterpret_cast<const uint32_t *>(row + 8 * c), 0u}
+                                       : *reinterpret_cast<const u32x2 *>(row + 16 * c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float v = I8 ? vs * (float)(int8_t)(x.x >> (8 * i))
+                                           : f16_bits_to_f32((i < 2 ? x.x : x.y) >> (16 * (i & 1)) & 0xFFFFu);
+                        if (!(fabsf(v) < INFINITY)) o[c / 4][4 * (c % 4) + i] += v;
+                    }
+                }
+            }
+        }
+    }
+
+    // Merge: the second group hands (O, m, l) over through its own buffers.
+    l = sum_xor_rows<32>(l);
+    if (G == 2) {
+        float *mb = reinterpret_cast<float *>(smem + 4 * TB);  // HD / 2 x 256 floats
+        if (gq == 1) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mb[(16 * dt + i) * 256 + tid] = o[dt][i];
+            mgl[tid] = m;
+            mgl[256 + tid] = l;
+        }
+        wait_lgkmcnt0();
+        lds_barrier();
+        if (gq == 1) return;
+        const float m1 = mgl[tid], l1 = mgl[256 + tid];
+        const float mm = fmaxf(m, m1);
+        const bool any = mm != -INFINITY;
+        const float c0 = any ? __builtin_amdgcn_exp2f(m - mm) : 0.0f;
+        const float c1 = any ? __builtin_amdgcn_exp2f(m1 - mm) : 0.0f;
+        l = l * c0 + l1 * c1;
+        m = mm;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[dt][i] = o[dt][i] * c0 + mb[(16 * dt + i) * 256 + tid] * c1;
+    }
+    if (!live_wave) return;
+    if (n_tiles > chunk_tiles) {  // the block has several chunks
+        if (row0 + r32 >= n_rows) return;
+        const int64_t at = ((int64_t)(span.row0 + tok) * p.n_heads + kvh * p.group + hj) * p.n_chunks + chunk;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<f32x4 *>(p.part + at * HD + 32 * dt + 8 * j + 4 * h) =
+                    f32x4{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
+        if (h == 0) {
+            p.stats[2 * at] = m;
+            p.stats[2 * at + 1] = l;
+        }
+        return;
+    }
+    // Output rows through the wave's own LDS rows: 16 bytes a lane, a row's
+    // bytes together (straight from the registers: 8-byte pieces of 32 rows).
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    constexpr int OP = 2 * HD + 16;  // LDS pitch of a staged row
+    static_assert(4 * 32 * OP <= 4 * TB, "the staged rows fit the group's buffers");
+    uint8_t *ow = lds + w * 32 * OP;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t a = pack2<RXQ4_DTYPE_F16>(o[dt][4 * j] * inv, o[dt][4 * j + 1] * inv);
+            const uint32_t c = pack2<RXQ4_DTYPE_F16>(o[dt][4 * j + 2] * inv, o[dt][4 * j + 3] * inv);
+            *reinterpret_cast<u32x2 *>(ow + r32 * OP + 2 * (32 * dt + 8 * j + 4 * h)) = u32x2{a, c};
+        }
+    wait_lgkmcnt0();
+#pragma unroll
+    for (int i = 0; i < 32 * CH / 64; ++i) {
+        const int id = lane + 64 * i, rr = id / CH, c = id % CH;
+        const int orow = row0 + rr;
+        if (orow < n_rows && c < n_ch) {
+            int t, jj;
+            rm.at(rr, t, jj);
+            *reinterpret_cast<u32x4 *>(p.out + ((int64_t)(span.row0 + t) * p.n_heads + kvh * p.group + jj) * hd + 8 * c) =
+                *reinterpret_cast<const u32x4 *>(ow + rr * OP + 16 * c);
+        }
+    }
+}
+
+// out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over a row's chunks in order.  A
+// wave takes a row: a lane's chunk for the weights, then a lane's dims.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_paged_block_combine_kernel(PagedParams p) {
+    constexpr int NE = (HD + 63) / 64;
+    const int lane = threadIdx.x & 63;
+    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= (int64_t)p.b.n_tokens * p.n_heads) return;
+    const int t = (int)(id / p.n_heads), head = (int)(id % p.n_heads);
+    const int seq = seq_of_row(p.b, t);
+    if (seq >= p.b.n_seqs) return;
+    const SeqSpan span = seq_span(p.b, seq);
+    const int n_rows = min(span.n, p.b.max_new) * p.group;
+    const int row = (t - span.row0) * p.group + head % p.group;
+    if (t < span.row0 || row >= n_rows || n_rows <= p.rows_limit) return;
+    const int blk_last = min(n_rows, (row / kPagedBlock + 1) * kPagedBlock) - 1;
+    const int tiles = block_tiles(min(span.pos0 + blk_last / p.group + 1, position_limit(p.b, p.c)));
+    const int chunk_tiles = p.chunk / kTile, n_c = (tiles + chunk_tiles - 1) / chunk_tiles;
+    if (n_c <= 1) return;  // written already
+    const int64_t at = id * p.n_chunks;
+    const int c = min(lane, n_c - 1);
+    const float mc = p.stats[2 * (at + c)], lc = p.stats[2 * (at + c) + 1];
+    const float M = butterfly_max<64>(mc);
+    const float e = M != -INFINITY && lane < n_c ? __builtin_amdgcn_exp2f(mc - M) : 0.0f;
+    const float L = butterfly_sum<64>(e * lc);
+    float acc[NE] = {};
+    const float *src = p.part + at * HD;
+    for (int i = 0; i < n_c; ++i) {
+        const float ei = __shfl(e, i, 64);
+        if (ei == 0.0f) continue;
+#pragma unroll
+        for (int k = 0; k < NE; ++k) {
+            const int d = lane + 64 * k;
+            if (d < HD) acc[k] += ei * src[(int64_t)i * HD + d];
+        }
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int k = 0; k < NE; ++k) {
+        const int d = lane + 64 * k;
+        if (d < p.c.hd) p.out[id * p.c.hd + d] = f32_to_f16_bits(acc[k] * inv);
+    }
+}
+
+constexpr int kBigDim = 128;  // larger heads: one wave group, 512 registers a wave
+int pad_dim(int hd) { return hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : 256; }
+
+template <int HD, bool I8>
+hipError_t launch_t(const PagedParams &p, hipStream_t st) {
+    constexpr int G = HD > kBigDim ? 1 : 2;
+    constexpr int lds = block_lds<HD, G>();
+    // the dynamic LDS limit, raised once per device (devices 0..63)
+    static std::atomic<uint64_t> raised{0};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(raised.load(std::memory_order_acquire) & bit)) {
+        e = hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_paged_block_kernel<HD, I8, G>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+        raised.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    const int64_t grid = (int64_t)p.n_blocks * p.c.n_kv * p.n_chunks;
+    if (grid > 0x3FFFFF) return hipErrorInvalidValue;
+    attn_paged_block_kernel<HD, I8, G><<<(unsigned)grid, 256 * G, lds, st>>>(p);
+    if (p.n_chunks > 1)
+        attn_paged_block_combine_kernel<HD>
+            <<<(unsigned)(((int64_t)p.b.n_tokens * p.n_heads + 3) / 4), 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+
+// Blocks of the batch at most: every sequence's rows past the limit, each with a
+// last block of its own.
+int64_t most_blocks(const PagedParams &p) {
+    const int64_t rows = (int64_t)p.b.n_tokens * p.group;
+    return rows / kPagedBlock + std::min<int64_t>(p.b.n_seqs, rows / (p.rows_limit + 1));
+}
+
+}  // namespace
+
+PagedBlockPlan plan_paged_blocks(const PagedParams &p, size_t room) {
+    const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
+    const int pad = pad_dim(p.c.hd), G = pad > kBigDim ? 1 : 2;
+    const int64_t len = std::max<int64_t>(1, std::min<int64_t>(p.b.max_len, (int64_t)p.c.width << p.c.shift));
+    const int tiles = (int)((len + kTile - 1) / kTile);
+    const size_t per = (size_t)p.b.n_tokens * p.n_heads * (pad + 2) * 4;
+    const int64_t units = most_blocks(p) * p.c.n_kv;
+    int64_t want = std::max<int64_t>(1, std::min<int64_t>({(cus + units - 1) / units, kMaxChunks, (int64_t)(room / per)}));
+    if (tuning().attn_split) want = std::min<int64_t>(want, tuning().attn_split);
+    int ct = (int)((tiles + want - 1) / want);
+    ct = (ct + G - 1) / G * G;
+    const int n_c = (tiles + ct - 1) / ct;
+    return PagedBlockPlan{ct * kTile, n_c, n_c > 1 ? per * n_c : 0};
+}
+
+hipError_t launch_paged_blocks(PagedParams p, const PagedBlockPlan &plan, float *ws, int i8, hipStream_t st) {
+    p.chunk = plan.chunk;
+    p.n_chunks = plan.n_chunks;
+    const int64_t blocks = most_blocks(p);
+    if (blocks > 0x3FFFFF) return hipErrorInvalidValue;
+    p.n_blocks = (int)blocks;
+    p.part = ws;
+    p.stats = ws + (size_t)p.b.n_tokens * p.n_heads * p.n_chunks * pad_dim(p.c.hd);
+    switch (pad_dim(p.c.hd)) {
+        case 64: return i8 ? launch_t<64, true>(p, st) : launch_t<64, false>(p, st);
+        case 96: return i8 ? launch_t<96, true>(p, st) : launch_t<96, false>(p, st);
+        case 128: return i8 ? launch_t<128, true>(p, st) : launch_t<128, false>(p, st);
+        default: return i8 ? launch_t<256, true>(p, st) : launch_t<256, false>(p, st);
+    }
+}
+
+}  // namespace rxq4
