@@ -12,6 +12,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_paged.h"
 #include "attn_tile.h"
@@ -23,66 +24,67 @@
 namespace rxq4 {
 namespace {
 
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-
+constexpr int kStep = 128;      // positions per step of a workgroup
 constexpr int kMaxChunks = 64;  // chunks of positions per sequence
+
+__device__ const float g_one = 1.0f;  // int8 caches without scales: read with stride 0
+
 __device__ __forceinline__ float log2_scale(float vs) {
     return fminf(fmaxf(__builtin_amdgcn_logf(fabsf(vs)), kMinScale), kMaxScale);
 }
 
-// 8 int8 (bytes of .x, .y) as 8 fp16 (exact).
-__device__ __forceinline__ u32x4 i8_to_f16(u32x2 v) {
-    uint32_t o[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const uint32_t wd = e < 2 ? v.x : v.y;
-        const int sh = 16 * (e & 1);
-        o[e] = pack2<RXQ4_DTYPE_F16>((float)(int8_t)(uint8_t)(wd >> sh), (float)(int8_t)(uint8_t)(wd >> (sh + 8)));
-    }
-    return u32x4{o[0], o[1], o[2], o[3]};
-}
-
-// Wave w takes positions 16 w .. + 15 of every 64-position tile of the chunk with
-// its own online softmax; the four waves merge at the end.  Per tile, lane l =
+// Wave w takes positions 32 w .. + 31 of every 128-position step of the chunk with
+// its own online softmax; the four waves merge at the end.  Per step, lane l =
 // 16 g + r:
 //   S^T = K . Q^T    v_mfma_f32_16x16x32_f16, src0 = 16 positions x 32 dims of K
 //                    straight from memory (16 bytes a lane), src1 = Q^T; the lane
-//                    gets positions 4 g + i of row r;
-//   O^T += V^T P^T   v_mfma_f32_16x16x16_f16, src0 = 16 dims x 16 positions of V^T
-//                    (ds_read_tr16_b64 of the wave's V rows in LDS), src1 = P^T as
-//                    the score registers hold it, in fp16 hi + lo parts (22 bits).
-// Lane r looks up the page of position r once; the V chunks' lanes get the row's
-// offset from it.  int8: P holds the V scales, so the reference point of the
-// exponentials follows the maximum of score + log2 |scale|, and neither end of
-// fp16 is met whatever the scales.
-// The loads of NB tiles go out before their arithmetic, the table entries of the
-// next ones with them.
-template <int HD, bool I8>
+//                    gets positions 16 st + 4 g + i of row r;
+//   softmax          as in attn_prefill.hip: the reference point m moves when the
+//                    row's maximum has outgrown it by 2^kLazy; a lane's sums stay its
+//                    own to the end; int8: P holds the V scales and m follows the
+//                    maximum of score + log2 |scale|;
+//   O^T += V^T P^T   the same MFMA, src0 = 16 dims x 32 positions of V^T (two
+//                    ds_read_tr16_b64 of the wave's V rows in LDS), src1 = P^T as the
+//                    score registers hold it (k of a lane group: its positions), in
+//                    fp16 hi + lo parts (22 bits).
+// The next step's K and V are loaded before this step's arithmetic, and the table
+// entries of the one after before those (loads are waited for in order).  Lane i
+// looks up position i.  Pages of 16 positions or more (BIG): the 16 rows of an
+// operand lie in one page, a buffer resource of the wave, so that a load needs no
+// address arithmetic; smaller ones: the rows' offsets through LDS.
+// Rows past the end or in holes are zeros (BIG: past the end of the operand's buffer
+// resource; else the pool's first row in their place, cleared), their scores
+// -infinity.
+template <int HD, bool I8, bool BIG>
 __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel(PagedParams p) {
-    constexpr int KS = HD / 32, DT = HD / 16, VROW = HD + 16, CH = HD / 8, NV = 16 * CH / 64;
-    constexpr int NB = HD <= 128 ? 4 : 2;
+    constexpr int KS = HD / 32, DT = HD / 16, VROW = HD + 16, CH = HD / 8, NV = 32 * CH / 64;
     constexpr int esz = I8 ? 1 : 2;
     constexpr int NM = DT * 4 + 2;  // merge values per lane: O, m, l
-    __shared__ __attribute__((aligned(16))) uint16_t vl[4][16 * VROW];
-    __shared__ float mg[4][NM][64];
+    constexpr int kV = 4 * 32 * VROW * 2, kM = 4 * NM * 64 * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[kV > kM ? kV : kM];
+    __shared__ int64_t rowoff[BIG ? 1 : 4][32];
+    __shared__ __attribute__((aligned(16))) float scl[4][3][I8 ? 32 : 1];
 
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
+    uint16_t *const vl = reinterpret_cast<uint16_t *>(smem) + w * 32 * VROW;
     const int kvh = blockIdx.x % p.c.n_kv, u = blockIdx.x / p.c.n_kv;
     const int s = u % p.b.n_seqs, c = u / p.b.n_seqs;
     const int beg = c * p.chunk;
     const int limit = position_limit(p.b, p.c);
     if (beg >= limit && c > 0) return;
 
-    // Table entries of the first tiles, before the sequence's length is known.
-    const int32_t *const table = p.c.table ? p.c.table + (int64_t)s * p.c.width : nullptr;
+    // Table entries of the first steps, before the sequence's length is known.  (No load
+    // of the walk stands in a branch: the compiler would wait for all of them.)
+    const bool has_table = p.c.table != nullptr && limit > 0;
+    const int32_t *const table = has_table ? p.c.table + (int64_t)s * p.c.width : p.b.lens;
+    const int p_lane = beg + 32 * w + (lane & 31);  // the lane's position of the first step
     auto entry = [&](int pos) {
-        const int i = pos >> p.c.shift;
-        return pos < limit ? (table ? table[i] : i) : -1;
+        const int i = max(min(pos, limit - 1), 0) >> p.c.shift;
+        const int x = table[has_table ? i : 0];
+        return has_table ? x : i;
     };
-    int ent[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) ent[b] = entry(beg + kTile * b + 16 * w + r);
+    int ent = entry(p_lane), ent_next = entry(p_lane + kStep);
     const SeqSpan span = seq_span(p.b, s);
     const int rows = min(span.n, p.b.max_new) * p.group;
     if (rows == 0 || rows > kPagedRows) return;
@@ -106,132 +108,218 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
         qf[ks] = 4 * ks + g < n_ch ? load16(p.q + orow + 8 * (4 * ks + g)) : u32x4{0u, 0u, 0u, 0u};
+    // Byte offsets within a 16-row operand: K row r, dims 32 ks + 8 g; V row of the
+    // lane's chunks.  Chunks past head_dim are past the operand's end (BIG), or the
+    // last one again.
+    constexpr int kPast = 0x7FFF0000;
+    int ko[KS], vo[NV];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const int ch = 4 * ks + g;
+        ko[ks] = BIG ? (ch < n_ch ? r * row_bytes + 8 * esz * ch : kPast) : 8 * esz * min(ch, n_ch - 1);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int id = lane + 64 * j, ch = id % CH;
+        vo[j] = BIG ? (ch < n_ch ? (id / CH & 15) * row_bytes + 8 * esz * ch : kPast) : 8 * esz * min(ch, n_ch - 1);
+    }
+    const float *const ksp = p.c.ks ? p.c.ks + kvh : &g_one, *const vsp = p.c.vs ? p.c.vs + kvh : &g_one;
+    const int s_stride = p.c.ks ? p.c.n_kv : 0, v_stride = p.c.vs ? p.c.n_kv : 0;
+    using Chunk = typename std::conditional<I8, u32x2, u32x4>::type;
+    struct Step {
+        Chunk k[2][KS], v[NV];
+        float ks, vs;
+        uint32_t seen;  // which of the wave's 32 positions there are
+    };
+    auto buffer = [](__amdgpu_buffer_rsrc_t rs, int at) {
+        if constexpr (I8) return buffer_load8(rs, at);
+        else return buffer_load16(rs, at);
+    };
+    auto load_step = [&](int j, int e, Step &S) {
+        const int pos = p_lane + kStep * j;
+        const bool ok = pos < end && (unsigned)e < (unsigned)p.c.n_pages;
+        S.seen = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
+        const int place = pos & ((1 << p.c.shift) - 1);
+        if constexpr (I8) {
+            const int64_t at = ok ? ((int64_t)e << p.c.shift) + place : 0;
+            S.ks = ksp[at * s_stride];
+            S.vs = vsp[at * v_stride];
+        }
+        if constexpr (BIG) {
+            // an operand's rows: those of its positions that there are, from the first
+            __amdgpu_buffer_rsrc_t kr[2], vr[2];
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                const int n = __builtin_popcount((S.seen >> (16 * st)) & 0xFFFFu);
+                const int page = n ? __builtin_amdgcn_readlane(e, 16 * st) : 0;
+                const int64_t base = (int64_t)page * p.c.page_bytes + (int64_t)__builtin_amdgcn_readlane(place, 16 * st) * row_bytes;
+                const int bytes = n ? (n - 1) * row_bytes + hd * esz : 0;
+                kr[st] = make_rsrc(kb + base, bytes);
+                vr[st] = make_rsrc(vb + base, bytes);
+            }
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) S.k[st][ks] = buffer(kr[st], ko[ks]);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                if constexpr (CH == 12) {  // (a load's rows may be in both operands)
+                    const bool first = (lane + 64 * j) / CH < 16;
+                    const Chunk a = buffer(vr[0], first ? vo[j] : kPast), b = buffer(vr[1], first ? kPast : vo[j]);
+                    S.v[j] = a | b;
+                } else {
+                    S.v[j] = buffer(vr[64 * j / CH / 16], vo[j]);
+                }
+            }
+        } else {
+            if (lane < 32) rowoff[w][lane] = ok ? (int64_t)e * p.c.page_bytes + (int64_t)place * row_bytes : 0;
+            wave_lds_fence();
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                const uint8_t *src = kb + rowoff[w][16 * st + r];
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) S.k[st][ks] = *reinterpret_cast<const Chunk *>(src + ko[ks]);
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                S.v[j] = *reinterpret_cast<const Chunk *>(vb + rowoff[w][(lane + 64 * j) / CH] + vo[j]);
+            wave_lds_fence();
+        }
+    };
+    auto widen = [](Chunk x) {
+        if constexpr (I8) {
+            const u32x2 a = i8x4_to_f16(x.x), b = i8x4_to_f16(x.y);
+            return u32x4{a.x, a.y, b.x, b.y};
+        } else {
+            return x;
+        }
+    };
 
     f32x4 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
-    bool bad = false;  // some V is not finite
-    const int n_tiles = (end - beg + kTile - 1) / kTile;
-
-    for (int j0 = 0; j0 < n_tiles; j0 += NB) {
-        u32x4 kf[NB][KS], vr[NB][NV];
-        float ksc[NB], vsc[NB];
-        uint32_t seen[NB];  // which of the wave's 16 positions there are
+    bool bad = false;  // some V (int8: V scale) is not finite
+    auto process = [&](int j, Step &S) {
+        const int p0 = beg + kStep * j + 32 * w;
+        f32x4 acc[2];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int pos = beg + kTile * (j0 + b) + 16 * w + r;
-            const bool ok = pos < end && (unsigned)ent[b] < (unsigned)p.c.n_pages;
-            const int slot = ok ? (ent[b] << p.c.shift) + (pos & ((1 << p.c.shift) - 1)) : -1;
-            seen[b] = (uint32_t)__builtin_amdgcn_ballot_w64(ok) & 0xFFFFu;
-            const int64_t off = ok ? slot_bytes(p.c, slot, row_bytes) : -1;
+        for (int st = 0; st < 2; ++st) {
+            acc[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                kf[b][ks] = u32x4{0u, 0u, 0u, 0u};
-                if (ok && 4 * ks + g < n_ch) {
-                    const uint8_t *src = kb + off + 8 * esz * (4 * ks + g);
-                    if constexpr (I8) kf[b][ks] = u32x4{reinterpret_cast<const uint32_t *>(src)[0], reinterpret_cast<const uint32_t *>(src)[1], 0u, 0u};
-                    else kf[b][ks] = load16(src);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int id = lane + 64 * j;
-                const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)off, id / CH, 64);
-                const int hi = __shfl((int)(off >> 32), id / CH, 64);
-                vr[b][j] = u32x4{0u, 0u, 0u, 0u};
-                if (hi >= 0 && id % CH < n_ch) {
-                    const uint8_t *src = vb + (((int64_t)hi << 32) | lo) + 8 * esz * (id % CH);
-                    if constexpr (I8) vr[b][j] = u32x4{reinterpret_cast<const uint32_t *>(src)[0], reinterpret_cast<const uint32_t *>(src)[1], 0u, 0u};
-                    else vr[b][j] = load16(src);
-                }
-            }
-            if constexpr (I8) {
-                const int64_t at = (int64_t)max(slot, 0) * p.c.n_kv + kvh;
-                ksc[b] = p.c.ks ? p.c.ks[at] : 1.0f;
-                vsc[b] = p.c.vs ? p.c.vs[at] : 1.0f;
+                u32x4 k = widen(S.k[st][ks]);
+                if (!I8 && !BIG && 4 * ks + 4 > n_ch && 4 * ks + g >= n_ch) k = u32x4{0u, 0u, 0u, 0u};
+                acc[st] = mfma<RXQ4_DTYPE_F16>(k, qf[ks], acc[st]);
             }
         }
-#pragma unroll
-        for (int b = 0; b < NB; ++b) ent[b] = entry(beg + kTile * (j0 + NB + b) + 16 * w + r);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            if (j0 + b >= n_tiles) break;  // uniform
-            const int p0 = beg + kTile * (j0 + b) + 16 * w;
-            if (seen[b] == 0) continue;    // uniform
-            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const u32x4 k = I8 ? i8_to_f16(u32x2{kf[b][ks].x, kf[b][ks].y}) : kf[b][ks];
-                acc = mfma<RXQ4_DTYPE_F16>(k, qf[ks], acc);
+        f32x4 vx[2], lg[2];
+        if constexpr (I8) {
+            if (lane < 32) {
+                scl[w][0][lane] = S.ks;
+                scl[w][1][lane] = S.vs;
+                scl[w][2][lane] = log2_scale(S.vs);
             }
-            float sv[4], vx[4], lg[4];
-            bool vis[4];
-            float mx = -INFINITY;
+            wave_lds_fence();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                vis[i] = ((seen[b] >> (4 * g + i)) & 1) && p0 + 4 * g + i <= qpos;
-                float x = acc[i] * p.sl2;
-                vx[i] = 1.0f;
-                lg[i] = 0.0f;
-                if constexpr (I8) {
-                    x *= __shfl(ksc[b], 4 * g + i, 64);
-                    vx[i] = __shfl(vsc[b], 4 * g + i, 64);
-                    lg[i] = log2_scale(vx[i]);
-                }
-                sv[i] = vis[i] ? x : -INFINITY;
-                mx = fmaxf(mx, sv[i] + lg[i]);
+            for (int st = 0; st < 2; ++st) {
+                acc[st] *= *reinterpret_cast<const f32x4 *>(&scl[w][0][16 * st + 4 * g]);
+                vx[st] = *reinterpret_cast<const f32x4 *>(&scl[w][1][16 * st + 4 * g]);
+                lg[st] = *reinterpret_cast<const f32x4 *>(&scl[w][2][16 * st + 4 * g]);
             }
-            mx = max_xor_rows<16>(mx);
-            mx = max_xor_rows<32>(mx);
-            const float m_new = fmaxf(m, mx);
-            const bool any = m_new != -INFINITY;
-            const float corr = any ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
-            const float m_use = any ? m_new - kShift : 0.0f;
-            float e[4], sum = 0.0f;
+            wave_lds_fence();
+        }
+        const bool part = S.seen != ~0u;
+        float sv[8], mx = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                e[i] = __builtin_amdgcn_exp2f(sv[i] - m_use);
-                sum += e[i];
-                if (I8) e[i] = vis[i] ? e[i] * vx[i] : 0.0f;
-            }
-            l = l * corr + sum;  // this lane's positions
+        for (int i = 0; i < 8; ++i) sv[i] = acc[i >> 2][i & 3] * p.sl2;
+        if (part || p0 + 31 > span.pos0) {  // uniform: not every row sees all of them
+            const uint32_t in = S.seen >> (4 * g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!((in >> (16 * (i >> 2) + (i & 3))) & 1u) || p0 + 16 * (i >> 2) + 4 * g + (i & 3) > qpos)
+                    sv[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, I8 ? sv[i] + lg[i >> 2][i & 3] : sv[i]);
+        mx = max_xor_rows<16>(mx);
+        mx = max_xor_rows<32>(mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m + kLazy) != 0) {
+            // (each row's by its own rule: no row depends on what others see)
+            const float m_new = mx > m + kLazy ? mx : m;
+            const float corr = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
             m = m_new;
-            const uint32_t h01 = pack2<RXQ4_DTYPE_F16>(e[0], e[1]), h23 = pack2<RXQ4_DTYPE_F16>(e[2], e[3]);
-            const f16x4 ph = __builtin_bit_cast(f16x4, u32x2{h01, h23});
-            const f16x4 pl = __builtin_bit_cast(f16x4, u32x2{low_halves(e[0], e[1], h01), low_halves(e[2], e[3], h23)});
-            // An infinity or NaN in V would reach the rows that do not see it as 0 times
-            // it, and the others through the low half of P: such values are staged as
-            // zeros, and the rows that see them get them at the end.
-            if constexpr (!I8) {
-                if (__builtin_amdgcn_ballot_w64(not_finite16<NV>(vr[b])) != 0) {
-                    zero_not_finite16<NV>(vr[b]);
-                    bad = true;
-                }
-            }
-            // (the wave's own earlier reads of its rows are ahead in its LDS queue)
+            l *= corr;
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int id = lane + 64 * j;
-                *reinterpret_cast<u32x4 *>(&vl[w][(id / CH) * VROW + 8 * (id % CH)]) =
-                    I8 ? i8_to_f16(u32x2{vr[b][j].x, vr[b][j].y}) : vr[b][j];
-            }
-            // lane r of group g supplies dims 16 dt + 4 (r & 3) .. + 3 of position
-            // 4 g + r / 4 and receives dim 16 dt + r of positions 4 g .. + 3
+            for (int dt = 0; dt < DT; ++dt) o[dt] *= corr;
+        }
+        const float m_use = m == -INFINITY ? 0.0f : m - kShift;
+        uint32_t ph[4], pl[4];
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const f16x4 a = __builtin_bit_cast(
-                    f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16 *)
-                                                                   &vl[w][(4 * g + (r >> 2)) * VROW + 16 * dt + 4 * (r & 3)]));
-                o[dt] *= corr;
-                o[dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(a, ph, o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(a, pl, o[dt], 0, 0, 0);
+        for (int i = 0; i < 8; i += 2) {
+            float e0 = __builtin_amdgcn_exp2f(sv[i] - m_use), e1 = __builtin_amdgcn_exp2f(sv[i + 1] - m_use);
+            l += e0;
+            l += e1;
+            if constexpr (I8) {
+                // (a position that the row does not see stays 0 whatever its scale)
+                e0 = sv[i] == -INFINITY ? 0.0f : e0 * vx[i >> 2][i & 3];
+                e1 = sv[i + 1] == -INFINITY ? 0.0f : e1 * vx[i >> 2][(i & 3) + 1];
+            }
+            ph[i >> 1] = pack2<RXQ4_DTYPE_F16>(e0, e1);
+            pl[i >> 1] = low_halves(e0, e1, ph[i >> 1]);
+        }
+        // Rows that are not there: zeros.  An infinity or NaN in V would reach the rows
+        // that do not see it as 0 times it, and the others through the low half of P: such
+        // values are staged as zeros, and the rows that see them get them at the end.
+        if constexpr (!I8) {
+            if (!BIG && part)  // uniform
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    if (!((S.seen >> ((lane + 64 * j) / CH)) & 1u)) S.v[j] = u32x4{0u, 0u, 0u, 0u};
+            if (__builtin_amdgcn_ballot_w64(not_finite16<NV>(S.v)) != 0) {
+                zero_not_finite16<NV>(S.v);
+                bad = true;
             }
         }
+        // (the wave's own earlier reads of its rows are ahead in its LDS queue)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int id = lane + 64 * j;
+            *reinterpret_cast<u32x4 *>(&vl[(id / CH) * VROW + 8 * (id % CH)]) = widen(S.v[j]);
+        }
+        // lane r of group g supplies dims 16 dt + 4 (r & 3) .. + 3 of positions 4 g + r / 4
+        // and 16 + 4 g + r / 4 and receives dim 16 dt + r of positions 4 g .. + 3 and 16 + 4 g ..
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            const uint16_t *vp = &vl[(4 * g + (r >> 2)) * VROW + 16 * dt + 4 * (r & 3)];
+            const u32x2 v0 = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16 *)vp));
+            const u32x2 v1 = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                           (__attribute__((address_space(3))) v4i16 *)(vp + 16 * VROW)));
+            const u32x4 a = u32x4{v0.x, v0.y, v1.x, v1.y};
+            o[dt] = mfma<RXQ4_DTYPE_F16>(a, u32x4{ph[0], ph[1], ph[2], ph[3]}, o[dt]);
+            o[dt] = mfma<RXQ4_DTYPE_F16>(a, u32x4{pl[0], pl[1], pl[2], pl[3]}, o[dt]);
+        }
+    };
+    const int n_steps = (end - beg + kStep - 1) / kStep;
+    Step A, B;
+    load_step(0, ent, A);
+    for (int j = 0;;) {
+        ent = entry(p_lane + kStep * (j + 2));
+        load_step(j + 1, ent_next, B);
+        __builtin_amdgcn_sched_barrier(0);  // (the compiler would move them behind the products)
+        process(j, A);
+        if (++j >= n_steps) break;
+        ent_next = entry(p_lane + kStep * (j + 2));
+        load_step(j + 1, ent, A);
+        __builtin_amdgcn_sched_barrier(0);
+        process(j, B);
+        if (++j >= n_steps) break;
     }
     if (bad) {  // uniform, rare: the wave's positions again
         for (int pos = beg; pos < end; ++pos) {
-            if (((pos - beg) >> 4 & 3) != w || pos > qpos) continue;
+            if (((pos - beg) / 32 & 3) != w || pos > qpos) continue;
             const int slot = slot_of(p.c, s, pos);
             if (slot < 0) continue;
             const uint16_t *v = reinterpret_cast<const uint16_t *>(vb + slot_bytes(p.c, slot, row_bytes));
@@ -250,6 +338,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel
 
     // Merge: lane l of every wave holds row r, dims 16 dt + 4 g + i; wave w merges
     // the dims of tiles dt = w, w + 4, ...
+    float (*const mg)[NM][64] = reinterpret_cast<float (*)[NM][64]>(smem);
+    __syncthreads();  // the V rows are read
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -367,7 +457,7 @@ RowsPlan plan_rows(PagedParams &p, size_t room) {
     const size_t per = (size_t)units * p.rows_blk * (pad + 2) * 4;
     want = std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)(room / per)));
     if (tuning().attn_split) want = std::min<int64_t>(want, tuning().attn_split);
-    p.chunk = (int)(((len + want - 1) / want + kTile - 1) / kTile * kTile);
+    p.chunk = (int)(((len + want - 1) / want + kStep - 1) / kStep * kStep);
     p.n_chunks = (int)((len + p.chunk - 1) / p.chunk);
     return RowsPlan{units, p.n_chunks > 1 ? (per * p.n_chunks + 255) / 256 * 256 : 0};
 }
@@ -378,8 +468,11 @@ hipError_t launch_rows(PagedParams &p, const RowsPlan &plan, float *ws, int i8, 
     p.part = ws;
     p.stats = ws + (size_t)plan.units * p.n_chunks * p.rows_blk * HD;
     const unsigned grid = (unsigned)(plan.units * p.n_chunks);
-    if (i8) attn_paged_rows_kernel<HD, true><<<grid, 256, 0, st>>>(p);
-    else attn_paged_rows_kernel<HD, false><<<grid, 256, 0, st>>>(p);
+    const bool big = p.c.shift >= 4;
+    if (i8 && big) attn_paged_rows_kernel<HD, true, true><<<grid, 256, 0, st>>>(p);
+    else if (i8) attn_paged_rows_kernel<HD, true, false><<<grid, 256, 0, st>>>(p);
+    else if (big) attn_paged_rows_kernel<HD, false, true><<<grid, 256, 0, st>>>(p);
+    else attn_paged_rows_kernel<HD, false, false><<<grid, 256, 0, st>>>(p);
     if (p.n_chunks > 1)
         attn_paged_combine_kernel<HD><<<(unsigned)(plan.units * p.rows_blk * ((HD + 63) / 64)), 256, 0, st>>>(p);
     return hipGetLastError();

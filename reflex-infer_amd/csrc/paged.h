@@ -9,6 +9,13 @@
 
 namespace rxq4 {
 
+// A wave's LDS accesses stay in order between its lanes.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // One sequence of a batch: rows [row0, row0 + n) of q, the first at position
 // pos0 (negative where seq_lens is below the new tokens).  Whatever the device
 // arrays hold, the rows lie within [0, n_tokens).

@@ -60,13 +60,6 @@ __device__ __forceinline__ void load8(const void *base, int64_t at, float *x) {
     }
 }
 
-// A wave's LDS accesses stay in order between its lanes.
-__device__ __forceinline__ void wave_lds_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // DT: type of q, k, v; L: lanes a head (8 L >= head_dim).
 template <int DT, int L, bool I8>
 __global__ __launch_bounds__(64 * kWaves) void qk_rope_kernel(RopeParams p) {

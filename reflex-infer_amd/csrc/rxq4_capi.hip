@@ -518,7 +518,7 @@ rxq4::PagedCache device_cache(const rxq4_paged_kv &c) {
     p.vs = c.kv_int8 ? c.v_scales : nullptr;
     p.table = c.page_table;
     p.page_bytes = (c.page_stride ? c.page_stride : dense) * (c.kv_int8 ? 1 : 2);
-    p.width = c.page_table ? c.table_stride : c.n_pages;
+    p.width = c.n_pages == 0 ? 0 : c.page_table ? c.table_stride : c.n_pages;  // (no pages: nothing to see)
     p.n_pages = c.n_pages;
     p.shift = __builtin_ctz((unsigned)c.page_size);
     p.n_kv = c.n_kv_heads;
