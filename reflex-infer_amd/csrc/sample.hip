@@ -5,21 +5,21 @@
 // it: top-k a rank, top-p and the draw a sum of weights, min-p a weight.  So the row
 // need not be sorted: counts and sums of weights over bins of the logits say in
 // which bin a place lies, and only that bin's logits (or, where the kept ones are
-// few, all bins down to there at once) are sorted.
+// few, all down to there at once) are sorted.
 // Weights exp((l - max) / T) are formed in 64 bits and summed as whole numbers, so
 // the sums depend on no order: off by half a unit (2^-49 of a slice's largest weight,
 // and 2^-(63 - log2 n_vocab) of the row's) a logit.
 //
-//   sample_slices_kernel  a workgroup per slice of a row (up to 16384 logits, in
-//       registers): its largest logit, the count and weight of 512 bins of 1/16 in
-//       (l / T) on a grid that all slices share (the last bin: all further down), and
+//   sample_slices_kernel  a workgroup per slice of a row (in registers): its largest
+//       logit, the count and weight of 512 bins of 1/16 in (l / T) on a grid that all
+//       slices share (the last bin: all further down) and of blocks of 16 bins, and
 //       its indices in the order of the bins (a counting sort in LDS);
-//   sample_pick_kernel    a workgroup per row: the slices' bins together, then the
-//       places; a window of up to 1024 logits of some bins sorted in LDS.  A bin with
-//       more logits is narrowed by their ordered bit patterns, 256 parts at a time,
-//       down to a window or to equal logits.
-// Bound: two launches, the reads of the row (the slices) and the chain of dependent
-// steps of one workgroup (the pick).
+//   sample_pick_kernel    a workgroup per row: the slices' blocks together, the bins
+//       of a block where they are asked for, then the places, in a window of up to
+//       1024 sorted logits.  A bin with more is narrowed by the logits' ordered bit
+//       patterns, 256 parts at a time, down to a window or to equal logits.
+// Bound: two launches, the 64-bit arithmetic of a slice (some 40 instructions a
+// logit), and the pick's chain of dependent steps in one workgroup.
 #include <math.h>
 
 #include <algorithm>
@@ -34,10 +34,9 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kThreads = 1024;
-constexpr int kPer = 16;                      // logits of a thread
-constexpr int kSlice = kThreads * kPer;       // of a slice, at most
-constexpr int kBins = 512;
+constexpr int kBins = 512, kBlock = 16, kBlocks = kBins / kBlock;
 constexpr double kBinsPerUnit = 16.0;
+constexpr int kSlices = 512;                  // of a row, at most
 constexpr int kWindow = 1024;                 // logits sorted at once
 constexpr int kParts = 256;                   // of a bin that holds more
 constexpr double kSliceUnit = 0x1p48;         // weight units of a slice
@@ -51,15 +50,16 @@ __device__ __forceinline__ uint32_t order_key(float l) {
 __device__ __forceinline__ float key_value(uint32_t k) {
     return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
-constexpr uint32_t kMinusInf = 0x007FFFFFu;  // order_key(-inf): it and NaN are no tokens
 
 // A slice's part of the workspace.
 struct Slice {
-    u64 mass[kBins];          // weight relative to the slice's largest logit
-    uint32_t top;             // its pattern (0: no token)
-    uint32_t first;           // its lowest index in the slice
-    double top_bin;           // its place on the grid
-    uint16_t end[kBins];      // indices before the end of each bin
+    u64 mass[kBins];           // weights relative to the slice's largest logit
+    u64 block_mass[kBlocks];
+    int top_bin;               // the last place of its first block on the grid
+    uint32_t top;              // the largest logit's pattern (0: no token)
+    uint32_t first, unused;    // its lowest index in the slice (temperature 0)
+    uint16_t end[kBins];       // indices before the end of each bin
+    uint16_t block_end[kBlocks];
 };
 
 struct SampleParams {
@@ -70,12 +70,45 @@ struct SampleParams {
     double unit;        // weight units of a row
 };
 
+// e^-d for d >= 0 (0 from 100 on): 2^-n of the nearest whole n = d / ln 2, and the
+// Taylor series of the rest to the 12th power (|r| <= ln 2 / 2: off by 2^-52).
+__device__ __forceinline__ double exp_neg(double d) {
+    d = fmin(d, 100.0);
+    const double n = rint(d * 1.4426950408889634);
+    double r = __builtin_fma(n, 0.69314718055994529, -d);   // ln 2 in two parts
+    r = __builtin_fma(n, 2.3190468138462996e-17, r);
+    double e = 1.0 / 479001600.0;
+    e = __builtin_fma(e, r, 1.0 / 39916800.0);
+    e = __builtin_fma(e, r, 1.0 / 3628800.0);
+    e = __builtin_fma(e, r, 1.0 / 362880.0);
+    e = __builtin_fma(e, r, 1.0 / 40320.0);
+    e = __builtin_fma(e, r, 1.0 / 5040.0);
+    e = __builtin_fma(e, r, 1.0 / 720.0);
+    e = __builtin_fma(e, r, 1.0 / 120.0);
+    e = __builtin_fma(e, r, 1.0 / 24.0);
+    e = __builtin_fma(e, r, 1.0 / 6.0);
+    e = __builtin_fma(e, r, 0.5);
+    e = __builtin_fma(e, r, 1.0);
+    e = __builtin_fma(e, r, 1.0);
+    return ldexp(e, -(int)n);
+}
+// The weight of a logit beside the largest (a finite one beside an infinity: 0; NaN
+// from 0 times infinity goes the same way).
 __device__ __forceinline__ double weight_of(float l, float top, double inv_t) {
-    return l == top ? 1.0 : top == INFINITY ? 0.0 : exp(((double)l - (double)top) * inv_t);
+    return l == top ? 1.0 : exp_neg(((double)top - (double)l) * inv_t);
+}
+// ... rounded to whole units, at most 2^51 of them: the low bits of 2^52 + w.
+__device__ __forceinline__ u64 whole(double w) {
+    return __builtin_bit_cast(u64, w + 0x1p52) & 0xFFFFFFFFFFFFFull;
 }
 
 __device__ __forceinline__ u64 shfl_up64(u64 v, int d) {
     const uint32_t lo = __shfl_up((int)(uint32_t)v, d, 64), hi = __shfl_up((int)(v >> 32), d, 64);
+    return (u64)hi << 32 | lo;
+}
+
+__device__ __forceinline__ u64 shfl_xor64(u64 v, int d) {
+    const uint32_t lo = __shfl_xor((int)(uint32_t)v, d, 64), hi = __shfl_xor((int)(v >> 32), d, 64);
     return (u64)hi << 32 | lo;
 }
 
@@ -108,72 +141,105 @@ __device__ uint32_t scan32(uint32_t v, u64 *wave) {
     return v;
 }
 
+// The place of a logit on the bins' grid: in fp32 and saturated, the same in every
+// slice, and no smaller for a larger logit, which is all the bins need.
+__device__ __forceinline__ int grid_place(float l, float grid) {
+    return (int)floorf(__builtin_amdgcn_fmed3f(l * grid, -0x1.fffffep30f, 0x1.fffffep30f));
+}
+
+// PER: logits of a thread.
+// A logit's weight e^-d, d = (top - l) / T: a table of e^-(n / 16) for the nearest n / 16 and
+// the series of the rest (|r| <= 1 / 32: its 7th power is below 2^-47 of the weight);
+// from d = 40 on less than half a unit.
+template <int PER>
 __global__ __launch_bounds__(kThreads) void sample_slices_kernel(SampleParams p) {
+    constexpr int kTable = 641;
     __shared__ uint32_t count[kBins];
     __shared__ u64 mass[kBins], wave[kThreads / 64];
-    __shared__ uint16_t sorted[kSlice];
-    __shared__ uint32_t top_key, top_first;
+    __shared__ double table[kTable];  // in units
+    __shared__ uint16_t sorted[kThreads * PER];
+    __shared__ uint32_t top_first;
+    __shared__ float tops[kThreads / 64];
     const int tid = threadIdx.x;
     const int s = blockIdx.x % p.n_slices, r = blockIdx.x / p.n_slices, row = p.row0 + r;
     const int n = min(p.per, p.a.n_vocab - s * p.per);
     const float *l = p.a.logits + (int64_t)row * p.a.stride + (int64_t)s * p.per;
-    uint32_t key[kPer];
+    float x[PER];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int at = i * kThreads + tid;
-        const float x = l[min(at, n - 1)];
-        key[i] = at < n ? order_key(x) : 0u;
-    }
+    for (int i = 0; i < PER; ++i) x[i] = l[min(i * kThreads + tid, n - 1)];
     const float t = p.a.temperature ? p.a.temperature[row] : 1.0f;
-    if (tid == 0) {
-        top_key = 0;
-        top_first = ~0u;
-    }
+    if (tid == 0) top_first = ~0u;
     if (tid < kBins) {
         count[tid] = 0;
         mass[tid] = 0;
     }
-    __syncthreads();
-    uint32_t best = 0;
+    if (tid < kTable) table[tid] = exp_neg(tid * 0.0625) * kSliceUnit;
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) best = max(best, (uint32_t)__shfl_xor((int)best, d, 64));
-    if ((tid & 63) == 0) atomicMax(&top_key, best);
+    for (int i = 0; i < PER; ++i) {
+        if (i * kThreads + tid >= n) x[i] = -INFINITY;
+        top = fmaxf(top, x[i]);  // (NaN is not taken)
+    }
+    top = butterfly_max<64>(top);
+    if ((tid & 63) == 0) tops[tid >> 6] = top;
     __syncthreads();
-    const uint32_t tk = top_key;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) top = fmaxf(top, tops[i]);
     Slice &out = p.slices[(int64_t)r * p.n_slices + s];
-    if (tk <= kMinusInf || !(t > 0.0f)) {  // uniform: no token, or the largest logit alone is asked for
-        if (tk > kMinusInf) {
+    const bool none = top == -INFINITY;
+    if (none || !(t > 0.0f)) {  // uniform: no token, or the largest logit alone is asked for
+        if (!none) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (key[i] == tk) atomicMin(&top_first, (uint32_t)(i * kThreads + tid));
+            for (int i = 0; i < PER; ++i)
+                if (x[i] == top) atomicMin(&top_first, (uint32_t)(i * kThreads + tid));
         }
         if (tid < kBins) {
             out.mass[tid] = 0;
             out.end[tid] = 0;
         }
+        if (tid < kBlocks) {
+            out.block_mass[tid] = 0;
+            out.block_end[tid] = 0;
+        }
         __syncthreads();
         if (tid == 0) {
-            out.top = tk <= kMinusInf ? 0u : tk;
+            out.top = none ? 0u : order_key(top);
             out.first = top_first;
-            out.top_bin = -INFINITY;
+            out.top_bin = 0;
         }
         return;
     }
-    const float top = key_value(tk);
-    const double inv_t = 1.0 / (double)t, grid = kBinsPerUnit * inv_t;
-    const double top_bin = top == INFINITY ? INFINITY : floor((double)top * grid);
-    uint32_t place[kPer];  // bin, and number in it
+    if (tid == 0) {
+        out.top = order_key(top);
+        out.first = ~0u;
+    }
+    if (top == INFINITY) {  // uniform, rare: beside infinities the others weigh nothing
+        top = 0x1.fffffep127f;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+        for (int i = 0; i < PER; ++i) x[i] = x[i] == INFINITY ? top : -INFINITY;
+    }
+    const double inv_t = 1.0 / (double)t;
+    const float grid = fminf((float)(kBinsPerUnit * inv_t), 0x1.fffffep127f);
+    // blocks are those of the grid, so that the slices' blocks match
+    const int top_bin = grid_place(top, grid) | (kBlock - 1);
+    uint32_t place[PER];  // bin, and number in it
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
         place[i] = ~0u;
-        if (key[i] > kMinusInf) {
-            const float x = key_value(key[i]);
-            const double below = x == top ? 0.0 : top_bin - floor((double)x * grid);
-            const int b = below < (double)(kBins - 1) ? (int)below : kBins - 1;
-            const u64 w = (u64)rint(weight_of(x, top, inv_t) * kSliceUnit);
-            place[i] = (uint32_t)b << 16 | atomicAdd(&count[b], 1u);
+        if (x[i] > -INFINITY) {
+            const uint32_t b = min((uint32_t)top_bin - (uint32_t)grid_place(x[i], grid), (uint32_t)(kBins - 1));
+            const double d = ((double)top - (double)x[i]) * inv_t;
+            const double at = rint(fmin(d * 16.0, 640.0));
+            const double q = at * 0.0625 - d;
+            double e = 1.0 / 720.0;
+            e = __builtin_fma(e, q, 1.0 / 120.0);
+            e = __builtin_fma(e, q, 1.0 / 24.0);
+            e = __builtin_fma(e, q, 1.0 / 6.0);
+            e = __builtin_fma(e, q, 0.5);
+            e = __builtin_fma(e, q, 1.0);
+            e = __builtin_fma(e, q, 1.0);
+            const u64 w = at < 640.0 ? whole(table[(int)at] * e) : 0;
+            place[i] = b << 16 | atomicAdd(&count[b], 1u);
             if (w) atomicAdd(&mass[b], w);
         }
     }
@@ -183,16 +249,19 @@ __global__ __launch_bounds__(kThreads) void sample_slices_kernel(SampleParams p)
     if (tid < kBins) {
         count[tid] = end - mine;
         out.end[tid] = (uint16_t)end;
-        out.mass[tid] = mass[tid];
+        u64 m = mass[tid];
+        out.mass[tid] = m;
+#pragma unroll
+        for (int d = 1; d < kBlock; d <<= 1) m += shfl_xor64(m, d);
+        if (tid % kBlock == kBlock - 1) {
+            out.block_mass[tid / kBlock] = m;
+            out.block_end[tid / kBlock] = (uint16_t)end;
+        }
     }
-    if (tid == 0) {
-        out.top = tk;
-        out.first = ~0u;
-        out.top_bin = top_bin;
-    }
+    if (tid == 0) out.top_bin = top_bin;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
+    for (int i = 0; i < PER; ++i)
         if (place[i] != ~0u) sorted[count[place[i] >> 16] + (place[i] & 0xFFFFu)] = (uint16_t)(i * kThreads + tid);
     __syncthreads();
     uint32_t *dst = reinterpret_cast<uint32_t *>(p.index + ((int64_t)r * p.n_slices + s) * p.per);
@@ -209,11 +278,15 @@ struct Found {
 };
 
 struct Pick {
-    // the row's bins: counts and weights up to the end of each
-    u64 mass_to[kBins];
-    uint32_t count_to[kBins];
-    uint16_t shift[512];    // bins of a slice below the row's top
-    double scale[512];      // a slice's weight unit in the row's
+    // up to the end of each block of the row's bins, and of each bin of one block
+    u64 block_mass[kBlocks], bin_mass[kBlock];
+    uint32_t block_count[kBlocks], bin_count[kBlock];
+    int shift[kSlices];     // bins of a slice below the row's top, kBins: it is all past the bins
+    double scale[kSlices];  // a slice's weight unit in the row's
+    // the logits of some bins: where they begin in a slice's indices, and how many there
+    // are up to the end of each slice
+    int from[kSlices];
+    uint32_t upto[kSlices];
     // the window: sorted (~pattern, index), weights up to the end of each
     u64 item[kWindow], mass[kWindow];
     u64 part_mass[kParts];
@@ -233,6 +306,8 @@ struct Picker {
     int n;
     uint32_t base_rank;
     u64 base_mass, end_mass;
+    int block;           // whose bins are in sh
+    uint32_t logits;     // of the bins last gathered
 
     __device__ u64 weight(uint32_t key) const {
         return (u64)rint(weight_of(key_value(key), top, inv_t) * p.unit);
@@ -242,61 +317,101 @@ struct Picker {
         return p.a.logits[(int64_t)row * p.a.stride + (int64_t)s * p.per + i];
     }
 
-    // f(slice, index in it, pattern) for the logits of the bins [b0, b1]: 32 threads a
-    // slice.
-    template <class F>
-    __device__ void each(int b0, int b1, F f) const {
-        for (int s = threadIdx.x >> 5; s < p.n_slices; s += kThreads / 32) {
-            const int sf = sh.shift[s], j0 = max(b0 - sf, 0), j1 = b1 == kBins - 1 ? kBins - 1 : b1 - sf;
-            if (j1 < j0) continue;
-            const Slice &sl = slice(s);
-            const int beg = j0 > 0 ? sl.end[j0 - 1] : 0, end = sl.end[j1];
-            const uint16_t *index = p.index + ((int64_t)r * p.n_slices + s) * p.per;
-            for (int i = beg + (threadIdx.x & 31); i < end; i += 32) {
-                const uint32_t at = index[i];
-                f(s, at, order_key(logit(s, at)));
+    // Gathers the bins [b0, b1]: their part of every slice's indices.
+    __device__ __forceinline__ void gather(int b0, int b1) {
+        const int tid = threadIdx.x;
+        uint32_t c = 0;
+        if (tid < p.n_slices) {
+            const int sf = sh.shift[tid], j0 = max(b0 - sf, 0), j1 = b1 == kBins - 1 ? kBins - 1 : b1 - sf;
+            int beg = 0;
+            if (j1 >= j0) {
+                const Slice &sl = slice(tid);
+                const int end = sl.end[j1];
+                beg = j0 > 0 ? sl.end[j0 - 1] : 0;
+                c = end - beg;
             }
+            sh.from[tid] = beg;
+        }
+        const uint32_t to = scan32(c, sh.wave);
+        if (tid < p.n_slices) sh.upto[tid] = to;
+        __syncthreads();
+        logits = sh.upto[p.n_slices - 1];
+    }
+    // f(index in the row, pattern) for the gathered logits, four of a thread at a time.
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        for (uint32_t i0 = threadIdx.x; i0 < logits; i0 += 4 * kThreads) {
+            int s[4];
+            uint32_t at[4];
+            float x[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t i = min(i0 + q * kThreads, logits - 1);
+                int a = 0, b = p.n_slices - 1;  // the first slice with upto > i
+                while (a < b) {
+                    const int m = (a + b) >> 1;
+                    if (sh.upto[m] > i) b = m;
+                    else a = m + 1;
+                }
+                s[q] = a;
+                at[q] = p.index[((int64_t)r * p.n_slices + a) * p.per + sh.from[a] + (i - (a > 0 ? sh.upto[a - 1] : 0))];
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] = logit(s[q], at[q]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (i0 + q * kThreads < logits) f((uint32_t)(s[q] * p.per) + at[q], order_key(x[q]));
         }
     }
 
-    // Sorts the logits of the bins [b0, b1] with patterns in [lo, hi], `count` <=
-    // kWindow of them, into the window.
-    __device__ void window(int b0, int b1, uint32_t lo, uint32_t hi, uint32_t count, uint32_t rank, u64 before) {
+    // Sorts the gathered logits with patterns in [lo, hi], `count` <= kWindow of them, into
+    // the window.
+    __device__ __forceinline__ void window(uint32_t lo, uint32_t hi, uint32_t count, uint32_t rank, u64 before) {
         const int tid = threadIdx.x;
         __syncthreads();
         if (tid == 0) sh.v[0] = 0;
         sh.item[tid] = ~0ull;
         __syncthreads();
-        each(b0, b1, [&](int s, uint32_t at, uint32_t key) {
+        each([&](uint32_t index, uint32_t key) {
             if (key < lo || key > hi) return;
             const uint32_t i = atomicAdd(&sh.v[0], 1u);
-            if (i < kWindow) sh.item[i] = (u64)~key << 32 | (uint32_t)(s * p.per + at);
+            if (i < kWindow) sh.item[i] = (u64)~key << 32 | index;
         });
         __syncthreads();
         // bitonic, ascending (the empty places last); partners of the same wave need no
-        // barrier
+        // barrier, and waves without items only take part in those
         int size = 64;
         while (size < (int)count) size <<= 1;
         u64 x = sh.item[tid];
+        const bool live = tid < size;  // the same for a wave
         for (int k = 2; k <= size; k <<= 1)
             for (int j = k >> 1; j > 0; j >>= 1) {
-                u64 y;
+                u64 y = x;
                 if (j >= 64) {
                     __syncthreads();
-                    sh.item[tid] = x;
+                    if (live) sh.item[tid] = x;
                     __syncthreads();
-                    y = sh.item[tid ^ j];
-                } else {
-                    const uint32_t a = __shfl_xor((int)(uint32_t)x, j, 64), b = __shfl_xor((int)(x >> 32), j, 64);
-                    y = (u64)b << 32 | a;
+                    if (live) y = sh.item[tid ^ j];
+                } else if (live) {
+                    y = shfl_xor64(x, j);
                 }
-                const bool up = (tid & k) == 0 || k == size, low = (tid & j) == 0;
+                const bool up = (tid & k) == 0, low = (tid & j) == 0;
                 if ((y < x) == (up == low)) x = y;
             }
+        u64 to = tid < (int)count ? weight(~(uint32_t)(x >> 32)) : 0;
+        if (live) {
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const u64 y = shfl_up64(to, d);
+                if ((tid & 63) >= d) to += y;
+            }
+        }
         __syncthreads();
+        if ((tid & 63) == 63) sh.wave[tid >> 6] = to;
         sh.item[tid] = x;
-        const u64 w = tid < (int)count ? weight(~(uint32_t)(x >> 32)) : 0;
-        const u64 to = scan64(w, sh.wave);
+        __syncthreads();
+        if (live)
+            for (int i = 0; i < tid >> 6; ++i) to += sh.wave[i];
         sh.mass[tid] = to;
         __syncthreads();
         n = (int)count;
@@ -305,33 +420,90 @@ struct Picker {
         end_mass = before + sh.mass[n - 1];
     }
 
-    __device__ Found at_window(int i) const {
+    __device__ __forceinline__ Found at_window(int i) const {
         const u64 x = sh.item[i], to = sh.mass[i], from = i > 0 ? sh.mass[i - 1] : 0;
         return Found{base_rank + i, base_mass + from, to - from, ~(uint32_t)(x >> 32), 0, (int)(uint32_t)x};
     }
 
+    // The first of `m` <= 64 ends (counts or masses up to there, on top of rank and
+    // before) past the target, or the last with a logit: every wave by itself.
+    __device__ __forceinline__ int first_past(const uint32_t *count, const u64 *mass, int m, uint32_t rank, u64 before, bool by_count,
+                              double target) const {
+        const int lane = threadIdx.x & 63, i = min(lane, m - 1);
+        const bool some = lane < m && count[i] > (lane > 0 ? count[i - 1] : 0);
+        const bool past = some && (by_count ? (double)(rank + count[i]) > target : (double)(before + mass[i]) > target);
+        const u64 a = __builtin_amdgcn_ballot_w64(past), b = __builtin_amdgcn_ballot_w64(some);
+        return a ? __builtin_ctzll(a) : 63 - __builtin_clzll(b);
+    }
+
+    // The counts and masses of the bins of block `b`, up to the end of each, on top of
+    // those before the block.
+    __device__ __forceinline__ void open_block(int b) {
+        const int tid = threadIdx.x;
+        if (b == block) return;  // uniform
+        block = b;
+        __syncthreads();
+        if (tid < kBlock) {
+            sh.bin_count[tid] = 0;
+            sh.bin_mass[tid] = 0;
+        }
+        __syncthreads();
+        if (b < kBlocks - 1) {  // 16 bins of a slice
+            for (int i = tid; i < p.n_slices * kBlock; i += kThreads)
+                add_bin(i / kBlock, b * kBlock - sh.shift[i / kBlock] + i % kBlock, i % kBlock);
+        } else {                // any past the other blocks
+            for (int i = tid; i < p.n_slices * kBins; i += kThreads) {
+                const int to = min(i % kBins + sh.shift[i / kBins], kBins - 1) - b * kBlock;
+                if (to >= 0) add_bin(i / kBins, i % kBins, to);
+            }
+        }
+        __syncthreads();
+        if (tid < 64) {
+            uint32_t c = tid < kBlock ? sh.bin_count[tid] : 0;
+            u64 m = tid < kBlock ? sh.bin_mass[tid] : 0;
+#pragma unroll
+            for (int d = 1; d < kBlock; d <<= 1) {
+                const uint32_t x = __shfl_up((int)c, d, 64);
+                const u64 y = shfl_up64(m, d);
+                if (tid >= d) {
+                    c += x;
+                    m += y;
+                }
+            }
+            if (tid < kBlock) {
+                sh.bin_count[tid] = c;
+                sh.bin_mass[tid] = m;
+            }
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ void add_bin(int s, int j, int to) {
+        if (j < 0) return;
+        const Slice &sl = slice(s);
+        const uint32_t c = sl.end[j] - (j > 0 ? sl.end[j - 1] : 0);
+        if (c == 0) return;
+        atomicAdd(&sh.bin_count[to], c);
+        atomicAdd(&sh.bin_mass[to], (u64)rint((double)sl.mass[j] * sh.scale[s]));
+    }
+
     // The first place at which the number (by_count) or the weight of the logits down to
     // it exceeds `target`; the last one if none does.
-    __device__ Found find(bool by_count, double target) {
+    __device__ __forceinline__ Found find(bool by_count, double target) {
         const int tid = threadIdx.x;
         if (n > 0 && by_count && target >= base_rank && target < base_rank + n) return at_window((int)target - (int)base_rank);
         if (n > 0 && !by_count && target >= (double)base_mass && target < (double)end_mass) return search(target);
-        // its bin: the first whose end exceeds the target, else the last with a logit
-        __syncthreads();
-        if (tid == 0) {
-            sh.v[1] = kBins;
-            sh.v[2] = 0;
+        const int b = first_past(sh.block_count, sh.block_mass, kBlocks, 0, 0, by_count, target);
+        uint32_t rank = b > 0 ? sh.block_count[b - 1] : 0;
+        u64 before = b > 0 ? sh.block_mass[b - 1] : 0;
+        open_block(b);
+        const int bin = first_past(sh.bin_count, sh.bin_mass, kBlock, rank, before, by_count, target);
+        uint32_t count = sh.bin_count[bin];
+        if (bin > 0) {
+            count -= sh.bin_count[bin - 1];
+            rank += sh.bin_count[bin - 1];
+            before += sh.bin_mass[bin - 1];
         }
-        __syncthreads();
-        if (tid < kBins) {
-            const bool some = sh.count_to[tid] > (tid > 0 ? sh.count_to[tid - 1] : 0);
-            if (some && (by_count ? (double)sh.count_to[tid] > target : (double)sh.mass_to[tid] > target)) atomicMin(&sh.v[1], (uint32_t)tid);
-            if (some) atomicMax(&sh.v[2], (uint32_t)tid);
-        }
-        __syncthreads();
-        const int b = sh.v[1] < kBins ? (int)sh.v[1] : (int)sh.v[2];
-        uint32_t rank = b > 0 ? sh.count_to[b - 1] : 0, count = sh.count_to[b] - rank;
-        u64 before = b > 0 ? sh.mass_to[b - 1] : 0;
+        gather(b * kBlock + bin, b * kBlock + bin);
         uint32_t lo = 0, hi = ~0u;
         while (count > kWindow) {  // narrow it
             __syncthreads();
@@ -345,7 +517,7 @@ struct Picker {
             }
             __syncthreads();
             uint32_t least = ~0u, most = 0;
-            each(b, b, [&](int, uint32_t, uint32_t key) {
+            each([&](uint32_t, uint32_t key) {
                 if (key >= lo && key <= hi) {
                     least = min(least, key);
                     most = max(most, key);
@@ -363,7 +535,7 @@ struct Picker {
                 return Found{rank + (uint32_t)nth, before + (u64)nth * w, w, lo, (uint32_t)nth, -1};
             }
             const u64 range = (u64)(hi - lo) + 1;
-            each(b, b, [&](int, uint32_t, uint32_t key) {
+            each([&](uint32_t, uint32_t key) {
                 if (key >= lo && key <= hi) {
                     const int part = (int)((u64)(hi - key) * kParts / range);
                     atomicAdd(&sh.part_count[part], 1u);
@@ -402,13 +574,13 @@ struct Picker {
             lo = hi - to;
             hi = hi - from;
         }
-        window(b, b, lo, hi, count, rank, before);
+        window(lo, hi, count, rank, before);
         if (by_count) return at_window(min(max((int)(target - (double)rank), 0), n - 1));
         return search(target);
     }
 
     // The window's first place whose weights exceed the target, or its last.
-    __device__ Found search(double target) {
+    __device__ __forceinline__ Found search(double target) {
         const int tid = threadIdx.x;
         __syncthreads();
         if (tid == 0) sh.v[1] = n - 1;
@@ -421,7 +593,7 @@ struct Picker {
 
 __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams p) {
     __shared__ Pick sh;
-    __shared__ double top_bin;
+    __shared__ int top_bin;
     __shared__ uint32_t top_key;
     const int tid = threadIdx.x, r = blockIdx.x, row = p.row0 + r;
     const SampleRows &a = p.a;
@@ -430,17 +602,25 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams p) {
     const float top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f;
     const float u = fminf(fmaxf(a.u[row], 0.0f), 0x1.fffffep-1f);
     const Slice *slices = p.slices + (int64_t)r * p.n_slices;
+    // the blocks of the first slices, a thread's one each, before what they are relative to
+    const int s_mine = tid / kBlocks, b_mine = tid % kBlocks;
+    uint32_t c_mine = 0;
+    u64 m_mine = 0;
+    if (s_mine < p.n_slices) {
+        c_mine = slices[s_mine].block_end[b_mine];
+        m_mine = slices[s_mine].block_mass[b_mine];
+    }
     if (tid == 0) {
         top_key = 0;
         sh.v[0] = ~0u;
     }
-    if (tid < kBins) {
-        sh.count_to[tid] = 0;
-        sh.mass_to[tid] = 0;
+    if (tid < kBlocks) {
+        sh.block_count[tid] = 0;
+        sh.block_mass[tid] = 0;
     }
     __syncthreads();
     uint32_t mine = 0;
-    double bin = 0.0;
+    int bin = 0;
     if (tid < p.n_slices) {
         mine = slices[tid].top;
         bin = slices[tid].top_bin;
@@ -463,97 +643,113 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams p) {
     if (tid < p.n_slices && mine == tk) top_bin = bin;  // (all that write it write the same)
     __syncthreads();
     if (tid < p.n_slices) {
-        const double below = mine == tk ? 0.0 : top_bin - bin;
-        sh.shift[tid] = mine != 0 && below < (double)(kBins - 1) ? (uint16_t)below : kBins - 1;
+        sh.shift[tid] = mine != 0 ? (int)min((uint32_t)top_bin - (uint32_t)bin, (uint32_t)kBins) : kBins;
         sh.scale[tid] = mine != 0 ? weight_of(key_value(mine), top, inv_t) * (p.unit / kSliceUnit) : 0.0;
     }
     __syncthreads();
-    for (int i = tid; i < p.n_slices * kBins; i += kThreads) {
-        const int s = i / kBins, j = i % kBins;
-        const uint32_t c = slices[s].end[j] - (j > 0 ? slices[s].end[j - 1] : 0);
-        if (c == 0) continue;
-        const int b = min(j + sh.shift[s], kBins - 1);
-        atomicAdd(&sh.count_to[b], c);
-        atomicAdd(&sh.mass_to[b], (u64)rint((double)slices[s].mass[j] * sh.scale[s]));
+    for (int s = s_mine; s < p.n_slices; s += kThreads / kBlocks) {
+        if (s != s_mine) {
+            c_mine = slices[s].block_end[b_mine];
+            m_mine = slices[s].block_mass[b_mine];
+        }
+        const int to = min(b_mine + sh.shift[s] / kBlock, kBlocks - 1);
+        const uint32_t prev = b_mine > 0 ? slices[s].block_end[b_mine - 1] : 0;
+        if (c_mine == prev) continue;
+        atomicAdd(&sh.block_count[to], c_mine - prev);
+        atomicAdd(&sh.block_mass[to], (u64)rint((double)m_mine * sh.scale[s]));
     }
     __syncthreads();
-    {
-        const uint32_t c = scan32(tid < kBins ? sh.count_to[tid] : 0, sh.wave);
-        const u64 m = scan64(tid < kBins ? sh.mass_to[tid] : 0, sh.wave);
-        __syncthreads();
-        if (tid < kBins) {
-            sh.count_to[tid] = c;
-            sh.mass_to[tid] = m;
-        }
-        __syncthreads();
-    }
-    Picker pick{p, sh, r, row, top, inv_t, 0, 0, 0, 0};
-    uint32_t keep = sh.count_to[kBins - 1];
-    u64 kept = sh.mass_to[kBins - 1];
-
-    // Bins that the kept logits cannot go past: all down to there in one window, if
-    // they fit it.
-    int last = kBins - 1;
-    {
-        const uint32_t want = k > 0 && (uint32_t)k < keep ? (uint32_t)k : keep;
-        if (tid == 0) {
-            sh.v[0] = kBins - 1;
-            sh.v[1] = kBins - 1;
-        }
-        __syncthreads();
-        if (tid < kBins && sh.count_to[tid] >= want) atomicMin(&sh.v[0], (uint32_t)tid);
-        __syncthreads();
-        last = (int)sh.v[0];
-        const double most = (double)top_p * (double)sh.mass_to[last];
-        if (top_p < 1.0f && tid < kBins && (double)sh.mass_to[tid] >= most && sh.count_to[tid] > 0) atomicMin(&sh.v[1], (uint32_t)tid);
-        __syncthreads();
-        if (top_p < 1.0f) last = min(last, (int)sh.v[1]);
-        // (a weight of min_p lies -log(min_p) below the top: one bin more for the grid's
-        // place and one for roundings)
-        if (min_p > 0.0f) last = min(last, (int)fmin(fmax(-log((double)min_p) * kBinsPerUnit, 0.0) + 2.0, (double)(kBins - 1)));
-        const bool filtered = want < keep || top_p < 1.0f || min_p > 0.0f;
-        if (filtered && sh.count_to[last] <= kWindow) pick.window(0, last, 0u, ~0u, sh.count_to[last], 0, 0);
-    }
-    if (k > 0 && (uint32_t)k < keep) {
-        const Found f = pick.find(true, (double)k - 1.0);
-        keep = f.rank + 1;
-        kept = f.before + f.w;
-    }
-    if (top_p < 1.0f) {
-        // the shortest prefix that reaches the target
-        const Found f = pick.find(false, nextafter((double)top_p * (double)kept, -INFINITY));
-        if (f.rank + 1 < keep) {
-            keep = f.rank + 1;
-            kept = f.before + f.w;
-        }
-    }
-    if (min_p > 0.0f) {
-        // how many logits weigh enough: those of the window, if it ends below them
-        __syncthreads();
-        if (tid == 0) sh.v[0] = 0;
-        __syncthreads();
-        uint32_t c = 0;
-        const auto enough = [&](uint32_t key) { return weight_of(key_value(key), top, inv_t) >= (double)min_p; };
-        const bool in_window = pick.n > 0 && pick.base_rank == 0 &&
-                               ((uint32_t)pick.n >= keep || !enough(~(uint32_t)(sh.item[pick.n - 1] >> 32)));
-        if (in_window) {
-            if (tid < pick.n) c = enough(~(uint32_t)(sh.item[tid] >> 32));
-        } else {
-            pick.each(0, last, [&](int, uint32_t, uint32_t key) { c += enough(key); });
-        }
+    if (tid < 64) {
+        uint32_t c = tid < kBlocks ? sh.block_count[tid] : 0;
+        u64 m = tid < kBlocks ? sh.block_mass[tid] : 0;
 #pragma unroll
-        for (int d = 32; d > 0; d >>= 1) c += __shfl_xor((int)c, d, 64);
-        if ((tid & 63) == 0) atomicAdd(&sh.v[0], c);
-        __syncthreads();
-        const uint32_t most = max(1u, sh.v[0]);
-        if (most < keep) {
-            const Found f = pick.find(true, (double)most - 1.0);
+        for (int d = 1; d < kBlocks; d <<= 1) {
+            const uint32_t x = __shfl_up((int)c, d, 64);
+            const u64 y = shfl_up64(m, d);
+            if (tid >= d) {
+                c += x;
+                m += y;
+            }
+        }
+        if (tid < kBlocks) {
+            sh.block_count[tid] = c;
+            sh.block_mass[tid] = m;
+        }
+    }
+    __syncthreads();
+    Picker pick{p, sh, r, row, top, inv_t, 0, 0, 0, 0, -1, 0};
+    uint32_t keep = sh.block_count[kBlocks - 1];
+    u64 kept = sh.block_mass[kBlocks - 1];
+    const bool by_k = k > 0 && (uint32_t)k < keep;
+
+    // The block that the kept logits cannot go past: all down to there in one window, if
+    // they fit it.  (Top-p's share is one of what top-k keeps, so that with both the
+    // window goes down to top-k's border.)
+    int last = kBlocks - 1;
+    if (by_k) last = pick.first_past(sh.block_count, sh.block_mass, kBlocks, 0, 0, true, (double)k - 1.0);
+    if (top_p < 1.0f && !(by_k && sh.block_count[last] <= kWindow))
+        last = min(last, pick.first_past(sh.block_count, sh.block_mass, kBlocks, 0, 0, false,
+                                         nextafter((double)top_p * (double)sh.block_mass[last], -INFINITY)));
+    // (a weight of min_p lies -log(min_p) below the top: a block more for the grid's
+    // place and roundings)
+    const int min_p_block =
+        min_p > 0.0f ? (int)fmin(fmax(-log((double)min_p) * (kBinsPerUnit / kBlock), 0.0) + 2.0, (double)(kBlocks - 1)) : 0;
+    if (min_p > 0.0f && !by_k && !(top_p < 1.0f)) last = min(last, min_p_block);
+    if (last < kBlocks - 1 && sh.block_count[last] <= kWindow) {
+        pick.gather(0, last * kBlock + kBlock - 1);
+        pick.window(0u, ~0u, sh.block_count[last], 0, 0);
+    }
+    // Top-k's, top-p's and min-p's borders, then the draw: places of the order, one
+    // after the other.
+    Found f{};
+    for (int step = 0; step < 5; ++step) {
+        bool by_count = true;
+        double target = 0.0;
+        if (step == 0) {
+            if (!by_k) continue;
+            target = (double)k - 1.0;
+        } else if (step == 1) {
+            // the shortest prefix that reaches the share (0: the first logit)
+            if (!(top_p < 1.0f)) continue;
+            by_count = false;
+            target = fmax(nextafter((double)top_p * (double)kept, -INFINITY), 0.0);
+        } else if (step == 2) {
+            // how many logits weigh enough: those of the window, if it ends below them, else
+            // down to the kept ones' border or to where none can
+            if (!(min_p > 0.0f)) continue;
+            __syncthreads();
+            if (tid == 0) sh.v[0] = 0;
+            __syncthreads();
+            uint32_t c = 0;
+            const auto enough = [&](uint32_t key) { return weight_of(key_value(key), top, inv_t) >= (double)min_p; };
+            const bool in_window = pick.n > 0 && pick.base_rank == 0 &&
+                                   ((uint32_t)pick.n >= keep || !enough(~(uint32_t)(sh.item[pick.n - 1] >> 32)));
+            if (in_window) {
+                if (tid < pick.n) c = enough(~(uint32_t)(sh.item[tid] >> 32));
+            } else {
+                pick.gather(0, min(last, min_p_block) * kBlock + kBlock - 1);
+                pick.each([&](uint32_t, uint32_t key) { c += enough(key); });
+            }
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) c += __shfl_xor((int)c, d, 64);
+            if ((tid & 63) == 0) atomicAdd(&sh.v[0], c);
+            __syncthreads();
+            const uint32_t most = max(1u, sh.v[0]);
+            if (most >= keep) continue;
+            target = (double)most - 1.0;
+        } else if (step == 3) {
+            by_count = false;
+            target = (double)u * (double)kept;
+        } else {
+            if (f.rank < keep) continue;
+            target = (double)keep - 1.0;
+        }
+        f = pick.find(by_count, target);
+        if (step < 3 && f.rank + 1 < keep) {
             keep = f.rank + 1;
             kept = f.before + f.w;
         }
     }
-    Found f = pick.find(false, (double)u * (double)kept);
-    if (f.rank >= keep) f = pick.find(true, (double)keep - 1.0);
     if (f.index >= 0) {  // uniform
         if (tid == 0) a.ids[row] = f.index;
         return;
@@ -591,7 +787,13 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams p) {
 hipError_t launch_sample(const SampleRows &rows, int n_rows, hipStream_t st) {
     SampleParams p{};
     p.a = rows;
-    p.n_slices = (rows.n_vocab + kSlice - 1) / kSlice;
+    // 8 logits of a thread for a few rows, which leave CUs free; 16 for many: fewer bins
+    // to put together
+    const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
+    const int64_t eights = (rows.n_vocab + 8 * kThreads - 1) / (8 * kThreads);
+    const bool few = eights <= kSlices && eights * n_rows <= 2 * cus;
+    const int most = (few ? 8 : 16) * kThreads;
+    p.n_slices = (rows.n_vocab + most - 1) / most;
     p.per = ((rows.n_vocab + p.n_slices - 1) / p.n_slices + 1) & ~1;
     int bits = 62;
     for (int n = 1; n < rows.n_vocab; n <<= 1) --bits;
@@ -605,7 +807,8 @@ hipError_t launch_sample(const SampleRows &rows, int n_rows, hipStream_t st) {
     p.index = reinterpret_cast<uint16_t *>(p.slices + (size_t)group * p.n_slices);
     for (p.row0 = 0; p.row0 < n_rows; p.row0 += group) {
         const int n = std::min(group, n_rows - p.row0);
-        sample_slices_kernel<<<n * p.n_slices, kThreads, 0, st>>>(p);
+        if (few) sample_slices_kernel<8><<<n * p.n_slices, kThreads, 0, st>>>(p);
+        else sample_slices_kernel<16><<<n * p.n_slices, kThreads, 0, st>>>(p);
         sample_pick_kernel<<<n, kThreads, 0, st>>>(p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
