@@ -16,7 +16,7 @@
 //       its indices in the order of the bins (a counting sort in LDS);
 //   sample_pick_kernel    a workgroup per row: the slices' blocks together, the bins
 //       of a block where they are asked for, then the places, in a window of up to
-//       1024 sorted logits.  A bin with more is narrowed by the logits' ordered bit
+//       512 sorted logits.  A bin with more is narrowed by the logits' ordered bit
 //       patterns, 256 parts at a time, down to a window or to equal logits.
 // Bound: two launches, the 64-bit arithmetic of a slice (some 40 instructions a
 // logit), and the pick's chain of dependent steps in one workgroup.
@@ -33,11 +33,11 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;                 // of the pick
 constexpr int kBins = 512, kBlock = 16, kBlocks = kBins / kBlock;
 constexpr double kBinsPerUnit = 16.0;
-constexpr int kSlices = 512;                  // of a row, at most
-constexpr int kWindow = 1024;                 // logits sorted at once
+constexpr int kSlices = kThreads;             // of a row, at most
+constexpr int kWindow = kThreads;               // logits sorted at once
 constexpr int kParts = 256;                   // of a bin that holds more
 constexpr double kSliceUnit = 0x1p48;         // weight units of a slice
 
@@ -112,9 +112,10 @@ __device__ __forceinline__ u64 shfl_xor64(u64 v, int d) {
     return (u64)hi << 32 | lo;
 }
 
-// Sums over the threads up to each one (inclusive); `wave`: 16 values of LDS.
+// Sums over the T threads up to each one (inclusive); `wave`: T / 64 values of LDS.
 // Every thread of the workgroup takes part.
-__device__ u64 scan64(u64 v, u64 *wave) {
+template <int T>
+__device__ __forceinline__ u64 scan64(u64 v, u64 *wave) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -124,10 +125,12 @@ __device__ u64 scan64(u64 v, u64 *wave) {
     __syncthreads();
     if (lane == 63) wave[w] = v;
     __syncthreads();
-    for (int i = 0; i < w; ++i) v += wave[i];
+#pragma unroll
+    for (int i = 0; i < T / 64 - 1; ++i) v += i < w ? wave[i] : 0;
     return v;
 }
-__device__ uint32_t scan32(uint32_t v, u64 *wave) {
+template <int T>
+__device__ __forceinline__ uint32_t scan32(uint32_t v, u64 *wave) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -137,7 +140,8 @@ __device__ uint32_t scan32(uint32_t v, u64 *wave) {
     __syncthreads();
     if (lane == 63) wave[w] = v;
     __syncthreads();
-    for (int i = 0; i < w; ++i) v += (uint32_t)wave[i];
+#pragma unroll
+    for (int i = 0; i < T / 64 - 1; ++i) v += i < w ? (uint32_t)wave[i] : 0u;
     return v;
 }
 
@@ -147,55 +151,61 @@ __device__ __forceinline__ int grid_place(float l, float grid) {
     return (int)floorf(__builtin_amdgcn_fmed3f(l * grid, -0x1.fffffep30f, 0x1.fffffep30f));
 }
 
-// PER: logits of a thread.
-// A logit's weight e^-d, d = (top - l) / T: a table of e^-(n / 16) for the nearest n / 16 and
-// the series of the rest (|r| <= 1 / 32: its 7th power is below 2^-47 of the weight);
-// from d = 40 on less than half a unit.
-template <int PER>
-__global__ __launch_bounds__(kThreads) void sample_slices_kernel(SampleParams p) {
-    constexpr int kTable = 641;
+// T threads, PER logits each.
+// A logit's weight e^-d, d = (top - l) / T: two tables for the nearest n / 16 and the
+// series of the rest (|r| <= 1 / 32: its 7th power is below 2^-47 of the weight); from
+// d = 40 on less than half a unit.
+template <int T, int PER>
+__global__ __launch_bounds__(T) void sample_slices_kernel(SampleParams p) {
+    constexpr int kEach = kBins > T ? kBins / T : 1;  // bins of a thread, of the first kBins / kEach
     __shared__ uint32_t count[kBins];
-    __shared__ u64 mass[kBins], wave[kThreads / 64];
-    __shared__ double table[kTable];  // in units
-    __shared__ uint16_t sorted[kThreads * PER];
+    __shared__ u64 mass[kBins], wave[T / 64];
+    __shared__ double ones[41], parts[16];  // e^-i in units, e^-(i / 16)
+    __shared__ uint16_t sorted[T * PER];
     __shared__ uint32_t top_first;
-    __shared__ float tops[kThreads / 64];
+    __shared__ float tops[T / 64];
     const int tid = threadIdx.x;
     const int s = blockIdx.x % p.n_slices, r = blockIdx.x / p.n_slices, row = p.row0 + r;
     const int n = min(p.per, p.a.n_vocab - s * p.per);
     const float *l = p.a.logits + (int64_t)row * p.a.stride + (int64_t)s * p.per;
     float x[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) x[i] = l[min(i * kThreads + tid, n - 1)];
+    for (int i = 0; i < PER; ++i) x[i] = l[min(i * T + tid, n - 1)];
     const float t = p.a.temperature ? p.a.temperature[row] : 1.0f;
     if (tid == 0) top_first = ~0u;
-    if (tid < kBins) {
-        count[tid] = 0;
-        mass[tid] = 0;
+#pragma unroll
+    for (int i = tid; i < kBins; i += T) {
+        count[i] = 0;
+        mass[i] = 0;
     }
-    if (tid < kTable) table[tid] = exp_neg(tid * 0.0625) * kSliceUnit;
+    if (tid < 41 + 16) {
+        const double e = exp_neg(tid < 41 ? (double)tid : (tid - 41) * 0.0625);
+        if (tid < 41) ones[tid] = e * kSliceUnit;
+        else parts[tid - 41] = e;
+    }
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        if (i * kThreads + tid >= n) x[i] = -INFINITY;
+        if (i * T + tid >= n) x[i] = -INFINITY;
         top = fmaxf(top, x[i]);  // (NaN is not taken)
     }
     top = butterfly_max<64>(top);
     if ((tid & 63) == 0) tops[tid >> 6] = top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) top = fmaxf(top, tops[i]);
+    for (int i = 0; i < T / 64; ++i) top = fmaxf(top, tops[i]);
     Slice &out = p.slices[(int64_t)r * p.n_slices + s];
     const bool none = top == -INFINITY;
     if (none || !(t > 0.0f)) {  // uniform: no token, or the largest logit alone is asked for
         if (!none) {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-                if (x[i] == top) atomicMin(&top_first, (uint32_t)(i * kThreads + tid));
+                if (x[i] == top) atomicMin(&top_first, (uint32_t)(i * T + tid));
         }
-        if (tid < kBins) {
-            out.mass[tid] = 0;
-            out.end[tid] = 0;
+#pragma unroll
+        for (int i = tid; i < kBins; i += T) {
+            out.mass[i] = 0;
+            out.end[i] = 0;
         }
         if (tid < kBlocks) {
             out.block_mass[tid] = 0;
@@ -230,6 +240,7 @@ __global__ __launch_bounds__(kThreads) void sample_slices_kernel(SampleParams p)
             const uint32_t b = min((uint32_t)top_bin - (uint32_t)grid_place(x[i], grid), (uint32_t)(kBins - 1));
             const double d = ((double)top - (double)x[i]) * inv_t;
             const double at = rint(fmin(d * 16.0, 640.0));
+            const int n16 = (int)at;
             const double q = at * 0.0625 - d;
             double e = 1.0 / 720.0;
             e = __builtin_fma(e, q, 1.0 / 120.0);
@@ -238,34 +249,46 @@ __global__ __launch_bounds__(kThreads) void sample_slices_kernel(SampleParams p)
             e = __builtin_fma(e, q, 0.5);
             e = __builtin_fma(e, q, 1.0);
             e = __builtin_fma(e, q, 1.0);
-            const u64 w = at < 640.0 ? whole(table[(int)at] * e) : 0;
+            const u64 w = n16 < 640 ? whole(ones[n16 >> 4] * parts[n16 & 15] * e) : 0;
             place[i] = b << 16 | atomicAdd(&count[b], 1u);
             if (w) atomicAdd(&mass[b], w);
         }
     }
     __syncthreads();
-    const uint32_t mine = tid < kBins ? count[tid] : 0u;
-    const uint32_t end = scan32(mine, wave);
-    if (tid < kBins) {
-        count[tid] = end - mine;
-        out.end[tid] = (uint16_t)end;
-        u64 m = mass[tid];
-        out.mass[tid] = m;
+    uint32_t mine = 0;
+    const bool has = tid * kEach < kBins;
+    if (has)
 #pragma unroll
-        for (int d = 1; d < kBlock; d <<= 1) m += shfl_xor64(m, d);
-        if (tid % kBlock == kBlock - 1) {
-            out.block_mass[tid / kBlock] = m;
-            out.block_end[tid / kBlock] = (uint16_t)end;
+        for (int i = 0; i < kEach; ++i) mine += count[tid * kEach + i];
+    uint32_t at = scan32<T>(mine, wave) - mine;
+    if (has) {
+        u64 m = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int b = tid * kEach + i;
+            const uint32_t c = count[b];
+            count[b] = at;
+            at += c;
+            out.end[b] = (uint16_t)at;
+            out.mass[b] = mass[b];
+            m += mass[b];
+        }
+        constexpr int kHold = kBlock / kEach;  // threads of a block
+#pragma unroll
+        for (int d = 1; d < kHold; d <<= 1) m += shfl_xor64(m, d);
+        if (tid % kHold == kHold - 1) {
+            out.block_mass[tid / kHold] = m;
+            out.block_end[tid / kHold] = (uint16_t)at;
         }
     }
     if (tid == 0) out.top_bin = top_bin;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-        if (place[i] != ~0u) sorted[count[place[i] >> 16] + (place[i] & 0xFFFFu)] = (uint16_t)(i * kThreads + tid);
+        if (place[i] != ~0u) sorted[count[place[i] >> 16] + (place[i] & 0xFFFFu)] = (uint16_t)(i * T + tid);
     __syncthreads();
     uint32_t *dst = reinterpret_cast<uint32_t *>(p.index + ((int64_t)r * p.n_slices + s) * p.per);
-    for (int i = tid; i < (n + 1) / 2; i += kThreads) dst[i] = reinterpret_cast<const uint32_t *>(sorted)[i];
+    for (int i = tid; i < (n + 1) / 2; i += T) dst[i] = reinterpret_cast<const uint32_t *>(sorted)[i];
 }
 
 // A place in the order.
@@ -289,6 +312,7 @@ struct Pick {
     uint32_t upto[kSlices];
     // the window: sorted (~pattern, index), weights up to the end of each
     u64 item[kWindow], mass[kWindow];
+    uint32_t place[256];
     u64 part_mass[kParts];
     uint32_t part_count[kParts];
     u64 wave[kThreads / 64];
@@ -332,14 +356,19 @@ struct Picker {
             }
             sh.from[tid] = beg;
         }
-        const uint32_t to = scan32(c, sh.wave);
+        const uint32_t to = scan32<kThreads>(c, sh.wave);
         if (tid < p.n_slices) sh.upto[tid] = to;
         __syncthreads();
         logits = sh.upto[p.n_slices - 1];
     }
-    // f(index in the row, pattern) for the gathered logits, four of a thread at a time.
+    // f(index in the row, pattern) for the gathered logits.
     template <class F>
     __device__ __forceinline__ void each(F f) const {
+        load([&](int, uint32_t index, uint32_t key) { f(index, key); });
+    }
+    // Four of a thread at a time.
+    template <class F>
+    __device__ __forceinline__ void load(F f) const {
         for (uint32_t i0 = threadIdx.x; i0 < logits; i0 += 4 * kThreads) {
             int s[4];
             uint32_t at[4];
@@ -360,7 +389,7 @@ struct Picker {
             for (int q = 0; q < 4; ++q) x[q] = logit(s[q], at[q]);
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                if (i0 + q * kThreads < logits) f((uint32_t)(s[q] * p.per) + at[q], order_key(x[q]));
+                if (i0 + q * kThreads < logits) f(q, (uint32_t)(s[q] * p.per) + at[q], order_key(x[q]));
         }
     }
 
@@ -378,26 +407,42 @@ struct Picker {
             if (i < kWindow) sh.item[i] = (u64)~key << 32 | index;
         });
         __syncthreads();
-        // bitonic, ascending (the empty places last); partners of the same wave need no
-        // barrier, and waves without items only take part in those
+        // ascending (the empty places last)
         int size = 64;
         while (size < (int)count) size <<= 1;
         u64 x = sh.item[tid];
         const bool live = tid < size;  // the same for a wave
-        for (int k = 2; k <= size; k <<= 1)
-            for (int j = k >> 1; j > 0; j >>= 1) {
-                u64 y = x;
-                if (j >= 64) {
-                    __syncthreads();
-                    if (live) sh.item[tid] = x;
-                    __syncthreads();
-                    if (live) y = sh.item[tid ^ j];
-                } else if (live) {
-                    y = shfl_xor64(x, j);
+        if (size <= 256) {
+            // an item's place is the number of smaller ones: kThreads / size threads an item
+            const int i = tid & (size - 1), each = size * size / kThreads, j0 = tid / size * each;
+            const u64 y = sh.item[i];
+            uint32_t smaller = 0;
+            for (int j = 0; j < each; ++j) smaller += sh.item[j0 + j] < y;
+            if (live) sh.place[tid] = 0;
+            __syncthreads();
+            atomicAdd(&sh.place[i], smaller);
+            __syncthreads();
+            if (tid < (int)count) sh.item[sh.place[tid]] = x;
+            __syncthreads();
+            x = sh.item[tid];
+        } else {
+            // bitonic; partners of the same wave need no barrier, and waves without items
+            // only take part in those
+            for (int k = 2; k <= size; k <<= 1)
+                for (int j = k >> 1; j > 0; j >>= 1) {
+                    u64 y = x;
+                    if (j >= 64) {
+                        __syncthreads();
+                        if (live) sh.item[tid] = x;
+                        __syncthreads();
+                        if (live) y = sh.item[tid ^ j];
+                    } else if (live) {
+                        y = shfl_xor64(x, j);
+                    }
+                    const bool up = (tid & k) == 0, low = (tid & j) == 0;
+                    if ((y < x) == (up == low)) x = y;
                 }
-                const bool up = (tid & k) == 0, low = (tid & j) == 0;
-                if ((y < x) == (up == low)) x = y;
-            }
+        }
         u64 to = tid < (int)count ? weight(~(uint32_t)(x >> 32)) : 0;
         if (live) {
 #pragma unroll
@@ -505,6 +550,19 @@ struct Picker {
         }
         gather(b * kBlock + bin, b * kBlock + bin);
         uint32_t lo = 0, hi = ~0u;
+        // the thread's patterns, where four a thread hold them (0: none)
+        uint32_t key4[4] = {0, 0, 0, 0};
+        const bool held = logits <= 4 * kThreads;
+        if (count > kWindow && held) load([&](int q, uint32_t, uint32_t key) { key4[q] = key; });
+        const auto each_key = [&](auto f) {
+            if (held) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (key4[q] != 0) f(key4[q]);
+            } else {
+                each([&](uint32_t, uint32_t key) { f(key); });
+            }
+        };
         while (count > kWindow) {  // narrow it
             __syncthreads();
             if (tid == 0) {
@@ -517,7 +575,7 @@ struct Picker {
             }
             __syncthreads();
             uint32_t least = ~0u, most = 0;
-            each([&](uint32_t, uint32_t key) {
+            each_key([&](uint32_t key) {
                 if (key >= lo && key <= hi) {
                     least = min(least, key);
                     most = max(most, key);
@@ -535,7 +593,7 @@ struct Picker {
                 return Found{rank + (uint32_t)nth, before + (u64)nth * w, w, lo, (uint32_t)nth, -1};
             }
             const u64 range = (u64)(hi - lo) + 1;
-            each([&](uint32_t, uint32_t key) {
+            each_key([&](uint32_t key) {
                 if (key >= lo && key <= hi) {
                     const int part = (int)((u64)(hi - key) * kParts / range);
                     atomicAdd(&sh.part_count[part], 1u);
@@ -545,8 +603,8 @@ struct Picker {
             __syncthreads();
             const uint32_t c = tid < kParts ? sh.part_count[tid] : 0;
             const u64 m = tid < kParts ? sh.part_mass[tid] : 0;
-            const uint32_t c_to = scan32(c, sh.wave);
-            const u64 m_to = scan64(m, sh.wave);
+            const uint32_t c_to = scan32<kThreads>(c, sh.wave);
+            const u64 m_to = scan64<kThreads>(m, sh.wave);
             __syncthreads();
             if (tid == 0) {
                 sh.v[1] = kParts;
@@ -579,15 +637,20 @@ struct Picker {
         return search(target);
     }
 
+    // How many of the window's first places f holds for, up to where it ends (f(i) for i
+    // < n; every wave by itself).
+    template <class F>
+    __device__ __forceinline__ int prefix(F f) const {
+        const int lane = threadIdx.x & 63;
+        for (int i0 = 0; i0 < n; i0 += 64) {
+            const u64 no = __builtin_amdgcn_ballot_w64(i0 + lane >= n || !f(min(i0 + lane, n - 1)));
+            if (no) return i0 + __builtin_ctzll(no);
+        }
+        return n;
+    }
     // The window's first place whose weights exceed the target, or its last.
-    __device__ __forceinline__ Found search(double target) {
-        const int tid = threadIdx.x;
-        __syncthreads();
-        if (tid == 0) sh.v[1] = n - 1;
-        __syncthreads();
-        if (tid < n && (double)(base_mass + sh.mass[tid]) > target) atomicMin(&sh.v[1], (uint32_t)tid);
-        __syncthreads();
-        return at_window((int)sh.v[1]);
+    __device__ __forceinline__ Found search(double target) const {
+        return at_window(min(prefix([&](int i) { return (double)(base_mass + sh.mass[i]) <= target; }), n - 1));
     }
 };
 
@@ -717,24 +780,23 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams p) {
             // how many logits weigh enough: those of the window, if it ends below them, else
             // down to the kept ones' border or to where none can
             if (!(min_p > 0.0f)) continue;
-            __syncthreads();
-            if (tid == 0) sh.v[0] = 0;
-            __syncthreads();
-            uint32_t c = 0;
             const auto enough = [&](uint32_t key) { return weight_of(key_value(key), top, inv_t) >= (double)min_p; };
-            const bool in_window = pick.n > 0 && pick.base_rank == 0 &&
-                                   ((uint32_t)pick.n >= keep || !enough(~(uint32_t)(sh.item[pick.n - 1] >> 32)));
-            if (in_window) {
-                if (tid < pick.n) c = enough(~(uint32_t)(sh.item[tid] >> 32));
-            } else {
+            uint32_t most = 0;
+            const bool from_top = pick.n > 0 && pick.base_rank == 0;
+            if (from_top) most = pick.prefix([&](int i) { return enough(~(uint32_t)(sh.item[i] >> 32)); });
+            if (!from_top || (most == (uint32_t)pick.n && most < keep)) {  // uniform
+                __syncthreads();
+                if (tid == 0) sh.v[0] = 0;
+                uint32_t c = 0;
                 pick.gather(0, min(last, min_p_block) * kBlock + kBlock - 1);
                 pick.each([&](uint32_t, uint32_t key) { c += enough(key); });
-            }
 #pragma unroll
-            for (int d = 32; d > 0; d >>= 1) c += __shfl_xor((int)c, d, 64);
-            if ((tid & 63) == 0) atomicAdd(&sh.v[0], c);
-            __syncthreads();
-            const uint32_t most = max(1u, sh.v[0]);
+                for (int d = 32; d > 0; d >>= 1) c += __shfl_xor((int)c, d, 64);
+                if ((tid & 63) == 0) atomicAdd(&sh.v[0], c);
+                __syncthreads();
+                most = sh.v[0];
+            }
+            most = max(most, 1u);
             if (most >= keep) continue;
             target = (double)most - 1.0;
         } else if (step == 3) {
@@ -760,7 +822,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams p) {
         const int n = min(p.per, a.n_vocab - s * p.per);
         uint32_t c = 0;
         for (int i = tid; i < n; i += kThreads) c += order_key(pick.logit(s, i)) == f.key;
-        const uint32_t to = scan32(c, sh.wave);
+        const uint32_t to = scan32<kThreads>(c, sh.wave);
         __syncthreads();
         if (tid == kThreads - 1) sh.v[0] = to;
         __syncthreads();
@@ -771,7 +833,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams p) {
         }
         for (int i0 = 0; i0 < n; i0 += kThreads) {
             const bool is = i0 + tid < n && order_key(pick.logit(s, i0 + tid)) == f.key;
-            const uint32_t upto = before + scan32(is, sh.wave);
+            const uint32_t upto = before + scan32<kThreads>(is, sh.wave);
             if (is && upto == f.nth + 1) a.ids[row] = s * p.per + i0 + tid;
             __syncthreads();
             if (tid == kThreads - 1) sh.v[0] = upto;
@@ -787,12 +849,12 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams p) {
 hipError_t launch_sample(const SampleRows &rows, int n_rows, hipStream_t st) {
     SampleParams p{};
     p.a = rows;
-    // 8 logits of a thread for a few rows, which leave CUs free; 16 for many: fewer bins
-    // to put together
+    // Slices of 2048 logits for a few rows, which leave CUs free, of 8192 for some, of
+    // 16384 for many: fewer bins to put together.
     const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
-    const int64_t eights = (rows.n_vocab + 8 * kThreads - 1) / (8 * kThreads);
-    const bool few = eights <= kSlices && eights * n_rows <= 2 * cus;
-    const int most = (few ? 8 : 16) * kThreads;
+    int most = 2048;
+    if ((int64_t)((rows.n_vocab + most - 1) / most) * n_rows > 2 * cus || rows.n_vocab > kSlices * most) most = 8192;
+    if ((int64_t)((rows.n_vocab + most - 1) / most) * n_rows > 2 * cus || rows.n_vocab > kSlices * most) most = 16384;
     p.n_slices = (rows.n_vocab + most - 1) / most;
     p.per = ((rows.n_vocab + p.n_slices - 1) / p.n_slices + 1) & ~1;
     int bits = 62;
@@ -807,8 +869,9 @@ hipError_t launch_sample(const SampleRows &rows, int n_rows, hipStream_t st) {
     p.index = reinterpret_cast<uint16_t *>(p.slices + (size_t)group * p.n_slices);
     for (p.row0 = 0; p.row0 < n_rows; p.row0 += group) {
         const int n = std::min(group, n_rows - p.row0);
-        if (few) sample_slices_kernel<8><<<n * p.n_slices, kThreads, 0, st>>>(p);
-        else sample_slices_kernel<16><<<n * p.n_slices, kThreads, 0, st>>>(p);
+        if (most == 2048) sample_slices_kernel<256, 8><<<n * p.n_slices, 256, 0, st>>>(p);
+        else if (most == 8192) sample_slices_kernel<1024, 8><<<n * p.n_slices, 1024, 0, st>>>(p);
+        else sample_slices_kernel<1024, 16><<<n * p.n_slices, 1024, 0, st>>>(p);
         sample_pick_kernel<<<n, kThreads, 0, st>>>(p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
