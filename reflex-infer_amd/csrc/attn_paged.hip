@@ -12,7 +12,6 @@
 #include <math.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "attn_paged.h"
 #include "attn_tile.h"
@@ -25,13 +24,19 @@ namespace rxq4 {
 namespace {
 
 constexpr int kStep = 128;      // positions per step of a workgroup
+constexpr int kNoStep = 1 << 22;  // past every position (2^24 at most): its loads are past the end
 constexpr int kMaxChunks = 64;  // chunks of positions per sequence
 
+typedef const float __attribute__((address_space(1))) *GlobalFloat;
 __device__ const float g_one = 1.0f;  // int8 caches without scales: read with stride 0
 
 __device__ __forceinline__ float log2_scale(float vs) {
     return fminf(fmaxf(__builtin_amdgcn_logf(fabsf(vs)), kMinScale), kMaxScale);
 }
+
+// Waves per SIMD that the registers are cut to: what is in flight is what counts, and
+// an int8 step holds half the bytes of an fp16 one.
+constexpr int rows_waves(int hd, bool i8) { return hd > 128 ? 1 : hd == 64 ? 4 : i8 ? 3 : 2; }
 
 // Wave w takes positions 32 w .. + 31 of every 128-position step of the chunk with
 // its own online softmax; the four waves merge at the end.  Per step, lane l =
@@ -47,17 +52,21 @@ __device__ __forceinline__ float log2_scale(float vs) {
 //                    ds_read_tr16_b64 of the wave's V rows in LDS), src1 = P^T as the
 //                    score registers hold it (k of a lane group: its positions), in
 //                    fp16 hi + lo parts (22 bits).
-// The next step's K and V are loaded before this step's arithmetic, and the table
-// entries of the one after before those (loads are waited for in order).  Lane i
-// looks up position i.  Pages of 16 positions or more (BIG): the 16 rows of an
+// The next step's K and V are loaded before this step's arithmetic.  Pages of 16 positions or more (BIG): the 16 rows of an
 // operand lie in one page, a buffer resource of the wave, so that a load needs no
-// address arithmetic; smaller ones: the rows' offsets through LDS.
+// address arithmetic, and the lanes hold the table entries of 32 steps; smaller ones:
+// lane i looks up position i, a step ahead, and the rows' offsets go through LDS.
 // Rows past the end or in holes are zeros (BIG: past the end of the operand's buffer
 // resource; else the pool's first row in their place, cleared), their scores
 // -infinity.
 template <int HD, bool I8, bool BIG>
-__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel(PagedParams p) {
-    constexpr int KS = HD / 32, DT = HD / 16, VROW = HD + 16, CH = HD / 8, NV = 32 * CH / 64;
+__global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kernel(PagedParams p) {
+    // A chunk is 16 bytes: 8 dims of fp16, 16 of int8, which are two k steps of a
+    // product (a lane's dims need only be the same in K and Q).
+    constexpr int EC = I8 ? 16 : 8;                     // dims of a chunk
+    constexpr int KL = (HD + 4 * EC - 1) / (4 * EC);    // K chunks of a lane and operand
+    constexpr int KS = I8 ? 2 * KL : KL;                // k steps
+    constexpr int DT = HD / 16, VROW = HD + 16, CH = HD / EC, NV = (32 * CH + 63) / 64;
     constexpr int esz = I8 ? 1 : 2;
     constexpr int NM = DT * 4 + 2;  // merge values per lane: O, m, l
     constexpr int kV = 4 * 32 * VROW * 2, kM = 4 * NM * 64 * 4;
@@ -68,8 +77,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
     uint16_t *const vl = reinterpret_cast<uint16_t *>(smem) + w * 32 * VROW;
-    const int kvh = blockIdx.x % p.c.n_kv, u = blockIdx.x / p.c.n_kv;
-    const int s = u % p.b.n_seqs, c = u / p.b.n_seqs;
+    // The KV heads of a sequence's chunk go to one XCD (workgroups are dealt to the eight in
+    // turn): they read the same pages and scales.  A sequence's chunks go to different ones.
+    const int x8 = blockIdx.x / 8, kvh = x8 % p.c.n_kv, u = x8 / p.c.n_kv * 8 + blockIdx.x % 8;
+    const int c = u / p.b.n_seqs, s = (u + 3 * c) % p.b.n_seqs;
+    if (c >= p.n_chunks) return;
     const int beg = c * p.chunk;
     const int limit = position_limit(p.b, p.c);
     if (beg >= limit && c > 0) return;
@@ -84,7 +96,10 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel
         const int x = table[has_table ? i : 0];
         return has_table ? x : i;
     };
-    int ent = entry(p_lane), ent_next = entry(p_lane + kStep);
+    // BIG: lane 2 j + st holds the entry of operand st of step j, for 32 steps; else the
+    // lane's position's, one step ahead
+    auto entries = [&](int j) { return entry(beg + 32 * w + kStep * (j + (lane >> 1)) + 16 * (lane & 1)); };
+    int ent = BIG ? entries(0) : entry(p_lane), ent_next = BIG ? 0 : entry(p_lane + kStep);
     const SeqSpan span = seq_span(p.b, s);
     const int rows = min(span.n, p.b.max_new) * p.group;
     if (rows == 0 || rows > kPagedRows) return;
@@ -93,11 +108,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel
     const int row = min(r, rows - 1);  // (columns past the last row repeat it)
     const int tok = row / p.group, head = kvh * p.group + row % p.group;
     const bool row_ok = r < rows;
-    const int hd = p.c.hd, n_ch = hd >> 3;
+    const int hd = p.c.hd, n_ch = hd / EC;
     const int64_t orow = ((int64_t)(span.row0 + tok) * p.n_heads + head) * hd;
     if (end <= beg) {  // uniform
         if (c == 0 && w == 0 && row_ok)  // the tokens see nothing
-            for (int ch = g; ch < n_ch; ch += 4) *reinterpret_cast<u32x4 *>(p.out + orow + 8 * ch) = u32x4{0u, 0u, 0u, 0u};
+            for (int ch = g; ch < hd / 8; ch += 4) *reinterpret_cast<u32x4 *>(p.out + orow + 8 * ch) = u32x4{0u, 0u, 0u, 0u};
         return;
     }
     const int qpos = span.pos0 + tok;
@@ -106,93 +121,101 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel
 
     u32x4 qf[KS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-        qf[ks] = 4 * ks + g < n_ch ? load16(p.q + orow + 8 * (4 * ks + g)) : u32x4{0u, 0u, 0u, 0u};
+    for (int ks = 0; ks < KS; ++ks) {
+        const int ch = I8 ? 2 * (4 * (ks / 2) + g) + ks % 2 : 4 * ks + g;  // of 8 dims
+        qf[ks] = ch < hd / 8 ? load16(p.q + orow + 8 * ch) : u32x4{0u, 0u, 0u, 0u};
+    }
     // Byte offsets within a 16-row operand: K row r, dims 32 ks + 8 g; V row of the
     // lane's chunks.  Chunks past head_dim are past the operand's end (BIG), or the
     // last one again.
     constexpr int kPast = 0x7FFF0000;
-    int ko[KS], vo[NV];
+    int ko[KL], vo[NV];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        const int ch = 4 * ks + g;
-        ko[ks] = BIG ? (ch < n_ch ? r * row_bytes + 8 * esz * ch : kPast) : 8 * esz * min(ch, n_ch - 1);
+    for (int i = 0; i < KL; ++i) {
+        const int ch = 4 * i + g;
+        ko[i] = BIG ? (ch < n_ch ? r * row_bytes + 16 * ch : kPast) : 16 * min(ch, n_ch - 1);
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int id = lane + 64 * j, ch = id % CH;
-        vo[j] = BIG ? (ch < n_ch ? (id / CH & 15) * row_bytes + 8 * esz * ch : kPast) : 8 * esz * min(ch, n_ch - 1);
+        vo[j] = BIG ? (ch < n_ch && id < 32 * CH ? (id / CH & 15) * row_bytes + 16 * ch : kPast) : 16 * min(ch, n_ch - 1);
     }
-    const float *const ksp = p.c.ks ? p.c.ks + kvh : &g_one, *const vsp = p.c.vs ? p.c.vs + kvh : &g_one;
+    // (global pointers: a generic load would be waited for with the LDS reads)
+    const GlobalFloat ksp = p.c.ks ? (GlobalFloat)(p.c.ks + kvh) : (GlobalFloat)&g_one;
+    const GlobalFloat vsp = p.c.vs ? (GlobalFloat)(p.c.vs + kvh) : (GlobalFloat)&g_one;
     const int s_stride = p.c.ks ? p.c.n_kv : 0, v_stride = p.c.vs ? p.c.n_kv : 0;
-    using Chunk = typename std::conditional<I8, u32x2, u32x4>::type;
     struct Step {
-        Chunk k[2][KS], v[NV];
+        u32x4 k[2][KL], v[NV];
         float ks, vs;
         uint32_t seen;  // which of the wave's 32 positions there are
     };
-    auto buffer = [](__amdgpu_buffer_rsrc_t rs, int at) {
-        if constexpr (I8) return buffer_load8(rs, at);
-        else return buffer_load16(rs, at);
-    };
     auto load_step = [&](int j, int e, Step &S) {
-        const int pos = p_lane + kStep * j;
-        const bool ok = pos < end && (unsigned)e < (unsigned)p.c.n_pages;
-        S.seen = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
-        const int place = pos & ((1 << p.c.shift) - 1);
-        if constexpr (I8) {
-            const int64_t at = ok ? ((int64_t)e << p.c.shift) + place : 0;
-            S.ks = ksp[at * s_stride];
-            S.vs = vsp[at * v_stride];
-        }
+        const int mask = (1 << p.c.shift) - 1;
         if constexpr (BIG) {
             // an operand's rows: those of its positions that there are, from the first
             __amdgpu_buffer_rsrc_t kr[2], vr[2];
+            S.seen = 0;
+            int page[2], place[2];
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-                const int n = __builtin_popcount((S.seen >> (16 * st)) & 0xFFFFu);
-                const int page = n ? __builtin_amdgcn_readlane(e, 16 * st) : 0;
-                const int64_t base = (int64_t)page * p.c.page_bytes + (int64_t)__builtin_amdgcn_readlane(place, 16 * st) * row_bytes;
-                const int bytes = n ? (n - 1) * row_bytes + hd * esz : 0;
+                const int pos = beg + 32 * w + kStep * j + 16 * st;
+                page[st] = __builtin_amdgcn_readlane(e, (2 * j + st) & 63);
+                const int n = (unsigned)page[st] < (unsigned)p.c.n_pages ? max(min(end - pos, 16), 0) : 0;
+                S.seen |= ((1u << n) - 1) << (16 * st);
+                page[st] = n > 0 ? page[st] : 0;
+                place[st] = pos & mask;
+                const int64_t base = (int64_t)page[st] * p.c.page_bytes + (int64_t)place[st] * row_bytes;
+                const int bytes = n > 0 ? (n - 1) * row_bytes + hd * esz : 0;
                 kr[st] = make_rsrc(kb + base, bytes);
                 vr[st] = make_rsrc(vb + base, bytes);
+            }
+            if constexpr (I8) {
+                const bool ok = (S.seen >> (lane & 31)) & 1;
+                const int64_t at = ok ? ((int64_t)(lane & 16 ? page[1] : page[0]) << p.c.shift) +
+                                            (lane & 16 ? place[1] : place[0]) + (lane & 15) : 0;
+                S.ks = ksp[at * s_stride];
+                S.vs = vsp[at * v_stride];
             }
 #pragma unroll
             for (int st = 0; st < 2; ++st)
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) S.k[st][ks] = buffer(kr[st], ko[ks]);
+                for (int i = 0; i < KL; ++i) S.k[st][i] = buffer_load16(kr[st], ko[i]);
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                if constexpr (CH == 12) {  // (a load's rows may be in both operands)
+                constexpr bool kSplit = 64 % CH != 0 || 64 / CH > 16;  // a load's rows may be in both operands
+                if constexpr (kSplit) {
                     const bool first = (lane + 64 * j) / CH < 16;
-                    const Chunk a = buffer(vr[0], first ? vo[j] : kPast), b = buffer(vr[1], first ? kPast : vo[j]);
-                    S.v[j] = a | b;
+                    S.v[j] = buffer_load16(vr[0], first ? vo[j] : kPast) | buffer_load16(vr[1], first ? kPast : vo[j]);
                 } else {
-                    S.v[j] = buffer(vr[64 * j / CH / 16], vo[j]);
+                    S.v[j] = buffer_load16(vr[64 * j / CH / 16], vo[j]);
                 }
             }
         } else {
+            const int pos = p_lane + kStep * j;
+            const bool ok = pos < end && (unsigned)e < (unsigned)p.c.n_pages;
+            S.seen = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
+            const int place = pos & mask;
+            if constexpr (I8) {
+                const int64_t at = ok ? ((int64_t)e << p.c.shift) + place : 0;
+                S.ks = ksp[at * s_stride];
+                S.vs = vsp[at * v_stride];
+            }
             if (lane < 32) rowoff[w][lane] = ok ? (int64_t)e * p.c.page_bytes + (int64_t)place * row_bytes : 0;
             wave_lds_fence();
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
                 const uint8_t *src = kb + rowoff[w][16 * st + r];
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) S.k[st][ks] = *reinterpret_cast<const Chunk *>(src + ko[ks]);
+                for (int i = 0; i < KL; ++i) S.k[st][i] = load16(src + ko[i]);
             }
 #pragma unroll
-            for (int j = 0; j < NV; ++j)
-                S.v[j] = *reinterpret_cast<const Chunk *>(vb + rowoff[w][(lane + 64 * j) / CH] + vo[j]);
+            for (int j = 0; j < NV; ++j) S.v[j] = load16(vb + rowoff[w][min((lane + 64 * j) / CH, 31)] + vo[j]);
             wave_lds_fence();
         }
     };
-    auto widen = [](Chunk x) {
-        if constexpr (I8) {
-            const u32x2 a = i8x4_to_f16(x.x), b = i8x4_to_f16(x.y);
-            return u32x4{a.x, a.y, b.x, b.y};
-        } else {
-            return x;
-        }
+    auto widen = [](uint32_t a, uint32_t b) {  // 8 int8
+        const u32x2 x = i8x4_to_f16(a), y = i8x4_to_f16(b);
+        return u32x4{x.x, x.y, y.x, y.y};
     };
 
     f32x4 o[DT];
@@ -208,7 +231,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel
             acc[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                u32x4 k = widen(S.k[st][ks]);
+                u32x4 k;
+                if constexpr (I8) k = ks % 2 ? widen(S.k[st][ks / 2].z, S.k[st][ks / 2].w) : widen(S.k[st][ks / 2].x, S.k[st][ks / 2].y);
+                else k = S.k[st][ks];
                 if (!I8 && !BIG && 4 * ks + 4 > n_ch && 4 * ks + g >= n_ch) k = u32x4{0u, 0u, 0u, 0u};
                 acc[st] = mfma<RXQ4_DTYPE_F16>(k, qf[ks], acc[st]);
             }
@@ -285,7 +310,15 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int id = lane + 64 * j;
-            *reinterpret_cast<u32x4 *>(&vl[(id / CH) * VROW + 8 * (id % CH)]) = widen(S.v[j]);
+            uint16_t *dst = &vl[(id / CH) * VROW + EC * (id % CH)];
+            if constexpr (I8) {
+                if (32 * CH % 64 == 0 || id < 32 * CH) {
+                    *reinterpret_cast<u32x4 *>(dst) = widen(S.v[j].x, S.v[j].y);
+                    *reinterpret_cast<u32x4 *>(dst + 8) = widen(S.v[j].z, S.v[j].w);
+                }
+            } else {
+                *reinterpret_cast<u32x4 *>(dst) = S.v[j];
+            }
         }
         // lane r of group g supplies dims 16 dt + 4 (r & 3) .. + 3 of positions 4 g + r / 4
         // and 16 + 4 g + r / 4 and receives dim 16 dt + r of positions 4 g .. + 3 and 16 + 4 g ..
@@ -304,18 +337,23 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_paged_rows_kernel
     };
     const int n_steps = (end - beg + kStep - 1) / kStep;
     Step A, B;
-    load_step(0, ent, A);
-    for (int j = 0;;) {
-        ent = entry(p_lane + kStep * (j + 2));
-        load_step(j + 1, ent_next, B);
-        __builtin_amdgcn_sched_barrier(0);  // (the compiler would move them behind the products)
-        process(j, A);
-        if (++j >= n_steps) break;
-        ent_next = entry(p_lane + kStep * (j + 2));
-        load_step(j + 1, ent, A);
-        __builtin_amdgcn_sched_barrier(0);
-        process(j, B);
-        if (++j >= n_steps) break;
+    for (int j0 = 0; j0 < n_steps; j0 += 32) {
+        const int j1 = BIG ? min(n_steps, j0 + 32) : n_steps;
+        if (j0 > 0) ent = entries(j0);
+        load_step(j0, ent, A);
+        for (int j = j0;;) {
+            if (!BIG) ent = entry(p_lane + kStep * (j + 2));
+            load_step(j + 1 < j1 ? j + 1 : kNoStep, BIG ? ent : ent_next, B);
+            __builtin_amdgcn_sched_barrier(0);  // (the compiler would move them behind the products)
+            process(j, A);
+            if (++j >= j1) break;
+            if (!BIG) ent_next = entry(p_lane + kStep * (j + 2));
+            load_step(j + 1 < j1 ? j + 1 : kNoStep, ent, A);
+            __builtin_amdgcn_sched_barrier(0);
+            process(j, B);
+            if (++j >= j1) break;
+        }
+        if (!BIG) break;
     }
     if (bad) {  // uniform, rare: the wave's positions again
         for (int pos = beg; pos < end; ++pos) {
@@ -467,7 +505,7 @@ hipError_t launch_rows(PagedParams &p, const RowsPlan &plan, float *ws, int i8, 
     if (plan.units * p.n_chunks > 0x7FFFFF) return hipErrorInvalidValue;
     p.part = ws;
     p.stats = ws + (size_t)plan.units * p.n_chunks * p.rows_blk * HD;
-    const unsigned grid = (unsigned)(plan.units * p.n_chunks);
+    const unsigned grid = (unsigned)(((int64_t)p.b.n_seqs * p.n_chunks + 7) / 8 * 8 * p.c.n_kv);
     const bool big = p.c.shift >= 4;
     if (i8 && big) attn_paged_rows_kernel<HD, true, true><<<grid, 256, 0, st>>>(p);
     else if (i8) attn_paged_rows_kernel<HD, true, false><<<grid, 256, 0, st>>>(p);

@@ -538,9 +538,9 @@ __global__ __launch_bounds__(256) void attn_paged_block_combine_kernel(PagedPara
     const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (id >= (int64_t)p.b.n_tokens * p.n_heads) return;
     const int t = (int)(id / p.n_heads), head = (int)(id % p.n_heads);
-    const int seq = seq_of_row(p.b, t);
+    SeqSpan span;
+    const int seq = seq_of_row(p.b, t, span);
     if (seq >= p.b.n_seqs) return;
-    const SeqSpan span = seq_span(p.b, seq);
     const int n_rows = min(span.n, p.b.max_new) * p.group;
     const int row = (t - span.row0) * p.group + head % p.group;
     if (t < span.row0 || row >= n_rows || n_rows <= p.rows_limit) return;

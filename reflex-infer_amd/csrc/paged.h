@@ -22,24 +22,31 @@ __device__ __forceinline__ void wave_lds_fence() {
 struct SeqSpan {
     int row0, n, pos0;
 };
+__device__ __forceinline__ SeqSpan seq_span(const SeqBatch &b, int start, int end, int len) {
+    const int a = min(max(start, 0), b.n_tokens);
+    const int e = min(max(end, a), b.n_tokens);
+    return SeqSpan{a, e - a, len - (e - a)};
+}
 __device__ __forceinline__ SeqSpan seq_span(const SeqBatch &b, int s) {
-    const int a = min(max(b.starts[s], 0), b.n_tokens);
-    const int e = min(max(b.starts[s + 1], a), b.n_tokens);
-    return SeqSpan{a, e - a, b.lens[s] - (e - a)};
+    return seq_span(b, b.starts[s], b.starts[s + 1], b.lens[s]);
 }
 
-// The sequence that row t belongs to (n_seqs: none), the same for a whole wave:
-// the number of sequences that end at or before t.
-__device__ __forceinline__ int seq_of_row(const SeqBatch &b, int t) {
+// The sequence that row t belongs to (n_seqs: none) and its rows, the same for a
+// whole wave: the number of sequences that end at or before t.  A lane loads all
+// of a sequence at once: one round trip to memory for up to 64 sequences.
+__device__ __forceinline__ int seq_of_row(const SeqBatch &b, int t, SeqSpan &span) {
     const int lane = threadIdx.x & 63;
-    int seq = 0;
     for (int i = 0; i < b.n_seqs; i += 64) {
-        const bool ends = i + lane < b.n_seqs && b.starts[i + lane + 1] <= t;
-        const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(ends));
-        seq += n;
-        if (n < 64) break;
+        const int j = min(i + lane, b.n_seqs - 1);
+        const int start = b.starts[j], end = b.starts[j + 1], len = b.lens[j];
+        const uint64_t ends = __builtin_amdgcn_ballot_w64(i + lane < b.n_seqs && end <= t);
+        const int n = __builtin_popcountll(ends);
+        if (n == 64 || i + n >= b.n_seqs) continue;
+        span = seq_span(b, __builtin_amdgcn_readlane(start, n), __builtin_amdgcn_readlane(end, n),
+                        __builtin_amdgcn_readlane(len, n));
+        return i + n;
     }
-    return __builtin_amdgcn_readfirstlane(seq);
+    return b.n_seqs;
 }
 
 // Positions that the batch's tokens may see or store: below the table's end.

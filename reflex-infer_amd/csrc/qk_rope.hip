@@ -11,11 +11,12 @@
 //             remainder in 32
 //   int8      scale = max |x| / 127, rint(x / scale), both divisions IEEE, so that
 //             the bytes follow from the 32-bit row alone
-// A workgroup takes one token and up to kWaves * kPasses * (heads a wave) of its
-// heads: its threads form the token's sines and cosines once, in LDS; then each
-// head belongs to L lanes of a wave, 8 dims a lane (16-byte loads and stores),
-// the sums over the L lanes by lane swaps and the pair's other half through the
-// wave's own LDS.
+// A workgroup takes one token and its heads, or a part of them: its threads form
+// the token's sines and cosines once, in LDS, while the first heads' rows are on
+// their way; then each head belongs to L lanes of a wave, 8 dims a lane (16-byte
+// loads and stores, the next head's loads ahead of this one's arithmetic), the
+// sums over the L lanes by lane swaps and the pair's other half through the wave's
+// own LDS.
 #include <math.h>
 
 #include "launch.h"
@@ -40,115 +41,165 @@ struct RopeParams {
     PagedCache c;
 };
 
+// Eight values of a row as they are stored, and widened.
 template <int DT>
-__device__ __forceinline__ void load8(const void *base, int64_t at, float *x) {
+struct Raw {
+    u32x4 a[DT == RXQ4_DTYPE_F32 ? 2 : 1];
+};
+
+template <int DT>
+__device__ __forceinline__ Raw<DT> load8(const void *base, int64_t at) {
+    Raw<DT> r;
+    const uint8_t *s = static_cast<const uint8_t *>(base) + at * (DT == RXQ4_DTYPE_F32 ? 4 : 2);
+    r.a[0] = load16(s);
+    if constexpr (DT == RXQ4_DTYPE_F32) r.a[1] = load16(s + 16);
+    return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void widen8(const Raw<DT> &r, float *x) {
     if constexpr (DT == RXQ4_DTYPE_F32) {
-        const f32x4 *s = reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + at);
-        const f32x4 a = s[0], b = s[1];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = a[i];
-            x[4 + i] = b[i];
-        }
+        for (int i = 0; i < 8; ++i) x[i] = __builtin_bit_cast(f32x4, r.a[i >> 2])[i & 3];
     } else {
-        const u32x4 a = load16(static_cast<const uint16_t *>(base) + at);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = DT == RXQ4_DTYPE_F16 ? f16_bits_to_f32(a[i] & 0xFFFFu) : bf16_bits_to_f32(a[i] & 0xFFFFu);
-            x[2 * i + 1] = DT == RXQ4_DTYPE_F16 ? f16_bits_to_f32(a[i] >> 16) : bf16_bits_to_f32(a[i] >> 16);
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t u = i & 1 ? r.a[0][i >> 1] >> 16 : r.a[0][i >> 1] & 0xFFFFu;
+            x[i] = DT == RXQ4_DTYPE_F16 ? f16_bits_to_f32(u) : bf16_bits_to_f32(u);
         }
     }
 }
 
+__device__ __forceinline__ void lds8(const float *s, float *x) {
+    const f32x4 a = reinterpret_cast<const f32x4 *>(s)[0], b = reinterpret_cast<const f32x4 *>(s)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[i] = a[i];
+        x[4 + i] = b[i];
+    }
+}
+
+// A head of the token: queries, keys and values in order.
+struct Head {
+    bool q, v;
+    int hk;  // its number among its kind
+};
+__device__ __forceinline__ Head head_of(const RopeParams &p, int h) {
+    const bool q = h < p.n_heads, v = h >= p.n_heads + p.c.n_kv;
+    return Head{q, v, q ? h : v ? h - p.n_heads - p.c.n_kv : h - p.n_heads};
+}
+
 // DT: type of q, k, v; L: lanes a head (8 L >= head_dim).
 template <int DT, int L, bool I8>
-__global__ __launch_bounds__(64 * kWaves) void qk_rope_kernel(RopeParams p) {
+__global__ __launch_bounds__(64 * kWaves, DT == RXQ4_DTYPE_F32 ? 7 : 8) void qk_rope_kernel(RopeParams p) {
     constexpr int HPW = 64 / L;  // heads of a wave at a time
     __shared__ float cs[128], sn[128];
-    __shared__ __attribute__((aligned(16))) float xl[kWaves][64 * 8];
+    __shared__ __attribute__((aligned(16))) float wts[2][256], xl[kWaves][64 * 8];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int t = blockIdx.x;
-    const int seq = seq_of_row(p.b, t);
+    const int hd = p.c.hd, half = p.n_rot >> 1;
+    const int sub = lane % L;
+    const bool dims = 8 * sub < hd;
+    const int d0 = dims ? 8 * sub : 0;
+    const int h_end = min(p.n_heads + 2 * p.c.n_kv, ((int)blockIdx.y + 1) * p.heads_wg);
+    // (lanes past the last head repeat it)
+    const auto load = [&](int h0) {
+        const Head h = head_of(p, min(h0 + lane / L, h_end - 1));
+        return load8<DT>(h.q ? p.q : h.v ? p.v : p.k, (int64_t)t * (h.q ? p.q_stride : p.kv_stride) + (int64_t)h.hk * hd + d0);
+    };
+    int h0 = blockIdx.y * p.heads_wg + w * HPW;
+    Raw<DT> next = load(h0);
+    const float freq = tid < half ? p.inv_freq[tid] : 0.0f;
+    if (tid < hd) {
+        if (p.qw) wts[0][tid] = p.qw[tid];
+        if (p.kw) wts[1][tid] = p.kw[tid];
+    }
+    SeqSpan span;
+    const int seq = seq_of_row(p.b, t, span);
     if (seq >= p.b.n_seqs) return;  // uniform
-    const SeqSpan span = seq_span(p.b, seq);
     if (t < span.row0 || t - span.row0 >= min(span.n, p.b.max_new)) return;
     const int pos = span.pos0 + (t - span.row0);
-    const int hd = p.c.hd, half = p.n_rot >> 1;
     const int slot = pos >= 0 && pos < position_limit(p.b, p.c) ? slot_of(p.c, seq, pos) : -1;
     if (tid < half) {
-        const double turns = (double)pos * (double)p.inv_freq[tid] * 0.15915494309189533577;
+        const double turns = (double)pos * (double)freq * 0.15915494309189533577;
         float s, c;
         sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
         cs[tid] = c;
         sn[tid] = s;
     }
     __syncthreads();
-    const int sub = lane % L;
-    const bool dims = 8 * sub < hd;
-    const int n_all = p.n_heads + 2 * p.c.n_kv;
-    const int h_end = min(n_all, ((int)blockIdx.y + 1) * p.heads_wg);
+    // This lane's part of the rotation, the same for every head: x c + y s with the
+    // pair's other half y; the sine's sign is in s.
+    float c[8], s[8];
+    uint32_t turn = 0;  // bit i: dim 8 sub + i is rotated
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int d = 8 * sub + i;
+        const bool first = p.interleaved ? !(i & 1) : d < half;
+        const int j = p.interleaved ? d >> 1 : first ? d : d - half;
+        const bool on = d < p.n_rot;
+        turn |= (uint32_t)on << i;
+        c[i] = on ? cs[j] : 1.0f;
+        s[i] = on ? first ? -sn[j] : sn[j] : 0.0f;
+    }
+    const bool whole = half % 8 == 0;  // a lane's eight dims are all of one half
     float *const mine = xl[w] + lane * 8;
-    float *const head = xl[w] + (lane - sub) * 8;
-    for (int h0 = blockIdx.y * p.heads_wg + w * HPW; h0 < h_end; h0 += kWaves * HPW) {
-        const int h = min(h0 + lane / L, h_end - 1);  // (lanes past the last head repeat it)
+    const float *const head = xl[w] + (lane - sub) * 8;
+    const float *const other = head + (8 * sub < half ? 8 * sub + half : 8 * sub < p.n_rot ? 8 * sub - half : 0);
+    for (; h0 < h_end; h0 += kWaves * HPW) {
         const bool live = h0 + lane / L < h_end && dims;
-        const bool is_q = h < p.n_heads, is_v = h >= p.n_heads + p.c.n_kv;
-        const int hk = is_q ? h : is_v ? h - p.n_heads - p.c.n_kv : h - p.n_heads;
-        const void *src = is_q ? p.q : is_v ? p.v : p.k;
-        const int d0 = dims ? 8 * sub : 0;
+        const Head h = head_of(p, min(h0 + lane / L, h_end - 1));
         float x[8];
-        load8<DT>(src, (int64_t)t * (is_q ? p.q_stride : p.kv_stride) + (int64_t)hk * hd + d0, x);
-        const float *wt = is_q ? p.qw : is_v ? nullptr : p.kw;
+        widen8<DT>(next, x);
+        next = load(h0 + kWaves * HPW);
         if (p.qw || p.kw) {  // uniform; lanes whose head has no weight leave theirs
             float ss = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss += dims ? x[i] * x[i] : 0.0f;
             ss = group_sum<L>(ss);
-            if (wt) {
+            if (!h.v && (h.q ? p.qw : p.kw)) {
                 const float r = 1.0f / sqrtf(ss / (float)hd + p.eps);
+                float wt[8];
+                lds8(wts[h.q ? 0 : 1] + d0, wt);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = x[i] * r * wt[d0 + i];
+                for (int i = 0; i < 8; ++i) x[i] = x[i] * r * wt[i];
             }
         }
         if (half > 0) {  // uniform
+            float y[8];
             if (p.interleaved) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int j = 4 * sub + i;
-                    if (!is_v && j < half) {
-                        const float a = x[2 * i], b = x[2 * i + 1];
-                        x[2 * i] = a * cs[j] - b * sn[j];
-                        x[2 * i + 1] = b * cs[j] + a * sn[j];
-                    }
-                }
+                for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
             } else {
                 wave_lds_fence();  // the reads of the heads before are done
-#pragma unroll
-                for (int i = 0; i < 8; ++i) mine[i] = x[i];
+                reinterpret_cast<f32x4 *>(mine)[0] = f32x4{x[0], x[1], x[2], x[3]};
+                reinterpret_cast<f32x4 *>(mine)[1] = f32x4{x[4], x[5], x[6], x[7]};
                 wave_lds_fence();
+                if (whole) {
+                    lds8(other, y);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int d = 8 * sub + i;
-                    if (!is_v && d < p.n_rot) {
-                        const bool first = d < half;
-                        const int j = first ? d : d - half;
-                        const float y = head[first ? d + half : d - half];
-                        x[i] = first ? x[i] * cs[j] - y * sn[j] : x[i] * cs[j] + y * sn[j];
+                    for (int i = 0; i < 8; ++i) {
+                        const int d = 8 * sub + i;
+                        y[i] = head[d < half ? d + half : d < p.n_rot ? d - half : 0];
                     }
                 }
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!h.v && (turn >> i & 1)) x[i] = x[i] * c[i] + y[i] * s[i];
         }
-        if (is_q) {
+        if (h.q) {
             const bool none = pos < 0;
             u32x4 r;
 #pragma unroll
             for (int i = 0; i < 4; ++i) r[i] = none ? 0u : pack2<RXQ4_DTYPE_F16>(x[2 * i], x[2 * i + 1]);
-            if (live) *reinterpret_cast<u32x4 *>(p.q_out + ((int64_t)t * p.n_heads + h) * hd + d0) = r;
+            if (live) *reinterpret_cast<u32x4 *>(p.q_out + ((int64_t)t * p.n_heads + h.hk) * hd + d0) = r;
         } else if constexpr (!I8) {
             u32x4 r;
 #pragma unroll
             for (int i = 0; i < 4; ++i) r[i] = pack2<RXQ4_DTYPE_F16>(x[2 * i], x[2 * i + 1]);
-            uint8_t *dst = (is_v ? p.c.v : p.c.k) + slot_bytes(p.c, max(slot, 0), p.c.n_kv * hd * 2) + (hk * hd + d0) * 2;
+            uint8_t *dst = (h.v ? p.c.v : p.c.k) + slot_bytes(p.c, max(slot, 0), p.c.n_kv * hd * 2) + (h.hk * hd + d0) * 2;
             if (live && slot >= 0) *reinterpret_cast<u32x4 *>(dst) = r;
         }
         if constexpr (I8) {
@@ -163,14 +214,14 @@ __global__ __launch_bounds__(64 * kWaves) void qk_rope_kernel(RopeParams p) {
             uint32_t b[2] = {0u, 0u};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float y = scale > 0.0f && scale < INFINITY ? rintf(x[i] / scale) : 0.0f;
-                const int n = (int)fminf(fmaxf(y, -127.0f), 127.0f);
+                const float z = scale > 0.0f && scale < INFINITY ? rintf(x[i] / scale) : 0.0f;
+                const int n = (int)fminf(fmaxf(z, -127.0f), 127.0f);
                 b[i >> 2] |= ((uint32_t)n & 0xFFu) << (8 * (i & 3));
             }
-            if (!is_q && live && slot >= 0) {
-                uint8_t *dst = (is_v ? p.c.v : p.c.k) + slot_bytes(p.c, slot, p.c.n_kv * hd) + hk * hd + d0;
+            if (!h.q && live && slot >= 0) {
+                uint8_t *dst = (h.v ? p.c.v : p.c.k) + slot_bytes(p.c, slot, p.c.n_kv * hd) + h.hk * hd + d0;
                 *reinterpret_cast<u32x2 *>(dst) = u32x2{b[0], b[1]};
-                if (sub == 0) (is_v ? p.c.vs : p.c.ks)[(int64_t)slot * p.c.n_kv + hk] = scale;
+                if (sub == 0) (h.v ? p.c.vs : p.c.ks)[(int64_t)slot * p.c.n_kv + h.hk] = scale;
             }
         }
     }
@@ -186,9 +237,9 @@ template <int DT>
 void launch_dt(RopeParams &p, int i8, hipStream_t st) {
     const int L = p.c.hd <= 64 ? 8 : p.c.hd <= 128 ? 16 : 32;
     const int n_all = p.n_heads + 2 * p.c.n_kv, at_once = kWaves * (64 / L);
-    p.heads_wg = n_all;
+    const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
+    p.heads_wg = p.b.n_tokens < cus ? at_once : n_all;
     const dim3 grid(p.b.n_tokens, (n_all + p.heads_wg - 1) / p.heads_wg);
-    (void)at_once;
     if (L == 8) launch_l<DT, 8>(p, grid, i8, st);
     else if (L == 16) launch_l<DT, 16>(p, grid, i8, st);
     else launch_l<DT, 32>(p, grid, i8, st);
