@@ -19,8 +19,11 @@ struct PagedParams {
     float sl2;            // scale * log2(e)
     int rows_limit;       // sequences of at most this many rows are the 16-row kernel's (0: none)
     int rows_blk;         // 16 rows: rows of a sequence that the partials hold
-    int n_blocks;         // 128 rows: at most this many blocks, over the sequences
-    int chunk, n_chunks;  // positions per chunk (a multiple of 64); chunks per block at most
+    int chunk;            // 16 rows: positions per chunk (a multiple of 64)
+    int n_chunks;         // chunks per 16 rows; per block at most
+    int max_units;        // 128 rows: blocks' chunks of the batch at most, per KV head
+    int most_tiles, min_tiles;  // tiles of a block, and of a chunk, at most and at least
+    int *chunk_tiles;     // tiles of a chunk, left for the combine
 };
 
 // Query rows of a workgroup of the smaller and of the larger kernel.
@@ -29,7 +32,7 @@ constexpr int kPagedRows = 16, kPagedBlock = 128;
 // Sequences of more than rows_limit rows (new tokens x group), 128 rows a
 // workgroup; partials within `room` bytes at `ws` (null: no split).
 struct PagedBlockPlan {
-    int chunk, n_chunks;
+    int units, n_chunks, tiles;
     size_t bytes;  // of partials
 };
 PagedBlockPlan plan_paged_blocks(const PagedParams &p, size_t room);

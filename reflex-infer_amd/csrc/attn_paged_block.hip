@@ -32,6 +32,8 @@ namespace rxq4 {
 namespace {
 
 constexpr int kMaxChunks = 64;  // chunks per block
+constexpr int kLeastTiles = 4;  // tiles per chunk, where a block is cut
+constexpr int kSplitSeqs = 1024;  // sequences of a batch whose blocks are cut
 // An int8 tile's floats in LDS: K scales, V scales, log2 |V scale|.
 constexpr int kScl = 3 * kTile;
 
@@ -49,18 +51,64 @@ constexpr int block_lds() {
            + G * 4 * 4;                  // a wave's flag: V not finite
 }
 
-// Blocks of sequence s.
-__device__ __forceinline__ int seq_blocks(const PagedParams &p, int s) {
-    const int rows = min(seq_span(p.b, s).n, p.b.max_new) * p.group;
-    return rows > p.rows_limit ? (rows + kPagedBlock - 1) / kPagedBlock : 0;
+template <typename Chunk>
+__device__ __forceinline__ Chunk load_chunk(__amdgpu_buffer_rsrc_t r, int at, int down) {
+    if constexpr (sizeof(Chunk) == 16) return __builtin_amdgcn_raw_buffer_load_b128(r, at, down, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b64(r, at, down, 0);
 }
 
-// The sequence and block of the idx-th block of the batch, the same for a whole
-// wave; false past the last one.
-__device__ __forceinline__ bool find_block(const PagedParams &p, int idx, int &seq, int &block) {
+// Tiles that a block seeing positions [0, pos_end) walks (one where it sees
+// nothing: its rows are zeros).
+__device__ __forceinline__ int block_tiles(int pos_end) { return (max(pos_end, 1) + kTile - 1) / kTile; }
+
+// Blocks of sequence s, and the tiles of its last.
+__device__ __forceinline__ void seq_blocks(const PagedParams &p, int s, int &blocks, int &tiles) {
+    blocks = 0;
+    tiles = 0;
+    if (s >= p.b.n_seqs) return;
+    const SeqSpan span = seq_span(p.b, s);
+    const int n = min(span.n, p.b.max_new), rows = n * p.group;
+    if (rows <= p.rows_limit) return;
+    blocks = (rows + kPagedBlock - 1) / kPagedBlock;
+    tiles = block_tiles(min(span.pos0 + n, position_limit(p.b, p.c)));
+}
+
+// A workgroup's part of the batch: a block of a sequence and one of the chunks, of
+// `chunk_tiles` tiles, that its tiles are cut into.
+struct Unit {
+    int seq, block, chunk, chunk_tiles;
+};
+
+// The idx-th unit of the batch, the same for a whole wave; false past the last one
+// (chunk_tiles is set all the same).  The chunks are as short as leaves at most
+// p.max_units of them (a sequence's blocks counted as long as its last), or the
+// blocks stay whole: every workgroup comes to the same length from the same sums.
+__device__ __forceinline__ bool find_unit(const PagedParams &p, int idx, Unit &u) {
     const int lane = threadIdx.x & 63;
+    int nb, nt;
+    seq_blocks(p, lane, nb, nt);
+    const auto sum = [&](auto f) {  // over the sequences
+        float x = nb > 0 ? f(nb, nt) : 0.0f;
+        for (int s0 = 64; s0 < p.b.n_seqs; s0 += 64) {
+            int b, t;
+            seq_blocks(p, s0 + lane, b, t);
+            x += b > 0 ? f(b, t) : 0.0f;
+        }
+        return butterfly_sum<64>(x);
+    };
+    int ct = p.most_tiles;
+    if (p.n_chunks > 1 && sum([](int b, int) { return (float)b; }) < (float)p.max_units) {
+        const float all = sum([](int b, int t) { return (float)b * (float)t; });
+        ct = max(p.min_tiles, (int)(all / (float)p.max_units));
+        while (ct < p.most_tiles &&
+               sum([&](int b, int t) { return (float)b * (float)((t + ct - 1) / ct); }) > (float)p.max_units)
+            ct += max(1, ct >> 4);
+        ct = min(ct, p.most_tiles);
+    }
+    u.chunk_tiles = ct = __builtin_amdgcn_readfirstlane(ct);
     for (int s0 = 0; s0 < p.b.n_seqs; s0 += 64) {
-        const int n = s0 + lane < p.b.n_seqs ? seq_blocks(p, s0 + lane) : 0;
+        if (s0 > 0) seq_blocks(p, s0 + lane, nb, nt);
+        const int n_c = (nt + ct - 1) / ct, n = nb * n_c;
         int upto = n;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -70,9 +118,12 @@ __device__ __forceinline__ bool find_block(const PagedParams &p, int idx, int &s
         const uint64_t past = __builtin_amdgcn_ballot_w64(upto > idx);
         if (past != 0) {
             const int at = __builtin_ctzll(past);
-            seq = s0 + at;
-            const int mine = __builtin_amdgcn_readlane(n, at);
-            block = mine - 1 - (idx - (__builtin_amdgcn_readlane(upto, at) - mine));
+            const int in = idx - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
+            const int chunks = __builtin_amdgcn_readlane(n_c, at);
+            const int from_last = __builtin_amdgcn_readfirstlane(in / chunks);
+            u.seq = s0 + at;
+            u.block = __builtin_amdgcn_readlane(nb, at) - 1 - from_last;  // the latest tokens first
+            u.chunk = in - from_last * chunks;
             return true;
         }
         idx -= __builtin_amdgcn_readlane(upto, 63);
@@ -80,11 +131,8 @@ __device__ __forceinline__ bool find_block(const PagedParams &p, int idx, int &s
     return false;
 }
 
-// Tiles that a block seeing positions [0, pos_end) walks (one where it sees
-// nothing: its rows are zeros).
-__device__ __forceinline__ int block_tiles(int pos_end) { return (max(pos_end, 1) + kTile - 1) / kTile; }
-
-template <int HD, bool I8, int G>
+// BIG: pages of 16 positions or more.
+template <int HD, bool I8, int G, bool BIG>
 __global__ __launch_bounds__(256 * G) void attn_paged_block_kernel(PagedParams p) {
     constexpr int KS = HD / 16;             // k-steps of the scores
     constexpr int DT = HD / 32;             // 32-dim tiles of O
@@ -103,19 +151,18 @@ __global__ __launch_bounds__(256 * G) void attn_paged_block_kernel(PagedParams p
     float *const mgl = reinterpret_cast<float *>(smem + G * 4 * TB + G * 8 * kScl);
     int *const bad_v = reinterpret_cast<int *>(mgl + 512) + gq * 4;
 
-    // Unit: a sequence's latest tokens first.
     const int kvh = blockIdx.x % p.c.n_kv;
-    const int v0 = blockIdx.x / p.c.n_kv;
-    const int chunk = v0 / p.n_blocks;
-    int seq, block;
-    if (!find_block(p, v0 % p.n_blocks, seq, block)) return;  // uniform
+    Unit unit;
+    const bool found = find_unit(p, blockIdx.x / p.c.n_kv, unit);
+    if (p.n_chunks > 1 && blockIdx.x == 0 && threadIdx.x == 0) *p.chunk_tiles = unit.chunk_tiles;
+    if (!found) return;  // uniform
+    const int seq = unit.seq, block = unit.block, chunk = unit.chunk, chunk_tiles = unit.chunk_tiles;
     const SeqSpan span = seq_span(p.b, seq);
     const int hd = p.c.hd;
     const int n_rows = min(span.n, p.b.max_new) * p.group;
     const int blk_last = min(n_rows, (block + 1) * kPagedBlock) - 1;
     const int limit = position_limit(p.b, p.c);
     const int pos_end = min(span.pos0 + blk_last / p.group + 1, limit);  // positions the block sees
-    const int chunk_tiles = p.chunk / kTile;
     const int n_tiles = block_tiles(pos_end);
     const int t_beg = chunk * chunk_tiles;
     const int t_end = min(n_tiles, t_beg + chunk_tiles);
@@ -187,6 +234,15 @@ __global__ __launch_bounds__(256 * G) void attn_paged_block_kernel(PagedParams p
         const int i = min(t * kTile + lane, limit - 1) >> p.c.shift;
         return limit <= 0 ? -1 : table ? table[i] : i;
     };
+    // Pages of 16 or more: the 64 chunks that a wave loads at once lie in one aligned
+    // group of 16 rows, so in one page, and the wave takes its address from the lane
+    // that looked it up: a resource over the 16 rows, of no bytes in a hole.
+    int at_row[BIG ? kPer : 1];
+    if constexpr (BIG) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+            at_row[j] = chunk_col(j) < n_ch ? chunk_row(j) % 16 * row_bytes + 8 * esz * chunk_col(j) : 0x7FFFFFFF - 15;
+    }
     int ent = 0;
     uint64_t there = 0;  // the tile's positions in the block's sight and in the pool
     Raw K, V;
@@ -195,17 +251,32 @@ __global__ __launch_bounds__(256 * G) void attn_paged_block_kernel(PagedParams p
         const bool ok = pos < pos_end && (unsigned)ent < (unsigned)p.c.n_pages;
         there = __builtin_amdgcn_ballot_w64(ok);
         const int slot = ok ? (ent << p.c.shift) + (pos & ((1 << p.c.shift) - 1)) : 0;
-        const int64_t off = ok ? slot_bytes(p.c, slot, row_bytes) : -1;
+        if constexpr (BIG) {
 #pragma unroll
-        for (int j = 0; j < NC; ++j) {
-            const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)off, chunk_row(j), 64);
-            const int hi = __shfl((int)(off >> 32), chunk_row(j), 64);
-            const int64_t at = (((int64_t)hi << 32) | lo) + 8 * esz * chunk_col(j);
-            K.c[j] = Chunk{};
-            V.c[j] = Chunk{};
-            if (hi >= 0 && chunk_col(j) < n_ch) {
-                K.c[j] = *reinterpret_cast<const Chunk *>(kb + at);
-                V.c[j] = *reinterpret_cast<const Chunk *>(vb + at);
+            for (int j = 0; j < NC; ++j) {
+                const int g = (64 * w + 256 * j) / (16 * CH);
+                const int page = __builtin_amdgcn_readlane(ent, 16 * g), p0 = t * kTile + 16 * g;
+                const bool in_pool = p0 < pos_end && (unsigned)page < (unsigned)p.c.n_pages;
+                const int64_t at = in_pool ? (int64_t)page * p.c.page_bytes + (p0 & ((1 << p.c.shift) - 1)) * row_bytes : 0;
+                const int bytes = in_pool ? 16 * row_bytes - kvh * hd * esz : 0;
+                const auto kr = make_rsrc(kb + at, bytes), vr = make_rsrc(vb + at, bytes);
+                const int place = kEven ? at_row[0] : at_row[j % kPer], down = kEven ? j * kRows % 16 * row_bytes : 0;
+                K.c[j] = load_chunk<Chunk>(kr, place, down);
+                V.c[j] = load_chunk<Chunk>(vr, place, down);
+            }
+        } else {
+            const int64_t off = ok ? slot_bytes(p.c, slot, row_bytes) : -1;
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)off, chunk_row(j), 64);
+                const int hi = __shfl((int)(off >> 32), chunk_row(j), 64);
+                const int64_t at = (((int64_t)hi << 32) | lo) + 8 * esz * chunk_col(j);
+                K.c[j] = Chunk{};
+                V.c[j] = Chunk{};
+                if (hi >= 0 && chunk_col(j) < n_ch) {
+                    K.c[j] = *reinterpret_cast<const Chunk *>(kb + at);
+                    V.c[j] = *reinterpret_cast<const Chunk *>(vb + at);
+                }
             }
         }
         if (I8) {
@@ -546,7 +617,7 @@ __global__ __launch_bounds__(256) void attn_paged_block_combine_kernel(PagedPara
     if (t < span.row0 || row >= n_rows || n_rows <= p.rows_limit) return;
     const int blk_last = min(n_rows, (row / kPagedBlock + 1) * kPagedBlock) - 1;
     const int tiles = block_tiles(min(span.pos0 + blk_last / p.group + 1, position_limit(p.b, p.c)));
-    const int chunk_tiles = p.chunk / kTile, n_c = (tiles + chunk_tiles - 1) / chunk_tiles;
+    const int ct = *p.chunk_tiles, n_c = min((tiles + ct - 1) / ct, p.n_chunks);
     if (n_c <= 1) return;  // written already
     const int64_t at = id * p.n_chunks;
     const int c = min(lane, n_c - 1);
@@ -556,13 +627,17 @@ __global__ __launch_bounds__(256) void attn_paged_block_combine_kernel(PagedPara
     const float L = butterfly_sum<64>(e * lc);
     float acc[NE] = {};
     const float *src = p.part + at * HD;
-    for (int i = 0; i < n_c; ++i) {
-        const float ei = __shfl(e, i, 64);
-        if (ei == 0.0f) continue;
+    for (int i = 0; i < n_c; i += 4) {  // (four chunks' loads at once)
+        float x[4][NE];
 #pragma unroll
-        for (int k = 0; k < NE; ++k) {
-            const int d = lane + 64 * k;
-            if (d < HD) acc[k] += ei * src[(int64_t)i * HD + d];
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int k = 0; k < NE; ++k) x[j][k] = src[(int64_t)min(i + j, n_c - 1) * HD + min(lane + 64 * k, HD - 1)];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float ei = __shfl(e, (i + j) & 63, 64);  // (0 past the last chunk)
+#pragma unroll
+            for (int k = 0; k < NE; ++k) acc[k] += ei == 0.0f ? 0.0f : ei * x[j][k];
         }
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
@@ -576,7 +651,14 @@ __global__ __launch_bounds__(256) void attn_paged_block_combine_kernel(PagedPara
 constexpr int kBigDim = 128;  // larger heads: one wave group, 512 registers a wave
 int pad_dim(int hd) { return hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : 256; }
 
-template <int HD, bool I8>
+// Blocks of the batch at most: every sequence's rows past the limit, each with a
+// last block of its own.
+int64_t most_blocks(const PagedParams &p) {
+    const int64_t rows = (int64_t)p.b.n_tokens * p.group;
+    return rows / kPagedBlock + std::min<int64_t>(p.b.n_seqs, rows / (p.rows_limit + 1));
+}
+
+template <int HD, bool I8, bool BIG>
 hipError_t launch_t(const PagedParams &p, hipStream_t st) {
     constexpr int G = HD > kBigDim ? 1 : 2;
     constexpr int lds = block_lds<HD, G>();
@@ -587,57 +669,55 @@ hipError_t launch_t(const PagedParams &p, hipStream_t st) {
     if (e != hipSuccess) return e;
     const uint64_t bit = 1ull << (dev & 63);
     if (!(raised.load(std::memory_order_acquire) & bit)) {
-        e = hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_paged_block_kernel<HD, I8, G>),
+        e = hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_paged_block_kernel<HD, I8, G, BIG>),
                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
         raised.fetch_or(bit, std::memory_order_acq_rel);
     }
-    const int64_t grid = (int64_t)p.n_blocks * p.c.n_kv * p.n_chunks;
+    const int64_t grid = (p.n_chunks > 1 ? std::max<int64_t>(p.max_units, most_blocks(p)) : most_blocks(p)) * p.c.n_kv;
     if (grid > 0x3FFFFF) return hipErrorInvalidValue;
-    attn_paged_block_kernel<HD, I8, G><<<(unsigned)grid, 256 * G, lds, st>>>(p);
+    attn_paged_block_kernel<HD, I8, G, BIG><<<(unsigned)grid, 256 * G, lds, st>>>(p);
     if (p.n_chunks > 1)
         attn_paged_block_combine_kernel<HD>
             <<<(unsigned)(((int64_t)p.b.n_tokens * p.n_heads + 3) / 4), 256, 0, st>>>(p);
     return hipGetLastError();
 }
 
-// Blocks of the batch at most: every sequence's rows past the limit, each with a
-// last block of its own.
-int64_t most_blocks(const PagedParams &p) {
-    const int64_t rows = (int64_t)p.b.n_tokens * p.group;
-    return rows / kPagedBlock + std::min<int64_t>(p.b.n_seqs, rows / (p.rows_limit + 1));
+template <int HD>
+hipError_t launch_hd(const PagedParams &p, int i8, hipStream_t st) {
+    const bool big = p.c.shift >= 4;
+    if (i8) return big ? launch_t<HD, true, true>(p, st) : launch_t<HD, true, false>(p, st);
+    return big ? launch_t<HD, false, true>(p, st) : launch_t<HD, false, false>(p, st);
 }
 
 }  // namespace
 
 PagedBlockPlan plan_paged_blocks(const PagedParams &p, size_t room) {
     const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
-    const int pad = pad_dim(p.c.hd), G = pad > kBigDim ? 1 : 2;
     const int64_t len = std::max<int64_t>(1, std::min<int64_t>(p.b.max_len, (int64_t)p.c.width << p.c.shift));
     const int tiles = (int)((len + kTile - 1) / kTile);
-    const size_t per = (size_t)p.b.n_tokens * p.n_heads * (pad + 2) * 4;
-    const int64_t units = most_blocks(p) * p.c.n_kv;
-    int64_t want = std::max<int64_t>(1, std::min<int64_t>({(cus + units - 1) / units, kMaxChunks, (int64_t)(room / per)}));
+    const size_t per = (size_t)p.b.n_tokens * p.n_heads * (pad_dim(p.c.hd) + 2) * 4;
+    const int64_t units = std::max(1, cus / p.c.n_kv);
+    int64_t want = 1;
+    if ((int64_t)p.b.n_tokens * p.group / kPagedBlock < units && p.b.n_seqs <= kSplitSeqs && room > 256)
+        want = std::max<int64_t>(1, std::min<int64_t>({tiles / kLeastTiles, kMaxChunks, (int64_t)((room - 256) / per)}));
     if (tuning().attn_split) want = std::min<int64_t>(want, tuning().attn_split);
-    int ct = (int)((tiles + want - 1) / want);
-    ct = (ct + G - 1) / G * G;
-    const int n_c = (tiles + ct - 1) / ct;
-    return PagedBlockPlan{ct * kTile, n_c, n_c > 1 ? per * n_c : 0};
+    return PagedBlockPlan{(int)units, (int)want, tiles, want > 1 ? per * want + 256 : 0};
 }
 
 hipError_t launch_paged_blocks(PagedParams p, const PagedBlockPlan &plan, float *ws, int i8, hipStream_t st) {
-    p.chunk = plan.chunk;
+    p.max_units = plan.units;
     p.n_chunks = plan.n_chunks;
-    const int64_t blocks = most_blocks(p);
-    if (blocks > 0x3FFFFF) return hipErrorInvalidValue;
-    p.n_blocks = (int)blocks;
-    p.part = ws;
-    p.stats = ws + (size_t)p.b.n_tokens * p.n_heads * p.n_chunks * pad_dim(p.c.hd);
+    p.most_tiles = plan.tiles;
+    p.min_tiles = std::max((plan.tiles + plan.n_chunks - 1) / plan.n_chunks, kLeastTiles);
+    p.chunk_tiles = reinterpret_cast<int *>(ws);
+    p.part = ws ? ws + 64 : nullptr;
+    p.stats = ws ? p.part + (size_t)p.b.n_tokens * p.n_heads * p.n_chunks * pad_dim(p.c.hd) : nullptr;
     switch (pad_dim(p.c.hd)) {
-        case 64: return i8 ? launch_t<64, true>(p, st) : launch_t<64, false>(p, st);
-        case 96: return i8 ? launch_t<96, true>(p, st) : launch_t<96, false>(p, st);
-        case 128: return i8 ? launch_t<128, true>(p, st) : launch_t<128, false>(p, st);
-        default: return i8 ? launch_t<256, true>(p, st) : launch_t<256, false>(p, st);
+        case 64: return launch_hd<64>(p, i8, st);
+        case 96: return launch_hd<96>(p, i8, st);
+        case 128: return launch_hd<128>(p, i8, st);
+        default: return launch_hd<256>(p, i8, st);
     }
 }
 
