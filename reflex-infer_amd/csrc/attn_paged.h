@@ -19,11 +19,13 @@ struct PagedParams {
     float sl2;            // scale * log2(e)
     int rows_limit;       // sequences of at most this many rows are the 16-row kernel's (0: none)
     int rows_blk;         // 16 rows: rows of a sequence that the partials hold
-    int chunk;            // 16 rows: positions per chunk (a multiple of 64)
-    int n_chunks;         // chunks per 16 rows; per block at most
-    int max_units;        // 128 rows: blocks' chunks of the batch at most, per KV head
-    int most_tiles, min_tiles;  // tiles of a block, and of a chunk, at most and at least
-    int *chunk_tiles;     // tiles of a chunk, left for the combine
+    int n_chunks;         // chunks of a sequence's or block's positions at most
+    int max_units;        // chunks of the batch per KV head, about (16 rows) or at most
+    int min_tiles;        // steps (16 rows) or tiles of a chunk at least
+    int *firsts;          // 16 rows: a sequence's first slot and its chunks, for the combine
+    int chunk;            // 16 rows: positions per chunk where the host cuts them
+    int most_tiles;       // 128 rows: tiles of a block at most
+    int *chunk_tiles;     // 128 rows: tiles of a chunk, left for the combine
 };
 
 // Query rows of a workgroup of the smaller and of the larger kernel.

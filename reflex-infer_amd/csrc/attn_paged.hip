@@ -26,6 +26,7 @@ namespace {
 constexpr int kStep = 128;      // positions per step of a workgroup
 constexpr int kNoStep = 1 << 22;  // past every position (2^24 at most): its loads are past the end
 constexpr int kMaxChunks = 64;  // chunks of positions per sequence
+constexpr int kSeqs = 256;      // sequences whose chunks a workgroup counts itself
 
 typedef const float __attribute__((address_space(1))) *GlobalFloat;
 __device__ const float g_one = 1.0f;  // int8 caches without scales: read with stride 0
@@ -37,6 +38,97 @@ __device__ __forceinline__ float log2_scale(float vs) {
 // Waves per SIMD that the registers are cut to: what is in flight is what counts, and
 // an int8 step holds half the bytes of an fp16 one.
 constexpr int rows_waves(int hd, bool i8) { return hd > 128 ? 1 : hd == 64 ? 4 : i8 ? 3 : 2; }
+
+// Steps of the walk over a sequence (0: not this kernel's; one where its tokens see
+// nothing, to write their zeros).
+__device__ __forceinline__ int seq_steps(const PagedParams &p, const SeqSpan &span) {
+    const int n = min(span.n, p.b.max_new);
+    if (n == 0 || n * p.group > kPagedRows) return 0;
+    return (max(min(span.pos0 + n, position_limit(p.b, p.c)), 1) + kStep - 1) / kStep;
+}
+
+// The chunks of the batch, sequence after sequence: of at most so many steps that there
+// are about p.max_units, a sequence's about equally long.  Lane l holds the sequences
+// per l, .. per l + per - 1; the same in every wave, from the same sums.
+constexpr int kPer = kSeqs / 64;
+struct RowsUnits {
+    int per;
+    SeqSpan span[kPer];
+    int steps[kPer], chunks[kPer];
+    int upto;  // chunks up to the lane's last
+};
+__device__ __forceinline__ RowsUnits rows_units(const PagedParams &p) {
+    RowsUnits u{};
+    const int lane = threadIdx.x & 63;
+    u.per = (p.b.n_seqs + 63) >> 6;
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (i < u.per) {  // uniform
+            const int s = lane * u.per + i;
+            u.span[i] = seq_span(p.b, min(s, p.b.n_seqs - 1));
+            u.steps[i] = s < p.b.n_seqs ? seq_steps(p, u.span[i]) : 0;
+            all += u.steps[i];
+        }
+    all = __builtin_amdgcn_readlane(wave_prefix(all), 63);
+    const int most = max(p.min_tiles, (all + p.max_units - 1) / p.max_units);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (i < u.per) {
+            u.chunks[i] = (u.steps[i] + most - 1) / most;
+            u.upto += u.chunks[i];
+        }
+    u.upto = wave_prefix(u.upto);
+    return u;
+}
+
+// A chunk of a sequence's steps.  With more than kSeqs sequences the chunks are of
+// p.chunk positions, every sequence with p.n_chunks of them.
+struct RowsUnit {
+    SeqSpan span;
+    int s, c;           // sequence (-1: none), chunk
+    int chunks, chunk;  // chunks of the sequence; positions of each
+    int64_t slot;       // of the chunk's partials
+};
+__device__ __forceinline__ RowsUnit rows_unit(const PagedParams &p, int idx) {
+    RowsUnit r{};
+    r.s = -1;
+    if (p.n_chunks == 1 || p.b.n_seqs > kSeqs) {
+        // (a sequence's chunks on different XCDs)
+        r.c = idx / p.b.n_seqs;
+        if (r.c >= p.n_chunks) return r;
+        const int s = (idx + 3 * r.c) % p.b.n_seqs;
+        r.span = seq_span(p.b, s);
+        r.chunk = p.chunk;
+        r.chunks = (seq_steps(p, r.span) * kStep + p.chunk - 1) / p.chunk;
+        r.slot = (int64_t)s * p.n_chunks + r.c;
+        if (r.c < r.chunks) r.s = s;
+        return r;
+    }
+    const RowsUnits u = rows_units(p);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(u.upto > idx);
+    if (past == 0) return r;
+    const int at = __builtin_ctzll(past);
+    int c = idx - __builtin_amdgcn_readlane(u.upto, at);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) c += __builtin_amdgcn_readlane(u.chunks[i], at);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int chunks = __builtin_amdgcn_readlane(u.chunks[i], at);
+        if (c >= 0 && c < chunks) {
+            const int n = __builtin_amdgcn_readlane(u.steps[i], at);
+            r.span = SeqSpan{__builtin_amdgcn_readlane(u.span[i].row0, at), __builtin_amdgcn_readlane(u.span[i].n, at),
+                             __builtin_amdgcn_readlane(u.span[i].pos0, at)};
+            r.s = at * u.per + i;
+            r.c = c;
+            r.chunks = chunks;
+            r.chunk = __builtin_amdgcn_readfirstlane((n + chunks - 1) / chunks) * kStep;
+        }
+        c -= chunks;
+    }
+    r.slot = idx;
+    return r;
+}
 
 // Wave w takes positions 32 w .. + 31 of every 128-position step of the chunk with
 // its own online softmax; the four waves merge at the end.  Per step, lane l =
@@ -79,15 +171,17 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
     uint16_t *const vl = reinterpret_cast<uint16_t *>(smem) + w * 32 * VROW;
     // The KV heads of a sequence's chunk go to one XCD (workgroups are dealt to the eight in
     // turn): they read the same pages and scales.  A sequence's chunks go to different ones.
-    const int x8 = blockIdx.x / 8, kvh = x8 % p.c.n_kv, u = x8 / p.c.n_kv * 8 + blockIdx.x % 8;
-    const int c = u / p.b.n_seqs, s = (u + 3 * c) % p.b.n_seqs;
-    if (c >= p.n_chunks) return;
-    const int beg = c * p.chunk;
+    const int x8 = blockIdx.x / 8, kvh = x8 % p.c.n_kv;
+    const RowsUnit unit = rows_unit(p, x8 / p.c.n_kv * 8 + blockIdx.x % 8);
+    const int s = unit.s, c = unit.c, beg = c * unit.chunk;
+    if (s < 0) return;  // uniform
+    if (p.n_chunks > 1 && c == 0 && kvh == 0 && tid == 0) {
+        p.firsts[2 * s] = (int)unit.slot;
+        p.firsts[2 * s + 1] = unit.chunks;
+    }
     const int limit = position_limit(p.b, p.c);
-    if (beg >= limit && c > 0) return;
 
-    // Table entries of the first steps, before the sequence's length is known.  (No load
-    // of the walk stands in a branch: the compiler would wait for all of them.)
+    // (No load of the walk stands in a branch: the compiler would wait for all of them.)
     const bool has_table = p.c.table != nullptr && limit > 0;
     const int32_t *const table = has_table ? p.c.table + (int64_t)s * p.c.width : p.b.lens;
     const int p_lane = beg + 32 * w + (lane & 31);  // the lane's position of the first step
@@ -100,11 +194,10 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
     // lane's position's, one step ahead
     auto entries = [&](int j) { return entry(beg + 32 * w + kStep * (j + (lane >> 1)) + 16 * (lane & 1)); };
     int ent = BIG ? entries(0) : entry(p_lane), ent_next = BIG ? 0 : entry(p_lane + kStep);
-    const SeqSpan span = seq_span(p.b, s);
+    const SeqSpan span = unit.span;
     const int rows = min(span.n, p.b.max_new) * p.group;
-    if (rows == 0 || rows > kPagedRows) return;
     const int end_seq = min(span.pos0 + (rows - 1) / p.group + 1, limit);
-    const int end = min(end_seq, beg + p.chunk);
+    const int end = min(end_seq, beg + unit.chunk);
     const int row = min(r, rows - 1);  // (columns past the last row repeat it)
     const int tok = row / p.group, head = kvh * p.group + row % p.group;
     const bool row_ok = r < rows;
@@ -398,9 +491,9 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
         L += mg[v][NM - 1][lane] * cw[v];
     }
     if (!row_ok) return;
-    const bool whole = end_seq <= p.chunk;  // one chunk: no partials
+    const bool whole = unit.chunks <= 1;  // one chunk: no partials
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    const int64_t at = ((int64_t)(s * p.c.n_kv + kvh) * p.n_chunks + c) * p.rows_blk + r;
+    const int64_t at = (unit.slot * p.c.n_kv + kvh) * p.rows_blk + r;
 #pragma unroll
     for (int dt = w; dt < DT; dt += 4) {
         f32x4 ov;
@@ -423,96 +516,105 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
     }
 }
 
-// out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over a row's chunks in a fixed
-// order.  Workgroup: a row and 64 of its dims; wave v sums the chunks v, v + 4, ..,
-// the waves add up in order.
+// out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over a row's chunks in order.  A
+// wave takes a row: a lane's chunk for the weights, then a lane's dims.
 template <int HD>
 __global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedParams p) {
-    constexpr int NS = (HD + 63) / 64;
-    __shared__ float part[4][64];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int d = blockIdx.x % NS * 64 + lane;
-    const int r = blockIdx.x / NS % p.rows_blk, u = blockIdx.x / NS / p.rows_blk;
-    const int kvh = u % p.c.n_kv, s = u / p.c.n_kv;
-    const int64_t at = (int64_t)u * p.n_chunks * p.rows_blk + r;
-    const float *st = p.stats + 2 * at, *src = p.part + at * HD + min(d, HD - 1);
-    const int64_t step = p.rows_blk;
-    // (the first loads before the sequence's length: what is past it is not used)
-    const int cl = min(lane, p.n_chunks - 1);
-    float mc = st[2 * cl * step], lc = st[2 * cl * step + 1];
-    constexpr int U = 4;
-    float x[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) x[i] = src[(int64_t)min(w + 4 * i, p.n_chunks - 1) * step * HD];
+    constexpr int VE = HD > 128 ? 4 : HD > 64 ? 2 : 1, U = 8;
+    typedef float Piece __attribute__((ext_vector_type(VE)));
+    const int lane = threadIdx.x & 63, r = 4 * blockIdx.y + (threadIdx.x >> 6);
+    const int kvh = blockIdx.x % p.c.n_kv, s = blockIdx.x / p.c.n_kv;
     const SeqSpan span = seq_span(p.b, s);
+    const int first = p.firsts[2 * s], n_c = p.firsts[2 * s + 1];
     const int rows = min(span.n, p.b.max_new) * p.group;
-    if (r >= rows || rows > kPagedRows) return;  // uniform
-    const int end = min(span.pos0 + (rows - 1) / p.group + 1, position_limit(p.b, p.c));
-    const int n_c = (max(end, 0) + p.chunk - 1) / p.chunk;
-    if (n_c <= 1) return;  // written already
-    if (lane >= n_c) {
-        mc = -INFINITY;
-        lc = 0.0f;
-    }
-    const float M = butterfly_max<64>(mc);
-    const float e = M != -INFINITY && lane < n_c ? __builtin_amdgcn_exp2f(mc - M) : 0.0f;
-    const float L = butterfly_sum<64>(e * lc);
-    float acc = 0.0f;
-    for (int c0 = 0; c0 < n_c; c0 += 4 * U) {
+    if (r >= rows || rows > kPagedRows || n_c <= 1 || n_c > p.n_chunks) return;  // not this kernel's, or written already
+    const int64_t at = ((int64_t)first * p.c.n_kv + kvh) * p.rows_blk + r, step = (int64_t)p.c.n_kv * p.rows_blk;
+    const float *st = p.stats + 2 * (at + min(lane, n_c - 1) * step);
+    const float mc = st[0], lc = st[1];
+    const int d = min(lane * VE, HD - VE);
+    const float *src = p.part + at * HD + d;
+    Piece acc{};
+    float e = 0.0f, L = 0.0f;
+    for (int c0 = 0; c0 < n_c; c0 += U) {
+        Piece x[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) x[i] = *reinterpret_cast<const Piece *>(src + min(c0 + i, n_c - 1) * step * HD);
+        if (c0 == 0) {
+            const float M = butterfly_max<64>(mc);
+            e = M != -INFINITY && lane < n_c ? __builtin_amdgcn_exp2f(mc - M) : 0.0f;
+            L = butterfly_sum<64>(e * lc);
+        }
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int c = c0 + w + 4 * i;
-            const float ec = __shfl(e, min(c, 63), 64);
-            if (c < n_c && ec != 0.0f) acc += ec * x[i];
+            const float ec = __builtin_bit_cast(
+                float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, e), min(c0 + i, 63)));
+            if (c0 + i < n_c && ec != 0.0f) acc += ec * x[i];  // uniform
         }
-        if (c0 + 4 * U < n_c)
-#pragma unroll
-            for (int i = 0; i < U; ++i) x[i] = src[(int64_t)min(c0 + 4 * U + w + 4 * i, n_c - 1) * step * HD];
     }
-    part[w][lane] = acc;
-    __syncthreads();
-    if (w == 0 && d < p.c.hd) {
-        const float sum = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
-        const int tok = r / p.group, head = kvh * p.group + r % p.group;
-        p.out[((int64_t)(span.row0 + tok) * p.n_heads + head) * p.c.hd + d] =
-            f32_to_f16_bits(L == 0.0f ? 0.0f : sum * (1.0f / L));
+    if (lane * VE >= p.c.hd) return;
+    const int tok = r / p.group, head = kvh * p.group + r % p.group;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    uint16_t *out = p.out + ((int64_t)(span.row0 + tok) * p.n_heads + head) * p.c.hd + d;
+    if constexpr (VE == 1) {
+        *out = f32_to_f16_bits(acc[0] * inv);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VE; i += 2)
+            *reinterpret_cast<uint32_t *>(out + i) = pack2<RXQ4_DTYPE_F16>(acc[i] * inv, acc[i + 1] * inv);
     }
 }
 
-// The 16-row launch's split: its partials within `room` bytes.
+// The 16-row launch's chunks: their partials within `room` bytes.  Some six chunks of
+// an fp16 and twelve of an int8 cache a CU (three to four of what runs at a time, for
+// sequences of any lengths): 64 sequences of 64 to 8000 positions, 8 heads, fp16, 5 / 6
+// / 8 / 12 a CU 98.7 / 91.7 / 94.6 / 103 us; 16 of 20000 to 40000, int8, 6 / 8 / 12 / 16
+// 213 / 208 / 202 / 204.  Past kSeqs sequences there is little to cut: the host's chunks.
 struct RowsPlan {
-    int64_t units;
+    int64_t slots;  // chunks of the batch at most, per KV head
     size_t bytes;
 };
-RowsPlan plan_rows(PagedParams &p, size_t room) {
+RowsPlan plan_rows(PagedParams &p, int i8, size_t room) {
     const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
     const int pad = p.c.hd <= 64 ? 64 : p.c.hd <= 96 ? 96 : p.c.hd <= 128 ? 128 : 256;
     p.rows_blk = (int)std::min<int64_t>((int64_t)std::min(p.b.max_new, p.b.n_tokens) * p.group, kPagedRows);
-    const int64_t units = (int64_t)p.b.n_seqs * p.c.n_kv;
     const int64_t len = std::max<int64_t>(1, std::min<int64_t>(p.b.max_len, (int64_t)p.c.width << p.c.shift));
-    int64_t want = std::max((4 * cus + units - 1) / units, (len + 1023) / 1024);
-    want = std::min<int64_t>({want, kMaxChunks, (len + 2 * kTile - 1) / (2 * kTile)});
-    const size_t per = (size_t)units * p.rows_blk * (pad + 2) * 4;
-    want = std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)(room / per)));
-    if (tuning().attn_split) want = std::min<int64_t>(want, tuning().attn_split);
-    p.chunk = (int)(((len + want - 1) / want + kStep - 1) / kStep * kStep);
-    p.n_chunks = (int)((len + p.chunk - 1) / p.chunk);
-    return RowsPlan{units, p.n_chunks > 1 ? (per * p.n_chunks + 255) / 256 * 256 : 0};
+    const int64_t steps = (len + kStep - 1) / kStep, n = p.b.n_seqs;
+    const size_t per = (size_t)p.c.n_kv * p.rows_blk * (pad + 2) * 4;  // bytes of a slot
+    room -= std::min<size_t>(room, 8 * n + 256);
+    int64_t most = std::min<int64_t>(steps, kMaxChunks);
+    if (tuning().attn_split) most = std::min<int64_t>(most, tuning().attn_split);
+    const int64_t units = std::min<int64_t>((i8 ? 12 : 6) * cus / p.c.n_kv, (int64_t)(room / per) - n);
+    if (n > kSeqs) {
+        most = std::min<int64_t>({most, std::max((4 * cus + n * p.c.n_kv - 1) / (n * p.c.n_kv), (len + 1023) / 1024), (int64_t)(room / per) / n});
+    } else if (units < 1) {
+        most = 1;
+    }
+    most = std::max<int64_t>(most, 1);
+    const int64_t least = (steps + most - 1) / most;  // steps of a chunk
+    p.min_tiles = (int)least;
+    p.max_units = (int)std::max<int64_t>(units, 1);
+    p.chunk = (int)least * kStep;
+    p.n_chunks = (int)((steps + least - 1) / least);
+    const int64_t slots = p.n_chunks == 1 || n > kSeqs ? n * p.n_chunks : std::min<int64_t>(units + n, n * p.n_chunks);
+    return RowsPlan{slots, p.n_chunks > 1 ? (per * slots + 8 * n + 255) / 256 * 256 : 0};
 }
 
 template <int HD>
 hipError_t launch_rows(PagedParams &p, const RowsPlan &plan, float *ws, int i8, hipStream_t st) {
-    if (plan.units * p.n_chunks > 0x7FFFFF) return hipErrorInvalidValue;
+    const int64_t grid = (plan.slots + 7) / 8 * 8 * p.c.n_kv;
+    if (grid > 0x7FFFFF) return hipErrorInvalidValue;
     p.part = ws;
-    p.stats = ws + (size_t)plan.units * p.n_chunks * p.rows_blk * HD;
-    const unsigned grid = (unsigned)(((int64_t)p.b.n_seqs * p.n_chunks + 7) / 8 * 8 * p.c.n_kv);
+    p.stats = ws + (size_t)plan.slots * p.c.n_kv * p.rows_blk * HD;
+    p.firsts = reinterpret_cast<int *>(p.stats + (size_t)plan.slots * p.c.n_kv * p.rows_blk * 2);
     const bool big = p.c.shift >= 4;
-    if (i8 && big) attn_paged_rows_kernel<HD, true, true><<<grid, 256, 0, st>>>(p);
-    else if (i8) attn_paged_rows_kernel<HD, true, false><<<grid, 256, 0, st>>>(p);
-    else if (big) attn_paged_rows_kernel<HD, false, true><<<grid, 256, 0, st>>>(p);
-    else attn_paged_rows_kernel<HD, false, false><<<grid, 256, 0, st>>>(p);
-    if (p.n_chunks > 1)
-        attn_paged_combine_kernel<HD><<<(unsigned)(plan.units * p.rows_blk * ((HD + 63) / 64)), 256, 0, st>>>(p);
+    if (i8 && big) attn_paged_rows_kernel<HD, true, true><<<(unsigned)grid, 256, 0, st>>>(p);
+    else if (i8) attn_paged_rows_kernel<HD, true, false><<<(unsigned)grid, 256, 0, st>>>(p);
+    else if (big) attn_paged_rows_kernel<HD, false, true><<<(unsigned)grid, 256, 0, st>>>(p);
+    else attn_paged_rows_kernel<HD, false, false><<<(unsigned)grid, 256, 0, st>>>(p);
+    if (p.n_chunks > 1) {
+        const dim3 rows((unsigned)(p.b.n_seqs * p.c.n_kv), (unsigned)(p.rows_blk + 3) / 4);
+        attn_paged_combine_kernel<HD><<<rows, 256, 0, st>>>(p);
+    }
     return hipGetLastError();
 }
 
@@ -538,7 +640,7 @@ hipError_t launch_attention_paged(uint16_t *out, const uint16_t *q, int n_heads,
     PagedParams pr = p;
     RowsPlan rp{};
     PagedBlockPlan bp{};
-    if (rows) rp = plan_rows(pr, (blocks ? kWorkspaceBytes / 2 : kWorkspaceBytes) - 256);
+    if (rows) rp = plan_rows(pr, kv_int8, (blocks ? kWorkspaceBytes / 2 : kWorkspaceBytes) - 256);
     if (blocks) bp = plan_paged_blocks(p, kWorkspaceBytes - rp.bytes);
     float *ws = nullptr;
     if (rp.bytes + bp.bytes > 0) {

@@ -31,6 +31,21 @@ __device__ __forceinline__ SeqSpan seq_span(const SeqBatch &b, int s) {
     return seq_span(b, b.starts[s], b.starts[s + 1], b.lens[s]);
 }
 
+// x summed over the lanes up to this one, on the VALU: shifts within rows of 16
+// lanes, then each row's last lane added to the rows behind it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add_from(int x) {
+    return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_prefix(int x) {
+    x = dpp_add_from<0x111, 0xF>(x);  // row_shr:1
+    x = dpp_add_from<0x112, 0xF>(x);
+    x = dpp_add_from<0x114, 0xF>(x);
+    x = dpp_add_from<0x118, 0xF>(x);
+    x = dpp_add_from<0x142, 0xA>(x);  // row_bcast:15 into rows 1 and 3
+    return dpp_add_from<0x143, 0xC>(x);  // row_bcast:31 into rows 2 and 3
+}
+
 // The sequence that row t belongs to (n_seqs: none) and its rows, the same for a
 // whole wave: the number of sequences that end at or before t.  A lane loads all
 // of a sequence at once: one round trip to memory for up to 64 sequences.
