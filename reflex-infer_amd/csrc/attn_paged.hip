@@ -71,11 +71,12 @@ __device__ __forceinline__ RowsUnits rows_units(const PagedParams &p) {
             all += u.steps[i];
         }
     all = __builtin_amdgcn_readlane(wave_prefix(all), 63);
-    const int most = max(p.min_tiles, (all + p.max_units - 1) / p.max_units);
+    // (a few short sequences: one step a chunk, no division)
+    const int most = all <= p.max_units ? p.min_tiles : max(p.min_tiles, (all + p.max_units - 1) / p.max_units);
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
         if (i < u.per) {
-            u.chunks[i] = (u.steps[i] + most - 1) / most;
+            u.chunks[i] = most == 1 ? u.steps[i] : (u.steps[i] + most - 1) / most;
             u.upto += u.chunks[i];
         }
     u.upto = wave_prefix(u.upto);
@@ -122,7 +123,7 @@ __device__ __forceinline__ RowsUnit rows_unit(const PagedParams &p, int idx) {
             r.s = at * u.per + i;
             r.c = c;
             r.chunks = chunks;
-            r.chunk = __builtin_amdgcn_readfirstlane((n + chunks - 1) / chunks) * kStep;
+            r.chunk = n == chunks ? kStep : __builtin_amdgcn_readfirstlane((n + chunks - 1) / chunks) * kStep;
         }
         c -= chunks;
     }
