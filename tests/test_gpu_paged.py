@@ -282,3 +282,46 @@ def test_captured_and_replayed_with_other_lengths(new, lens):
         check(p, out, 0.09)
         eager = attend(p, 0.09, cache, batch)
         assert torch.equal(eager, out)
+
+
+@pytest.mark.parametrize("n,heads,page,int8", [(64, (8, 2, 64), 16, False), (65, (8, 2, 64), 4, True),
+                                               (256, (4, 2, 64), 16, True), (257, (4, 2, 64), 16, False),
+                                               (700, (4, 1, 64), 1, False)])
+def test_many_sequences_decoding(n, heads, page, int8):
+    """A lane's one sequence, several, and more than a workgroup counts; some of no
+    new tokens, some of no positions."""
+    new = [0 if i % 13 == 5 else 1 + i % 3 for i in range(n)]
+    lens = [0 if i % 31 == 7 else 1 + (i * 97) % 400 + (1500 if i % 50 == 0 else 0) for i in range(n)]
+    p = ref.Paged(35, *heads, page, new, lens, int8)
+    check(p, attend(p, 0.125), 0.125)
+
+
+@pytest.mark.parametrize("n", [65, 1024, 1030])
+def test_many_sequences_of_chunks(n):
+    """Blocks found among more sequences than lanes, and among more than are cut."""
+    new = [0 if i % 13 == 5 else 1 + i % 29 for i in range(n)]
+    lens = [m + (i * 37) % 90 for i, m in enumerate(new)]
+    lens[3] += 1500
+    p = ref.Paged(36, 2, 1, 16, 16, new, lens)
+    check(p, attend(p, 0.25), 0.25)
+
+
+@pytest.mark.parametrize("new,int8", [([1, 1, 1], False), ([1, 1, 1], True), ([1, 40, 2], False), ([90, 30, 20], True)])
+def test_limits_of_a_whole_context(new, int8):
+    """max_len and the table at a capacity far above the lengths, as for a captured
+    step: the chunks follow the lengths."""
+    p = ref.Paged(37, 16, 2, 128, 16, new, [9000] * 3, int8)
+    for lens in ([9000, 900, 90], [130, 129, 95], [200, 8000, 3000]):
+        p.lens, p.seq_lens = lens, torch.tensor(lens, dtype=torch.int32)
+        check(p, attend(p, 0.09, max_len=9000), 0.09)
+
+
+@pytest.mark.parametrize("hd", [64, 80, 96, 128, 200, 256])
+@pytest.mark.parametrize("new,length", [(1, 700), (40, 700)])
+def test_pages_of_sixteen_or_more_with_holes(hd, new, length):
+    """The page of a wave's 16 rows from the lane that looked it up: every head
+    width, pages that end inside a tile, holes between them, K and V apart."""
+    p = ref.Paged(38, 4, 2, hd, 16, [new], [length], holes=[(0, 1), (0, 2), (0, 9), (0, 42)], apart=True)
+    check(p, attend(p, 0.125), 0.125)
+    p = ref.Paged(39, 4, 2, hd - hd % 16, 32, [new], [length], True, holes=[(0, 3), (0, 20)])
+    check(p, attend(p, 0.0625), 0.0625)
