@@ -364,17 +364,17 @@ struct Picker {
     // f(index in the row, pattern) for the gathered logits.
     template <class F>
     __device__ __forceinline__ void each(F f) const {
-        load([&](int, uint32_t index, uint32_t key) { f(index, key); });
+        load<4>([&](int, uint32_t index, uint32_t key) { f(index, key); });
     }
-    // Four of a thread at a time.
-    template <class F>
+    // Q of a thread at a time.
+    template <int Q, class F>
     __device__ __forceinline__ void load(F f) const {
-        for (uint32_t i0 = threadIdx.x; i0 < logits; i0 += 4 * kThreads) {
-            int s[4];
-            uint32_t at[4];
-            float x[4];
+        for (uint32_t i0 = threadIdx.x; i0 < logits; i0 += Q * kThreads) {
+            int s[Q];
+            uint32_t at[Q];
+            float x[Q];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < Q; ++q) {
                 const uint32_t i = min(i0 + q * kThreads, logits - 1);
                 int a = 0, b = p.n_slices - 1;  // the first slice with upto > i
                 while (a < b) {
@@ -386,9 +386,9 @@ struct Picker {
                 at[q] = p.index[((int64_t)r * p.n_slices + a) * p.per + sh.from[a] + (i - (a > 0 ? sh.upto[a - 1] : 0))];
             }
 #pragma unroll
-            for (int q = 0; q < 4; ++q) x[q] = logit(s[q], at[q]);
+            for (int q = 0; q < Q; ++q) x[q] = logit(s[q], at[q]);
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < Q; ++q)
                 if (i0 + q * kThreads < logits) f(q, (uint32_t)(s[q] * p.per) + at[q], order_key(x[q]));
         }
     }
@@ -396,12 +396,17 @@ struct Picker {
     // Sorts the gathered logits with patterns in [lo, hi], `count` <= kWindow of them, into
     // the window.
     __device__ __forceinline__ void window(uint32_t lo, uint32_t hi, uint32_t count, uint32_t rank, u64 before) {
+        window(lo, hi, count, rank, before, [&](auto f) { each(f); });
+    }
+    template <class Each>
+    __device__ __forceinline__ void window(uint32_t lo, uint32_t hi, uint32_t count, uint32_t rank, u64 before,
+                                           Each each_item) {
         const int tid = threadIdx.x;
         __syncthreads();
         if (tid == 0) sh.v[0] = 0;
         sh.item[tid] = ~0ull;
         __syncthreads();
-        each([&](uint32_t index, uint32_t key) {
+        each_item([&](uint32_t index, uint32_t key) {
             if (key < lo || key > hi) return;
             const uint32_t i = atomicAdd(&sh.v[0], 1u);
             if (i < kWindow) sh.item[i] = (u64)~key << 32 | index;
@@ -550,18 +555,26 @@ struct Picker {
         }
         gather(b * kBlock + bin, b * kBlock + bin);
         uint32_t lo = 0, hi = ~0u;
-        // the thread's patterns, where four a thread hold them (0: none)
-        uint32_t key4[4] = {0, 0, 0, 0};
-        const bool held = logits <= 4 * kThreads;
-        if (count > kWindow && held) load([&](int q, uint32_t, uint32_t key) { key4[q] = key; });
-        const auto each_key = [&](auto f) {
+        // the thread's logits, where eight a thread hold them (pattern 0: none)
+        constexpr int kHeld = 8;
+        uint32_t key[kHeld] = {}, index[kHeld];
+        const bool held = count > kWindow && logits <= kHeld * kThreads;
+        if (held)
+            load<kHeld>([&](int q, uint32_t i, uint32_t x) {
+                key[q] = x;
+                index[q] = i;
+            });
+        const auto each_item = [&](auto f) {
             if (held) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (key4[q] != 0) f(key4[q]);
+                for (int q = 0; q < kHeld; ++q)
+                    if (key[q] != 0) f(index[q], key[q]);
             } else {
-                each([&](uint32_t, uint32_t key) { f(key); });
+                each(f);
             }
+        };
+        const auto each_key = [&](auto f) {
+            each_item([&](uint32_t, uint32_t x) { f(x); });
         };
         while (count > kWindow) {  // narrow it
             __syncthreads();
@@ -632,7 +645,7 @@ struct Picker {
             lo = hi - to;
             hi = hi - from;
         }
-        window(lo, hi, count, rank, before);
+        window(lo, hi, count, rank, before, each_item);
         if (by_count) return at_window(min(max((int)(target - (double)rank), 0), n - 1));
         return search(target);
     }
