@@ -102,14 +102,40 @@ __device__ __forceinline__ u64 whole(double w) {
     return __builtin_bit_cast(u64, w + 0x1p52) & 0xFFFFFFFFFFFFFull;
 }
 
-__device__ __forceinline__ u64 shfl_up64(u64 v, int d) {
-    const uint32_t lo = __shfl_up((int)(uint32_t)v, d, 64), hi = __shfl_up((int)(v >> 32), d, 64);
-    return (u64)hi << 32 | lo;
-}
-
 __device__ __forceinline__ u64 shfl_xor64(u64 v, int d) {
     const uint32_t lo = __shfl_xor((int)(uint32_t)v, d, 64), hi = __shfl_xor((int)(v >> 32), d, 64);
     return (u64)hi << 32 | lo;
+}
+
+// Sums over a wave's lanes up to each one, and the largest of its values, on the VALU.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_add_from64(u64 x) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xF, false);
+    return x + ((u64)hi << 32 | lo);
+}
+__device__ __forceinline__ u64 wave_prefix64(u64 x) {
+    x = dpp_add_from64<0x111, 0xF>(x);  // as in wave_prefix
+    x = dpp_add_from64<0x112, 0xF>(x);
+    x = dpp_add_from64<0x114, 0xF>(x);
+    x = dpp_add_from64<0x118, 0xF>(x);
+    x = dpp_add_from64<0x142, 0xA>(x);
+    return dpp_add_from64<0x143, 0xC>(x);
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+    float a, b;
+    swap_rows<32>(__builtin_bit_cast(float, x), a, b);
+    x = max(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+    swap_rows<16>(__builtin_bit_cast(float, x), a, b);
+    x = max(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+    x = dpp_max<0x128>(x);  // row_ror:8, 4, 2, 1
+    x = dpp_max<0x124>(x);
+    x = dpp_max<0x122>(x);
+    return dpp_max<0x121>(x);
 }
 
 // Sums over the T threads up to each one (inclusive); `wave`: T / 64 values of LDS.
@@ -117,11 +143,7 @@ __device__ __forceinline__ u64 shfl_xor64(u64 v, int d) {
 template <int T>
 __device__ __forceinline__ u64 scan64(u64 v, u64 *wave) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 x = shfl_up64(v, d);
-        if (lane >= d) v += x;
-    }
+    v = wave_prefix64(v);
     __syncthreads();
     if (lane == 63) wave[w] = v;
     __syncthreads();
@@ -132,11 +154,7 @@ __device__ __forceinline__ u64 scan64(u64 v, u64 *wave) {
 template <int T>
 __device__ __forceinline__ uint32_t scan32(uint32_t v, u64 *wave) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t x = __shfl_up((int)v, d, 64);
-        if (lane >= d) v += x;
-    }
+    v = (uint32_t)wave_prefix((int)v);
     __syncthreads();
     if (lane == 63) wave[w] = v;
     __syncthreads();
@@ -449,13 +467,7 @@ struct Picker {
                 }
         }
         u64 to = tid < (int)count ? weight(~(uint32_t)(x >> 32)) : 0;
-        if (live) {
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const u64 y = shfl_up64(to, d);
-                if ((tid & 63) >= d) to += y;
-            }
-        }
+        if (live) to = wave_prefix64(to);
         __syncthreads();
         if ((tid & 63) == 63) sh.wave[tid >> 6] = to;
         sh.item[tid] = x;
@@ -511,15 +523,8 @@ struct Picker {
         if (tid < 64) {
             uint32_t c = tid < kBlock ? sh.bin_count[tid] : 0;
             u64 m = tid < kBlock ? sh.bin_mass[tid] : 0;
-#pragma unroll
-            for (int d = 1; d < kBlock; d <<= 1) {
-                const uint32_t x = __shfl_up((int)c, d, 64);
-                const u64 y = shfl_up64(m, d);
-                if (tid >= d) {
-                    c += x;
-                    m += y;
-                }
-            }
+            c = (uint32_t)wave_prefix((int)c);
+            m = wave_prefix64(m);
             if (tid < kBlock) {
                 sh.bin_count[tid] = c;
                 sh.bin_mass[tid] = m;
@@ -594,8 +599,12 @@ struct Picker {
                     most = max(most, key);
                 }
             });
-            atomicMin(&sh.v[1], least);
-            atomicMax(&sh.v[2], most);
+            least = ~wave_max(~least);
+            most = wave_max(most);
+            if ((tid & 63) == 0) {
+                atomicMin(&sh.v[1], least);
+                atomicMax(&sh.v[2], most);
+            }
             __syncthreads();
             lo = sh.v[1];
             hi = sh.v[2];
@@ -605,45 +614,59 @@ struct Picker {
                 nth = fmin(fmax(nth, 0.0), (double)(count - 1));
                 return Found{rank + (uint32_t)nth, before + (u64)nth * w, w, lo, (uint32_t)nth, -1};
             }
-            const u64 range = (u64)(hi - lo) + 1;
+            const int shift = max(24 - (int)__builtin_clz(hi - lo), 0);  // to at most kParts
             each_key([&](uint32_t key) {
                 if (key >= lo && key <= hi) {
-                    const int part = (int)((u64)(hi - key) * kParts / range);
+                    const uint32_t part = (hi - key) >> shift;
                     atomicAdd(&sh.part_count[part], 1u);
                     atomicAdd(&sh.part_mass[part], weight(key));
                 }
             });
             __syncthreads();
-            const uint32_t c = tid < kParts ? sh.part_count[tid] : 0;
-            const u64 m = tid < kParts ? sh.part_mass[tid] : 0;
-            const uint32_t c_to = scan32<kThreads>(c, sh.wave);
-            const u64 m_to = scan64<kThreads>(m, sh.wave);
-            __syncthreads();
-            if (tid == 0) {
-                sh.v[1] = kParts;
-                sh.v[2] = 0;
+            // every wave for itself: its lanes' four parts each
+            const int lane = tid & 63;
+            uint32_t c[kParts / 64], c_to = 0;
+            u64 m[kParts / 64], m_to = 0;
+#pragma unroll
+            for (int i = 0; i < kParts / 64; ++i) {
+                c_to += c[i] = sh.part_count[kParts / 64 * lane + i];
+                m_to += m[i] = sh.part_mass[kParts / 64 * lane + i];
             }
-            __syncthreads();
-            if (c > 0) {
-                if (by_count ? (double)(rank + c_to) > target : (double)(before + m_to) > target) atomicMin(&sh.v[1], (uint32_t)tid);
-                atomicMax(&sh.v[2], (uint32_t)tid);
+            c_to = (uint32_t)wave_prefix((int)c_to);
+            m_to = wave_prefix64(m_to);
+            // from the lane's last part back to its first: the first part past the target, or
+            // the last with a logit
+            uint32_t first = kParts, last_of = 0, c_before = 0, c_last = 0;
+            u64 m_before = 0, m_last = 0;
+#pragma unroll
+            for (int i = kParts / 64 - 1; i >= 0; --i) {
+                if (c[i] > 0) {
+                    if (last_of == 0) {
+                        last_of = kParts / 64 * lane + i + 1;
+                        c_last = c_to - c[i];
+                        m_last = m_to - m[i];
+                    }
+                    if (by_count ? (double)(rank + c_to) > target : (double)(before + m_to) > target) {
+                        first = kParts / 64 * lane + i;
+                        c_before = c_to - c[i];
+                        m_before = m_to - m[i];
+                    }
+                }
+                c_to -= c[i];
+                m_to -= m[i];
             }
-            __syncthreads();
-            const uint32_t part = sh.v[1] < kParts ? sh.v[1] : sh.v[2];
-            if (tid == (int)part) {
-                sh.v[3] = c_to - c;
-                sh.u[0] = m_to - m;
-                sh.v[0] = c;
-            }
-            __syncthreads();
-            rank += sh.v[3];
-            before += sh.u[0];
-            count = sh.v[0];
-            // the patterns of the part: (hi - key) * kParts / range == part
-            const uint32_t from = (uint32_t)(((u64)part * range + kParts - 1) / kParts);
-            const uint32_t to = (uint32_t)((((u64)part + 1) * range + kParts - 1) / kParts - 1);
-            lo = hi - to;
-            hi = hi - from;
+            const u64 past = __builtin_amdgcn_ballot_w64(first < kParts), some = __builtin_amdgcn_ballot_w64(last_of > 0);
+            const int from_lane = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+            const uint32_t part = (uint32_t)__builtin_amdgcn_readlane((int)(past ? first : last_of - 1), from_lane);
+            const u64 mass = past ? m_before : m_last;
+            rank += (uint32_t)__builtin_amdgcn_readlane((int)(past ? c_before : c_last), from_lane);
+            before += (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mass, from_lane) |
+                      (u64)(uint32_t)__builtin_amdgcn_readlane((int)(mass >> 32), from_lane) << 32;
+            count = sh.part_count[part];
+            // the patterns of the part: (hi - key) >> shift == part
+            const uint32_t top_of = hi - (part << shift), width = (1u << shift) - 1;
+            lo = top_of - lo > width ? top_of - width : lo;
+            hi = top_of;
         }
         window(lo, hi, count, rank, before, each_item);
         if (by_count) return at_window(min(max((int)(target - (double)rank), 0), n - 1));
@@ -700,7 +723,10 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams p) {
     if (tid < p.n_slices) {
         mine = slices[tid].top;
         bin = slices[tid].top_bin;
-        atomicMax(&top_key, mine);
+    }
+    {
+        const uint32_t most = wave_max(mine);
+        if ((tid & 63) == 0) atomicMax(&top_key, most);
     }
     __syncthreads();
     const uint32_t tk = top_key;
@@ -738,15 +764,8 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams p) {
     if (tid < 64) {
         uint32_t c = tid < kBlocks ? sh.block_count[tid] : 0;
         u64 m = tid < kBlocks ? sh.block_mass[tid] : 0;
-#pragma unroll
-        for (int d = 1; d < kBlocks; d <<= 1) {
-            const uint32_t x = __shfl_up((int)c, d, 64);
-            const u64 y = shfl_up64(m, d);
-            if (tid >= d) {
-                c += x;
-                m += y;
-            }
-        }
+        c = (uint32_t)wave_prefix((int)c);
+        m = wave_prefix64(m);
         if (tid < kBlocks) {
             sh.block_count[tid] = c;
             sh.block_mass[tid] = m;
