@@ -8,7 +8,9 @@
  * the C++ API of include/reflex/infer.h is implemented on top of them.  The
  * entry points marked NEW have no reference counterpart: they expose work
  * the reference API cannot express (bf16 GEMM, batched embedding gather,
- * small-batch decode, the quantiser used to build inputs).
+ * small-batch decode, the quantiser used to build inputs, and the operators
+ * of a serving step between the projections: head norms, rotation and the
+ * store in a paged cache, attention over it, the next token's draw).
  *
  * Conventions for every entry point:
  *   - `w` is a DEVICE pointer to raw GGML blocks of `ggml_type`: Q4_K (12,
@@ -23,7 +25,8 @@
  *     work; no entry point but rxq4_release_workspace synchronises the
  *     device or the stream.  The one allocation is the fp32 workspace of the
  *     split launches (split-K GEMM with few output tiles, small-batch
- *     products on long rows, attention over long cached contexts): 48 MiB
+ *     products on long rows, attention over long cached contexts) and of
+ *     rxq4_sample_f32's bins: 48 MiB
  *     per (device, stream), made by the first such launch on that stream,
  *     never resized, and kept until rxq4_release_workspace(stream) frees it,
  *     so a HIP graph captured on a stream stays valid whatever runs later,
@@ -271,7 +274,9 @@ int rxq4_qk_norm_rope(void *q_out, const void *q, const void *k, const void *v, 
  * does not reach its row, infinities and NaN included.  Few tokens on long
  * contexts split over the stream's workspace described above (a graph captured
  * with such a call uses the capturing stream's, also where it is replayed on
- * another).
+ * another).  The split follows the lengths of the whole batch as they are on the
+ * device: the same batch gives the same bits, a sequence in another batch the
+ * same within rounding.
  * No counterpart in the reference, whose KernelSupport names
  * paged_decode_attention. */
 int rxq4_attention_paged_f16(void *out, const void *q, int n_heads, float scale,

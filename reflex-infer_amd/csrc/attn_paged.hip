@@ -8,7 +8,18 @@
 // Query rows.  The rows of a sequence and KV head are numbered t * group + j (new
 // token t, j-th head of the group).  A workgroup takes 16 of them, the columns of
 // a 16 x 16 MFMA tile, and one chunk of positions: each K and V row is read once
-// for all of them, which is what bounds decoding (one to a few new tokens).
+// for all of them.
+//
+// Bound: reading the cache, in pieces of a head's row (256 bytes at head_dim 128,
+// fp16), which a plain read of the same pieces does at 5.6 to 5.8 TB/s (128-byte
+// pieces of int8: 5.1 to 5.3).  So a step's loads are issued a step ahead, nothing
+// of K passes LDS, and the chunks are cut from the batch's own lengths, which only
+// the device knows.
+// Measured, 32 / 8 heads of 128, one new token a sequence, pages of 16: 512
+// sequences of 1023 positions 366 us (5.9 TB/s), 256 of 2047 380 (5.7), 64 of 64 to
+// 8000 92 (4.7); int8 512 of 1023 214 (5.2), 256 of 2047 228 (4.9), 16 of 20000 to
+// 40000 202 (4.9).  A call's fixed part (launch, first loads, the chunks' ends, the
+// combine) is about 20 us at 64 sequences and 8 at one.
 #include <math.h>
 
 #include <algorithm>
@@ -145,10 +156,11 @@ __device__ __forceinline__ RowsUnit rows_unit(const PagedParams &p, int idx) {
 //                    ds_read_tr16_b64 of the wave's V rows in LDS), src1 = P^T as the
 //                    score registers hold it (k of a lane group: its positions), in
 //                    fp16 hi + lo parts (22 bits).
-// The next step's K and V are loaded before this step's arithmetic.  Pages of 16 positions or more (BIG): the 16 rows of an
-// operand lie in one page, a buffer resource of the wave, so that a load needs no
-// address arithmetic, and the lanes hold the table entries of 32 steps; smaller ones:
-// lane i looks up position i, a step ahead, and the rows' offsets go through LDS.
+// The next step's K and V are loaded before this step's arithmetic.  Pages of 16
+// positions or more (BIG): the 16 rows of an operand lie in one page, a buffer resource
+// of the wave, so that a load needs no address arithmetic, and the lanes hold the table
+// entries of 32 steps; smaller ones: lane i looks up position i, a step ahead, and the
+// rows' offsets go through LDS.
 // Rows past the end or in holes are zeros (BIG: past the end of the operand's buffer
 // resource; else the pool's first row in their place, cleared), their scores
 // -infinity.
@@ -171,7 +183,8 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
     const int r = lane & 15, g = lane >> 4;
     uint16_t *const vl = reinterpret_cast<uint16_t *>(smem) + w * 32 * VROW;
     // The KV heads of a sequence's chunk go to one XCD (workgroups are dealt to the eight in
-    // turn): they read the same pages and scales.  A sequence's chunks go to different ones.
+    // turn): they read the same pages and scales (int8, 512 sequences of 1023 positions, 244
+    // us with the heads on all, 216 so).  A sequence's chunks go to different ones.
     const int x8 = blockIdx.x / 8, kvh = x8 % p.c.n_kv;
     const RowsUnit unit = rows_unit(p, x8 / p.c.n_kv * 8 + blockIdx.x % 8);
     const int s = unit.s, c = unit.c, beg = c * unit.chunk;

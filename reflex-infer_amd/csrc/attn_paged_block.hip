@@ -10,11 +10,25 @@
 //            sequence and block by a sum over the sequences' block counts, a lane a
 //            sequence;
 //   pages    lane i of a wave looks up row i of the next tile (its page's table
-//            entry is loaded a tile earlier) and hands its offset to the lanes that
-//            load the row's chunks; rows in holes or past the block's sight are
-//            zeros, and their scores -infinity;
-//   splits   a workgroup leaves (O, m, l) per query row; attn_paged_block_combine
-//            adds a row's chunks in order.
+//            entry is loaded a tile earlier).  Pages of 16 positions or more: what a
+//            wave loads at once lies in one page, whose address it takes from the
+//            lane that looked it up; smaller ones: each row's offset goes to the
+//            lanes that load its chunks.  Scores in holes or past the block's sight
+//            are -infinity;
+//   splits   where the blocks leave CUs idle, every workgroup works out the same
+//            chunk length from the batch's lengths: the shortest that leaves at most
+//            a workgroup a CU (their 130 KB of LDS).  Chunks cut by the host from the
+//            lengths' limit took 34.7 us on 12 drafts of 3 to 6 tokens after 500 to 6000
+//            positions (28 / 4 heads), so 25.4.  A workgroup leaves (O, m, l) per query
+//            row; attn_paged_block_combine adds a row's chunks in order.
+// Bound: the chain of a tile in a wave (scores, maximum, exponentials, staging, P.V: 7000
+// to 8500 cycles, 1536 of them its matrix instructions) between two barriers; the two
+// waves of a SIMD are in the same part of it.
+// Measured, 32 / 8 heads of 128, fp16: 512 tokens of 16 / 2 heads after 7000 positions
+// 64.8 us (469 TFLOP/s), four prompts of 1254 to 3615 tokens 323 to 336 (525 to 546).
+// The second wave group a phase later (V weighed an iteration after its scores, a third V
+// buffer) made the prompts 341, a table load outside branches 356, raised priorities for
+// the products or fences between the phases 332 to 336.
 #include <math.h>
 
 #include <algorithm>

@@ -8,7 +8,7 @@
 namespace rxq4 {
 
 // The fp32 workspace of the split launches (split-K partials, attention
-// chunks): kWorkspaceBytes per (device, stream) (per (device, thread) for
+// chunks, the sampler's slices): kWorkspaceBytes per (device, stream) (per (device, thread) for
 // hipStreamPerThread), allocated by the first split launch on that stream,
 // never resized, freed only by release_stream_workspace.  Launchers choose
 // split counts whose partials fit in it.

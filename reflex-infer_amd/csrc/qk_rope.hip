@@ -17,6 +17,12 @@
 // loads and stores, the next head's loads ahead of this one's arithmetic), the
 // sums over the L lanes by lane swaps and the pair's other half through the wave's
 // own LDS.
+// Bound: for many tokens the rows' bytes, in and out; for a few the chain of lengths,
+// table entry, sine and store.  So a few tokens' heads are spread over workgroups, a pass
+// each; many tokens keep all heads in one, which shares the sines.
+// Measured, 32 / 8 heads of 128: 3595 tokens from bf16 24.1 us (3.7 TB/s; a copy of the
+// bytes 17; 31 with each row's loads after the sines), 64 tokens into int8 4.9, one token
+// of 16 / 2 heads 4.1.
 #include <math.h>
 
 #include "launch.h"

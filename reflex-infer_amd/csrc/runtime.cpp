@@ -2,7 +2,8 @@
 // the split launches and the tuning overrides read from the environment.
 //
 // Workspace (split-K GEMM partials, small-batch K-split partials of every
-// weight type, attention chunk partials of decode and prefill):
+// weight type, attention chunk partials of decode, prefill and paged batches,
+// what the sampler's slices of a row hand on):
 // One buffer of kWorkspaceBytes per (device, stream), allocated the first
 // time a split launch is enqueued on that stream and kept until
 // rxq4_release_workspace frees it or the process ends.  Hence:
