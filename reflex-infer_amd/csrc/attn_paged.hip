@@ -599,7 +599,7 @@ RowsPlan plan_rows(PagedParams &p, int i8, size_t room) {
     if (tuning().attn_split) most = std::min<int64_t>(most, tuning().attn_split);
     const int64_t units = std::min<int64_t>((i8 ? 12 : 6) * cus / p.c.n_kv, (int64_t)(room / per) - n);
     if (n > kSeqs) {
-        most = std::min<int64_t>({most, std::max((4 * cus + n * p.c.n_kv - 1) / (n * p.c.n_kv), (len + 1023) / 1024), (int64_t)(room / per) / n});
+        most = std::min<int64_t>({most, std::max((4 * cus + n * p.c.n_kv - 1) / (n * p.c.n_kv), (len + 2047) / 2048), (int64_t)(room / per) / n});
     } else if (units < 1) {
         most = 1;
     }

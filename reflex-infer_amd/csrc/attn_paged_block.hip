@@ -94,7 +94,7 @@ struct Unit {
 };
 
 // The idx-th unit of the batch, the same for a whole wave; false past the last one
-// (chunk_tiles is set all the same).  The chunks are as short as leaves at most
+// (chunk_tiles is set all the same).  The chunks are about as short as leaves at most
 // p.max_units of them (a sequence's blocks counted as long as its last), or the
 // blocks stay whole: every workgroup comes to the same length from the same sums.
 __device__ __forceinline__ bool find_unit(const PagedParams &p, int idx, Unit &u) {
@@ -111,12 +111,20 @@ __device__ __forceinline__ bool find_unit(const PagedParams &p, int idx, Unit &u
         return butterfly_sum<64>(x);
     };
     int ct = p.most_tiles;
-    if (p.n_chunks > 1 && sum([](int b, int) { return (float)b; }) < (float)p.max_units) {
+    const float most = (float)p.max_units;
+    const float blocks = p.n_chunks > 1 ? sum([](int b, int) { return (float)b; }) : most;
+    if (blocks < most) {
         const float all = sum([](int b, int t) { return (float)b * (float)t; });
-        ct = max(p.min_tiles, (int)(all / (float)p.max_units));
-        while (ct < p.most_tiles &&
-               sum([&](int b, int t) { return (float)b * (float)((t + ct - 1) / ct); }) > (float)p.max_units)
+        ct = max(p.min_tiles, (int)(all / most));
+        int tries = 6;
+        while (sum([&](int b, int t) { return (float)b * (float)((t + ct - 1) / ct); }) > most) {
+            // (a chunk a block more than their tiles' share at most: this many do)
+            if (--tries == 0) {
+                ct = max(ct, (int)fminf(all / (most - blocks), 0x1p24f) + 1);
+                break;
+            }
             ct += max(1, ct >> 4);
+        }
         ct = min(ct, p.most_tiles);
     }
     u.chunk_tiles = ct = __builtin_amdgcn_readfirstlane(ct);

@@ -47,21 +47,24 @@ __device__ __forceinline__ int wave_prefix(int x) {
 }
 
 // The sequence that row t belongs to (n_seqs: none) and its rows, the same for a
-// whole wave: the number of sequences that end at or before t.  A lane loads all
-// of a sequence at once: one round trip to memory for up to 64 sequences.
+// whole wave: the number of sequences that end at or before t, 64 parts at a time.
+// Of the last 64 a lane loads all of one at once: a round trip to memory for up to 64
+// sequences, two for up to 4096.
 __device__ __forceinline__ int seq_of_row(const SeqBatch &b, int t, SeqSpan &span) {
     const int lane = threadIdx.x & 63;
-    for (int i = 0; i < b.n_seqs; i += 64) {
-        const int j = min(i + lane, b.n_seqs - 1);
-        const int start = b.starts[j], end = b.starts[j + 1], len = b.lens[j];
-        const uint64_t ends = __builtin_amdgcn_ballot_w64(i + lane < b.n_seqs && end <= t);
-        const int n = __builtin_popcountll(ends);
-        if (n == 64 || i + n >= b.n_seqs) continue;
-        span = seq_span(b, __builtin_amdgcn_readlane(start, n), __builtin_amdgcn_readlane(end, n),
-                        __builtin_amdgcn_readlane(len, n));
-        return i + n;
+    int base = 0;
+    for (int part = b.n_seqs > 4096 ? 4096 : b.n_seqs > 64 ? 64 : 1; part > 1; part >>= 6) {
+        const int end = base + (lane + 1) * part;
+        const bool ends = end <= b.n_seqs && b.starts[end] <= t;
+        base += part * __builtin_popcountll(__builtin_amdgcn_ballot_w64(ends));
     }
-    return b.n_seqs;
+    const int j = min(base + lane, b.n_seqs - 1);
+    const int start = b.starts[j], end = b.starts[j + 1], len = b.lens[j];
+    const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(base + lane < b.n_seqs && end <= t));
+    if (n == 64 || base + n >= b.n_seqs) return b.n_seqs;
+    span = seq_span(b, __builtin_amdgcn_readlane(start, n), __builtin_amdgcn_readlane(end, n),
+                    __builtin_amdgcn_readlane(len, n));
+    return __builtin_amdgcn_readfirstlane(base + n);
 }
 
 // Positions that the batch's tokens may see or store: below the table's end.

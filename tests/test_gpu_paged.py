@@ -325,3 +325,23 @@ def test_pages_of_sixteen_or_more_with_holes(hd, new, length):
     check(p, attend(p, 0.125), 0.125)
     p = ref.Paged(39, 4, 2, hd - hd % 16, 32, [new], [length], True, holes=[(0, 3), (0, 20)])
     check(p, attend(p, 0.0625), 0.0625)
+
+
+@pytest.mark.parametrize("n", [300, 1000])
+def test_chunks_among_many_decoding(n):
+    """Split blocks of a few sequences among many that decode."""
+    new, lens = [1] * n, [1 + (i * 53) % 60 for i in range(n)]
+    for i, m in ((7, 40), (n // 2, 100), (n - 1, 33)):
+        new[i], lens[i] = m, 2000 + i
+    p = ref.Paged(40, 4, 2, 64, 16, new, lens)
+    check(p, attend(p, 0.125), 0.125)
+
+
+@pytest.mark.parametrize("n", [1, 20, 100, 126, 127])
+def test_blocks_up_to_one_a_cu(n):
+    """As many blocks as nearly fill the CUs, of very different lengths: the chunks'
+    length where few divisions fit."""
+    new = [17] * n
+    lens = [17 + (i * i * 13) % 700 + (6000 if i == n // 2 else 0) for i in range(n)]
+    p = ref.Paged(41, 2, 2, 16, 16, new, lens)
+    check(p, attend(p, 0.25), 0.25)

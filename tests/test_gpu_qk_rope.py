@@ -221,3 +221,71 @@ def test_large_pool_offsets():
     slot = (p.slots(0, 1030)[1025:] + (n - far) * page).cuda()
     assert torch.equal(v.view(-1, kv, hd)[slot].cpu(), x[2])
     assert int((v != 0).any(-1).any(-1).sum()) == 5
+
+
+@pytest.mark.parametrize("n", [65, 4096, 4100, 9000])
+def test_many_sequences(n):
+    """A token's sequence among more than a wave's lanes hold, some without new tokens,
+    rows of no sequence around them."""
+    new = [0 if i % 11 == 4 else 1 + (i % 3 == 0) for i in range(n)]
+    lens = [m + i % 5 for i, m in enumerate(new)]
+    p = ref.Paged(53, 1, 1, 8, 4, new, lens, lead=3, pad=5)
+    args = (freqs(8), None, None, 1e-6, False)
+    x = inputs(p, F16, True)
+    got, cache = run(p, x, *args)
+    check(p, x, got, cache, *args)
+
+
+def test_captured_and_replayed_at_other_positions():
+    """A captured call follows seq_lens, the table and its inputs as they are at its
+    replay."""
+    p = ref.Paged(54, 8, 2, 64, 16, [1, 3, 1], [200] * 3)
+    cache, batch = p.device(capi)
+    before = [t.clone() for t in cache.tensors[:2]]
+    f = torch.zeros((p.rows, p.heads + 2 * p.kv, p.hd), dtype=F16, device="cuda")
+    q, k, v = f[:, :p.heads], f[:, p.heads:p.heads + p.kv], f[:, p.heads + p.kv:]
+    out = torch.full((p.rows, p.heads, p.hd), 7.0, dtype=F16, device="cuda")
+    inv_freq = freqs(64).cuda()
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    capi.qk_norm_rope(out, q, k, v, batch, cache, inv_freq, stream=s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        capi.qk_norm_rope(out, q, k, v, batch, cache, inv_freq, stream=s)
+    for step in range(3):
+        p.lens = [1 + 50 * step, 3 + 60 * step, 17 * (step + 1)]
+        batch.tensors[1].copy_(torch.tensor(p.lens, dtype=torch.int32))
+        x = inputs(p, F16, True, seed=60 + step)
+        f.copy_(x[3])
+        for t, b in zip(cache.tensors, before):
+            t.copy_(b)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            graph.replay()
+        torch.cuda.synchronize()
+        check(p, x, out, cache, freqs(64), None, None, 1e-6, False)
+
+
+def test_two_streams_at_once():
+    """Two calls into different pages of one cache, at once."""
+    p = ref.Paged(55, 8, 2, 64, 16, [300, 200], [400, 200])
+    args = (freqs(64), None, None, 1e-6, False)
+    x = inputs(p, F16, False)
+    cache, _ = p.device(capi)
+    q, k, v = (t.cuda() for t in x[:3])
+    out = torch.full((p.rows, p.heads, p.hd), 7.0, dtype=F16, device="cuda")
+    parts = []
+    for i, (a, b) in enumerate(((0, 300), (300, 500))):
+        one = capi.PagedKV(*cache.tensors[:2], cache.tensors[2][i:i + 1])
+        batch = capi.SeqBatch(torch.tensor([0, b - a], dtype=torch.int32, device="cuda"),
+                              torch.tensor([p.lens[i]], dtype=torch.int32, device="cuda"), b - a, b - a, p.lens[i])
+        parts.append((out[a:b], q[a:b], k[a:b], v[a:b], batch, one))
+    inv_freq = freqs(64).cuda()
+    streams = [torch.cuda.Stream() for _ in parts]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, part in zip(streams, parts):
+            capi.qk_norm_rope(*part, inv_freq, stream=s)
+    torch.cuda.synchronize()
+    check(p, x, out, cache, *args)

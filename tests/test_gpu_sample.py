@@ -179,3 +179,32 @@ def test_repeats_and_replays():
         assert torch.equal(eager, ids)
         host = l.cpu().numpy()
         assert ids.tolist() == [ref.sample(host[i], np.float32(u[i].item()), top_k=5 + 10 * step) for i in range(n)]
+
+
+@pytest.mark.parametrize("spread", [1e-6, 0.01, 0.05, 0.3])
+def test_bins_of_thousands_of_logits(spread):
+    """Borders and draws among logits that share a bin: narrowed from registers or, with
+    more than they hold, from memory."""
+    g = torch.Generator().manual_seed(91)
+    l = (spread * torch.randn((6, 60001), generator=g)).numpy()
+    u = torch.rand(6, generator=g).numpy()
+    check(l, u, top_p=torch.tensor([0.2, 0.5, 0.9, 0.99, 1.0, 0.7]))
+    check(l, u, top_k=torch.tensor([3000, 700, 0, 40000, 513, 5], dtype=torch.int32),
+          temperature=torch.tensor([1.0, 0.5, 2.0, 1.0, 4.0, 1.0]))
+
+
+def test_two_streams_at_once():
+    g = torch.Generator().manual_seed(92)
+    ls = [torch.randn((n, 30000), generator=g) for n in (3, 40)]
+    us = [torch.rand(len(l), generator=g) for l in ls]
+    on = [(torch.zeros(len(l), dtype=torch.int32, device="cuda"), l.cuda(), u.cuda()) for l, u in zip(ls, us)]
+    streams = [torch.cuda.Stream() for _ in on]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for s, args in zip(streams, on):
+            capi.sample_f32(*args, stream=s)
+    torch.cuda.synchronize()
+    for (ids, _, _), l, u in zip(on, ls, us):
+        assert ids.tolist() == [ref.sample(a, x) for a, x in zip(l.numpy(), u.numpy())]
+    for s in streams:
+        capi.release_workspace(s)
