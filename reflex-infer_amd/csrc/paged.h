@@ -18,14 +18,14 @@ __device__ __forceinline__ void wave_lds_fence() {
 
 // One sequence of a batch: rows [row0, row0 + n) of q, the first at position
 // pos0 (negative where seq_lens is below the new tokens).  Whatever the device
-// arrays hold, the rows lie within [0, n_tokens).
+// arrays hold, the rows lie within [0, n_tokens) and no sum of theirs overflows.
 struct SeqSpan {
     int row0, n, pos0;
 };
 __device__ __forceinline__ SeqSpan seq_span(const SeqBatch &b, int start, int end, int len) {
     const int a = min(max(start, 0), b.n_tokens);
     const int e = min(max(end, a), b.n_tokens);
-    return SeqSpan{a, e - a, len - (e - a)};
+    return SeqSpan{a, e - a, max(len, -(1 << 30)) - (e - a)};
 }
 __device__ __forceinline__ SeqSpan seq_span(const SeqBatch &b, int s) {
     return seq_span(b, b.starts[s], b.starts[s + 1], b.lens[s]);

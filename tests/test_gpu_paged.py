@@ -345,3 +345,15 @@ def test_blocks_up_to_one_a_cu(n):
     lens = [17 + (i * i * 13) % 700 + (6000 if i == n // 2 else 0) for i in range(n)]
     p = ref.Paged(41, 2, 2, 16, 16, new, lens)
     check(p, attend(p, 0.25), 0.25)
+
+
+@pytest.mark.parametrize("n", [1, 33])
+def test_lengths_outside_the_limits(n):
+    """seq_lens past max_len and below zero, to the type's ends: the cache as far as it
+    goes, and nothing."""
+    p = ref.Paged(42, 4, 2, 64, 16, [n] * 4, [64] * 4)
+    p.seq_lens = torch.tensor([2 ** 31 - 1, -5, -2 ** 31, 64], dtype=torch.int32)
+    got = attend(p, 0.125, max_len=64)
+    assert not got[n:3 * n].any()
+    p.lens = [64 + n, -5, -64, 64]  # past the table: every position is seen by every row
+    check(p, got, 0.125)
