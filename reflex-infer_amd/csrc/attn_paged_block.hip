@@ -46,7 +46,6 @@ namespace rxq4 {
 namespace {
 
 constexpr int kMaxChunks = 64;  // chunks per block
-constexpr int kLeastTiles = 4;  // tiles per chunk, where a block is cut
 constexpr int kSplitSeqs = 1024;  // sequences of a batch whose blocks are cut
 // An int8 tile's floats in LDS: K scales, V scales, log2 |V scale|.
 constexpr int kScl = 3 * kTile;
@@ -672,6 +671,11 @@ __global__ __launch_bounds__(256) void attn_paged_block_combine_kernel(PagedPara
 
 constexpr int kBigDim = 128;  // larger heads: one wave group, 512 registers a wave
 int pad_dim(int hd) { return hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : 256; }
+// Tiles per chunk at least, where a block is cut: one a wave group (27 drafts of 3 to 6
+// tokens after up to 1181 positions 19.7 us with four, 17.7 so; head_dim 256, three
+// chunks of 67 to 134 tokens 52.4 and 40.5).  Blocks of four tiles or less stay whole: the
+// combine takes longer than their walk (5 drafts after up to 250 positions 10.5, cut 12.1).
+constexpr int least_tiles(int pad) { return pad > kBigDim ? 1 : 2; }
 
 // Blocks of the batch at most: every sequence's rows past the limit, each with a
 // last block of its own.
@@ -721,8 +725,8 @@ PagedBlockPlan plan_paged_blocks(const PagedParams &p, size_t room) {
     const size_t per = (size_t)p.b.n_tokens * p.n_heads * (pad_dim(p.c.hd) + 2) * 4;
     const int64_t units = std::max(1, cus / p.c.n_kv);
     int64_t want = 1;
-    if ((int64_t)p.b.n_tokens * p.group / kPagedBlock < units && p.b.n_seqs <= kSplitSeqs && room > 256)
-        want = std::max<int64_t>(1, std::min<int64_t>({tiles / kLeastTiles, kMaxChunks, (int64_t)((room - 256) / per)}));
+    if ((int64_t)p.b.n_tokens * p.group / kPagedBlock < units && p.b.n_seqs <= kSplitSeqs && tiles > 4 && room > 256)
+        want = std::max<int64_t>(1, std::min<int64_t>({tiles / least_tiles(pad_dim(p.c.hd)), kMaxChunks, (int64_t)((room - 256) / per)}));
     if (tuning().attn_split) want = std::min<int64_t>(want, tuning().attn_split);
     return PagedBlockPlan{(int)units, (int)want, tiles, want > 1 ? per * want + 256 : 0};
 }
@@ -731,7 +735,7 @@ hipError_t launch_paged_blocks(PagedParams p, const PagedBlockPlan &plan, float 
     p.max_units = plan.units;
     p.n_chunks = plan.n_chunks;
     p.most_tiles = plan.tiles;
-    p.min_tiles = std::max((plan.tiles + plan.n_chunks - 1) / plan.n_chunks, kLeastTiles);
+    p.min_tiles = std::max((plan.tiles + plan.n_chunks - 1) / plan.n_chunks, least_tiles(pad_dim(p.c.hd)));
     p.chunk_tiles = reinterpret_cast<int *>(ws);
     p.part = ws ? ws + 64 : nullptr;
     p.stats = ws ? p.part + (size_t)p.b.n_tokens * p.n_heads * p.n_chunks * pad_dim(p.c.hd) : nullptr;
