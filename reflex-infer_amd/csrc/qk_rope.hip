@@ -6,9 +6,11 @@
 //   norm      x w / sqrt(mean x^2 + eps)
 //   rotation  (a, b) -> (a cos - b sin, b cos + a sin) of the pairs (i, i + n_rot / 2)
 //             or (2 i, 2 i + 1), the angle position * inv_freq[i]: its product and
-//             its remainder to whole turns in 64 bits (in 32 the angle of position
-//             100000 would be off by 2^-8 of a turn), sine and cosine of the
-//             remainder in 32
+//             its remainder to whole turns in 64 bits (a product of 32 bits is off by up to
+//             2^-8 radians at positions 65536 to 131071), sine and cosine in 32 of the
+//             remainder's nearest fp32 number of half turns, turned on by what that
+//             rounds off (up to 2^-25 half turns, 9e-8 of the sine: next to a half
+//             turn more than all of its other errors)
 //   int8      scale = max |x| / 127, rint(x / scale), both divisions IEEE, so that
 //             the bytes follow from the 32-bit row alone
 // A workgroup takes one token and its heads, or a part of them: its threads form
@@ -128,10 +130,12 @@ __global__ __launch_bounds__(64 * kWaves, DT == RXQ4_DTYPE_F32 ? 7 : 8) void qk_
     const int slot = pos >= 0 && pos < position_limit(p.b, p.c) ? slot_of(p.c, seq, pos) : -1;
     if (tid < half) {
         const double turns = (double)pos * (double)freq * 0.15915494309189533577;
+        const double halves = 2.0 * (turns - rint(turns));
+        const float near = (float)halves, rest = (float)((halves - (double)near) * 3.14159265358979323846);
         float s, c;
-        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-        cs[tid] = c;
-        sn[tid] = s;
+        sincospif(near, &s, &c);
+        cs[tid] = __builtin_fmaf(-s, rest, c);
+        sn[tid] = __builtin_fmaf(c, rest, s);
     }
     __syncthreads();
     // This lane's part of the rotation, the same for every head: x c + y s with the

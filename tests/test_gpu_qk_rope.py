@@ -289,3 +289,24 @@ def test_two_streams_at_once():
             capi.qk_norm_rope(*part, inv_freq, stream=s)
     torch.cuda.synchronize()
     check(p, x, out, cache, *args)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_sines_next_to_half_turns(interleaved):
+    """(1000, 0) turned by nearly pi: 1000 times a sine of 1e-4 to 2e-4, whose angle is
+    its remainder's distance to half a turn.  That distance in fp32 steps next to a half
+    turn is off by 2^-25 half turns, 9.4e-5 in the output; kept whole, the sine is off by
+    its function's 4 units in the last place (8 u), the correction's three roundings of
+    9.4e-8 and the sum's: 12 u of the value and 1e-10."""
+    p = ref.Paged(56, 4, 2, 64, 16, [1], [2])  # position 1
+    f = torch.tensor(np.pi * (1 + np.linspace(0.32e-4, 0.63e-4, 32)), dtype=F32)
+    q, k, v, _ = inputs(p, F16, False)
+    q[:] = 0.0
+    at, to = (slice(0, 64, 2), slice(1, 64, 2)) if interleaved else (slice(0, 32), slice(32, 64))
+    q[..., at] = 1000.0
+    got, _ = run(p, (q, k, v, None), f, None, None, 0.0, interleaved)
+    want = 1000.0 * np.sin(f.double().numpy())
+    assert (np.abs(want) > 0.09).all()
+    bound = 12 * ref.U * np.abs(want) + 1e-10 + ref.H16 * np.abs(want) + ref.TINY16
+    off = np.abs(got[0, :, to].cpu().double().numpy() - want)
+    assert (off <= bound).all(), (off / bound).max()
