@@ -265,13 +265,16 @@ class PagedKV:
                                        (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
             raise ValueError("PagedKV: page_table must be int32 [n_seqs, pages], its rows dense")
         _same_device("PagedKV", k, v, page_table, k_scales, v_scales)
+        # (a table of no entries needs an address too: none at all means a contiguous cache)
+        self._table = page_table.new_empty(1) if page_table is not None and page_table.numel() == 0 else page_table
         self.tensors = (k, v, page_table, k_scales, v_scales)
         self.n_seqs = 1 if page_table is None else page_table.shape[0]
         self.n_kv_heads, self.head_dim = n_kv, hd
         pages = 0 if page_table is None else page_table.shape[1]
         if pages > 0 and self.n_seqs > 1 and page_table.stride(0) != pages:
             raise ValueError("PagedKV: page_table must be dense")
-        self.struct = PagedKVStruct(_ptr(k), _ptr(v), _ptr(k_scales), _ptr(v_scales), _ptr(page_table), stride, pages,
+        self.struct = PagedKVStruct(_ptr(k), _ptr(v), _ptr(k_scales), _ptr(v_scales),
+                                    _ptr(self._table), stride, pages,
                                     n_pages, page_size, n_kv, hd, int(k.dtype == torch.int8))
         self.ref = ctypes.byref(self.struct)
 

@@ -139,3 +139,21 @@ def test_prompts_then_decoding_eager_and_replayed(page, int8):
     assert again == said
     for t, b in zip(cache.tensors, after):
         assert t is None or torch.equal(t, b)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_table_without_entries(new, int8):
+    """No position has a slot: nothing is stored, and every token sees nothing."""
+    p = ref.Paged(51, HEADS, KV, HD, 16, [new], [new], int8)
+    p.table = p.table[:, :0]
+    cache, batch = p.device(capi)
+    before = [None if t is None else t.clone() for t in cache.tensors]
+    g = torch.Generator().manual_seed(52)
+    x = [torch.randn((new, n, HD), generator=g).half().cuda() for n in (HEADS, KV, KV)]
+    q, out = (torch.full((new, HEADS, HD), 7.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    capi.qk_norm_rope(q, *x, batch, cache, freqs(HD).cuda())
+    capi.attention_paged_f16(out, q, batch, cache, SCALE)
+    assert not out.any() and not (q == 7.0).any()
+    for t, b in zip(cache.tensors, before):
+        assert t is None or torch.equal(t, b)

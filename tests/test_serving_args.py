@@ -154,3 +154,13 @@ def test_python_binding_refuses():
         capi.sample_f32(torch.zeros(3, dtype=torch.int32), logits, u[:2])
     with pytest.raises(ValueError):
         capi.sample_f32(torch.zeros(3, dtype=torch.int32), logits.t().contiguous().t(), u)
+
+
+@pytest.mark.parametrize("n_seqs", [1, 2])
+def test_an_empty_page_table_is_a_table(n_seqs):
+    """A table without entries, whose tensor has no address, is no contiguous cache: the
+    descriptor names a table of width 0, and no position is in it."""
+    k = torch.zeros((4, 16, 2, 64), dtype=torch.float16)
+    cache = capi.PagedKV(k, k, torch.zeros((n_seqs, 0), dtype=torch.int32))
+    assert cache.struct.page_table and cache.struct.table_stride == 0
+    assert cache.n_seqs == n_seqs
