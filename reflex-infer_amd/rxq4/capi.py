@@ -258,6 +258,8 @@ class PagedKV:
         for t in (k, v):
             if t.stride()[1:] != (n_kv * hd, hd, 1) or (n_pages > 1 and t.stride(0) != stride):
                 raise ValueError("PagedKV: a page must be dense, and K and V pages lie alike")
+        if stride < page_size * n_kv * hd:
+            raise ValueError("PagedKV: pages must not share memory")
         for t in (k_scales, v_scales):
             if t is not None and (t.dtype != torch.float32 or t.shape != k.shape[:3] or not t.is_contiguous()):
                 raise ValueError("PagedKV: scales must be contiguous fp32 [n_pages, page_size, n_kv_heads]")

@@ -164,3 +164,18 @@ def test_an_empty_page_table_is_a_table(n_seqs):
     cache = capi.PagedKV(k, k, torch.zeros((n_seqs, 0), dtype=torch.int32))
     assert cache.struct.page_table and cache.struct.table_stride == 0
     assert cache.n_seqs == n_seqs
+
+
+def test_pages_that_share_memory_are_refused():
+    """An expanded page (stride 0, which the C side takes for dense) and pages that
+    overlap; one page may have any stride."""
+    page = torch.zeros((1, 16, 2, 64), dtype=torch.float16)
+    table = torch.zeros((1, 4), dtype=torch.int32)
+    with pytest.raises(ValueError):
+        capi.PagedKV(page.expand(4, -1, -1, -1), page.expand(4, -1, -1, -1), table)
+    half = torch.zeros(4096, dtype=torch.float16).as_strided((3, 16, 2, 64), (1024, 128, 64, 1))
+    with pytest.raises(ValueError):
+        capi.PagedKV(half, half, table)
+    apart = torch.zeros((3, 2, 16, 2, 64), dtype=torch.float16)
+    assert capi.PagedKV(apart[:, 0], apart[:, 1], table).struct.page_stride == 4096
+    assert capi.PagedKV(page, page, table).struct.page_stride == 2048
