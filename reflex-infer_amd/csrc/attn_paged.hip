@@ -329,7 +329,8 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
-    bool bad = false;  // some V (int8: V scale) is not finite
+    bool bad = false;  // some V is not finite
+    uint32_t most_vs = 0;  // int8: the lane's largest |V scale|
     auto process = [&](int j, Step &S) {
         const int p0 = beg + kStep * j + 32 * w;
         f32x4 acc[2];
@@ -347,6 +348,13 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
         }
         f32x4 vx[2], lg[2];
         if constexpr (I8) {
+            // An infinite or NaN V scale: as an fp16 V below.  (Small pages: looked at after the
+            // walk; a ballot here spills 27 registers.  Larger ones: the lanes' sizes spill 2.)
+            const uint32_t size = __builtin_bit_cast(uint32_t, S.vs) & 0x7FFFFFFFu;
+            const uint32_t here = (S.seen >> (lane & 31)) & 1u ? size : 0u;
+            if constexpr (BIG) bad |= __builtin_amdgcn_ballot_w64(here >= 0x7F800000u) != 0;
+            else most_vs = max(most_vs, here);
+            S.vs = size < 0x7F800000u ? S.vs : 0.0f;
             if (lane < 32) {
                 scl[w][0][lane] = S.ks;
                 scl[w][1][lane] = S.vs;
@@ -402,7 +410,8 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
         }
         // Rows that are not there: zeros.  An infinity or NaN in V would reach the rows
         // that do not see it as 0 times it, and the others through the low half of P: such
-        // values are staged as zeros, and the rows that see them get them at the end.
+        // values (int8: V scales) are staged as zeros, and the rows that see them get them
+        // at the end.
         if constexpr (!I8) {
             if (!BIG && part)  // uniform
 #pragma unroll
@@ -462,22 +471,7 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
         }
         if (!BIG) break;
     }
-    if (bad) {  // uniform, rare: the wave's positions again
-        for (int pos = beg; pos < end; ++pos) {
-            if (((pos - beg) / 32 & 3) != w || pos > qpos) continue;
-            const int slot = slot_of(p.c, s, pos);
-            if (slot < 0) continue;
-            const uint16_t *v = reinterpret_cast<const uint16_t *>(vb + slot_bytes(p.c, slot, row_bytes));
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int d = 16 * dt + 4 * g + i;
-                    const float x = d < hd ? f16_bits_to_f32(v[d]) : 0.0f;
-                    if (!(fabsf(x) < INFINITY)) o[dt][i] += x;
-                }
-        }
-    }
+    if constexpr (I8 && !BIG) bad = __builtin_amdgcn_ballot_w64(most_vs >= 0x7F800000u) != 0;
     l = sum_xor_rows<16>(l);
     l = sum_xor_rows<32>(l);
 
@@ -491,6 +485,28 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
         for (int i = 0; i < 4; ++i) mg[w][4 * dt + i][lane] = o[dt][i];
     mg[w][NM - 2][lane] = m;
     mg[w][NM - 1][lane] = l;
+    if (bad) {  // uniform, rare: the wave's positions again (onto its part in LDS: no registers held for it)
+        for (int pos = beg; pos < end; ++pos) {
+            if (((pos - beg) / 32 & 3) != w || pos > qpos) continue;
+            const int slot = slot_of(p.c, s, pos);
+            if (slot < 0) continue;
+            const uint8_t *v = vb + slot_bytes(p.c, slot, row_bytes);
+            const float vs = I8 ? vsp[(int64_t)slot * v_stride] : 1.0f;
+            if (I8 && fabsf(vs) < INFINITY) continue;
+            for (int dt = 0; dt < DT; ++dt) {
+                const int d = 16 * dt + 4 * g;
+                if (d >= hd) continue;
+                const u32x2 x = I8 ? u32x2{*reinterpret_cast<const uint32_t *>(v + d), 0u}
+                                   : *reinterpret_cast<const u32x2 *>(v + 2 * d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float y = I8 ? vs * (float)(int8_t)(x.x >> (8 * i))
+                                       : f16_bits_to_f32((i < 2 ? x.x : x.y) >> (16 * (i & 1)) & 0xFFFFu);
+                    if (!(fabsf(y) < INFINITY)) mg[w][4 * dt + i][lane] += y;
+                }
+            }
+        }
+    }
     __syncthreads();
     float mw[4], M = -INFINITY;
 #pragma unroll

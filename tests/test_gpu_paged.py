@@ -357,3 +357,25 @@ def test_lengths_outside_the_limits(n):
     assert not got[n:3 * n].any()
     p.lens = [64 + n, -5, -64, 64]  # past the table: every position is seen by every row
     check(p, got, 0.125)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("new,length,page", [(1, 100, 16), (1, 3000, 8), (3, 100, 8), (20, 150, 16), (100, 333, 8)])
+@pytest.mark.parametrize("hd", [64, 80, 128])
+def test_int8_scales_that_are_not_finite_in_places_seen(bad, new, length, page, hd):
+    """A V scale of a seen position: the rows that see it get that times its bytes, NaN
+    where a byte is 0, whichever kernel takes them; no other row or head changes."""
+    p = ref.Paged(43, 8, 2, hd, page, [new], [length], True)
+    clean = attend(p, 0.0625).cpu()
+    at = length - (new + 1) // 2
+    slot = int(p.slots(0, length)[at])
+    p.v.view(-1, 2, hd)[slot, 1, 7] = 0
+    p.vs.view(-1, 2)[slot, 1] = bad
+    got = attend(p, 0.0625).cpu()
+    first = at - (length - new)  # the first token that sees it
+    want = p.v.view(-1, 2, hd)[slot, 1].float() * bad
+    for head in range(4, 8):
+        assert torch.equal(got[:first, head], clean[:first, head])
+        assert torch.equal(torch.nan_to_num(got[first:, head].float(), 3.0, 2.0, 1.0),
+                           torch.nan_to_num(want, 3.0, 2.0, 1.0).expand(new - first, hd))
+    assert torch.equal(got[:, :4], clean[:, :4])
