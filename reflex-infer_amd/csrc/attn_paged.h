@@ -3,6 +3,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include "launch.h"
@@ -27,6 +28,13 @@ struct PagedParams {
     int most_tiles;       // 128 rows: tiles of a block at most
     int *chunk_tiles;     // 128 rows: tiles of a chunk, left for the combine
 };
+
+// sum + w x, x a part relative to its own maximum and w its weight beside the other
+// parts.  Infinities and NaN (a V that is none, seen by the row) stay what they are where
+// w is below fp32's range: their weight is never 0.
+__device__ __forceinline__ float add_weighed(float sum, float w, float x) {
+    return __builtin_fmaf(fabsf(x) < INFINITY ? w : 1.0f, x, sum);
+}
 
 // Query rows of a workgroup of the smaller and of the larger kernel.
 constexpr int kPagedRows = 16, kPagedBlock = 128;

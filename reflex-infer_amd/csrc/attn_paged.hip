@@ -526,13 +526,17 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
     const int64_t at = (unit.slot * p.c.n_kv + kvh) * p.rows_blk + r;
 #pragma unroll
     for (int dt = w; dt < DT; dt += 4) {
-        f32x4 ov;
+        f32x4 ov{};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float x = 0.0f;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) x += mg[v][4 * dt + i][lane] * cw[v];
-            ov[i] = x;
+            for (int v = 0; v < 4; ++v) ov[i] = __builtin_fmaf(cw[v], mg[v][4 * dt + i][lane], ov[i]);
+        if (!(fabsf(ov[0]) + fabsf(ov[1]) + fabsf(ov[2]) + fabsf(ov[3]) < INFINITY)) {  // rare: the same sums
+            ov = f32x4{};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) ov[i] = add_weighed(ov[i], cw[v], mg[v][4 * dt + i][lane]);
         }
         const int d = 16 * dt + 4 * g;
         if (!whole) *reinterpret_cast<f32x4 *>(p.part + at * HD + d) = ov;
@@ -578,7 +582,11 @@ __global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedParams p) 
         for (int i = 0; i < U; ++i) {
             const float ec = __builtin_bit_cast(
                 float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, e), min(c0 + i, 63)));
-            if (c0 + i < n_c && ec != 0.0f) acc += ec * x[i];  // uniform
+            if (c0 + i >= n_c) continue;  // uniform
+            if (ec != 0.0f) acc += ec * x[i];
+            else
+#pragma unroll
+                for (int k = 0; k < VE; ++k) acc[k] = add_weighed(acc[k], 0.0f, x[i][k]);
         }
     }
     if (lane * VE >= p.c.hd) return;

@@ -565,6 +565,10 @@ __global__ __launch_bounds__(256 * G) void attn_paged_block_kernel(PagedParams p
         wait_lgkmcnt0();
         lds_barrier();
         if (gq == 1) return;
+        int bad = 0;  // either group's V
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bad |= bad_v[i];
+        bad = __builtin_amdgcn_readfirstlane(bad);
         const float m1 = mgl[tid], l1 = mgl[256 + tid];
         const float mm = fmaxf(m, m1);
         const bool any = mm != -INFINITY;
@@ -572,10 +576,18 @@ __global__ __launch_bounds__(256 * G) void attn_paged_block_kernel(PagedParams p
         const float c1 = any ? __builtin_amdgcn_exp2f(m1 - mm) : 0.0f;
         l = l * c0 + l1 * c1;
         m = mm;
+        if (bad != 0) {  // uniform, rare; the same sums
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[dt][i] = o[dt][i] * c0 + mb[(16 * dt + i) * 256 + tid] * c1;
+                for (int i = 0; i < 16; ++i)
+                    o[dt][i] = add_weighed(add_weighed(0.0f, c0, o[dt][i]), c1, mb[(16 * dt + i) * 256 + tid]);
+        } else {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[dt][i] = __builtin_fmaf(c1, mb[(16 * dt + i) * 256 + tid], c0 * o[dt][i]);
+        }
     }
     if (!live_wave) return;
     if (n_tiles > chunk_tiles) {  // the block has several chunks
@@ -656,9 +668,9 @@ __global__ __launch_bounds__(256) void attn_paged_block_combine_kernel(PagedPara
             for (int k = 0; k < NE; ++k) x[j][k] = src[(int64_t)min(i + j, n_c - 1) * HD + min(lane + 64 * k, HD - 1)];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float ei = __shfl(e, (i + j) & 63, 64);  // (0 past the last chunk)
+            const float ei = __shfl(e, (i + j) & 63, 64);  // (past the last chunk: that again, 0 times)
 #pragma unroll
-            for (int k = 0; k < NE; ++k) acc[k] += ei == 0.0f ? 0.0f : ei * x[j][k];
+            for (int k = 0; k < NE; ++k) acc[k] = add_weighed(acc[k], ei, x[j][k]);
         }
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;

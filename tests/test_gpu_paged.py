@@ -379,3 +379,25 @@ def test_int8_scales_that_are_not_finite_in_places_seen(bad, new, length, page, 
         assert torch.equal(torch.nan_to_num(got[first:, head].float(), 3.0, 2.0, 1.0),
                            torch.nan_to_num(want, 3.0, 2.0, 1.0).expand(new - first, hd))
     assert torch.equal(got[:, :4], clean[:, :4])
+
+
+@pytest.mark.parametrize("new,length", [(1, 100), (1, 3000), (3, 2000), (20, 150), (20, 3000), (100, 333)])
+@pytest.mark.parametrize("gap", [30.0, 900.0])
+def test_infinities_seen_with_little_weight(new, length, gap):
+    """Infinite V at positions whose weights are e^-gap of the largest's, with e^-900 below
+    fp32's range: any weight times them is infinite, however the positions are split
+    over waves and chunks, of which one alone holds the position that weighs."""
+    p = ref.Paged(44, 4, 1, 64, 16, [new], [length])
+    p.q[:] = 0.0
+    p.q[..., 0] = 1.0
+    slots = p.slots(0, length)
+    k, v = p.k.view(-1, 64), p.v.view(-1, 64)
+    k[slots, 0] = 0.0
+    k[slots[length - new], 0] = gap
+    for at in (1, 40, 77):
+        v[slots[at], at % 64] = float("inf") if at % 2 else float("-inf")
+    got = attend(p, 1.0).cpu()
+    assert (got[..., 1] == float("inf")).all() and (got[..., 40] == float("-inf")).all()
+    assert (got[..., 13] == float("inf")).all()
+    got[..., [1, 13, 40]] = 0.0
+    assert torch.isfinite(got).all()
