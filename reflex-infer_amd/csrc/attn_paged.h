@@ -43,9 +43,12 @@ constexpr int kPagedRows = 16, kPagedBlock = 128;
 // workgroup; partials within `room` bytes at `ws` (null: no split).
 struct PagedBlockPlan {
     int units, n_chunks, tiles;
+    int64_t grid;  // workgroups
     size_t bytes;  // of partials
 };
 PagedBlockPlan plan_paged_blocks(const PagedParams &p, size_t room);
+// (more workgroups than this are refused)
+constexpr int64_t kPagedMostRows = 0x7FFFFF, kPagedMostBlocks = 0x3FFFFF;
 hipError_t launch_paged_blocks(PagedParams p, const PagedBlockPlan &plan, float *ws, int kv_int8, hipStream_t st);
 
 }  // namespace rxq4

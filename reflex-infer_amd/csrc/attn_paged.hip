@@ -609,6 +609,7 @@ __global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedParams p) 
 // 213 / 208 / 202 / 204.  Past kSeqs sequences there is little to cut: the host's chunks.
 struct RowsPlan {
     int64_t slots;  // chunks of the batch at most, per KV head
+    int64_t grid;   // workgroups
     size_t bytes;
 };
 RowsPlan plan_rows(PagedParams &p, int i8, size_t room) {
@@ -634,21 +635,20 @@ RowsPlan plan_rows(PagedParams &p, int i8, size_t room) {
     p.chunk = (int)least * kStep;
     p.n_chunks = (int)((steps + least - 1) / least);
     const int64_t slots = p.n_chunks == 1 || n > kSeqs ? n * p.n_chunks : std::min<int64_t>(units + n, n * p.n_chunks);
-    return RowsPlan{slots, p.n_chunks > 1 ? (per * slots + 8 * n + 255) / 256 * 256 : 0};
+    return RowsPlan{slots, (slots + 7) / 8 * 8 * p.c.n_kv, p.n_chunks > 1 ? (per * slots + 8 * n + 255) / 256 * 256 : 0};
 }
 
 template <int HD>
 hipError_t launch_rows(PagedParams &p, const RowsPlan &plan, float *ws, int i8, hipStream_t st) {
-    const int64_t grid = (plan.slots + 7) / 8 * 8 * p.c.n_kv;
-    if (grid > 0x7FFFFF) return hipErrorInvalidValue;
+    const unsigned grid = (unsigned)plan.grid;
     p.part = ws;
     p.stats = ws + (size_t)plan.slots * p.c.n_kv * p.rows_blk * HD;
     p.firsts = reinterpret_cast<int *>(p.stats + (size_t)plan.slots * p.c.n_kv * p.rows_blk * 2);
     const bool big = p.c.shift >= 4;
-    if (i8 && big) attn_paged_rows_kernel<HD, true, true><<<(unsigned)grid, 256, 0, st>>>(p);
-    else if (i8) attn_paged_rows_kernel<HD, true, false><<<(unsigned)grid, 256, 0, st>>>(p);
-    else if (big) attn_paged_rows_kernel<HD, false, true><<<(unsigned)grid, 256, 0, st>>>(p);
-    else attn_paged_rows_kernel<HD, false, false><<<(unsigned)grid, 256, 0, st>>>(p);
+    if (i8 && big) attn_paged_rows_kernel<HD, true, true><<<grid, 256, 0, st>>>(p);
+    else if (i8) attn_paged_rows_kernel<HD, true, false><<<grid, 256, 0, st>>>(p);
+    else if (big) attn_paged_rows_kernel<HD, false, true><<<grid, 256, 0, st>>>(p);
+    else attn_paged_rows_kernel<HD, false, false><<<grid, 256, 0, st>>>(p);
     if (p.n_chunks > 1) {
         const dim3 rows((unsigned)(p.b.n_seqs * p.c.n_kv), (unsigned)(p.rows_blk + 3) / 4);
         attn_paged_combine_kernel<HD><<<rows, 256, 0, st>>>(p);
@@ -680,6 +680,8 @@ hipError_t launch_attention_paged(uint16_t *out, const uint16_t *q, int n_heads,
     PagedBlockPlan bp{};
     if (rows) rp = plan_rows(pr, kv_int8, (blocks ? kWorkspaceBytes / 2 : kWorkspaceBytes) - 256);
     if (blocks) bp = plan_paged_blocks(p, kWorkspaceBytes - rp.bytes);
+    // (before the first of the launches)
+    if (rp.grid > kPagedMostRows || bp.grid > kPagedMostBlocks) return hipErrorInvalidValue;
     float *ws = nullptr;
     if (rp.bytes + bp.bytes > 0) {
         const hipError_t e = Scratch{}.get(st, rp.bytes + bp.bytes, &ws);

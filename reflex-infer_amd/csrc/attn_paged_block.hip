@@ -697,7 +697,7 @@ int64_t most_blocks(const PagedParams &p) {
 }
 
 template <int HD, bool I8, bool BIG>
-hipError_t launch_t(const PagedParams &p, hipStream_t st) {
+hipError_t launch_t(const PagedParams &p, int64_t grid, hipStream_t st) {
     constexpr int G = HD > kBigDim ? 1 : 2;
     constexpr int lds = block_lds<HD, G>();
     // the dynamic LDS limit, raised once per device (devices 0..63)
@@ -712,8 +712,6 @@ hipError_t launch_t(const PagedParams &p, hipStream_t st) {
         if (e != hipSuccess) return e;
         raised.fetch_or(bit, std::memory_order_acq_rel);
     }
-    const int64_t grid = (p.n_chunks > 1 ? std::max<int64_t>(p.max_units, most_blocks(p)) : most_blocks(p)) * p.c.n_kv;
-    if (grid > 0x3FFFFF) return hipErrorInvalidValue;
     attn_paged_block_kernel<HD, I8, G, BIG><<<(unsigned)grid, 256 * G, lds, st>>>(p);
     if (p.n_chunks > 1)
         attn_paged_block_combine_kernel<HD>
@@ -722,10 +720,10 @@ hipError_t launch_t(const PagedParams &p, hipStream_t st) {
 }
 
 template <int HD>
-hipError_t launch_hd(const PagedParams &p, int i8, hipStream_t st) {
+hipError_t launch_hd(const PagedParams &p, int64_t grid, int i8, hipStream_t st) {
     const bool big = p.c.shift >= 4;
-    if (i8) return big ? launch_t<HD, true, true>(p, st) : launch_t<HD, true, false>(p, st);
-    return big ? launch_t<HD, false, true>(p, st) : launch_t<HD, false, false>(p, st);
+    if (i8) return big ? launch_t<HD, true, true>(p, grid, st) : launch_t<HD, true, false>(p, grid, st);
+    return big ? launch_t<HD, false, true>(p, grid, st) : launch_t<HD, false, false>(p, grid, st);
 }
 
 }  // namespace
@@ -740,7 +738,8 @@ PagedBlockPlan plan_paged_blocks(const PagedParams &p, size_t room) {
     if ((int64_t)p.b.n_tokens * p.group / kPagedBlock < units && p.b.n_seqs <= kSplitSeqs && tiles > 4 && room > 256)
         want = std::max<int64_t>(1, std::min<int64_t>({tiles / least_tiles(pad_dim(p.c.hd)), kMaxChunks, (int64_t)((room - 256) / per)}));
     if (tuning().attn_split) want = std::min<int64_t>(want, tuning().attn_split);
-    return PagedBlockPlan{(int)units, (int)want, tiles, want > 1 ? per * want + 256 : 0};
+    const int64_t grid = (want > 1 ? std::max(units, most_blocks(p)) : most_blocks(p)) * p.c.n_kv;
+    return PagedBlockPlan{(int)units, (int)want, tiles, grid, want > 1 ? per * want + 256 : 0};
 }
 
 hipError_t launch_paged_blocks(PagedParams p, const PagedBlockPlan &plan, float *ws, int i8, hipStream_t st) {
@@ -752,10 +751,10 @@ hipError_t launch_paged_blocks(PagedParams p, const PagedBlockPlan &plan, float 
     p.part = ws ? ws + 64 : nullptr;
     p.stats = ws ? p.part + (size_t)p.b.n_tokens * p.n_heads * p.n_chunks * pad_dim(p.c.hd) : nullptr;
     switch (pad_dim(p.c.hd)) {
-        case 64: return launch_hd<64>(p, i8, st);
-        case 96: return launch_hd<96>(p, i8, st);
-        case 128: return launch_hd<128>(p, i8, st);
-        default: return launch_hd<256>(p, i8, st);
+        case 64: return launch_hd<64>(p, plan.grid, i8, st);
+        case 96: return launch_hd<96>(p, plan.grid, i8, st);
+        case 128: return launch_hd<128>(p, plan.grid, i8, st);
+        default: return launch_hd<256>(p, plan.grid, i8, st);
     }
 }
 

@@ -401,3 +401,20 @@ def test_infinities_seen_with_little_weight(new, length, gap):
     assert (got[..., 13] == float("inf")).all()
     got[..., [1, 13, 40]] = 0.0
     assert torch.isfinite(got).all()
+
+
+def test_a_batch_too_large_for_one_kernel_writes_nothing():
+    """A mixed batch whose chunk fits its launch and whose decoding sequences do not."""
+    n, kv = 16500, 512
+    q = torch.zeros((n + 199, kv, 8), dtype=torch.float16, device="cuda")
+    k = torch.zeros((1, 1024, kv, 8), dtype=torch.float16, device="cuda")
+    starts = torch.arange(n + 1, dtype=torch.int32)
+    starts[1:] += 199
+    lens = torch.ones(n, dtype=torch.int32)
+    lens[0] = 200
+    cache = capi.PagedKV(k, k, torch.zeros((n, 1), dtype=torch.int32, device="cuda"))
+    batch = capi.SeqBatch(starts.cuda(), lens.cuda(), n + 199, 200, 200)
+    out = torch.full_like(q, 7.0)
+    with pytest.raises(rxq4.RxQ4Error):
+        capi.attention_paged_f16(out, q, batch, cache, 1.0)
+    assert (out == 7.0).all()
