@@ -248,7 +248,7 @@ typedef struct rxq4_seq_batch {
  * in pairs (i, i + n_rot / 2), or (2 i, 2 i + 1) where `interleaved`, and the
  * store of keys and values into the cache's slots of their positions.
  *   q_out   fp16 [n_tokens][n_heads][head_dim]; may be q itself where that is
- *           fp16 with the same stride, and overlap it in no other way
+ *           fp16 with the same stride, and overlap q, k and v in no other way
  *   q, k, v x_dtype (F16, BF16, F32), 16-byte aligned, rows q_stride / kv_stride
  *           elements apart (multiples of 8): slices of one fused output, or
  *           three arrays

@@ -565,11 +565,15 @@ int rxq4_qk_norm_rope(void *q_out, const void *q, const void *k, const void *v, 
         return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: an int8 cache needs both scale arrays", fn);
     const int64_t esz = x_dtype == RXQ4_DTYPE_F32 ? 4 : 2;
     const uintptr_t o0 = reinterpret_cast<uintptr_t>(q_out), o1 = o0 + (uintptr_t)(batch->n_tokens * q_row * 2);
-    const uintptr_t i0 = reinterpret_cast<uintptr_t>(q),
-                    i1 = i0 + (uintptr_t)(((batch->n_tokens - 1) * q_stride + q_row) * esz);
-    if (o0 < i1 && i0 < o1 && !(o0 == i0 && x_dtype == RXQ4_DTYPE_F16 && q_stride == q_row))
+    const auto over = [&](const void *x, int64_t stride, int64_t row) {
+        const uintptr_t i0 = reinterpret_cast<uintptr_t>(x);
+        return o0 < i0 + (uintptr_t)(((batch->n_tokens - 1) * stride + row) * esz) && i0 < o1;
+    };
+    if (over(q, q_stride, q_row) && !(q_out == q && x_dtype == RXQ4_DTYPE_F16 && q_stride == q_row))
         return set_error(RXQ4_STATUS_INVALID_ARGUMENT,
                          "%s: q_out overlaps q (it may be q itself, fp16 and without gaps)", fn);
+    if (over(k, kv_stride, kv_row) || over(v, kv_stride, kv_row))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: q_out overlaps k or v", fn);
     if ((s = check_device(fn)) != RXQ4_STATUS_SUCCESS) return s;
     return from_hip(rxq4::launch_qk_norm_rope(static_cast<uint16_t *>(q_out), q, k, v, x_dtype, q_stride,
                                               kv_stride, n_heads, q_weight, k_weight, eps, inv_freq, n_rot,

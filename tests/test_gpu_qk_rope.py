@@ -310,3 +310,15 @@ def test_sines_next_to_half_turns(interleaved):
     bound = 12 * ref.U * np.abs(want) + 1e-10 + ref.H16 * np.abs(want) + ref.TINY16
     off = np.abs(got[0, :, to].cpu().double().numpy() - want)
     assert (off <= bound).all(), (off / bound).max()
+
+
+def test_output_between_its_inputs():
+    """q_out right behind the values and right before the keys: no overlap."""
+    p = ref.Paged(57, 8, 2, 64, 16, [9], [30])
+    x = inputs(p, F16, False)
+    args = (freqs(64), None, None, 1e-6, False)
+    flat = torch.cat([x[2].flatten(), torch.full((9 * 8 * 64,), 7.0, dtype=F16), x[1].flatten()]).cuda()
+    v, out, k = flat[:9 * 128].view(9, 2, 64), flat[9 * 128:-9 * 128].view(9, 8, 64), flat[-9 * 128:].view(9, 2, 64)
+    cache, batch = p.device(capi)
+    capi.qk_norm_rope(out, x[0].cuda(), k, v, batch, cache, args[0].cuda())
+    check(p, x, out, cache, *args)

@@ -179,3 +179,11 @@ def test_pages_that_share_memory_are_refused():
     apart = torch.zeros((3, 2, 16, 2, 64), dtype=torch.float16)
     assert capi.PagedKV(apart[:, 0], apart[:, 1], table).struct.page_stride == 4096
     assert capi.PagedKV(page, page, table).struct.page_stride == 2048
+
+
+@pytest.mark.parametrize("over", [dict(q_out=3 * P), dict(q_out=4 * P), dict(q_out=3 * P - 16),
+                                  dict(q_out=4 * P + 1264), dict(q_out=4 * P + 2544, x_dtype=0),
+                                  dict(q_out=3 * P + 8192, kv_stride=4096)])
+def test_rope_output_over_keys_or_values(over):
+    """5 rows of 128 elements: 1280 bytes of fp16, 2560 of fp32."""
+    refused(_rope(**over), "overlaps")
