@@ -268,9 +268,9 @@ int rxq4_qk_norm_rope(void *q_out, const void *q, const void *k, const void *v, 
 
 /* NEW.  Attention of each sequence's new tokens over its pages: a token at
  * position p attends to positions [0, p] (causal), holes left out; fp32
- * softmax, fp16 out [n_tokens][n_heads][head_dim].  A batch may mix decoding
- * sequences (one new token), drafts and prompt chunks.  A token that sees
- * nothing gets zeros.  What the cache holds at positions a token does not see
+ * softmax, fp16 q and out [n_tokens][n_heads][head_dim]; out may be q itself, and
+ * overlap it in no other way.  A batch may mix decoding sequences (one new
+ * token), drafts and prompt chunks.  A token that sees nothing gets zeros.  What the cache holds at positions a token does not see
  * does not reach its row, infinities and NaN included.  Few tokens on long
  * contexts split over the stream's workspace described above (a graph captured
  * with such a call uses the capturing stream's, also where it is replayed on

@@ -593,6 +593,9 @@ int rxq4_attention_paged_f16(void *out, const void *q, int n_heads, float scale,
     if (batch->n_seqs == 0 || batch->n_tokens == 0 || batch->max_new == 0) return ok();
     if (!out || !q || !aligned16(out) || !aligned16(q))
         return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: q/out null or not 16-byte aligned", fn);
+    const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(q);
+    if (o != i && (o < i ? i - o : o - i) < (uintptr_t)((int64_t)batch->n_tokens * n_heads * cache->head_dim * 2))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: out overlaps q (it may be q itself)", fn);
     if ((s = check_device(fn)) != RXQ4_STATUS_SUCCESS) return s;
     return from_hip(rxq4::launch_attention_paged(static_cast<uint16_t *>(out), static_cast<const uint16_t *>(q),
                                                  n_heads, scale, device_batch(*batch), device_cache(*cache),

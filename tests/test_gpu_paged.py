@@ -418,3 +418,16 @@ def test_a_batch_too_large_for_one_kernel_writes_nothing():
     with pytest.raises(rxq4.RxQ4Error):
         capi.attention_paged_f16(out, q, batch, cache, 1.0)
     assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [700, 40, 1]), ([1, 3], [5000, 2000]), ([33, 70], [300, 3000]),
+                                      ([1, 150, 1, 2], [900, 400, 1, 3000]), ([300], [300])])
+@pytest.mark.parametrize("int8", [False, True])
+def test_in_place(new, lens, int8):
+    """out is q: whole rows and split ones, both kernels, alone and together."""
+    p = ref.Paged(45, 16, 2, 128, 16, new, lens, int8)
+    cache, batch = p.device(capi)
+    want = attend(p, 0.09, cache, batch)
+    q = p.q.cuda()
+    capi.attention_paged_f16(q, q, batch, cache, 0.09)
+    assert torch.equal(q, want)

@@ -187,3 +187,9 @@ def test_pages_that_share_memory_are_refused():
 def test_rope_output_over_keys_or_values(over):
     """5 rows of 128 elements: 1280 bytes of fp16, 2560 of fp32."""
     refused(_rope(**over), "overlaps")
+
+
+@pytest.mark.parametrize("out,q", [(P, P + 16), (P + 16, P), (P, P + 5104), (P + 5104, P)])
+def test_attention_output_partly_over_the_queries(out, q):
+    """5 rows of 8 heads of 64: 5120 bytes."""
+    refused(_attend(out=out, q=q), "overlaps")
