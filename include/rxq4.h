@@ -64,7 +64,7 @@ extern "C" {
 #define RXQ4_GGML_TYPE_Q6_K 14
 #define RXQ4_MAX_K 65536
 /* Limits of the serving entry points (rxq4_qk_norm_rope, rxq4_attention_paged_f16,
- * rxq4_sample_f32). */
+ * rxq4_sample_f32, whose n_rows is at most RXQ4_MAX_TOKENS). */
 #define RXQ4_MAX_SEQS 65536
 #define RXQ4_MAX_TOKENS 1048576
 #define RXQ4_MAX_POSITIONS 16777216

@@ -607,9 +607,10 @@ int rxq4_sample_f32(int32_t *ids, const float *logits, int64_t row_stride, int n
                     int n_vocab, const float *temperature, const int32_t *top_k,
                     const float *top_p, const float *min_p, const float *u, void *stream) {
     const char *fn = "rxq4_sample_f32";
-    if (n_rows < 0 || n_vocab <= 0 || n_vocab > RXQ4_MAX_VOCAB || row_stride < n_vocab)
-        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: n_rows=%d n_vocab=%d (1 to %d) row_stride=%lld", fn,
-                         n_rows, n_vocab, RXQ4_MAX_VOCAB, (long long)row_stride);
+    if (n_rows < 0 || n_rows > RXQ4_MAX_TOKENS || n_vocab <= 0 || n_vocab > RXQ4_MAX_VOCAB || row_stride < n_vocab)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT,
+                         "%s: n_rows=%d (at most %d) n_vocab=%d (1 to %d) row_stride=%lld", fn, n_rows,
+                         RXQ4_MAX_TOKENS, n_vocab, RXQ4_MAX_VOCAB, (long long)row_stride);
     if (n_rows == 0) return ok();
     if (!ids || !logits || !u) return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: null ids, logits or u", fn);
     const int s = check_device(fn);

@@ -193,3 +193,8 @@ def test_rope_output_over_keys_or_values(over):
 def test_attention_output_partly_over_the_queries(out, q):
     """5 rows of 8 heads of 64: 5120 bytes."""
     refused(_attend(out=out, q=q), "overlaps")
+
+
+def test_more_rows_than_the_limit():
+    """2^20 rows, as for the other operators; the launches count them in 32 bits."""
+    refused(_sample(n_rows=(1 << 20) + 1), "n_rows")
