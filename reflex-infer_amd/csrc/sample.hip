@@ -7,8 +7,11 @@
 // which bin a place lies, and only that bin's logits (or, where the kept ones are
 // few, all down to there at once) are sorted.
 // Weights exp((l - max) / T) are formed in 64 bits and summed as whole numbers, so
-// the sums depend on no order: off by half a unit (2^-49 of a slice's largest weight,
-// and 2^-(63 - log2 n_vocab) of the row's) a logit.
+// the sums depend on no order: off by half a unit (2^-49 of a slice's largest weight) a
+// logit, and by 2^-(63 - log2 n_vocab) of the row's largest for each block of a slice.
+// Within a block the unit is as small as the row's sum leaves room for (2^-61 of it):
+// with 2^-(62 - log2 n_vocab) of the largest weight a draw among a million equal weights
+// of 2^-23 went a token wide.
 //
 //   sample_slices_kernel  a workgroup per slice of a row (in registers): its largest
 //       logit, the count and weight of 512 bins of 1/16 in (l / T) on a grid that all
@@ -70,7 +73,7 @@ struct SampleParams {
     Slice *slices;      // [row][slice]
     uint16_t *index;    // [row][slice][per]: indices in the slice, by bin
     int row0, n_slices, per;
-    double unit;        // weight units of a row
+    double unit;        // weight units of a row's blocks
 };
 
 // e^-d for d >= 0 (0 from 100 on): 2^-n of the nearest whole n = d / ln 2, and the
@@ -124,6 +127,10 @@ __device__ __forceinline__ u64 wave_prefix64(u64 x) {
     x = dpp_add_from64<0x118, 0xF>(x);
     x = dpp_add_from64<0x142, 0xA>(x);
     return dpp_add_from64<0x143, 0xC>(x);
+}
+__device__ __forceinline__ u64 lane_63(u64 x) {
+    return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, 63) |
+           (u64)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32;
 }
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
@@ -346,7 +353,7 @@ struct Picker {
     Pick &sh;
     int r, row;
     float top;
-    double inv_t;
+    double inv_t, unit;
     // the window: n places from rank base_rank on
     int n;
     uint32_t base_rank;
@@ -355,7 +362,7 @@ struct Picker {
     uint32_t logits;     // of the bins last gathered
 
     __device__ u64 weight(uint32_t key) const {
-        return (u64)rint(weight_of(key_value(key), top, inv_t) * p.unit);
+        return (u64)rint(weight_of(key_value(key), top, inv_t) * unit);
     }
     __device__ const Slice &slice(int s) const { return p.slices[(int64_t)r * p.n_slices + s]; }
     __device__ float logit(int s, uint32_t i) const {
@@ -695,7 +702,7 @@ struct Picker {
 
 __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams p) {
     __shared__ Pick sh;
-    __shared__ int top_bin;
+    __shared__ int top_bin, finer;
     __shared__ uint32_t top_key;
     const int tid = threadIdx.x, r = blockIdx.x, row = p.row0 + r;
     const SampleRows &a = p.a;
@@ -769,13 +776,18 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams p) {
         u64 m = tid < kBlocks ? sh.block_mass[tid] : 0;
         c = (uint32_t)wave_prefix((int)c);
         m = wave_prefix64(m);
+        // the row's sum to 2^61 up to 2^62: room for the roundings of its parts
+        const int up = max(__builtin_clzll(lane_63(m)) - 2, 0);
         if (tid < kBlocks) {
             sh.block_count[tid] = c;
-            sh.block_mass[tid] = m;
+            sh.block_mass[tid] = m << up;
         }
+        if (tid == 0) finer = up;
     }
     __syncthreads();
-    Picker pick{p, sh, r, row, top, inv_t, 0, 0, 0, 0, -1, 0};
+    const double fine = ldexp(1.0, finer);
+    if (tid < p.n_slices) sh.scale[tid] *= fine;
+    Picker pick{p, sh, r, row, top, inv_t, p.unit * fine, 0, 0, 0, 0, -1, 0};
     uint32_t keep = sh.block_count[kBlocks - 1];
     u64 kept = sh.block_mass[kBlocks - 1];
     const bool by_k = k > 0 && (uint32_t)k < keep;

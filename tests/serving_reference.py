@@ -161,3 +161,31 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     x = min(max(0.0 if np.isnan(u) else float(u), 0.0), 1 - 2.0 ** -24)
     c = np.cumsum(w[:n])
     return int(order[min(n - 1, int((c <= x * c[-1]).sum()))])
+
+
+def sample_margin(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    """How near a row's token (of `sample`, finite logits) is to another one: the
+    smallest distance of top-p's share and of the draw from a sum of weights, over the
+    largest weight, and of min-p from a weight, over it."""
+    if temperature is not None and not float(temperature) > 0:
+        return 1.0
+    x = -np.sort(-logits.astype(np.float64))
+    w = np.exp((x - x[0]) / (1.0 if temperature is None else float(temperature)))
+    n, near = len(w), 1.0
+    if top_k is not None and top_k > 0:
+        n = min(n, int(top_k))
+
+    def border(sums, at):
+        i = int(np.searchsorted(sums, at))
+        return min(abs(s - at) for s in sums[max(i - 1, 0):i + 1])
+
+    if top_p is not None and float(top_p) < 1:
+        c = np.cumsum(w[:n])
+        share = float(top_p) * c[-1]
+        near = min(near, border(c, share))
+        n = max(1, int((np.concatenate([[0.0], c[:-1]]) < share).sum()))
+    if min_p is not None and float(min_p) > 0:
+        near = min(near, float((abs(w[:n] - float(min_p)) / float(min_p)).min()))
+        n = max(1, min(n, int((w[:n] >= float(min_p)).sum())))
+    c = np.cumsum(w[:n])
+    return min(near, border(c, min(max(float(u), 0.0), 1 - 2.0 ** -24) * c[-1])) if n > 1 else near

@@ -208,3 +208,90 @@ def test_two_streams_at_once():
         assert ids.tolist() == [ref.sample(a, x) for a, x in zip(l.numpy(), u.numpy())]
     for s in streams:
         capi.release_workspace(s)
+
+
+# What the sums may be off by, over the row's largest weight W: a weight of a slice half
+# of 2^-48 of the slice's largest, a block's sum of a slice (32 of each, 512 slices at most)
+# half a unit of 2^-(62 - log2 n) W, the 64-bit sums of the reference n 2^-53 of n W.
+def sums_off(vocab, total):
+    bits = int(vocab - 1).bit_length()
+    return vocab * 2.0 ** -49 + 512 * 32 * 2.0 ** -(63 - bits) + vocab * 2.0 ** -53 * total
+
+
+@pytest.mark.parametrize("vocab", [151936, 1048576, 1048577, 4194304])
+def test_a_draw_among_many_small_weights(vocab):
+    """One logit 16 above all others, which are equal: the token is the draw's place
+    among weights of 2^-23 of the largest.  Draws are taken whose place is 0.2 tokens or
+    more from the next, which is more than the sums are off."""
+    top, w = 12345, np.exp(-16.0)
+    total = 1 + (vocab - 1) * w
+    assert 0.2 * w > sums_off(vocab, total)
+    u = (np.arange(1, 4000) / 4000).astype(np.float32)
+    at = (u.astype(np.float64) * total - 1) / w
+    ok = np.flatnonzero((at > 1) & (at % 1 > 0.2) & (at % 1 < 0.8))
+    ok = ok[::len(ok) // 20]
+    u, at = u[ok], at[ok].astype(np.int64)
+    l = np.zeros((1, vocab), np.float32)
+    l[0, top] = 16.0
+    dev = torch.from_numpy(l).cuda()
+    ids = torch.empty(1, dtype=I, device="cuda")
+    us = torch.from_numpy(u).cuda()
+    got = []
+    for i in range(len(u)):
+        capi.sample_f32(ids, dev, us[i:i + 1])
+        got.append(int(ids.item()))
+    assert got == [int(j) + (j >= top) for j in at]
+
+
+@pytest.mark.parametrize("vocab", [1048576, 1048577, 4194304])
+@pytest.mark.parametrize("kind", ["model", "equal"])
+def test_vocabularies_to_the_limit(vocab, kind):
+    """512 slices of 2048 logits, the switch to 8192, and 512 of those."""
+    print(f"sample vocab={vocab} {kind}", flush=True)
+    l = logits_of(vocab, 1, vocab, kind)
+    weight = float(np.exp(l[0].astype(np.float64) - l[0].max()).sum())
+    off = sums_off(vocab, weight) if kind == "model" else weight * 2.0 ** -50  # (equal weights: whole numbers)
+    for i, params in enumerate([dict(temperature=[0.0]), dict(top_k=[50]), dict(top_k=[100000]), dict(top_p=[0.9]),
+                                dict(min_p=[0.05]), dict(temperature=[0.7], top_k=[3000], top_p=[0.95], min_p=[0.02])]):
+        one = {k: int(v[0]) if k == "top_k" else np.float32(v[0]) for k, v in params.items()}
+        # the first of a few draws that no error of the sums could move
+        u = next(x for x in np.float32([0.13, 0.37, 0.59, 0.71, 0.83, 0.97])
+                 if ref.sample_margin(l[0], x, **one) > off)
+        check(l, [u], **params)
+
+
+def test_repeats_and_replays_of_known_draws():
+    """As above with seeded inputs, every draw and share further from a border than the
+    sums are off."""
+    n, vocab = 6, 40000
+    g = torch.Generator().manual_seed(93)
+    l = torch.from_numpy(logits_of(11, n, vocab, "model")).cuda()
+    u, p = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    ids = torch.empty(n, dtype=I, device="cuda")
+    k = torch.full((n,), 30, dtype=I, device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    capi.sample_f32(ids, l, u, top_k=k, top_p=p, stream=s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        capi.sample_f32(ids, l, u, top_k=k, top_p=p, stream=s)
+    for step in range(5):
+        host = l.cpu() + 0.1 * torch.randn((n, vocab), generator=g)
+        l.copy_(host)
+        draws, shares = torch.rand(n, generator=g), 0.5 + 0.5 * torch.rand(n, generator=g)
+        u.copy_(draws)
+        p.copy_(shares)
+        k.fill_(5 + 2000 * step)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            graph.replay()
+        torch.cuda.synchronize()
+        eager = torch.empty_like(ids)
+        capi.sample_f32(eager, l, u, top_k=k, top_p=p)
+        assert torch.equal(eager, ids)
+        rows = list(zip(host.numpy(), draws.numpy(), shares.numpy()))
+        for row, x, share in rows:
+            total = float(np.exp(row.astype(np.float64) - row.max()).sum())
+            assert ref.sample_margin(row, x, top_k=5 + 2000 * step, top_p=share) > sums_off(vocab, total)
+        assert ids.tolist() == [ref.sample(row, x, top_k=5 + 2000 * step, top_p=share) for row, x, share in rows]
