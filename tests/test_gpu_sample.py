@@ -295,3 +295,20 @@ def test_repeats_and_replays_of_known_draws():
             total = float(np.exp(row.astype(np.float64) - row.max()).sum())
             assert ref.sample_margin(row, x, top_k=5 + 2000 * step, top_p=share) > sums_off(vocab, total)
         assert ids.tolist() == [ref.sample(row, x, top_k=5 + 2000 * step, top_p=share) for row, x, share in rows]
+
+
+@pytest.mark.parametrize("bits", [0x7F800001, 0x7FA00000, 0xFFBFFFFF, 0x7FFFFFFF, 0xFFC00001])
+@pytest.mark.parametrize("vocab", [5, 1000, 9000])
+def test_nan_of_every_kind(bits, vocab):
+    """Signalling ones and those with a sign: as -infinity, the row's first and last logit
+    and others between."""
+    l = logits_of(vocab, 3, vocab, "wide") if vocab < 64 else logits_of(vocab, 3, vocab, "model")
+    at = np.unique(np.array([0, vocab // 3, vocab - 1]))
+    l[:, at] = np.array(bits, np.uint32).view(np.float32)
+    l[2, :] = np.array(bits, np.uint32).view(np.float32)
+    assert (l.view(np.uint32)[:, at] == bits).all()
+    got = [run(l, [0.3, 0.9, 0.5], temperature=t) for t in (None, [0.0] * 3)]
+    clean = np.where(np.isnan(l), -np.inf, l).astype(np.float32)
+    for g, t in zip(got, (None, 0.0)):
+        assert g.tolist() == [ref.sample(c, x, temperature=t) for c, x in zip(clean, [0.3, 0.9, 0.5])]
+        assert g[2] == -1
