@@ -274,9 +274,16 @@ int rxq4_qk_norm_rope(void *q_out, const void *q, const void *k, const void *v, 
  * does not reach its row, infinities and NaN included.  Few tokens on long
  * contexts split over the stream's workspace described above (a graph captured
  * with such a call uses the capturing stream's, also where it is replayed on
- * another).  The split follows the lengths of the whole batch as they are on the
- * device: the same batch gives the same bits, a sequence in another batch the
- * same within rounding.
+ * another).  The split depends on the whole batch: the same batch gives the same
+ * bits, a sequence in another batch the same within rounding.
+ * What the split follows, rows being new tokens x n_heads / n_kv_heads:
+ *   sequences of up to 16 rows   the lengths on the device, in batches of up to 256
+ *       sequences; max_len and table_stride may be capacities.  Past 256 the host's
+ *       limits: max_len or table_stride far above the lengths leave long chunks
+ *   sequences of more            the lengths on the device too, but only where
+ *       n_tokens * n_heads is below 128 per CU and the batch has at most 1024
+ *       sequences.  Above either no sequence is split: a short chunk after a long
+ *       context goes apart from some hundred decoding sequences or padding rows
  * No counterpart in the reference, whose KernelSupport names
  * paged_decode_attention. */
 int rxq4_attention_paged_f16(void *out, const void *q, int n_heads, float scale,

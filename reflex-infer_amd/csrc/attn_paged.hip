@@ -11,15 +11,16 @@
 // for all of them.
 //
 // Bound: reading the cache, in pieces of a head's row (256 bytes at head_dim 128,
-// fp16), which a plain read of the same pieces does at 5.6 to 5.8 TB/s (128-byte
-// pieces of int8: 5.1 to 5.3).  So a step's loads are issued a step ahead, nothing
-// of K passes LDS, and the chunks are cut from the batch's own lengths, which only
-// the device knows.
+// fp16).  Loops that do nothing else read such pieces, 8 heads' rows together, at 5.3 to
+// 5.8 TB/s, by which lane and XCD takes what, 128-byte pieces of int8 at 4.9 to 5.4, and
+// 4 KB pieces at 6.0.  So a step's loads are issued a step ahead, nothing of K passes
+// LDS, and the chunks are cut from the batch's own lengths, which only the device knows
+// (up to kSeqs sequences).
 // Measured, 32 / 8 heads of 128, one new token a sequence, pages of 16: 512
-// sequences of 1023 positions 366 us (5.9 TB/s), 256 of 2047 380 (5.7), 64 of 64 to
-// 8000 92 (4.7); int8 512 of 1023 214 (5.2), 256 of 2047 228 (4.9), 16 of 20000 to
-// 40000 202 (4.9).  A call's fixed part (launch, first loads, the chunks' ends, the
-// combine) is about 20 us at 64 sequences and 8 at one.
+// sequences of 1023 positions 372 us (5.8 TB/s), 256 of 2047 397 (5.4), 64 of 64 to
+// 8000 92 (4.7); int8 512 of 1023 231 (4.8; pages of 64 221), 256 of 2047 246 (4.5), 16
+// of 20000 to 40000, pages of 64, 202 (4.9).  A call's fixed part (launch, first loads,
+// the chunks' ends, the combine) is about 20 us at 64 sequences and 8 at one.
 #include <math.h>
 
 #include <algorithm>
@@ -606,7 +607,9 @@ __global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedParams p) 
 // an fp16 and twelve of an int8 cache a CU (three to four of what runs at a time, for
 // sequences of any lengths): 64 sequences of 64 to 8000 positions, 8 heads, fp16, 5 / 6
 // / 8 / 12 a CU 98.7 / 91.7 / 94.6 / 103 us; 16 of 20000 to 40000, int8, 6 / 8 / 12 / 16
-// 213 / 208 / 202 / 204.  Past kSeqs sequences there is little to cut: the host's chunks.
+// 213 / 208 / 202 / 204.  Past kSeqs sequences the host cuts them from the limits: 299
+// sequences of 500 positions and one of 13000 159 us, with max_len 131072 271; 255 and one
+// on the device 125 and 134.
 struct RowsPlan {
     int64_t slots;  // chunks of the batch at most, per KV head
     int64_t grid;   // workgroups

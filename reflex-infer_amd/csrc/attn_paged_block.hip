@@ -19,13 +19,17 @@
 //            chunk length from the batch's lengths: the shortest that leaves at most
 //            a workgroup a CU (their 130 KB of LDS).  Chunks cut by the host from the
 //            lengths' limit took 34.7 us on 12 drafts of 3 to 6 tokens after 500 to 6000
-//            positions (28 / 4 heads), so 25.4.  A workgroup leaves (O, m, l) per query
-//            row; attn_paged_block_combine adds a row's chunks in order.
+//            positions (28 / 4 heads), so 25.  A workgroup leaves (O, m, l) per query
+//            row; attn_paged_block_combine adds a row's chunks in order.  The host
+//            allows it (it launches the combine and lays the partials out by rows) where
+//            the rows of the batch could not fill the CUs, decoding and padding rows
+//            counted: 16 tokens of 64 / 8 heads after 30000 positions 51 us, with 584 rows
+//            of padding or beside 512 decoding sequences, unsplit, 641 and 790.
 // Bound: the chain of a tile in a wave (scores, maximum, exponentials, staging, P.V: 7000
 // to 8500 cycles, 1536 of them its matrix instructions) between two barriers; the two
 // waves of a SIMD are in the same part of it.
 // Measured, 32 / 8 heads of 128, fp16: 512 tokens of 16 / 2 heads after 7000 positions
-// 64.8 us (469 TFLOP/s), four prompts of 1254 to 3615 tokens 323 to 336 (525 to 546).
+// 65 us (467 TFLOP/s), four prompts of 1254 to 3615 tokens 323 to 340 (519 to 546).
 // The second wave group a phase later (V weighed an iteration after its scores, a third V
 // buffer) made the prompts 341, a table load outside branches 356, raised priorities for
 // the products or fences between the phases 332 to 336.

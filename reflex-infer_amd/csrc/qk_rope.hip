@@ -22,7 +22,7 @@
 // Bound: for many tokens the rows' bytes, in and out; for a few the chain of lengths,
 // table entry, sine and store.  So a few tokens' heads are spread over workgroups, a pass
 // each; many tokens keep all heads in one, which shares the sines.
-// Measured, 32 / 8 heads of 128: 3595 tokens from bf16 24.1 us (3.7 TB/s; a copy of the
+// Measured, 32 / 8 heads of 128: 3595 tokens from bf16 24.4 us (3.6 TB/s; a copy of the
 // bytes 17; 31 with each row's loads after the sines), 64 tokens into int8 4.9, one token
 // of 16 / 2 heads 4.1.
 #include <math.h>

@@ -24,7 +24,7 @@
 // Bound: two launches, the 64-bit arithmetic of a slice (some 40 instructions a
 // logit), and the pick's chain of dependent steps in one workgroup.
 // Measured, 151936 logits a row: one row 17 us (slices 5, pick 11), 128 rows of mixed
-// settings 78 to 83 (slices 46, pick 35: a row whose nucleus ends among thousands of
+// settings 78 to 83 (slices 45, pick 35: a row whose nucleus ends among thousands of
 // equally likely logits takes 35, the others 8 to 12).
 #include <math.h>
 
