@@ -63,13 +63,16 @@ extern "C" {
 #define RXQ4_GGML_TYPE_Q5_K 13
 #define RXQ4_GGML_TYPE_Q6_K 14
 #define RXQ4_MAX_K 65536
-/* Limits of the serving entry points (rxq4_qk_norm_rope, rxq4_attention_paged_f16,
- * rxq4_sample_f32, whose n_rows is at most RXQ4_MAX_TOKENS). */
+/* Limits of the serving entry points (rxq4_qk_norm_rope and _axes, rxq4_attention_paged_f16,
+ * rxq4_kv_bounds, rxq4_select_pages, rxq4_attention_selected_f16, rxq4_sample_f32, whose
+ * n_rows is at most RXQ4_MAX_TOKENS). */
 #define RXQ4_MAX_SEQS 65536
 #define RXQ4_MAX_TOKENS 1048576
 #define RXQ4_MAX_POSITIONS 16777216
 #define RXQ4_MAX_HEADS 1024
 #define RXQ4_MAX_VOCAB 4194304
+#define RXQ4_MAX_AXES 16
+#define RXQ4_MAX_SELECT 4096
 
 /* Element types for the typed GEMM entry point. */
 #define RXQ4_DTYPE_F32 0
@@ -289,6 +292,79 @@ int rxq4_qk_norm_rope(void *q_out, const void *q, const void *k, const void *v, 
 int rxq4_attention_paged_f16(void *out, const void *q, int n_heads, float scale,
                              const rxq4_seq_batch *batch, const rxq4_paged_kv *cache,
                              void *stream);
+
+/* NEW.  rxq4_qk_norm_rope with the angles from coordinates of the caller's instead of
+ * the position in the cache: tokens of images and video have a time, a height and a
+ * width, and text behind them does not go on at the cache's position.
+ *   positions  int32, device: the coordinate of token t (a row of q) on axis a is
+ *              positions[a * position_stride + t], any whole number; n_axes axes, 1 to 16
+ *   axis_of    int32 [n_rot / 2], device: the axis whose coordinate turns pair i, times
+ *              inv_freq[i]; a value outside [0, n_axes) counts as coordinate 0.  NULL:
+ *              axis 0 for every pair
+ * Everything else is rxq4_qk_norm_rope's, the slots of keys and values included: they
+ * follow from seq_lens.  With the cache's positions on one axis the results are its, bit
+ * for bit.  q_out may not overlap positions or axis_of.
+ * No counterpart in the reference (rxq4_qk_norm_rope). */
+int rxq4_qk_norm_rope_axes(void *q_out, const void *q, const void *k, const void *v, int x_dtype,
+                           int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_weight,
+                           const float *k_weight, float eps, const float *inv_freq, int n_rot,
+                           int interleaved, const int32_t *positions, int64_t position_stride,
+                           int n_axes, const int32_t *axis_of, const rxq4_seq_batch *batch,
+                           const rxq4_paged_kv *cache, void *stream);
+
+/* NEW.  Attention over chosen pages, for long contexts, is three calls beside a paged
+ * cache: bounds of the pages' keys, kept up as tokens are stored; the choice of each
+ * token's pages by a score against the bounds; attention over the chosen pages.
+ *
+ * rxq4_kv_bounds: for every page that new tokens of the batch went to (rxq4_qk_norm_rope
+ * has stored them), and each KV head, the smallest and the largest key of each dim over
+ * the page's positions that its sequence has filled, computed anew.
+ *   bounds  int8 [n_pages][n_kv_heads][head_dim / 8][2][8], 16-byte aligned: of each 8 dims
+ *           the smallest, then the largest, rint(x / scale)
+ *   scales  fp32 [n_pages][n_kv_heads]: max(|smallest|, |largest|) / 127 over the dims
+ * lying beside the pool as the int8 scales do.  A NaN key is left out (a dim with
+ * nothing else gets 0); an infinity counts as fp32's largest number.  Positions and pages
+ * that rxq4_qk_norm_rope would not store to are left out.  Two sequences with new tokens
+ * in one page race.  A prompt's pages that came with their keys (a prefix that is shared
+ * or loaded) get theirs from a call whose batch has all its tokens as new ones; the batch's
+ * rows stand for no arrays here. */
+int rxq4_kv_bounds(void *bounds, float *scales, const rxq4_seq_batch *batch,
+                   const rxq4_paged_kv *cache, void *stream);
+
+/* NEW.  The pages that each new token's queries (fp16 [n_tokens][n_heads][head_dim], 16-byte
+ * aligned, after rotation) attend to, for each KV head.
+ *   pages    int32 [n_tokens][n_kv_heads][n_select]: places in the sequence's row of
+ *            page_table, ascending; -1 behind the last.  n_select: 1 to 4096
+ *   chosen   of the pages in the pool with a position that the token sees: the first
+ *            n_first and the last n_last of the sequence (holes among them are left out),
+ *            and those with the largest scores until there are n_select, of equal scores
+ *            the first pages.  n_first + n_last is at most n_select.  (n_last 1 or more
+ *            keeps the page that the token itself is in)
+ *   score    the largest, over the heads of the KV head's group, of
+ *            (sum_d max(z_d lo_d, z_d hi_d)) * step * scale, in this order in fp32, where
+ *            lo, hi and scale are the page's bounds, step = max |q| / 127 and z = rint(q /
+ *            step) of the head's query (NaN as 0, infinities as 65504): up to the
+ *            steps no key of the page has a larger product with the query.  The sum is
+ *            exact, so the lists do not depend on how the work is cut
+ * Tokens that see nothing get -1s.  Rows of no sequence are left as they are.  A few
+ * tokens with many pages use the stream's workspace described above. */
+int rxq4_select_pages(int32_t *pages, int n_select, int n_first, int n_last, const void *q,
+                      int n_heads, const void *bounds, const float *scales,
+                      const rxq4_seq_batch *batch, const rxq4_paged_kv *cache, void *stream);
+
+/* NEW.  rxq4_attention_paged_f16 over the positions of listed pages alone: each token's
+ * query heads attend to the positions up to its own of the pages that `pages`
+ * [n_tokens][n_kv_heads][n_select] (int32, device; rxq4_select_pages) lists for the token
+ * and KV head.  Entries in any order; those that name no page with a position that the
+ * token sees (-1, holes, pages behind its own) are left out; one that is there twice counts
+ * twice.  n_select: 1 to 4096.  out may be q itself and overlap it in no other way, nor
+ * pages.  A token that sees nothing gets zeros; what lies where a token does not look does
+ * not reach its row, infinities and NaN included.  Few tokens split their lists over the
+ * stream's workspace described above, by the host's sizes alone.
+ * No counterpart in the reference (rxq4_attention_paged_f16). */
+int rxq4_attention_selected_f16(void *out, const void *q, int n_heads, float scale,
+                                const int32_t *pages, int n_select, const rxq4_seq_batch *batch,
+                                const rxq4_paged_kv *cache, void *stream);
 
 /* NEW.  The next token of each row of logits [n_rows][n_vocab] (fp32, rows
  * row_stride elements apart), from u[row] in [0, 1) (clamped to it; NaN: 0).

@@ -27,6 +27,9 @@ struct PagedParams {
     int chunk;            // 16 rows: positions per chunk where the host cuts them
     int most_tiles;       // 128 rows: tiles of a block at most
     int *chunk_tiles;     // 128 rows: tiles of a chunk, left for the combine
+    const int32_t *lists;  // selected pages: those of each token and KV head
+    int n_select;          // entries of a list
+    int head_blocks;       // selected pages: blocks of 16 heads of a group
 };
 
 // sum + w x, x a part relative to its own maximum and w its weight beside the other

@@ -48,8 +48,11 @@ __device__ __forceinline__ float log2_scale(float vs) {
 }
 
 // Waves per SIMD that the registers are cut to: what is in flight is what counts, and
-// an int8 step holds half the bytes of an fp16 one.
-constexpr int rows_waves(int hd, bool i8) { return hd > 128 ? 1 : hd == 64 ? 4 : i8 ? 3 : 2; }
+// an int8 step holds half the bytes of an fp16 one.  (With a list's page beside the entry,
+// small fp16 pages spill at four.)
+constexpr int rows_waves(int hd, bool i8, bool big, bool sel) {
+    return hd > 128 ? 1 : hd == 64 ? (sel && !i8 && !big ? 3 : 4) : i8 ? 3 : 2;
+}
 
 // Steps of the walk over a sequence (0: not this kernel's; one where its tokens see
 // nothing, to write their zeros).
@@ -102,6 +105,7 @@ struct RowsUnit {
     int s, c;           // sequence (-1: none), chunk
     int chunks, chunk;  // chunks of the sequence; positions of each
     int64_t slot;       // of the chunk's partials
+    int tok;            // selected pages: the token of the sequence
 };
 __device__ __forceinline__ RowsUnit rows_unit(const PagedParams &p, int idx) {
     RowsUnit r{};
@@ -143,6 +147,32 @@ __device__ __forceinline__ RowsUnit rows_unit(const PagedParams &p, int idx) {
     return r;
 }
 
+// Selected pages: a token, its KV head kvh, the heads of the group from head0 on, and a chunk
+// of the places.  An XCD (workgroups are dealt to the eight in turn) takes tokens of one KV
+// head one after another: a prompt's neighbours list much the same pages.
+__device__ __forceinline__ RowsUnit selected_unit(const PagedParams &p, int &kvh, int &head0) {
+    RowsUnit r{};
+    r.s = -1;
+    const int per = gridDim.x / 8;  // (a multiple of 8)
+    const int idx = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+    r.c = idx % p.n_chunks;
+    int at = idx / p.n_chunks;
+    const int block = at % p.head_blocks;
+    at /= p.head_blocks;
+    const int t = at % p.b.n_tokens;
+    kvh = at / p.b.n_tokens;
+    head0 = block * kPagedRows;
+    if (kvh >= p.c.n_kv) return r;
+    const int s = seq_of_row(p.b, t, r.span);
+    r.tok = t - r.span.row0;
+    if (s >= p.b.n_seqs || r.tok < 0 || r.tok >= min(r.span.n, p.b.max_new)) return r;
+    r.s = s;
+    r.chunk = p.chunk;
+    r.chunks = p.n_chunks;
+    r.slot = ((int64_t)t * p.n_chunks + r.c) * p.head_blocks + block;
+    return r;
+}
+
 // Wave w takes positions 32 w .. + 31 of every 128-position step of the chunk with
 // its own online softmax; the four waves merge at the end.  Per step, lane l =
 // 16 g + r:
@@ -165,8 +195,12 @@ __device__ __forceinline__ RowsUnit rows_unit(const PagedParams &p, int idx) {
 // Rows past the end or in holes are zeros (BIG: past the end of the operand's buffer
 // resource; else the pool's first row in their place, cleared), their scores
 // -infinity.
-template <int HD, bool I8, bool BIG>
-__global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kernel(PagedParams p) {
+//
+// SEL: a workgroup takes one token, up to 16 heads of a KV head's group, and one chunk of
+// the places of its listed pages, page_size a list entry; all rows see the same, so the
+// masks are the entries'.
+template <int HD, bool I8, bool BIG, bool SEL>
+__global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, SEL)) void attn_paged_rows_kernel(PagedParams p) {
     // A chunk is 16 bytes: 8 dims of fp16, 16 of int8, which are two k steps of a
     // product (a lane's dims need only be the same in K and Q).
     constexpr int EC = I8 ? 16 : 8;                     // dims of a chunk
@@ -186,11 +220,18 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
     // The KV heads of a sequence's chunk go to one XCD (workgroups are dealt to the eight in
     // turn): they read the same pages and scales (int8, 512 sequences of 1023 positions, 244
     // us with the heads on all, 216 so).  A sequence's chunks go to different ones.
-    const int x8 = blockIdx.x / 8, kvh = x8 % p.c.n_kv;
-    const RowsUnit unit = rows_unit(p, x8 / p.c.n_kv * 8 + blockIdx.x % 8);
+    int kvh, head0 = 0;
+    RowsUnit unit;
+    if constexpr (SEL) {
+        unit = selected_unit(p, kvh, head0);
+    } else {
+        const int x8 = blockIdx.x / 8;
+        kvh = x8 % p.c.n_kv;
+        unit = rows_unit(p, x8 / p.c.n_kv * 8 + blockIdx.x % 8);
+    }
     const int s = unit.s, c = unit.c, beg = c * unit.chunk;
     if (s < 0) return;  // uniform
-    if (p.n_chunks > 1 && c == 0 && kvh == 0 && tid == 0) {
+    if (!SEL && p.n_chunks > 1 && c == 0 && kvh == 0 && tid == 0) {
         p.firsts[2 * s] = (int)unit.slot;
         p.firsts[2 * s + 1] = unit.chunks;
     }
@@ -207,14 +248,51 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
     };
     // BIG: lane 2 j + st holds the entry of operand st of step j, for 32 steps; else the
     // lane's position's, one step ahead
-    auto entries = [&](int j) { return entry(beg + 32 * w + kStep * (j + (lane >> 1)) + 16 * (lane & 1)); };
-    int ent = BIG ? entries(0) : entry(p_lane), ent_next = BIG ? 0 : entry(p_lane + kStep);
     const SeqSpan span = unit.span;
-    const int rows = min(span.n, p.b.max_new) * p.group;
-    const int end_seq = min(span.pos0 + (rows - 1) / p.group + 1, limit);
+    // SEL: the list's page at place `at` (-1: none that the token sees), its page of the pool
+    // (-1: a hole), and how many of its positions from the place on the token sees
+    const int sees = SEL ? min(limit, span.pos0 + unit.tok + 1) : 0;
+    const int pages_seen = sees > 0 ? ((sees - 1) >> p.c.shift) + 1 : 0;
+    const int32_t *const list =
+        SEL ? p.lists + ((int64_t)(span.row0 + unit.tok) * p.c.n_kv + kvh) * p.n_select : nullptr;
+    auto listed = [&](int at) {
+        const int i = at >> p.c.shift, x = list[min(i, p.n_select - 1)];
+        return i < p.n_select && x >= 0 && x < pages_seen ? x : -1;
+    };
+    auto page_of = [&](int x) {
+        const int e = table[has_table ? max(x, 0) : 0], page = has_table ? e : x;
+        return x >= 0 && (unsigned)page < (unsigned)p.c.n_pages ? page : -1;
+    };
+    auto seen_from = [&](int x, int at) { return sees - (x << p.c.shift) - (at & ((1 << p.c.shift) - 1)); };
+    int there = 0;    // SEL, BIG: beside the entry, the operand's positions that the token sees
+    int x_ahead = 0;  // SEL, small pages: the list's page of the step after the newest entry's
+    auto entries = [&](int j) {
+        const int at = beg + 32 * w + kStep * (j + (lane >> 1)) + 16 * (lane & 1);
+        if constexpr (SEL) {
+            const int x = listed(at), page = page_of(x);
+            there = page >= 0 ? min(max(seen_from(x, at), 0), 16) : 0;
+            return page;
+        } else {
+            return entry(at);
+        }
+    };
+    auto next_entry = [&](int j) {  // small pages: the lane's position's of step j, asked for in order
+        const int at = p_lane + kStep * j;
+        if constexpr (SEL) {
+            const int x = j == 0 ? listed(at) : x_ahead;
+            x_ahead = listed(at + kStep);
+            const int page = page_of(x);
+            return seen_from(x, at) > 0 ? page : -1;
+        } else {
+            return entry(at);
+        }
+    };
+    int ent = BIG ? entries(0) : next_entry(0), ent_next = BIG ? 0 : next_entry(1);
+    const int rows = SEL ? min(p.group - head0, kPagedRows) : min(span.n, p.b.max_new) * p.group;
+    const int end_seq = SEL ? (limit > 0 ? p.n_select << p.c.shift : 0) : min(span.pos0 + (rows - 1) / p.group + 1, limit);
     const int end = min(end_seq, beg + unit.chunk);
     const int row = min(r, rows - 1);  // (columns past the last row repeat it)
-    const int tok = row / p.group, head = kvh * p.group + row % p.group;
+    const int tok = SEL ? unit.tok : row / p.group, head = kvh * p.group + (SEL ? head0 + row : row % p.group);
     const bool row_ok = r < rows;
     const int hd = p.c.hd, n_ch = hd / EC;
     const int64_t orow = ((int64_t)(span.row0 + tok) * p.n_heads + head) * hd;
@@ -268,7 +346,8 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
             for (int st = 0; st < 2; ++st) {
                 const int pos = beg + 32 * w + kStep * j + 16 * st;
                 page[st] = __builtin_amdgcn_readlane(e, (2 * j + st) & 63);
-                const int n = (unsigned)page[st] < (unsigned)p.c.n_pages ? max(min(end - pos, 16), 0) : 0;
+                const int n = SEL ? (pos < end ? __builtin_amdgcn_readlane(there, (2 * j + st) & 63) : 0)
+                              : (unsigned)page[st] < (unsigned)p.c.n_pages ? max(min(end - pos, 16), 0) : 0;
                 S.seen |= ((1u << n) - 1) << (16 * st);
                 page[st] = n > 0 ? page[st] : 0;
                 place[st] = pos & mask;
@@ -333,6 +412,7 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
     bool bad = false;  // some V is not finite
     uint32_t most_vs = 0;  // int8: the lane's largest |V scale|
     auto process = [&](int j, Step &S) {
+        if (SEL && S.seen == 0) return;  // uniform
         const int p0 = beg + kStep * j + 32 * w;
         f32x4 acc[2];
 #pragma unroll
@@ -374,11 +454,11 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
         float sv[8], mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sv[i] = acc[i >> 2][i & 3] * p.sl2;
-        if (part || p0 + 31 > span.pos0) {  // uniform: not every row sees all of them
+        if (part || (!SEL && p0 + 31 > span.pos0)) {  // uniform: not every row sees all of them
             const uint32_t in = S.seen >> (4 * g);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (!((in >> (16 * (i >> 2) + (i & 3))) & 1u) || p0 + 16 * (i >> 2) + 4 * g + (i & 3) > qpos)
+                if (!((in >> (16 * (i >> 2) + (i & 3))) & 1u) || (!SEL && p0 + 16 * (i >> 2) + 4 * g + (i & 3) > qpos))
                     sv[i] = -INFINITY;
         }
 #pragma unroll
@@ -459,12 +539,12 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
         if (j0 > 0) ent = entries(j0);
         load_step(j0, ent, A);
         for (int j = j0;;) {
-            if (!BIG) ent = entry(p_lane + kStep * (j + 2));
+            if (!BIG) ent = next_entry(j + 2);
             load_step(j + 1 < j1 ? j + 1 : kNoStep, BIG ? ent : ent_next, B);
             __builtin_amdgcn_sched_barrier(0);  // (the compiler would move them behind the products)
             process(j, A);
             if (++j >= j1) break;
-            if (!BIG) ent_next = entry(p_lane + kStep * (j + 2));
+            if (!BIG) ent_next = next_entry(j + 2);
             load_step(j + 1 < j1 ? j + 1 : kNoStep, ent, A);
             __builtin_amdgcn_sched_barrier(0);
             process(j, B);
@@ -488,8 +568,14 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
     mg[w][NM - 1][lane] = l;
     if (bad) {  // uniform, rare: the wave's positions again (onto its part in LDS: no registers held for it)
         for (int pos = beg; pos < end; ++pos) {
-            if (((pos - beg) / 32 & 3) != w || pos > qpos) continue;
-            const int slot = slot_of(p.c, s, pos);
+            if (((pos - beg) / 32 & 3) != w || (!SEL && pos > qpos)) continue;
+            int slot;
+            if constexpr (SEL) {
+                const int x = listed(pos);
+                slot = x >= 0 && seen_from(x, pos) > 0 ? slot_of(p.c, s, (x << p.c.shift) + (pos & ((1 << p.c.shift) - 1))) : -1;
+            } else {
+                slot = slot_of(p.c, s, pos);
+            }
             if (slot < 0) continue;
             const uint8_t *v = vb + slot_bytes(p.c, slot, row_bytes);
             const float vs = I8 ? vsp[(int64_t)slot * v_stride] : 1.0f;
@@ -551,19 +637,14 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8)) void attn_paged_rows_kerne
     }
 }
 
-// out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over a row's chunks in order.  A
-// wave takes a row: a lane's chunk for the weights, then a lane's dims.
+// out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over a row's n_c chunks in order,
+// partials `at` and every `step` behind.  A wave takes a row: a lane's chunk for the
+// weights, then a lane's dims.
 template <int HD>
-__global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedParams p) {
+__device__ __forceinline__ void combine_row(const PagedParams &p, int64_t at, int64_t step, int n_c, uint16_t *out) {
     constexpr int VE = HD > 128 ? 4 : HD > 64 ? 2 : 1, U = 8;
     typedef float Piece __attribute__((ext_vector_type(VE)));
-    const int lane = threadIdx.x & 63, r = 4 * blockIdx.y + (threadIdx.x >> 6);
-    const int kvh = blockIdx.x % p.c.n_kv, s = blockIdx.x / p.c.n_kv;
-    const SeqSpan span = seq_span(p.b, s);
-    const int first = p.firsts[2 * s], n_c = p.firsts[2 * s + 1];
-    const int rows = min(span.n, p.b.max_new) * p.group;
-    if (r >= rows || rows > kPagedRows || n_c <= 1 || n_c > p.n_chunks) return;  // not this kernel's, or written already
-    const int64_t at = ((int64_t)first * p.c.n_kv + kvh) * p.rows_blk + r, step = (int64_t)p.c.n_kv * p.rows_blk;
+    const int lane = threadIdx.x & 63;
     const float *st = p.stats + 2 * (at + min(lane, n_c - 1) * step);
     const float mc = st[0], lc = st[1];
     const int d = min(lane * VE, HD - VE);
@@ -591,9 +672,8 @@ __global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedParams p) 
         }
     }
     if (lane * VE >= p.c.hd) return;
-    const int tok = r / p.group, head = kvh * p.group + r % p.group;
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    uint16_t *out = p.out + ((int64_t)(span.row0 + tok) * p.n_heads + head) * p.c.hd + d;
+    out += d;
     if constexpr (VE == 1) {
         *out = f32_to_f16_bits(acc[0] * inv);
     } else {
@@ -601,6 +681,34 @@ __global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedParams p) 
         for (int i = 0; i < VE; i += 2)
             *reinterpret_cast<uint32_t *>(out + i) = pack2<RXQ4_DTYPE_F16>(acc[i] * inv, acc[i + 1] * inv);
     }
+}
+
+template <int HD>
+__global__ __launch_bounds__(256) void attn_paged_combine_kernel(PagedParams p) {
+    const int r = 4 * blockIdx.y + (threadIdx.x >> 6);
+    const int kvh = blockIdx.x % p.c.n_kv, s = blockIdx.x / p.c.n_kv;
+    const SeqSpan span = seq_span(p.b, s);
+    const int first = p.firsts[2 * s], n_c = p.firsts[2 * s + 1];
+    const int rows = min(span.n, p.b.max_new) * p.group;
+    if (r >= rows || rows > kPagedRows || n_c <= 1 || n_c > p.n_chunks) return;  // not this kernel's, or written already
+    const int64_t at = ((int64_t)first * p.c.n_kv + kvh) * p.rows_blk + r, step = (int64_t)p.c.n_kv * p.rows_blk;
+    const int tok = r / p.group, head = kvh * p.group + r % p.group;
+    combine_row<HD>(p, at, step, n_c, p.out + ((int64_t)(span.row0 + tok) * p.n_heads + head) * p.c.hd);
+}
+
+// Selected pages: a row is a token's head.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_selected_combine_kernel(PagedParams p) {
+    const int t = blockIdx.x, head = 4 * blockIdx.y + (threadIdx.x >> 6);
+    if (head >= p.n_heads) return;
+    SeqSpan span;
+    const int s = seq_of_row(p.b, t, span);
+    if (s >= p.b.n_seqs || t < span.row0 || t - span.row0 >= min(span.n, p.b.max_new)) return;
+    const int kvh = head / p.group, j = head % p.group;
+    const int64_t slot = (int64_t)t * p.n_chunks * p.head_blocks + j / kPagedRows;
+    const int64_t at = (slot * p.c.n_kv + kvh) * p.rows_blk + j % kPagedRows;
+    combine_row<HD>(p, at, (int64_t)p.head_blocks * p.c.n_kv * p.rows_blk, p.n_chunks,
+                    p.out + ((int64_t)t * p.n_heads + head) * p.c.hd);
 }
 
 // The 16-row launch's chunks: their partials within `room` bytes.  Some six chunks of
@@ -648,10 +756,10 @@ hipError_t launch_rows(PagedParams &p, const RowsPlan &plan, float *ws, int i8, 
     p.stats = ws + (size_t)plan.slots * p.c.n_kv * p.rows_blk * HD;
     p.firsts = reinterpret_cast<int *>(p.stats + (size_t)plan.slots * p.c.n_kv * p.rows_blk * 2);
     const bool big = p.c.shift >= 4;
-    if (i8 && big) attn_paged_rows_kernel<HD, true, true><<<grid, 256, 0, st>>>(p);
-    else if (i8) attn_paged_rows_kernel<HD, true, false><<<grid, 256, 0, st>>>(p);
-    else if (big) attn_paged_rows_kernel<HD, false, true><<<grid, 256, 0, st>>>(p);
-    else attn_paged_rows_kernel<HD, false, false><<<grid, 256, 0, st>>>(p);
+    if (i8 && big) attn_paged_rows_kernel<HD, true, true, false><<<grid, 256, 0, st>>>(p);
+    else if (i8) attn_paged_rows_kernel<HD, true, false, false><<<grid, 256, 0, st>>>(p);
+    else if (big) attn_paged_rows_kernel<HD, false, true, false><<<grid, 256, 0, st>>>(p);
+    else attn_paged_rows_kernel<HD, false, false, false><<<grid, 256, 0, st>>>(p);
     if (p.n_chunks > 1) {
         const dim3 rows((unsigned)(p.b.n_seqs * p.c.n_kv), (unsigned)(p.rows_blk + 3) / 4);
         attn_paged_combine_kernel<HD><<<rows, 256, 0, st>>>(p);
@@ -659,7 +767,75 @@ hipError_t launch_rows(PagedParams &p, const RowsPlan &plan, float *ws, int i8, 
     return hipGetLastError();
 }
 
+// The chunks of the listed places: steps enough for `want` workgroups, partials within the
+// workspace.
+struct SelectedPlan {
+    int64_t grid;
+    size_t bytes;
+};
+SelectedPlan plan_selected(PagedParams &p, int i8) {
+    const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
+    const int pad = p.c.hd <= 64 ? 64 : p.c.hd <= 96 ? 96 : p.c.hd <= 128 ? 128 : 256;
+    p.rows_blk = std::min(p.group, kPagedRows);
+    p.head_blocks = (p.group + kPagedRows - 1) / kPagedRows;
+    const int64_t units = (int64_t)p.b.n_tokens * p.c.n_kv * p.head_blocks;
+    const int64_t per = units * p.rows_blk * (pad + 2) * 4;  // bytes of one chunk of every unit
+    const int64_t steps = std::min<int64_t>(p.b.max_len, (int64_t)p.c.width << p.c.shift) > 0
+                              ? (((int64_t)p.n_select << p.c.shift) + kStep - 1) / kStep : 1;
+    const int64_t want = (int64_t)(i8 ? 12 : 6) * cus;
+    int64_t most = std::min<int64_t>({steps, kMaxChunks, (want + units - 1) / units, (int64_t)kWorkspaceBytes / per});
+    if (tuning().attn_split) most = std::min<int64_t>(most, tuning().attn_split);
+    most = std::max<int64_t>(most, 1);
+    const int64_t least = (steps + most - 1) / most;
+    p.chunk = (int)least * kStep;
+    p.n_chunks = (int)((steps + least - 1) / least);
+    return SelectedPlan{(units * p.n_chunks + 7) / 8 * 8, p.n_chunks > 1 ? (size_t)(per * p.n_chunks) : 0};
+}
+
+template <int HD>
+hipError_t launch_selected(PagedParams &p, const SelectedPlan &plan, float *ws, int i8, hipStream_t st) {
+    const unsigned grid = (unsigned)plan.grid;
+    p.part = ws;
+    p.stats = ws + (size_t)p.b.n_tokens * p.n_chunks * p.head_blocks * p.c.n_kv * p.rows_blk * HD;
+    const bool big = p.c.shift >= 4;
+    if (i8 && big) attn_paged_rows_kernel<HD, true, true, true><<<grid, 256, 0, st>>>(p);
+    else if (i8) attn_paged_rows_kernel<HD, true, false, true><<<grid, 256, 0, st>>>(p);
+    else if (big) attn_paged_rows_kernel<HD, false, true, true><<<grid, 256, 0, st>>>(p);
+    else attn_paged_rows_kernel<HD, false, false, true><<<grid, 256, 0, st>>>(p);
+    if (p.n_chunks > 1) {
+        const dim3 rows((unsigned)p.b.n_tokens, (unsigned)(p.n_heads + 3) / 4);
+        attn_selected_combine_kernel<HD><<<rows, 256, 0, st>>>(p);
+    }
+    return hipGetLastError();
+}
+
 }  // namespace
+
+hipError_t launch_attention_selected(uint16_t *out, const uint16_t *q, int n_heads, float scale,
+                                     const int32_t *pages, int n_select, const SeqBatch &batch,
+                                     const PagedCache &cache, int kv_int8, hipStream_t st) {
+    PagedParams p{};
+    p.out = out;
+    p.q = q;
+    p.b = batch;
+    p.c = cache;
+    p.n_heads = n_heads;
+    p.group = n_heads / cache.n_kv;
+    p.sl2 = scale * 1.4426950408889634f;
+    p.lists = pages;
+    p.n_select = n_select;
+    const SelectedPlan plan = plan_selected(p, kv_int8);
+    if (plan.grid > kPagedMostRows) return hipErrorInvalidValue;
+    float *ws = nullptr;
+    if (plan.bytes > 0) {
+        const hipError_t e = Scratch{}.get(st, plan.bytes, &ws);
+        if (e != hipSuccess) return e;
+    }
+    if (cache.hd <= 64) return launch_selected<64>(p, plan, ws, kv_int8, st);
+    if (cache.hd <= 96) return launch_selected<96>(p, plan, ws, kv_int8, st);
+    if (cache.hd <= 128) return launch_selected<128>(p, plan, ws, kv_int8, st);
+    return launch_selected<256>(p, plan, ws, kv_int8, st);
+}
 
 hipError_t launch_attention_paged(uint16_t *out, const uint16_t *q, int n_heads, float scale,
                                   const SeqBatch &batch, const PagedCache &cache, int kv_int8,

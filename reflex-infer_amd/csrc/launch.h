@@ -197,14 +197,39 @@ struct SeqBatch {
     const int32_t *starts, *lens;
     int n_seqs, n_tokens, max_new, max_len;
 };
+// Coordinates of the tokens on n axes, and the axis of each rotated pair (null: 0).
+struct RopeAxes {
+    const int32_t *at;  // [n][stride]; null: the position in the cache is the one coordinate
+    int64_t stride;
+    int n;
+    const int32_t *axis_of;
+};
 hipError_t launch_qk_norm_rope(uint16_t *q_out, const void *q, const void *k, const void *v, int x_dtype,
                                int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_weight,
                                const float *k_weight, float eps, const float *inv_freq, int n_rot,
-                               int interleaved, const SeqBatch &batch, const PagedCache &cache, int kv_int8,
-                               hipStream_t stream);
+                               int interleaved, const RopeAxes &axes, const SeqBatch &batch,
+                               const PagedCache &cache, int kv_int8, hipStream_t stream);
 hipError_t launch_attention_paged(uint16_t *out, const uint16_t *q, int n_heads, float scale,
                                   const SeqBatch &batch, const PagedCache &cache, int kv_int8,
                                   hipStream_t stream);
+
+// The same over the positions of the pages listed for a token and KV head: pages
+// [n_tokens][n_kv][n_select], places in the sequence's table row.
+hipError_t launch_attention_selected(uint16_t *out, const uint16_t *q, int n_heads, float scale,
+                                     const int32_t *pages, int n_select, const SeqBatch &batch,
+                                     const PagedCache &cache, int kv_int8, hipStream_t stream);
+
+// Bounds of a page's keys: per page and KV head 8 dims' smallest, then their largest in
+// steps of the scale, dims after dims.
+struct PageBounds {
+    int8_t *bounds;  // [n_pages][n_kv][hd / 8][2][8]
+    float *scales;   // [n_pages][n_kv]
+};
+hipError_t launch_kv_bounds(const PageBounds &bounds, const SeqBatch &batch, const PagedCache &cache,
+                            int kv_int8, hipStream_t stream);
+hipError_t launch_select_pages(int32_t *pages, int n_select, int n_first, int n_last, const uint16_t *q,
+                               int n_heads, const PageBounds &bounds, const SeqBatch &batch,
+                               const PagedCache &cache, hipStream_t stream);
 
 struct SampleRows {
     int32_t *ids;

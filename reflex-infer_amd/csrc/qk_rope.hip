@@ -47,6 +47,7 @@ struct RopeParams {
     int heads_wg;  // heads (queries, keys, values in order) of a workgroup
     SeqBatch b;
     PagedCache c;
+    RopeAxes a;
 };
 
 // Eight values of a row as they are stored, and widened.
@@ -97,8 +98,9 @@ __device__ __forceinline__ Head head_of(const RopeParams &p, int h) {
     return Head{q, v, q ? h : v ? h - p.n_heads - p.c.n_kv : h - p.n_heads};
 }
 
-// DT: type of q, k, v; L: lanes a head (8 L >= head_dim).
-template <int DT, int L, bool I8>
+// DT: type of q, k, v; L: lanes a head (8 L >= head_dim); AX: the angles from p.a's
+// coordinates, their loads beside the first rows' (the slot follows from the lengths).
+template <int DT, int L, bool I8, bool AX>
 __global__ __launch_bounds__(64 * kWaves, DT == RXQ4_DTYPE_F32 ? 7 : 8) void qk_rope_kernel(RopeParams p) {
     constexpr int HPW = 64 / L;  // heads of a wave at a time
     __shared__ float cs[128], sn[128];
@@ -118,6 +120,11 @@ __global__ __launch_bounds__(64 * kWaves, DT == RXQ4_DTYPE_F32 ? 7 : 8) void qk_
     int h0 = blockIdx.y * p.heads_wg + w * HPW;
     Raw<DT> next = load(h0);
     const float freq = tid < half ? p.inv_freq[tid] : 0.0f;
+    int coord = 0;
+    if constexpr (AX) {
+        const int axis = tid < half && p.a.axis_of ? p.a.axis_of[tid] : 0;
+        if (tid < half && (unsigned)axis < (unsigned)p.a.n) coord = p.a.at[axis * p.a.stride + t];
+    }
     if (tid < hd) {
         if (p.qw) wts[0][tid] = p.qw[tid];
         if (p.kw) wts[1][tid] = p.kw[tid];
@@ -129,7 +136,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == RXQ4_DTYPE_F32 ? 7 : 8) void qk_
     const int pos = span.pos0 + (t - span.row0);
     const int slot = pos >= 0 && pos < position_limit(p.b, p.c) ? slot_of(p.c, seq, pos) : -1;
     if (tid < half) {
-        const double turns = (double)pos * (double)freq * 0.15915494309189533577;
+        const double turns = (double)(AX ? coord : pos) * (double)freq * 0.15915494309189533577;
         const double halves = 2.0 * (turns - rint(turns));
         const float near = (float)halves, rest = (float)((halves - (double)near) * 3.14159265358979323846);
         float s, c;
@@ -239,8 +246,13 @@ __global__ __launch_bounds__(64 * kWaves, DT == RXQ4_DTYPE_F32 ? 7 : 8) void qk_
 
 template <int DT, int L>
 void launch_l(const RopeParams &p, dim3 grid, int i8, hipStream_t st) {
-    if (i8) qk_rope_kernel<DT, L, true><<<grid, 64 * kWaves, 0, st>>>(p);
-    else qk_rope_kernel<DT, L, false><<<grid, 64 * kWaves, 0, st>>>(p);
+    if (p.a.at) {
+        if (i8) qk_rope_kernel<DT, L, true, true><<<grid, 64 * kWaves, 0, st>>>(p);
+        else qk_rope_kernel<DT, L, false, true><<<grid, 64 * kWaves, 0, st>>>(p);
+    } else {
+        if (i8) qk_rope_kernel<DT, L, true, false><<<grid, 64 * kWaves, 0, st>>>(p);
+        else qk_rope_kernel<DT, L, false, false><<<grid, 64 * kWaves, 0, st>>>(p);
+    }
 }
 
 template <int DT>
@@ -260,10 +272,10 @@ void launch_dt(RopeParams &p, int i8, hipStream_t st) {
 hipError_t launch_qk_norm_rope(uint16_t *q_out, const void *q, const void *k, const void *v, int x_dtype,
                                int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_weight,
                                const float *k_weight, float eps, const float *inv_freq, int n_rot,
-                               int interleaved, const SeqBatch &batch, const PagedCache &cache, int kv_int8,
-                               hipStream_t st) {
+                               int interleaved, const RopeAxes &axes, const SeqBatch &batch,
+                               const PagedCache &cache, int kv_int8, hipStream_t st) {
     RopeParams p{q_out, q, k, v, q_stride, kv_stride, q_weight, k_weight, inv_freq, eps,
-                 n_heads, n_rot, interleaved, 0, batch, cache};
+                 n_heads, n_rot, interleaved, 0, batch, cache, axes};
     if (x_dtype == RXQ4_DTYPE_F32) launch_dt<RXQ4_DTYPE_F32>(p, kv_int8, st);
     else if (x_dtype == RXQ4_DTYPE_F16) launch_dt<RXQ4_DTYPE_F16>(p, kv_int8, st);
     else launch_dt<RXQ4_DTYPE_BF16>(p, kv_int8, st);

@@ -530,16 +530,19 @@ rxq4::SeqBatch device_batch(const rxq4_seq_batch &b) {
     return rxq4::SeqBatch{b.q_starts, b.seq_lens, b.n_seqs, b.n_tokens, b.max_new, b.max_len};
 }
 
-}  // namespace
+// Whether two ranges of memory share a byte.
+bool overlap(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a_bytes > 0 && b_bytes > 0 && x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
+bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
-extern "C" {
-
-int rxq4_qk_norm_rope(void *q_out, const void *q, const void *k, const void *v, int x_dtype,
-                      int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_weight,
-                      const float *k_weight, float eps, const float *inv_freq, int n_rot,
-                      int interleaved, const rxq4_seq_batch *batch, const rxq4_paged_kv *cache,
-                      void *stream) {
-    const char *fn = "rxq4_qk_norm_rope";
+// rxq4_qk_norm_rope and, where axes has coordinates, rxq4_qk_norm_rope_axes.
+int qk_norm_rope(const char *fn, void *q_out, const void *q, const void *k, const void *v, int x_dtype,
+                 int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_weight,
+                 const float *k_weight, float eps, const float *inv_freq, int n_rot, int interleaved,
+                 const rxq4::RopeAxes &axes, const rxq4_seq_batch *batch, const rxq4_paged_kv *cache,
+                 void *stream) {
     int s = check_batch(fn, batch);
     if (s != RXQ4_STATUS_SUCCESS) return s;
     if ((s = check_cache(fn, cache, n_heads, batch->n_seqs)) != RXQ4_STATUS_SUCCESS) return s;
@@ -574,11 +577,148 @@ int rxq4_qk_norm_rope(void *q_out, const void *q, const void *k, const void *v, 
                          "%s: q_out overlaps q (it may be q itself, fp16 and without gaps)", fn);
     if (over(k, kv_stride, kv_row) || over(v, kv_stride, kv_row))
         return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: q_out overlaps k or v", fn);
+    const int64_t o_bytes = batch->n_tokens * q_row * 2;
+    if (axes.at && (overlap(q_out, o_bytes, axes.at, ((axes.n - 1) * axes.stride + batch->n_tokens) * 4) ||
+                    (axes.axis_of && overlap(q_out, o_bytes, axes.axis_of, n_rot * 2))))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: q_out overlaps positions or axis_of", fn);
     if ((s = check_device(fn)) != RXQ4_STATUS_SUCCESS) return s;
     return from_hip(rxq4::launch_qk_norm_rope(static_cast<uint16_t *>(q_out), q, k, v, x_dtype, q_stride,
                                               kv_stride, n_heads, q_weight, k_weight, eps, inv_freq, n_rot,
-                                              interleaved ? 1 : 0, device_batch(*batch), device_cache(*cache),
+                                              interleaved ? 1 : 0, axes, device_batch(*batch), device_cache(*cache),
                                               cache->kv_int8 ? 1 : 0, static_cast<hipStream_t>(stream)),
+                    fn);
+}
+
+int64_t bounds_bytes(const rxq4_paged_kv &c) { return (int64_t)c.n_pages * c.n_kv_heads * c.head_dim * 2; }
+int64_t bound_scales_bytes(const rxq4_paged_kv &c) { return (int64_t)c.n_pages * c.n_kv_heads * 4; }
+
+int check_n_select(const char *fn, int n_select) {
+    if (n_select <= 0 || n_select > RXQ4_MAX_SELECT)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: n_select=%d must be 1 to %d", fn, n_select, RXQ4_MAX_SELECT);
+    return RXQ4_STATUS_SUCCESS;
+}
+
+// Attention's shared arguments; where the batch has no rows, out and q are not looked at.
+int check_attention_batch(const char *fn, const void *out, const void *q, int n_heads, float scale,
+                          const rxq4_seq_batch *batch, const rxq4_paged_kv *cache) {
+    int s = check_batch(fn, batch);
+    if (s != RXQ4_STATUS_SUCCESS) return s;
+    if ((s = check_cache(fn, cache, n_heads, batch->n_seqs)) != RXQ4_STATUS_SUCCESS) return s;
+    if (!(scale - scale == 0.0f)) return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: scale=%g", fn, scale);
+    if (batch->n_seqs == 0 || batch->n_tokens == 0 || batch->max_new == 0) return RXQ4_STATUS_SUCCESS;
+    if (!out || !q || !aligned16(out) || !aligned16(q))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: q/out null or not 16-byte aligned", fn);
+    const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(q);
+    if (o != i && (o < i ? i - o : o - i) < (uintptr_t)((int64_t)batch->n_tokens * n_heads * cache->head_dim * 2))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: out overlaps q (it may be q itself)", fn);
+    return RXQ4_STATUS_SUCCESS;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rxq4_qk_norm_rope(void *q_out, const void *q, const void *k, const void *v, int x_dtype,
+                      int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_weight,
+                      const float *k_weight, float eps, const float *inv_freq, int n_rot,
+                      int interleaved, const rxq4_seq_batch *batch, const rxq4_paged_kv *cache,
+                      void *stream) {
+    return qk_norm_rope("rxq4_qk_norm_rope", q_out, q, k, v, x_dtype, q_stride, kv_stride, n_heads, q_weight,
+                        k_weight, eps, inv_freq, n_rot, interleaved, rxq4::RopeAxes{}, batch, cache, stream);
+}
+
+int rxq4_qk_norm_rope_axes(void *q_out, const void *q, const void *k, const void *v, int x_dtype,
+                           int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_weight,
+                           const float *k_weight, float eps, const float *inv_freq, int n_rot,
+                           int interleaved, const int32_t *positions, int64_t position_stride, int n_axes,
+                           const int32_t *axis_of, const rxq4_seq_batch *batch,
+                           const rxq4_paged_kv *cache, void *stream) {
+    const char *fn = "rxq4_qk_norm_rope_axes";
+    const int s = check_batch(fn, batch);
+    if (s != RXQ4_STATUS_SUCCESS) return s;
+    if (n_axes <= 0 || n_axes > RXQ4_MAX_AXES)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: n_axes=%d must be 1 to %d", fn, n_axes, RXQ4_MAX_AXES);
+    if (position_stride < batch->n_tokens || position_stride > (int64_t(1) << 32))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: position_stride=%lld must hold n_tokens=%d", fn,
+                         (long long)position_stride, batch->n_tokens);
+    if (batch->n_seqs > 0 && batch->n_tokens > 0 && (!positions || !aligned4(positions) || !aligned4(axis_of)))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: positions null, or positions/axis_of not 4-byte aligned", fn);
+    return qk_norm_rope(fn, q_out, q, k, v, x_dtype, q_stride, kv_stride, n_heads, q_weight, k_weight, eps,
+                        inv_freq, n_rot, interleaved, rxq4::RopeAxes{positions, position_stride, n_axes, axis_of},
+                        batch, cache, stream);
+}
+
+int rxq4_kv_bounds(void *bounds, float *scales, const rxq4_seq_batch *batch,
+                   const rxq4_paged_kv *cache, void *stream) {
+    const char *fn = "rxq4_kv_bounds";
+    int s = check_batch(fn, batch);
+    if (s != RXQ4_STATUS_SUCCESS) return s;
+    if ((s = check_cache(fn, cache, cache ? cache->n_kv_heads : 0, batch->n_seqs)) != RXQ4_STATUS_SUCCESS) return s;
+    if (batch->n_seqs == 0 || batch->n_tokens == 0 || batch->max_new == 0 || cache->n_pages == 0) return ok();
+    if (!bounds || !scales || !aligned16(bounds) || !aligned4(scales))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: bounds null or not 16-byte aligned, or scales null or not "
+                         "4-byte aligned", fn);
+    const rxq4::PagedCache c = device_cache(*cache);
+    const int64_t page = (int64_t)cache->page_size * cache->n_kv_heads * cache->head_dim * (cache->kv_int8 ? 1 : 2);
+    const int64_t k_bytes = (cache->n_pages - 1) * c.page_bytes + page;
+    const int64_t b_bytes = bounds_bytes(*cache), s_bytes = bound_scales_bytes(*cache);
+    if (overlap(bounds, b_bytes, scales, s_bytes) || overlap(bounds, b_bytes, cache->k, k_bytes) ||
+        overlap(scales, s_bytes, cache->k, k_bytes))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: bounds, scales and keys overlap", fn);
+    if ((s = check_device(fn)) != RXQ4_STATUS_SUCCESS) return s;
+    return from_hip(rxq4::launch_kv_bounds(rxq4::PageBounds{static_cast<int8_t *>(bounds), scales}, device_batch(*batch),
+                                           c, cache->kv_int8 ? 1 : 0, static_cast<hipStream_t>(stream)),
+                    fn);
+}
+
+int rxq4_select_pages(int32_t *pages, int n_select, int n_first, int n_last, const void *q,
+                      int n_heads, const void *bounds, const float *scales,
+                      const rxq4_seq_batch *batch, const rxq4_paged_kv *cache, void *stream) {
+    const char *fn = "rxq4_select_pages";
+    int s = check_batch(fn, batch);
+    if (s != RXQ4_STATUS_SUCCESS) return s;
+    if ((s = check_cache(fn, cache, n_heads, batch->n_seqs)) != RXQ4_STATUS_SUCCESS) return s;
+    if ((s = check_n_select(fn, n_select)) != RXQ4_STATUS_SUCCESS) return s;
+    if (n_first < 0 || n_last < 0 || (int64_t)n_first + n_last > n_select)
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: n_first=%d and n_last=%d must fit n_select=%d", fn, n_first,
+                         n_last, n_select);
+    if (batch->n_seqs == 0 || batch->n_tokens == 0 || batch->max_new == 0) return ok();
+    if (!pages || !q || !aligned4(pages) || !aligned16(q))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: pages null or not 4-byte aligned, or q null or not 16-byte "
+                         "aligned", fn);
+    if (cache->n_pages > 0 && (!bounds || !scales || !aligned16(bounds) || !aligned4(scales)))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: bounds null or not 16-byte aligned, or scales null or not "
+                         "4-byte aligned", fn);
+    const int64_t p_bytes = (int64_t)batch->n_tokens * cache->n_kv_heads * n_select * 4;
+    if (overlap(pages, p_bytes, q, (int64_t)batch->n_tokens * n_heads * cache->head_dim * 2) ||
+        overlap(pages, p_bytes, bounds, bounds_bytes(*cache)) ||
+        overlap(pages, p_bytes, scales, bound_scales_bytes(*cache)))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: pages overlaps q, bounds or scales", fn);
+    if ((s = check_device(fn)) != RXQ4_STATUS_SUCCESS) return s;
+    const rxq4::PageBounds b{static_cast<int8_t *>(const_cast<void *>(bounds)), const_cast<float *>(scales)};
+    return from_hip(rxq4::launch_select_pages(pages, n_select, n_first, n_last, static_cast<const uint16_t *>(q), n_heads,
+                                              b, device_batch(*batch), device_cache(*cache),
+                                              static_cast<hipStream_t>(stream)),
+                    fn);
+}
+
+int rxq4_attention_selected_f16(void *out, const void *q, int n_heads, float scale,
+                                const int32_t *pages, int n_select, const rxq4_seq_batch *batch,
+                                const rxq4_paged_kv *cache, void *stream) {
+    const char *fn = "rxq4_attention_selected_f16";
+    int s = check_attention_batch(fn, out, q, n_heads, scale, batch, cache);
+    if (s != RXQ4_STATUS_SUCCESS) return s;
+    if ((s = check_n_select(fn, n_select)) != RXQ4_STATUS_SUCCESS) return s;
+    if (batch->n_seqs == 0 || batch->n_tokens == 0 || batch->max_new == 0) return ok();
+    if (!pages || !aligned4(pages))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: pages null or not 4-byte aligned", fn);
+    if (overlap(out, (int64_t)batch->n_tokens * n_heads * cache->head_dim * 2, pages,
+                (int64_t)batch->n_tokens * cache->n_kv_heads * n_select * 4))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: out overlaps pages", fn);
+    if ((s = check_device(fn)) != RXQ4_STATUS_SUCCESS) return s;
+    return from_hip(rxq4::launch_attention_selected(static_cast<uint16_t *>(out), static_cast<const uint16_t *>(q), n_heads,
+                                                    scale, pages, n_select, device_batch(*batch), device_cache(*cache),
+                                                    cache->kv_int8 ? 1 : 0, static_cast<hipStream_t>(stream)),
                     fn);
 }
 
@@ -586,16 +726,9 @@ int rxq4_attention_paged_f16(void *out, const void *q, int n_heads, float scale,
                              const rxq4_seq_batch *batch, const rxq4_paged_kv *cache,
                              void *stream) {
     const char *fn = "rxq4_attention_paged_f16";
-    int s = check_batch(fn, batch);
+    int s = check_attention_batch(fn, out, q, n_heads, scale, batch, cache);
     if (s != RXQ4_STATUS_SUCCESS) return s;
-    if ((s = check_cache(fn, cache, n_heads, batch->n_seqs)) != RXQ4_STATUS_SUCCESS) return s;
-    if (!(scale - scale == 0.0f)) return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: scale=%g", fn, scale);
     if (batch->n_seqs == 0 || batch->n_tokens == 0 || batch->max_new == 0) return ok();
-    if (!out || !q || !aligned16(out) || !aligned16(q))
-        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: q/out null or not 16-byte aligned", fn);
-    const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(q);
-    if (o != i && (o < i ? i - o : o - i) < (uintptr_t)((int64_t)batch->n_tokens * n_heads * cache->head_dim * 2))
-        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: out overlaps q (it may be q itself)", fn);
     if ((s = check_device(fn)) != RXQ4_STATUS_SUCCESS) return s;
     return from_hip(rxq4::launch_attention_paged(static_cast<uint16_t *>(out), static_cast<const uint16_t *>(q),
                                                  n_heads, scale, device_batch(*batch), device_cache(*cache),

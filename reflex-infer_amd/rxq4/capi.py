@@ -62,6 +62,16 @@ SIGNATURES = {
                                   ctypes.POINTER(SeqBatchStruct), ctypes.POINTER(PagedKVStruct), c_void_p]),
     "rxq4_attention_paged_f16": (c_int, [c_void_p, c_void_p, c_int, ctypes.c_float, ctypes.POINTER(SeqBatchStruct),
                                          ctypes.POINTER(PagedKVStruct), c_void_p]),
+    "rxq4_qk_norm_rope_axes": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p,
+                                       c_void_p, ctypes.c_float, c_void_p, c_int, c_int, c_void_p, c_int64, c_int,
+                                       c_void_p, ctypes.POINTER(SeqBatchStruct), ctypes.POINTER(PagedKVStruct),
+                                       c_void_p]),
+    "rxq4_kv_bounds": (c_int, [c_void_p, c_void_p, ctypes.POINTER(SeqBatchStruct), ctypes.POINTER(PagedKVStruct),
+                               c_void_p]),
+    "rxq4_select_pages": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                                  ctypes.POINTER(SeqBatchStruct), ctypes.POINTER(PagedKVStruct), c_void_p]),
+    "rxq4_attention_selected_f16": (c_int, [c_void_p, c_void_p, c_int, ctypes.c_float, c_void_p, c_int,
+                                            ctypes.POINTER(SeqBatchStruct), ctypes.POINTER(PagedKVStruct), c_void_p]),
     "rxq4_sample_f32": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                 c_void_p, c_void_p]),
     "rxq4_host_gemv": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int,
@@ -302,36 +312,113 @@ def _fits(name, batch, cache):
     _same_device(name, batch.tensors[0], cache.tensors[0])
 
 
+def _rope_args(name, q_out, q, k, v, batch, cache, inv_freq, q_weight, k_weight, eps, interleaved):
+    """The shared arguments of qk_norm_rope and qk_norm_rope_axes, checked."""
+    _fits(name, batch, cache)
+    n, heads, hd = q.shape
+    want = (batch.n_tokens, cache.n_kv_heads, cache.head_dim)
+    if (n, hd) != (want[0], want[2]) or k.shape != want or v.shape != want or q_out.shape != q.shape:
+        raise ValueError(f"{name}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, q_out "
+                         f"{tuple(q_out.shape)} for {want[0]} tokens, {want[1]} KV heads of {want[2]}")
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    if sq[1:] != (hd, 1) or sk[1:] != (hd, 1) or sv[1:] != (hd, 1) or (sk[0] != sv[0] and n > 1) or \
+            q.dtype != k.dtype or q.dtype != v.dtype or q_out.dtype != torch.float16 or not q_out.is_contiguous():
+        raise ValueError(f"{name}: rows must be dense, k and v rows equally far apart, q, k, v of one type, "
+                         "q_out contiguous fp16")
+    for t in (inv_freq, q_weight, k_weight):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous()):
+            raise ValueError(f"{name}: inv_freq and weights must be contiguous fp32")
+    for t in (q_weight, k_weight):
+        if t is not None and t.numel() != hd:
+            raise ValueError(f"{name}: weights must have head_dim={hd} values")
+    _same_device(name, cache.tensors[0], q_out, q, k, v, inv_freq, q_weight, k_weight)
+    _on_current_device(name, q)
+    return (_ptr(q_out), _ptr(q), _ptr(k), _ptr(v), _dtype_code(q), sq[0] if n > 1 else heads * hd,
+            sk[0] if n > 1 else want[1] * hd, heads, _ptr(q_weight), _ptr(k_weight), eps, _ptr(inv_freq),
+            0 if inv_freq is None else 2 * inv_freq.numel(), int(interleaved))
+
+
 def qk_norm_rope(q_out, q, k, v, batch, cache, inv_freq, q_weight=None, k_weight=None, eps=1e-6, interleaved=False,
                  stream=None):
     """q [n_tokens, n_heads, head_dim] and k, v [n_tokens, n_kv_heads, head_dim]
     (fp16, bf16 or fp32, e.g. slices of one fused projection): head norms,
     rotation by position * inv_freq, queries to q_out, keys and values into the
     cache's pages."""
-    _fits("qk_norm_rope", batch, cache)
-    n, heads, hd = q.shape
-    want = (batch.n_tokens, cache.n_kv_heads, cache.head_dim)
-    if (n, hd) != (want[0], want[2]) or k.shape != want or v.shape != want or q_out.shape != q.shape:
-        raise ValueError(f"qk_norm_rope: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, q_out "
-                         f"{tuple(q_out.shape)} for {want[0]} tokens, {want[1]} KV heads of {want[2]}")
-    sq, sk, sv = q.stride(), k.stride(), v.stride()
-    if sq[1:] != (hd, 1) or sk[1:] != (hd, 1) or sv[1:] != (hd, 1) or (sk[0] != sv[0] and n > 1) or \
-            q.dtype != k.dtype or q.dtype != v.dtype or q_out.dtype != torch.float16 or not q_out.is_contiguous():
-        raise ValueError("qk_norm_rope: rows must be dense, k and v rows equally far apart, q, k, v of one type, "
-                         "q_out contiguous fp16")
-    for t in (inv_freq, q_weight, k_weight):
-        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous()):
-            raise ValueError("qk_norm_rope: inv_freq and weights must be contiguous fp32")
-    for t in (q_weight, k_weight):
-        if t is not None and t.numel() != hd:
-            raise ValueError(f"qk_norm_rope: weights must have head_dim={hd} values")
-    _same_device("qk_norm_rope", cache.tensors[0], q_out, q, k, v, inv_freq, q_weight, k_weight)
-    _on_current_device("qk_norm_rope", q)
-    return _check(lib().rxq4_qk_norm_rope(
-        _ptr(q_out), _ptr(q), _ptr(k), _ptr(v), _dtype_code(q), sq[0] if n > 1 else heads * hd,
-        sk[0] if n > 1 else want[1] * hd, heads, _ptr(q_weight), _ptr(k_weight), eps, _ptr(inv_freq),
-        0 if inv_freq is None else 2 * inv_freq.numel(), int(interleaved), batch.ref, cache.ref, _stream(stream)),
-        "rxq4_qk_norm_rope")
+    args = _rope_args("qk_norm_rope", q_out, q, k, v, batch, cache, inv_freq, q_weight, k_weight, eps, interleaved)
+    return _check(lib().rxq4_qk_norm_rope(*args, batch.ref, cache.ref, _stream(stream)), "rxq4_qk_norm_rope")
+
+
+def qk_norm_rope_axes(q_out, q, k, v, batch, cache, inv_freq, positions, axis_of=None, q_weight=None, k_weight=None,
+                      eps=1e-6, interleaved=False, stream=None):
+    """qk_norm_rope with the angles from coordinates: positions int32 [n_axes,
+    n_tokens] (rows may lie apart), axis_of int32, the axis of each value of inv_freq
+    (None: axis 0)."""
+    name = "qk_norm_rope_axes"
+    args = _rope_args(name, q_out, q, k, v, batch, cache, inv_freq, q_weight, k_weight, eps, interleaved)
+    n_axes, n = positions.shape
+    if positions.dtype != torch.int32 or n != batch.n_tokens or (n > 1 and positions.stride(1) != 1):
+        raise ValueError(f"{name}: positions must be int32 [n_axes, {batch.n_tokens}], its rows dense")
+    if axis_of is not None and _int32(axis_of, "axis_of").numel() != (0 if inv_freq is None else inv_freq.numel()):
+        raise ValueError(f"{name}: axis_of must have a value for each of inv_freq")
+    _same_device(name, q, positions, axis_of)
+    return _check(lib().rxq4_qk_norm_rope_axes(
+        *args, _ptr(positions), positions.stride(0) if n_axes > 1 else n, n_axes, _ptr(axis_of), batch.ref, cache.ref,
+        _stream(stream)), "rxq4_qk_norm_rope_axes")
+
+
+def _bounds_fit(name, bounds, scales, cache):
+    n_pages, kv, hd = cache.struct.n_pages, cache.n_kv_heads, cache.head_dim
+    if bounds.dtype != torch.int8 or tuple(bounds.shape) != (n_pages, kv, hd // 8, 2, 8) or not bounds.is_contiguous() or \
+            scales.dtype != torch.float32 or tuple(scales.shape) != (n_pages, kv) or not scales.is_contiguous():
+        raise ValueError(f"{name}: bounds must be contiguous int8 {(n_pages, kv, hd // 8, 2, 8)}, scales fp32 "
+                         f"{(n_pages, kv)}")
+
+
+def kv_bounds(bounds, scales, batch, cache, stream=None):
+    """The bounds of the pages that the batch's new tokens went to: bounds int8
+    [n_pages, n_kv_heads, head_dim / 8, 2, 8] (of each 8 dims the smallest, then the
+    largest), scales fp32 [n_pages, n_kv_heads]."""
+    _fits("kv_bounds", batch, cache)
+    _bounds_fit("kv_bounds", bounds, scales, cache)
+    _same_device("kv_bounds", cache.tensors[0], bounds, scales)
+    _on_current_device("kv_bounds", bounds)
+    return _check(lib().rxq4_kv_bounds(_ptr(bounds), _ptr(scales), batch.ref, cache.ref, _stream(stream)),
+                  "rxq4_kv_bounds")
+
+
+def _rows_fit(name, q, batch, cache, pages):
+    if q.dim() != 3 or q.shape[0] != batch.n_tokens or q.shape[2] != cache.head_dim or q.dtype != torch.float16 or \
+            not q.is_contiguous():
+        raise ValueError(f"{name}: q must be contiguous fp16 [{batch.n_tokens}, n_heads, {cache.head_dim}]")
+    if _int32(pages, "pages").dim() != 3 or pages.shape[:2] != (batch.n_tokens, cache.n_kv_heads):
+        raise ValueError(f"{name}: pages must be int32 [{batch.n_tokens}, {cache.n_kv_heads}, n_select]")
+
+
+def select_pages(pages, q, bounds, scales, batch, cache, n_first=1, n_last=1, stream=None):
+    """pages int32 [n_tokens, n_kv_heads, n_select] = the pages that each new token's
+    queries q (fp16 [n_tokens, n_heads, head_dim]) attend to: the first n_first and the
+    last n_last of its sequence and those with the largest bound of a score."""
+    _fits("select_pages", batch, cache)
+    _rows_fit("select_pages", q, batch, cache, pages)
+    _bounds_fit("select_pages", bounds, scales, cache)
+    _same_device("select_pages", cache.tensors[0], pages, q, bounds, scales)
+    _on_current_device("select_pages", q)
+    return _check(lib().rxq4_select_pages(_ptr(pages), pages.shape[2], n_first, n_last, _ptr(q), q.shape[1], _ptr(bounds),
+                                          _ptr(scales), batch.ref, cache.ref, _stream(stream)), "rxq4_select_pages")
+
+
+def attention_selected_f16(out, q, pages, batch, cache, scale, stream=None):
+    """attention_paged_f16 over the listed pages alone: pages int32 [n_tokens,
+    n_kv_heads, n_select], places in the sequence's row of the page table."""
+    _fits("attention_selected_f16", batch, cache)
+    _rows_fit("attention_selected_f16", q, batch, cache, pages)
+    if out.shape != q.shape or out.dtype != torch.float16 or not out.is_contiguous():
+        raise ValueError(f"attention_selected_f16: out must be contiguous fp16 {tuple(q.shape)}")
+    _same_device("attention_selected_f16", cache.tensors[0], out, q, pages)
+    _on_current_device("attention_selected_f16", q)
+    return _check(lib().rxq4_attention_selected_f16(_ptr(out), _ptr(q), q.shape[1], scale, _ptr(pages), pages.shape[2],
+                                                    batch.ref, cache.ref, _stream(stream)),
+                  "rxq4_attention_selected_f16")
 
 
 def attention_paged_f16(out, q, batch, cache, scale, stream=None):
