@@ -321,7 +321,8 @@ int rxq4_qk_norm_rope_axes(void *q_out, const void *q, const void *k, const void
  * the page's positions that its sequence has filled, computed anew.
  *   bounds  int8 [n_pages][n_kv_heads][head_dim / 8][2][8], 16-byte aligned: of each 8 dims
  *           the smallest, then the largest, rint(x / scale)
- *   scales  fp32 [n_pages][n_kv_heads]: max(|smallest|, |largest|) / 127 over the dims
+ *   scales  fp32 [n_pages][n_kv_heads]: max(|smallest|, |largest|) * fp32(1 / 127) over
+ *           the dims,
  * lying beside the pool as the int8 scales do.  A NaN key is left out (a dim with
  * nothing else gets 0); an infinity counts as fp32's largest number.  Positions and pages
  * that rxq4_qk_norm_rope would not store to are left out.  Two sequences with new tokens
@@ -342,8 +343,8 @@ int rxq4_kv_bounds(void *bounds, float *scales, const rxq4_seq_batch *batch,
  *            keeps the page that the token itself is in)
  *   score    the largest, over the heads of the KV head's group, of
  *            (sum_d max(z_d lo_d, z_d hi_d)) * step * scale, in this order in fp32, where
- *            lo, hi and scale are the page's bounds, step = max |q| / 127 and z = rint(q /
- *            step) of the head's query (NaN as 0, infinities as 65504): up to the
+ *            lo, hi and scale are the page's bounds, step = max |q| * fp32(1 / 127) and z =
+ *            rint(q / step) of the head's query (NaN as 0, infinities as 65504): up to the
  *            steps no key of the page has a larger product with the query.  The sum is
  *            exact, so the lists do not depend on how the work is cut
  * Tokens that see nothing get -1s.  Rows of no sequence are left as they are.  A few

@@ -3,12 +3,12 @@
 // cores.
 //
 //   bounds  a page's smallest and largest key of each dim over its filled positions, lo
-//           and hi, in steps of scale = max(|lo|, |hi|) / 127: rint(lo / scale),
+//           and hi, in steps of scale = max(|lo|, |hi|) * fp32(1 / 127): rint(lo / scale),
 //           rint(hi / scale).  NaN keys are left out, infinities count as the largest
 //           fp32 numbers.
 //   score   of a page for a query q: no key of it has a larger product than
 //           sum_d max(q_d lo_d, q_d hi_d) (up to the steps).  The query in steps of its
-//           own, max |q| / 127: with q- = min(q, 0), q+ = max(q, 0) the sum is q- . lo +
+//           own, max |q| * fp32(1 / 127): with q- = min(q, 0), q+ = max(q, 0) the sum is q- . lo +
 //           q+ . hi, a product of whole numbers below 2^23, exact in any order; times the
 //           query's step, times the page's scale, both rounded.  A page's score for a token
 //           is the largest over the heads of the KV head's group.
@@ -30,6 +30,7 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
+constexpr float kStepOfMax = 1.0f / 127.0f;
 __device__ __forceinline__ int to_step(float x, float scale) {
     const float z = scale > 0.0f ? rintf(x / scale) : 0.0f;  // (IEEE: the bytes follow from x alone)
     return (int)fminf(fmaxf(z, -127.0f), 127.0f);
@@ -120,7 +121,7 @@ __device__ __forceinline__ void bound_page(const BoundsParams &p, int page, int 
     const int hc = c / n_ch;
     if (hc >= heads) return;
     for (int j = 0; j < n_ch; ++j) top = fmaxf(top, most[hc * n_ch + j]);
-    const float scale = top / 127.0f;
+    const float scale = top * kStepOfMax;
     const int64_t row = (int64_t)page * p.c.n_kv + head0 + hc;
     int8_t *dst = p.out.bounds + row * 2 * hd + 16 * (c % n_ch) + i;
     dst[0] = (int8_t)to_step(l, scale);
@@ -245,7 +246,7 @@ __device__ __forceinline__ void score_pages(const SelectParams &p, const Tile &t
             for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(value(ks, i)));
         top = max_xor_rows<16>(top);
         top = max_xor_rows<32>(top);
-        const float qstep = top / 127.0f;
+        const float qstep = top * kStepOfMax;
         i32x4 qa[KS];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {

@@ -11,6 +11,9 @@ import torch
 from tests.serving_reference import H16, TINY16, U, Paged
 
 
+STEP = np.float32(1) / np.float32(127)  # of a largest value: the steps of a byte
+
+
 def rope_axes(x, weight, eps, coords, inv_freq, interleaved):
     """serving_reference.rope with a coordinate of its own for every pair: coords
     [rows, pairs].  The same steps, so the same bound: 24 u of |a| + |b| for the angle,
@@ -69,7 +72,7 @@ def bounds(p: Paged, page, held):
         hi = np.where(some, np.fmax.reduce(k, 0), 0).astype(np.float32)
         top = np.finfo(np.float32).max
         lo, hi = np.clip(lo, -top, top), np.clip(hi, -top, top)
-        scale = np.maximum(np.abs(lo), np.abs(hi)).max(-1) / np.float32(127)
+        scale = np.maximum(np.abs(lo), np.abs(hi)).max(-1) * STEP
         step = np.where(scale > 0, scale, np.float32(1))[:, None]
         both = np.stack([np.where(scale[:, None] > 0, np.clip(np.rint(x / step), -127, 127), 0) for x in (lo, hi)], 1)
     kv, _, hd = both.shape
@@ -101,7 +104,7 @@ def scores(q, both, scale):
     are whole numbers; the rest are single fp32 operations."""
     pages, kv, n8 = both.shape[:3]
     q = np.nan_to_num(q.astype(np.float32), nan=0.0, posinf=65504.0, neginf=-65504.0)
-    step = np.abs(q).max(-1) / np.float32(127)
+    step = np.abs(q).max(-1) * STEP
     safe = np.where(step > 0, step, np.float32(1))[:, None]
     z = np.where(step[:, None] > 0, np.rint(q / safe), 0).astype(np.int64).reshape(kv, -1, n8 * 8)
     lo, hi = (both[:, :, :, i].reshape(pages, kv, n8 * 8).astype(np.float64).transpose(1, 0, 2) for i in (0, 1))
