@@ -30,6 +30,7 @@ struct PagedParams {
     const int32_t *lists;  // selected pages: those of each token and KV head
     int n_select;          // entries of a list
     int head_blocks;       // selected pages: blocks of 16 heads of a group
+    int tile;              // selected pages: tokens of a tile at most
 };
 
 // sum + w x, x a part relative to its own maximum and w its weight beside the other

@@ -105,7 +105,8 @@ struct RowsUnit {
     int s, c;           // sequence (-1: none), chunk
     int chunks, chunk;  // chunks of the sequence; positions of each
     int64_t slot;       // of the chunk's partials
-    int tok;            // selected pages: the token of the sequence
+    int tok;            // listed pages: the (first) token of the sequence
+    int tokens;         // a tile's
 };
 __device__ __forceinline__ RowsUnit rows_unit(const PagedParams &p, int idx) {
     RowsUnit r{};
@@ -173,6 +174,101 @@ __device__ __forceinline__ RowsUnit selected_unit(const PagedParams &p, int &kvh
     return r;
 }
 
+// Listed pages: the tokens of a tile and their KV head kvh.  Unit u of the first
+// ceil(n_tokens / tile): the rows from u * tile up to the next such row that are of the
+// sequence of the first; the units behind them: a sequence's rows before its first multiple
+// of `tile`.  Every row is in one.
+__device__ __forceinline__ RowsUnit tile_unit(const PagedParams &p, int &kvh) {
+    RowsUnit r{};
+    r.s = -1;
+    const int whole = (p.b.n_tokens + p.tile - 1) / p.tile, units = whole + p.b.n_seqs;
+    const int idx = (int)(blockIdx.x % 8) * (gridDim.x / 8) + (int)(blockIdx.x / 8), u = idx % units;
+    kvh = idx / units;
+    if (kvh >= p.c.n_kv) return r;
+    int from, s;
+    if (u < whole) {
+        from = u * p.tile;
+        s = seq_of_row(p.b, from, r.span);
+        if (s >= p.b.n_seqs || from < r.span.row0) return r;
+    } else {
+        s = u - whole;
+        r.span = seq_span(p.b, s);
+        from = r.span.row0;
+        if (from % p.tile == 0) return r;
+    }
+    r.tok = from - r.span.row0;
+    r.tokens = min((from / p.tile + 1) * p.tile, r.span.row0 + min(r.span.n, p.b.max_new)) - from;
+    if (r.tokens <= 0) return r;
+    r.s = s;
+    r.chunks = 1;
+    r.chunk = 1 << 30;
+    return r;
+}
+
+// The pages that a tile's tokens list, each once with the tokens that do, in the order of
+// the first token's list, then what the second's adds, ..: work[k] the page of the pool,
+// work[tile * n_select + k] its place in the table | tokens << 24; how many.  Found by
+// binary search where every list ascends (rxq4_select_pages'); of others every entry stays
+// its own.  By the whole workgroup.
+__device__ __forceinline__ int merge_lists(const PagedParams &p, const RowsUnit &unit, int kvh, int *work) {
+    __shared__ int counts[2][4], out_of_order;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = p.n_select, total = unit.tokens * n;
+    const int limit = position_limit(p.b, p.c);
+    int *const lists = work + 2 * p.tile * n;
+    constexpr int kEnd = 0x7FFFFFFF;
+    if (tid == 0) out_of_order = 0;
+    const int32_t *const table = p.c.table ? p.c.table + (int64_t)unit.s * p.c.width : nullptr;
+    const auto value = [&](int t, int i) {
+        const int x = p.lists[((int64_t)(unit.span.row0 + unit.tok + t) * p.c.n_kv + kvh) * n + i];
+        const int sees = min(limit, unit.span.pos0 + unit.tok + t + 1);
+        const int pages = sees > 0 ? ((sees - 1) >> p.c.shift) + 1 : 0;
+        return x >= 0 && x < pages ? x : kEnd;
+    };
+    for (int e = tid; e < total; e += 256) lists[e] = value(e / n, e % n);
+    __syncthreads();
+    bool wrong = false;
+    for (int e = tid; e < total; e += 256)
+        wrong |= e % n > 0 && lists[e] <= lists[e - 1] && !(lists[e] == kEnd && lists[e - 1] == kEnd);
+    if (wrong) out_of_order = 1;
+    __syncthreads();
+    const bool ascend = out_of_order == 0;
+    int found = 0;
+    for (int e0 = 0, odd = 0; e0 < total; e0 += 256, odd ^= 1) {
+        const int e = e0 + tid, t = min(e, total - 1) / n, x = e < total ? lists[e] : kEnd;
+        uint32_t tokens = 1u << t;
+        if (ascend && x != kEnd)
+            for (int o = 0; o < unit.tokens; ++o) {
+                if (o == t) continue;
+                const int *l = lists + o * n;
+                int a = 0, b = n;  // the first entry not below x
+                while (a < b) {
+                    const int m = (a + b) >> 1;
+                    if (l[m] < x) a = m + 1;
+                    else b = m;
+                }
+                if (a < n && l[a] == x) tokens |= 1u << o;
+            }
+        int page = -1;
+        if (x != kEnd && (tokens & ((1u << t) - 1u)) == 0) page = table ? table[x] : x;  // (the first that lists it)
+        const bool keep = (unsigned)page < (unsigned)p.c.n_pages;
+        const uint64_t kept = __builtin_amdgcn_ballot_w64(keep);
+        if (lane == 0) counts[odd][w] = __builtin_popcountll(kept);
+        __syncthreads();
+        int at = found + __builtin_popcountll(kept & ((uint64_t(1) << lane) - 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            at += i < w ? counts[odd][i] : 0;
+            found += counts[odd][i];
+        }
+        if (keep) {
+            work[at] = page;
+            work[p.tile * n + at] = x | (int)(tokens << 24);
+        }
+    }
+    __syncthreads();
+    return found;
+}
+
 // Wave w takes positions 32 w .. + 31 of every 128-position step of the chunk with
 // its own online softmax; the four waves merge at the end.  Per step, lane l =
 // 16 g + r:
@@ -196,11 +292,16 @@ __device__ __forceinline__ RowsUnit selected_unit(const PagedParams &p, int &kvh
 // resource; else the pool's first row in their place, cleared), their scores
 // -infinity.
 //
-// SEL: a workgroup takes one token, up to 16 heads of a KV head's group, and one chunk of
-// the places of its listed pages, page_size a list entry; all rows see the same, so the
-// masks are the entries'.
-template <int HD, bool I8, bool BIG, bool SEL>
-__global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, SEL)) void attn_paged_rows_kernel(PagedParams p) {
+// Listed pages.  kTokenLists: a workgroup takes one token, up to 16 heads of a KV head's group,
+// and one chunk of the places of its listed pages, page_size a list entry; all rows see the
+// same, so the masks are the entries'.  kTileLists: several tokens of a sequence, as many as 16
+// rows hold, and the pages that any of them lists, each read once (the lists of a prompt's
+// neighbours agree on most); a row's mask is its token's bit beside the page.
+enum Lists { kNoLists, kTokenLists, kTileLists };
+template <int HD, bool I8, bool BIG, Lists LISTS>
+__global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists)) void attn_paged_rows_kernel(PagedParams p) {
+    constexpr bool SEL = LISTS == kTokenLists, TILE = LISTS == kTileLists;
+    static_assert(!TILE || BIG, "an operand of a tile lies in one page");
     // A chunk is 16 bytes: 8 dims of fp16, 16 of int8, which are two k steps of a
     // product (a lane's dims need only be the same in K and Q).
     constexpr int EC = I8 ? 16 : 8;                     // dims of a chunk
@@ -222,8 +323,13 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, SEL)) void attn_paged_
     // us with the heads on all, 216 so).  A sequence's chunks go to different ones.
     int kvh, head0 = 0;
     RowsUnit unit;
+    int listed_pages = 0;  // TILE: pages that the tile's tokens list
+    extern __shared__ int work[];  // TILE: their pages of the pool; their places | tokens << 24; the lists
     if constexpr (SEL) {
         unit = selected_unit(p, kvh, head0);
+    } else if constexpr (TILE) {
+        unit = tile_unit(p, kvh);
+        if (unit.s >= 0) listed_pages = merge_lists(p, unit, kvh, work);
     } else {
         const int x8 = blockIdx.x / 8;
         kvh = x8 % p.c.n_kv;
@@ -231,7 +337,7 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, SEL)) void attn_paged_
     }
     const int s = unit.s, c = unit.c, beg = c * unit.chunk;
     if (s < 0) return;  // uniform
-    if (!SEL && p.n_chunks > 1 && c == 0 && kvh == 0 && tid == 0) {
+    if (LISTS == kNoLists && p.n_chunks > 1 && c == 0 && kvh == 0 && tid == 0) {
         p.firsts[2 * s] = (int)unit.slot;
         p.firsts[2 * s + 1] = unit.chunks;
     }
@@ -266,9 +372,17 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, SEL)) void attn_paged_
     auto seen_from = [&](int x, int at) { return sees - (x << p.c.shift) - (at & ((1 << p.c.shift) - 1)); };
     int there = 0;    // SEL, BIG: beside the entry, the operand's positions that the token sees
     int x_ahead = 0;  // SEL, small pages: the list's page of the step after the newest entry's
+    int of_tokens = 0;  // TILE: beside the entry, its place and tokens
     auto entries = [&](int j) {
         const int at = beg + 32 * w + kStep * (j + (lane >> 1)) + 16 * (lane & 1);
-        if constexpr (SEL) {
+        if constexpr (TILE) {
+            const int i = at >> p.c.shift, k = min(i, max(listed_pages - 1, 0));
+            of_tokens = work[p.tile * p.n_select + k];
+            const int last = min(limit, span.pos0 + unit.tok + unit.tokens);  // positions that the last token sees
+            const int place = ((of_tokens & 0xFFFFFF) << p.c.shift) + (at & ((1 << p.c.shift) - 1));
+            there = i < listed_pages ? min(max(last - place, 0), 16) : 0;
+            return work[k];
+        } else if constexpr (SEL) {
             const int x = listed(at), page = page_of(x);
             there = page >= 0 ? min(max(seen_from(x, at), 0), 16) : 0;
             return page;
@@ -288,11 +402,12 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, SEL)) void attn_paged_
         }
     };
     int ent = BIG ? entries(0) : next_entry(0), ent_next = BIG ? 0 : next_entry(1);
-    const int rows = SEL ? min(p.group - head0, kPagedRows) : min(span.n, p.b.max_new) * p.group;
-    const int end_seq = SEL ? (limit > 0 ? p.n_select << p.c.shift : 0) : min(span.pos0 + (rows - 1) / p.group + 1, limit);
+    const int rows = SEL ? min(p.group - head0, kPagedRows) : (TILE ? unit.tokens : min(span.n, p.b.max_new)) * p.group;
+    const int end_seq = TILE ? listed_pages << p.c.shift : SEL ? (limit > 0 ? p.n_select << p.c.shift : 0) : min(span.pos0 + (rows - 1) / p.group + 1, limit);
     const int end = min(end_seq, beg + unit.chunk);
     const int row = min(r, rows - 1);  // (columns past the last row repeat it)
-    const int tok = SEL ? unit.tok : row / p.group, head = kvh * p.group + (SEL ? head0 + row : row % p.group);
+    const int mine = SEL ? 0 : row / p.group;  // the row's token
+    const int tok = LISTS != kNoLists ? unit.tok + mine : mine, head = kvh * p.group + (SEL ? head0 + row : row % p.group);
     const bool row_ok = r < rows;
     const int hd = p.c.hd, n_ch = hd / EC;
     const int64_t orow = ((int64_t)(span.row0 + tok) * p.n_heads + head) * hd;
@@ -334,6 +449,8 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, SEL)) void attn_paged_
         u32x4 k[2][KL], v[NV];
         float ks, vs;
         uint32_t seen;  // which of the wave's 32 positions there are
+        int of[2];      // TILE: an operand's page and tokens
+        bool all[2];    // TILE: every token sees all of the operand
     };
     auto load_step = [&](int j, int e, Step &S) {
         const int mask = (1 << p.c.shift) - 1;
@@ -346,11 +463,17 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, SEL)) void attn_paged_
             for (int st = 0; st < 2; ++st) {
                 const int pos = beg + 32 * w + kStep * j + 16 * st;
                 page[st] = __builtin_amdgcn_readlane(e, (2 * j + st) & 63);
-                const int n = SEL ? (pos < end ? __builtin_amdgcn_readlane(there, (2 * j + st) & 63) : 0)
+                const int n = LISTS != kNoLists ? (pos < end ? __builtin_amdgcn_readlane(there, (2 * j + st) & 63) : 0)
                               : (unsigned)page[st] < (unsigned)p.c.n_pages ? max(min(end - pos, 16), 0) : 0;
                 S.seen |= ((1u << n) - 1) << (16 * st);
                 page[st] = n > 0 ? page[st] : 0;
                 place[st] = pos & mask;
+                if constexpr (TILE) {
+                    S.of[st] = __builtin_amdgcn_readlane(of_tokens, (2 * j + st) & 63);
+                    const int first = ((S.of[st] & 0xFFFFFF) << p.c.shift) + place[st];
+                    S.all[st] = n > 0 && (uint32_t)S.of[st] >> 24 == (1u << unit.tokens) - 1u &&
+                                first + 16 <= min(limit, span.pos0 + unit.tok + 1);
+                }
                 const int64_t base = (int64_t)page[st] * p.c.page_bytes + (int64_t)place[st] * row_bytes;
                 const int bytes = n > 0 ? (n - 1) * row_bytes + hd * esz : 0;
                 kr[st] = make_rsrc(kb + base, bytes);
@@ -412,7 +535,7 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, SEL)) void attn_paged_
     bool bad = false;  // some V is not finite
     uint32_t most_vs = 0;  // int8: the lane's largest |V scale|
     auto process = [&](int j, Step &S) {
-        if (SEL && S.seen == 0) return;  // uniform
+        if (LISTS != kNoLists && S.seen == 0) return;  // uniform
         const int p0 = beg + kStep * j + 32 * w;
         f32x4 acc[2];
 #pragma unroll
@@ -454,7 +577,19 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, SEL)) void attn_paged_
         float sv[8], mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sv[i] = acc[i >> 2][i & 3] * p.sl2;
-        if (part || (!SEL && p0 + 31 > span.pos0)) {  // uniform: not every row sees all of them
+        if constexpr (TILE) {
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+                if (!S.all[st]) {  // uniform
+                    // places of the operand that the row's token lists and sees
+                    const int first = ((S.of[st] & 0xFFFFFF) << p.c.shift) + ((p0 + 16 * st) & ((1 << p.c.shift) - 1));
+                    const int n = S.of[st] >> (24 + mine) & 1 ? min(limit, qpos + 1) - first : 0;
+                    const int here = (S.seen >> (16 * st) & 0xFFFFu) != 0 ? n : 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (4 * g + i >= here) sv[4 * st + i] = -INFINITY;
+                }
+        } else if (part || (!SEL && p0 + 31 > span.pos0)) {  // uniform: not every row sees all of them
             const uint32_t in = S.seen >> (4 * g);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -568,9 +703,13 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, SEL)) void attn_paged_
     mg[w][NM - 1][lane] = l;
     if (bad) {  // uniform, rare: the wave's positions again (onto its part in LDS: no registers held for it)
         for (int pos = beg; pos < end; ++pos) {
-            if (((pos - beg) / 32 & 3) != w || (!SEL && pos > qpos)) continue;
+            if (((pos - beg) / 32 & 3) != w || (LISTS == kNoLists && pos > qpos)) continue;
             int slot;
-            if constexpr (SEL) {
+            if constexpr (TILE) {
+                const int k = pos >> p.c.shift, in = pos & ((1 << p.c.shift) - 1), of = work[p.tile * p.n_select + k];
+                const bool sees_it = of >> (24 + mine) & 1 && ((of & 0xFFFFFF) << p.c.shift) + in < min(limit, qpos + 1);
+                slot = sees_it ? (work[k] << p.c.shift) + in : -1;
+            } else if constexpr (SEL) {
                 const int x = listed(pos);
                 slot = x >= 0 && seen_from(x, pos) > 0 ? slot_of(p.c, s, (x << p.c.shift) + (pos & ((1 << p.c.shift) - 1))) : -1;
             } else {
@@ -756,10 +895,10 @@ hipError_t launch_rows(PagedParams &p, const RowsPlan &plan, float *ws, int i8, 
     p.stats = ws + (size_t)plan.slots * p.c.n_kv * p.rows_blk * HD;
     p.firsts = reinterpret_cast<int *>(p.stats + (size_t)plan.slots * p.c.n_kv * p.rows_blk * 2);
     const bool big = p.c.shift >= 4;
-    if (i8 && big) attn_paged_rows_kernel<HD, true, true, false><<<grid, 256, 0, st>>>(p);
-    else if (i8) attn_paged_rows_kernel<HD, true, false, false><<<grid, 256, 0, st>>>(p);
-    else if (big) attn_paged_rows_kernel<HD, false, true, false><<<grid, 256, 0, st>>>(p);
-    else attn_paged_rows_kernel<HD, false, false, false><<<grid, 256, 0, st>>>(p);
+    if (i8 && big) attn_paged_rows_kernel<HD, true, true, kNoLists><<<grid, 256, 0, st>>>(p);
+    else if (i8) attn_paged_rows_kernel<HD, true, false, kNoLists><<<grid, 256, 0, st>>>(p);
+    else if (big) attn_paged_rows_kernel<HD, false, true, kNoLists><<<grid, 256, 0, st>>>(p);
+    else attn_paged_rows_kernel<HD, false, false, kNoLists><<<grid, 256, 0, st>>>(p);
     if (p.n_chunks > 1) {
         const dim3 rows((unsigned)(p.b.n_seqs * p.c.n_kv), (unsigned)(p.rows_blk + 3) / 4);
         attn_paged_combine_kernel<HD><<<rows, 256, 0, st>>>(p);
@@ -773,17 +912,28 @@ struct SelectedPlan {
     int64_t grid;
     size_t bytes;
 };
+constexpr int kListEntries = 2048;  // of a tile's lists: 24 KB of LDS
 SelectedPlan plan_selected(PagedParams &p, int i8) {
     const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
     const int pad = p.c.hd <= 64 ? 64 : p.c.hd <= 96 ? 96 : p.c.hd <= 128 ? 128 : 256;
     p.rows_blk = std::min(p.group, kPagedRows);
     p.head_blocks = (p.group + kPagedRows - 1) / kPagedRows;
+    // Tiles where the sequences have tokens to fill them, the pages hold whole operands and the
+    // tiles are enough for the CUs.
+    p.tile = (int)std::min<int64_t>({(int64_t)kPagedRows / p.group, 8, kListEntries / p.n_select});
+    if (p.tile > 1 && p.c.shift >= 4 && p.b.max_new > 1 && p.b.n_tokens >= 4 * (int64_t)p.b.n_seqs) {
+        const int64_t tiles = ((p.b.n_tokens + p.tile - 1) / p.tile + p.b.n_seqs) * (int64_t)p.c.n_kv;
+        if (tiles >= cus) {
+            p.n_chunks = 1;
+            return SelectedPlan{(tiles + 7) / 8 * 8, 0};
+        }
+    }
+    p.tile = 1;
     const int64_t units = (int64_t)p.b.n_tokens * p.c.n_kv * p.head_blocks;
     const int64_t per = units * p.rows_blk * (pad + 2) * 4;  // bytes of one chunk of every unit
     const int64_t steps = std::min<int64_t>(p.b.max_len, (int64_t)p.c.width << p.c.shift) > 0
                               ? (((int64_t)p.n_select << p.c.shift) + kStep - 1) / kStep : 1;
-    const int64_t want = (int64_t)(i8 ? 12 : 6) * cus;
-    int64_t most = std::min<int64_t>({steps, kMaxChunks, (want + units - 1) / units, (int64_t)kWorkspaceBytes / per});
+    int64_t most = std::min<int64_t>({steps, kMaxChunks, cus / units, (int64_t)kWorkspaceBytes / per});
     if (tuning().attn_split) most = std::min<int64_t>(most, tuning().attn_split);
     most = std::max<int64_t>(most, 1);
     const int64_t least = (steps + most - 1) / most;
@@ -798,10 +948,16 @@ hipError_t launch_selected(PagedParams &p, const SelectedPlan &plan, float *ws, 
     p.part = ws;
     p.stats = ws + (size_t)p.b.n_tokens * p.n_chunks * p.head_blocks * p.c.n_kv * p.rows_blk * HD;
     const bool big = p.c.shift >= 4;
-    if (i8 && big) attn_paged_rows_kernel<HD, true, true, true><<<grid, 256, 0, st>>>(p);
-    else if (i8) attn_paged_rows_kernel<HD, true, false, true><<<grid, 256, 0, st>>>(p);
-    else if (big) attn_paged_rows_kernel<HD, false, true, true><<<grid, 256, 0, st>>>(p);
-    else attn_paged_rows_kernel<HD, false, false, true><<<grid, 256, 0, st>>>(p);
+    if (p.tile > 1) {
+        const size_t lds = (size_t)3 * p.tile * p.n_select * 4;
+        if (i8) attn_paged_rows_kernel<HD, true, true, kTileLists><<<grid, 256, lds, st>>>(p);
+        else attn_paged_rows_kernel<HD, false, true, kTileLists><<<grid, 256, lds, st>>>(p);
+        return hipGetLastError();
+    }
+    if (i8 && big) attn_paged_rows_kernel<HD, true, true, kTokenLists><<<grid, 256, 0, st>>>(p);
+    else if (i8) attn_paged_rows_kernel<HD, true, false, kTokenLists><<<grid, 256, 0, st>>>(p);
+    else if (big) attn_paged_rows_kernel<HD, false, true, kTokenLists><<<grid, 256, 0, st>>>(p);
+    else attn_paged_rows_kernel<HD, false, false, kTokenLists><<<grid, 256, 0, st>>>(p);
     if (p.n_chunks > 1) {
         const dim3 rows((unsigned)p.b.n_tokens, (unsigned)(p.n_heads + 3) / 4);
         attn_selected_combine_kernel<HD><<<rows, 256, 0, st>>>(p);
