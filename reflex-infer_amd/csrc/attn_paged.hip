@@ -50,7 +50,8 @@ __device__ __forceinline__ float log2_scale(float vs) {
 // Waves per SIMD that the registers are cut to: what is in flight is what counts, and
 // an int8 step holds half the bytes of an fp16 one.  (With a list's page beside the entry,
 // small fp16 pages spill at four.)
-constexpr int rows_waves(int hd, bool i8, bool big, bool sel) {
+constexpr int rows_waves(int hd, bool i8, bool big, bool sel, bool tile) {
+    if (tile) return hd > 128 ? 1 : hd == 64 ? 4 : 3;
     return hd > 128 ? 1 : hd == 64 ? (sel && !i8 && !big ? 3 : 4) : i8 ? 3 : 2;
 }
 
@@ -148,22 +149,22 @@ __device__ __forceinline__ RowsUnit rows_unit(const PagedParams &p, int idx) {
     return r;
 }
 
-// Selected pages: a token, its KV head kvh, the heads of the group from head0 on, and a chunk
-// of the places.  An XCD (workgroups are dealt to the eight in turn) takes tokens of one KV
-// head one after another: a prompt's neighbours list much the same pages.
+// Listed pages: a token, its KV head kvh, the heads of the group from head0 on, and a chunk
+// of the places.  An XCD (workgroups are dealt to the eight in turn) takes tokens one after
+// another, which list much the same pages in a prompt, and all of a token's KV heads: their
+// rows lie beside one another, one head's alone in a part of the L2's channels.
 __device__ __forceinline__ RowsUnit selected_unit(const PagedParams &p, int &kvh, int &head0) {
     RowsUnit r{};
     r.s = -1;
     const int per = gridDim.x / 8;  // (a multiple of 8)
     const int idx = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-    r.c = idx % p.n_chunks;
-    int at = idx / p.n_chunks;
-    const int block = at % p.head_blocks;
-    at /= p.head_blocks;
-    const int t = at % p.b.n_tokens;
-    kvh = at / p.b.n_tokens;
+    kvh = idx % p.c.n_kv;
+    int at = idx / p.c.n_kv;
+    r.c = at % p.n_chunks;
+    at /= p.n_chunks;
+    const int block = at % p.head_blocks, t = at / p.head_blocks;
     head0 = block * kPagedRows;
-    if (kvh >= p.c.n_kv) return r;
+    if (t >= p.b.n_tokens) return r;
     const int s = seq_of_row(p.b, t, r.span);
     r.tok = t - r.span.row0;
     if (s >= p.b.n_seqs || r.tok < 0 || r.tok >= min(r.span.n, p.b.max_new)) return r;
@@ -182,9 +183,9 @@ __device__ __forceinline__ RowsUnit tile_unit(const PagedParams &p, int &kvh) {
     RowsUnit r{};
     r.s = -1;
     const int whole = (p.b.n_tokens + p.tile - 1) / p.tile, units = whole + p.b.n_seqs;
-    const int idx = (int)(blockIdx.x % 8) * (gridDim.x / 8) + (int)(blockIdx.x / 8), u = idx % units;
-    kvh = idx / units;
-    if (kvh >= p.c.n_kv) return r;
+    const int idx = (int)(blockIdx.x % 8) * (gridDim.x / 8) + (int)(blockIdx.x / 8), u = idx / p.c.n_kv;
+    kvh = idx % p.c.n_kv;
+    if (u >= units) return r;
     int from, s;
     if (u < whole) {
         from = u * p.tile;
@@ -299,7 +300,7 @@ __device__ __forceinline__ int merge_lists(const PagedParams &p, const RowsUnit 
 // neighbours agree on most); a row's mask is its token's bit beside the page.
 enum Lists { kNoLists, kTokenLists, kTileLists };
 template <int HD, bool I8, bool BIG, Lists LISTS>
-__global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists)) void attn_paged_rows_kernel(PagedParams p) {
+__global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, LISTS == kTileLists)) void attn_paged_rows_kernel(PagedParams p) {
     constexpr bool SEL = LISTS == kTokenLists, TILE = LISTS == kTileLists;
     static_assert(!TILE || BIG, "an operand of a tile lies in one page");
     // A chunk is 16 bytes: 8 dims of fp16, 16 of int8, which are two k steps of a
@@ -445,18 +446,49 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists))
     const GlobalFloat ksp = p.c.ks ? (GlobalFloat)(p.c.ks + kvh) : (GlobalFloat)&g_one;
     const GlobalFloat vsp = p.c.vs ? (GlobalFloat)(p.c.vs + kvh) : (GlobalFloat)&g_one;
     const int s_stride = p.c.ks ? p.c.n_kv : 0, v_stride = p.c.vs ? p.c.n_kv : 0;
+    // K as the products take it; TILE: by rows as V, turned in LDS (16 rows side by side are 64
+    // lookups of the L1 a load and bound a tile whose pages come from the L2, rows one after
+    // another 16)
+    struct Rows {
+        u32x4 k[TILE ? 1 : 2][TILE ? NV : KL], v[NV];
+    };
     struct Step {
-        u32x4 k[2][KL], v[NV];
         float ks, vs;
         uint32_t seen;  // which of the wave's 32 positions there are
         int of[2];      // TILE: an operand's page and tokens
         bool all[2];    // TILE: every token sees all of the operand
     };
-    auto load_step = [&](int j, int e, Step &S) {
+    // TILE: the loads of K and of V are left to the caller, from the operands' buffers
+    struct Operands {
+        __amdgpu_buffer_rsrc_t k[2], v[2];
+    };
+    auto load_rows = [&](const __amdgpu_buffer_rsrc_t *from, u32x4 *x) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            constexpr bool kSplit = 64 % CH != 0 || 64 / CH > 16;  // a load's rows may be in both operands
+            if constexpr (kSplit) {
+                const bool first = (lane + 64 * j) / CH < 16;
+                x[j] = buffer_load16(from[0], first ? vo[j] : kPast) | buffer_load16(from[1], first ? kPast : vo[j]);
+            } else {
+                x[j] = buffer_load16(from[64 * j / CH / 16], vo[j]);
+            }
+        }
+    };
+    auto load_k = [&](const Operands &from, Rows &R) {
+        if constexpr (TILE) {
+            load_rows(from.k, R.k[0]);
+        } else {
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int i = 0; i < KL; ++i) R.k[st][i] = buffer_load16(from.k[st], ko[i]);
+        }
+    };
+    auto load_v = [&](const Operands &from, Rows &R) { load_rows(from.v, R.v); };
+    auto load_step = [&](int j, int e, Step &S, Rows &R, Operands &from) {
         const int mask = (1 << p.c.shift) - 1;
         if constexpr (BIG) {
             // an operand's rows: those of its positions that there are, from the first
-            __amdgpu_buffer_rsrc_t kr[2], vr[2];
             S.seen = 0;
             int page[2], place[2];
 #pragma unroll
@@ -476,8 +508,8 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists))
                 }
                 const int64_t base = (int64_t)page[st] * p.c.page_bytes + (int64_t)place[st] * row_bytes;
                 const int bytes = n > 0 ? (n - 1) * row_bytes + hd * esz : 0;
-                kr[st] = make_rsrc(kb + base, bytes);
-                vr[st] = make_rsrc(vb + base, bytes);
+                from.k[st] = make_rsrc(kb + base, bytes);
+                from.v[st] = make_rsrc(vb + base, bytes);
             }
             if constexpr (I8) {
                 const bool ok = (S.seen >> (lane & 31)) & 1;
@@ -486,19 +518,9 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists))
                 S.ks = ksp[at * s_stride];
                 S.vs = vsp[at * v_stride];
             }
-#pragma unroll
-            for (int st = 0; st < 2; ++st)
-#pragma unroll
-                for (int i = 0; i < KL; ++i) S.k[st][i] = buffer_load16(kr[st], ko[i]);
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                constexpr bool kSplit = 64 % CH != 0 || 64 / CH > 16;  // a load's rows may be in both operands
-                if constexpr (kSplit) {
-                    const bool first = (lane + 64 * j) / CH < 16;
-                    S.v[j] = buffer_load16(vr[0], first ? vo[j] : kPast) | buffer_load16(vr[1], first ? kPast : vo[j]);
-                } else {
-                    S.v[j] = buffer_load16(vr[64 * j / CH / 16], vo[j]);
-                }
+            if constexpr (!TILE) {
+                load_k(from, R);
+                load_v(from, R);
             }
         } else {
             const int pos = p_lane + kStep * j;
@@ -516,10 +538,10 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists))
             for (int st = 0; st < 2; ++st) {
                 const uint8_t *src = kb + rowoff[w][16 * st + r];
 #pragma unroll
-                for (int i = 0; i < KL; ++i) S.k[st][i] = load16(src + ko[i]);
+                for (int i = 0; i < KL; ++i) R.k[st][i] = load16(src + ko[i]);
             }
 #pragma unroll
-            for (int j = 0; j < NV; ++j) S.v[j] = load16(vb + rowoff[w][min((lane + 64 * j) / CH, 31)] + vo[j]);
+            for (int j = 0; j < NV; ++j) R.v[j] = load16(vb + rowoff[w][min((lane + 64 * j) / CH, 31)] + vo[j]);
             wave_lds_fence();
         }
     };
@@ -534,22 +556,42 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists))
     float m = -INFINITY, l = 0.0f;
     bool bad = false;  // some V is not finite
     uint32_t most_vs = 0;  // int8: the lane's largest |V scale|
-    auto process = [&](int j, Step &S) {
-        if (LISTS != kNoLists && S.seen == 0) return;  // uniform
+    auto process = [&](int j, Step &S, Rows &R, auto after_k, auto after_v) {
+        if (SEL && S.seen == 0) return;  // uniform
         const int p0 = beg + kStep * j + 32 * w;
         f32x4 acc[2];
+        // (the wave's own reads of its V rows are ahead in its LDS queue, and these ahead of the next)
+        constexpr int kPitch = HD * esz + 16;  // bytes of a K row
+        uint8_t *const kl = reinterpret_cast<uint8_t *>(vl);
+        if constexpr (TILE) {
+            wave_lds_fence();
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int id = lane + 64 * j;
+                if (32 * CH % 64 == 0 || id < 32 * CH) *reinterpret_cast<u32x4 *>(kl + (id / CH) * kPitch + 16 * (id % CH)) = R.k[0][j];
+            }
+            wave_lds_fence();
+        }
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
             acc[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            u32x4 kf[KL];
+#pragma unroll
+            for (int i = 0; i < KL; ++i) {
+                if constexpr (TILE) kf[i] = *reinterpret_cast<const u32x4 *>(kl + (16 * st + r) * kPitch + 16 * (4 * i + g));
+                else kf[i] = R.k[st][i];
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 u32x4 k;
-                if constexpr (I8) k = ks % 2 ? widen(S.k[st][ks / 2].z, S.k[st][ks / 2].w) : widen(S.k[st][ks / 2].x, S.k[st][ks / 2].y);
-                else k = S.k[st][ks];
+                if constexpr (I8) k = ks % 2 ? widen(kf[ks / 2].z, kf[ks / 2].w) : widen(kf[ks / 2].x, kf[ks / 2].y);
+                else k = kf[ks];
                 if (!I8 && !BIG && 4 * ks + 4 > n_ch && 4 * ks + g >= n_ch) k = u32x4{0u, 0u, 0u, 0u};
                 acc[st] = mfma<RXQ4_DTYPE_F16>(k, qf[ks], acc[st]);
             }
         }
+        if constexpr (TILE) wave_lds_fence();
+        after_k();
         f32x4 vx[2], lg[2];
         if constexpr (I8) {
             // An infinite or NaN V scale: as an fp16 V below.  (Small pages: looked at after the
@@ -632,9 +674,9 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists))
             if (!BIG && part)  // uniform
 #pragma unroll
                 for (int j = 0; j < NV; ++j)
-                    if (!((S.seen >> ((lane + 64 * j) / CH)) & 1u)) S.v[j] = u32x4{0u, 0u, 0u, 0u};
-            if (__builtin_amdgcn_ballot_w64(not_finite16<NV>(S.v)) != 0) {
-                zero_not_finite16<NV>(S.v);
+                    if (!((S.seen >> ((lane + 64 * j) / CH)) & 1u)) R.v[j] = u32x4{0u, 0u, 0u, 0u};
+            if (__builtin_amdgcn_ballot_w64(not_finite16<NV>(R.v)) != 0) {
+                zero_not_finite16<NV>(R.v);
                 bad = true;
             }
         }
@@ -645,13 +687,14 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists))
             uint16_t *dst = &vl[(id / CH) * VROW + EC * (id % CH)];
             if constexpr (I8) {
                 if (32 * CH % 64 == 0 || id < 32 * CH) {
-                    *reinterpret_cast<u32x4 *>(dst) = widen(S.v[j].x, S.v[j].y);
-                    *reinterpret_cast<u32x4 *>(dst + 8) = widen(S.v[j].z, S.v[j].w);
+                    *reinterpret_cast<u32x4 *>(dst) = widen(R.v[j].x, R.v[j].y);
+                    *reinterpret_cast<u32x4 *>(dst + 8) = widen(R.v[j].z, R.v[j].w);
                 }
             } else {
-                *reinterpret_cast<u32x4 *>(dst) = S.v[j];
+                *reinterpret_cast<u32x4 *>(dst) = R.v[j];
             }
         }
+        after_v();
         // lane r of group g supplies dims 16 dt + 4 (r & 3) .. + 3 of positions 4 g + r / 4
         // and 16 + 4 g + r / 4 and receives dim 16 dt + r of positions 4 g .. + 3 and 16 + 4 g ..
 #pragma unroll
@@ -665,27 +708,59 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists))
             const u32x4 a = u32x4{v0.x, v0.y, v1.x, v1.y};
             o[dt] = mfma<RXQ4_DTYPE_F16>(a, u32x4{ph[0], ph[1], ph[2], ph[3]}, o[dt]);
             o[dt] = mfma<RXQ4_DTYPE_F16>(a, u32x4{pl[0], pl[1], pl[2], pl[3]}, o[dt]);
+            if (TILE && dt % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // (all reads at once: 32 registers)
         }
     };
     const int n_steps = (end - beg + kStep - 1) / kStep;
+    const auto nothing = [] {};
     Step A, B;
-    for (int j0 = 0; j0 < n_steps; j0 += 32) {
-        const int j1 = BIG ? min(n_steps, j0 + 32) : n_steps;
-        if (j0 > 0) ent = entries(j0);
-        load_step(j0, ent, A);
-        for (int j = j0;;) {
-            if (!BIG) ent = next_entry(j + 2);
-            load_step(j + 1 < j1 ? j + 1 : kNoStep, BIG ? ent : ent_next, B);
-            __builtin_amdgcn_sched_barrier(0);  // (the compiler would move them behind the products)
-            process(j, A);
-            if (++j >= j1) break;
-            if (!BIG) ent_next = next_entry(j + 2);
-            load_step(j + 1 < j1 ? j + 1 : kNoStep, ent, A);
-            __builtin_amdgcn_sched_barrier(0);
-            process(j, B);
-            if (++j >= j1) break;
+    Operands next;
+    if constexpr (TILE) {
+        // The matrix and vector units bound it, not memory: K and V of one step in registers,
+        // the next step's loaded where this one's products and stores are done with them, so
+        // that another wave fits a SIMD.
+        Rows R;
+        for (int j0 = 0; j0 < n_steps; j0 += 32) {
+            const int j1 = min(n_steps, j0 + 32);
+            if (j0 > 0) ent = entries(j0);
+            load_step(j0, ent, A, R, next);
+            load_k(next, R);
+            load_v(next, R);
+            for (int j = j0; j < j1; ++j) {
+                load_step(j + 1 < j1 ? j + 1 : kNoStep, ent, B, R, next);
+                // (kept there: earlier they would need registers of their own)
+                process(j, A, R, [&] {
+                    __builtin_amdgcn_sched_barrier(0);
+                    load_k(next, R);
+                    __builtin_amdgcn_sched_barrier(0);
+                }, [&] {
+                    __builtin_amdgcn_sched_barrier(0);
+                    load_v(next, R);
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                A = B;
+            }
         }
-        if (!BIG) break;
+    } else {
+        Rows RA, RB;
+        for (int j0 = 0; j0 < n_steps; j0 += 32) {
+            const int j1 = BIG ? min(n_steps, j0 + 32) : n_steps;
+            if (j0 > 0) ent = entries(j0);
+            load_step(j0, ent, A, RA, next);
+            for (int j = j0;;) {
+                if (!BIG) ent = next_entry(j + 2);
+                load_step(j + 1 < j1 ? j + 1 : kNoStep, BIG ? ent : ent_next, B, RB, next);
+                __builtin_amdgcn_sched_barrier(0);  // (the compiler would move them behind the products)
+                process(j, A, RA, nothing, nothing);
+                if (++j >= j1) break;
+                if (!BIG) ent_next = next_entry(j + 2);
+                load_step(j + 1 < j1 ? j + 1 : kNoStep, ent, A, RA, next);
+                __builtin_amdgcn_sched_barrier(0);
+                process(j, B, RB, nothing, nothing);
+                if (++j >= j1) break;
+            }
+            if (!BIG) break;
+        }
     }
     if constexpr (I8 && !BIG) bad = __builtin_amdgcn_ballot_w64(most_vs >= 0x7F800000u) != 0;
     l = sum_xor_rows<16>(l);
