@@ -35,6 +35,8 @@
 namespace rxq4 {
 namespace {
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int kStep = 128;      // positions per step of a workgroup
 constexpr int kNoStep = 1 << 22;  // past every position (2^24 at most): its loads are past the end
 constexpr int kMaxChunks = 64;  // chunks of positions per sequence
@@ -302,7 +304,6 @@ enum Lists { kNoLists, kTokenLists, kTileLists };
 template <int HD, bool I8, bool BIG, Lists LISTS>
 __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, LISTS == kTileLists)) void attn_paged_rows_kernel(PagedParams p) {
     constexpr bool SEL = LISTS == kTokenLists, TILE = LISTS == kTileLists;
-    static_assert(!TILE || BIG, "an operand of a tile lies in one page");
     // A chunk is 16 bytes: 8 dims of fp16, 16 of int8, which are two k steps of a
     // product (a lane's dims need only be the same in K and Q).
     constexpr int EC = I8 ? 16 : 8;                     // dims of a chunk
@@ -315,6 +316,7 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
     __shared__ __attribute__((aligned(16))) uint8_t smem[kV > kM ? kV : kM];
     __shared__ int64_t rowoff[BIG ? 1 : 4][32];
     __shared__ __attribute__((aligned(16))) float scl[4][3][I8 ? 32 : 1];
+    __shared__ __attribute__((aligned(16))) int tokens_of[TILE && !BIG ? 4 : 1][32];  // that see each position
 
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
@@ -393,7 +395,9 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
     };
     auto next_entry = [&](int j) {  // small pages: the lane's position's of step j, asked for in order
         const int at = p_lane + kStep * j;
-        if constexpr (SEL) {
+        if constexpr (TILE) {
+            return 0;  // (in LDS: looked up with the loads)
+        } else if constexpr (SEL) {
             const int x = j == 0 ? listed(at) : x_ahead;
             x_ahead = listed(at + kStep);
             const int page = page_of(x);
@@ -455,16 +459,20 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
     struct Step {
         float ks, vs;
         uint32_t seen;  // which of the wave's 32 positions there are
-        int of[2];      // TILE: an operand's page and tokens
-        bool all[2];    // TILE: every token sees all of the operand
+        int of[2];      // TILE: an operand's page and tokens; small pages: the lane's position's tokens
+        bool all[2];    // TILE: every token sees all of the operand (small pages: of both)
     };
     // TILE: the loads of K and of V are left to the caller, from the operands' buffers
     struct Operands {
         __amdgpu_buffer_rsrc_t k[2], v[2];
     };
-    auto load_rows = [&](const __amdgpu_buffer_rsrc_t *from, u32x4 *x) {
+    auto load_rows = [&](const __amdgpu_buffer_rsrc_t *from, const uint8_t *base, u32x4 *x) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
+            if constexpr (!BIG) {
+                x[j] = load16(base + rowoff[w][min((lane + 64 * j) / CH, 31)] + vo[j]);
+                continue;
+            }
             constexpr bool kSplit = 64 % CH != 0 || 64 / CH > 16;  // a load's rows may be in both operands
             if constexpr (kSplit) {
                 const bool first = (lane + 64 * j) / CH < 16;
@@ -476,7 +484,7 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
     };
     auto load_k = [&](const Operands &from, Rows &R) {
         if constexpr (TILE) {
-            load_rows(from.k, R.k[0]);
+            load_rows(from.k, kb, R.k[0]);
         } else {
 #pragma unroll
             for (int st = 0; st < 2; ++st)
@@ -484,8 +492,8 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
                 for (int i = 0; i < KL; ++i) R.k[st][i] = buffer_load16(from.k[st], ko[i]);
         }
     };
-    auto load_v = [&](const Operands &from, Rows &R) { load_rows(from.v, R.v); };
-    auto load_step = [&](int j, int e, Step &S, Rows &R, Operands &from) {
+    auto load_v = [&](const Operands &from, Rows &R) { load_rows(from.v, vb, R.v); };
+    auto load_step = [&](int j, [[maybe_unused]] int e, Step &S, Rows &R, Operands &from) {
         const int mask = (1 << p.c.shift) - 1;
         if constexpr (BIG) {
             // an operand's rows: those of its positions that there are, from the first
@@ -524,7 +532,17 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
             }
         } else {
             const int pos = p_lane + kStep * j;
-            const bool ok = pos < end && (unsigned)e < (unsigned)p.c.n_pages;
+            bool ok = pos < end && (unsigned)e < (unsigned)p.c.n_pages;
+            if constexpr (TILE) {
+                const int k = min(pos >> p.c.shift, listed_pages - 1), of = work[p.tile * p.n_select + k];
+                const int at = ((of & 0xFFFFFF) << p.c.shift) + (pos & mask);  // the place of the sequence
+                // of the tokens that list it those that are not before it
+                const int before = max(at - (span.pos0 + unit.tok), 0);
+                S.of[0] = pos < end && at < limit && before < 8 ? (of >> 24 & 0xFF) >> before << before : 0;
+                ok = S.of[0] != 0;
+                e = ok ? work[k] : 0;
+                S.all[0] = __builtin_amdgcn_ballot_w64(S.of[0] != (1 << unit.tokens) - 1) == 0;
+            }
             S.seen = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
             const int place = pos & mask;
             if constexpr (I8) {
@@ -532,8 +550,10 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
                 S.ks = ksp[at * s_stride];
                 S.vs = vsp[at * v_stride];
             }
+            if constexpr (TILE) wave_lds_fence();  // the rows before are asked for
             if (lane < 32) rowoff[w][lane] = ok ? (int64_t)e * p.c.page_bytes + (int64_t)place * row_bytes : 0;
             wave_lds_fence();
+            if constexpr (TILE) return;
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
                 const uint8_t *src = kb + rowoff[w][16 * st + r];
@@ -619,7 +639,20 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
         float sv[8], mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sv[i] = acc[i >> 2][i & 3] * p.sl2;
-        if constexpr (TILE) {
+        if constexpr (TILE && !BIG) {
+            if (!S.all[0]) {  // uniform
+                if (lane < 32) tokens_of[w][lane] = S.of[0];
+                wave_lds_fence();
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    const i32x4 of = *reinterpret_cast<const i32x4 *>(&tokens_of[w][16 * st + 4 * g]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!(of[i] >> mine & 1)) sv[4 * st + i] = -INFINITY;
+                }
+                wave_lds_fence();
+            }
+        } else if constexpr (TILE) {
 #pragma unroll
             for (int st = 0; st < 2; ++st)
                 if (!S.all[st]) {  // uniform
@@ -722,7 +755,7 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
         Rows R;
         for (int j0 = 0; j0 < n_steps; j0 += 32) {
             const int j1 = min(n_steps, j0 + 32);
-            if (j0 > 0) ent = entries(j0);
+            if (BIG && j0 > 0) ent = entries(j0);
             load_step(j0, ent, A, R, next);
             load_k(next, R);
             load_v(next, R);
@@ -993,10 +1026,9 @@ SelectedPlan plan_selected(PagedParams &p, int i8) {
     const int pad = p.c.hd <= 64 ? 64 : p.c.hd <= 96 ? 96 : p.c.hd <= 128 ? 128 : 256;
     p.rows_blk = std::min(p.group, kPagedRows);
     p.head_blocks = (p.group + kPagedRows - 1) / kPagedRows;
-    // Tiles where the sequences have tokens to fill them, the pages hold whole operands and the
-    // tiles are enough for the CUs.
+    // Tiles where the sequences have tokens to fill them and the tiles are enough for the CUs.
     p.tile = (int)std::min<int64_t>({(int64_t)kPagedRows / p.group, 8, kListEntries / p.n_select});
-    if (p.tile > 1 && p.c.shift >= 4 && p.b.max_new > 1 && p.b.n_tokens >= 4 * (int64_t)p.b.n_seqs) {
+    if (p.tile > 1 && p.b.max_new > 1 && p.b.n_tokens >= 4 * (int64_t)p.b.n_seqs) {
         const int64_t tiles = ((p.b.n_tokens + p.tile - 1) / p.tile + p.b.n_seqs) * (int64_t)p.c.n_kv;
         if (tiles >= cus) {
             p.n_chunks = 1;
@@ -1025,8 +1057,10 @@ hipError_t launch_selected(PagedParams &p, const SelectedPlan &plan, float *ws, 
     const bool big = p.c.shift >= 4;
     if (p.tile > 1) {
         const size_t lds = (size_t)3 * p.tile * p.n_select * 4;
-        if (i8) attn_paged_rows_kernel<HD, true, true, kTileLists><<<grid, 256, lds, st>>>(p);
-        else attn_paged_rows_kernel<HD, false, true, kTileLists><<<grid, 256, lds, st>>>(p);
+        if (i8 && big) attn_paged_rows_kernel<HD, true, true, kTileLists><<<grid, 256, lds, st>>>(p);
+        else if (i8) attn_paged_rows_kernel<HD, true, false, kTileLists><<<grid, 256, lds, st>>>(p);
+        else if (big) attn_paged_rows_kernel<HD, false, true, kTileLists><<<grid, 256, lds, st>>>(p);
+        else attn_paged_rows_kernel<HD, false, false, kTileLists><<<grid, 256, lds, st>>>(p);
         return hipGetLastError();
     }
     if (i8 && big) attn_paged_rows_kernel<HD, true, true, kTokenLists><<<grid, 256, 0, st>>>(p);

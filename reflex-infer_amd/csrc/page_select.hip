@@ -66,7 +66,7 @@ __device__ __forceinline__ void bound_page(const BoundsParams &p, int page, int 
         lo[i] = INFINITY;
         hi[i] = -INFINITY;
     }
-    constexpr int U = 4;
+    constexpr int U = 8;
     for (int at = grp; at < held; at += U * kGroups) {
         u32x4 x[U];
         float s[U];
@@ -895,10 +895,12 @@ hipError_t launch_select(SelectParams p, hipStream_t st) {
 
 hipError_t launch_kv_bounds(const PageBounds &bounds, const SeqBatch &batch, const PagedCache &cache,
                             int kv_int8, hipStream_t st) {
-    // Few rows: one a workgroup; many: as many as leave some thousand workgroups, a page's at most.
-    BoundsParams p{bounds, batch, cache, std::max(1, std::min(1 << cache.shift, batch.n_tokens / 1024))};
-    const int heads = kPieces / (cache.hd / 8);
-    const dim3 grid((batch.n_tokens + p.rows_wg - 1) / p.rows_wg, (cache.n_kv + heads - 1) / heads);
+    // Few rows: one a workgroup; many: as many as leave a thousand workgroups, a page's at most
+    // (those without a page's first row end after the lookup of their sequence).
+    const int heads = kPieces / (cache.hd / 8), parts = (cache.n_kv + heads - 1) / heads;
+    const int64_t rows = (int64_t)batch.n_tokens * parts / 1024;
+    BoundsParams p{bounds, batch, cache, (int)std::max<int64_t>(1, std::min<int64_t>(1 << cache.shift, rows))};
+    const dim3 grid((batch.n_tokens + p.rows_wg - 1) / p.rows_wg, parts);
     if (kv_int8) kv_bounds_kernel<true><<<grid, 256, 0, st>>>(p);
     else kv_bounds_kernel<false><<<grid, 256, 0, st>>>(p);
     return hipGetLastError();

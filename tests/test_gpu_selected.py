@@ -308,6 +308,88 @@ def test_attention(heads, page, int8, new, lens, n_select):
     check_attend(p, run_attend(p, lists, scale), lists, scale)
 
 
+# heads, page, int8, new, lens, n_select: several tokens' lists walked together (256 tiles or more)
+TILES = [
+    ((32, 32, 16), 16, False, [70, 1, 3], [300, 200, 3], 6),     # eight tokens a tile
+    ((64, 32, 64), 16, True, [60, 9, 5], [400, 9, 64], 9),       # of 2 heads: eight
+    ((48, 16, 80), 32, False, [90, 1, 1], [300, 40, 200], 5),    # of 3: five
+    ((64, 16, 128), 16, False, [75, 20, 2], [600, 33, 90], 12),  # of 4: four
+    ((80, 16, 64), 64, True, [60], [500], 4),                    # of 5: three
+    ((112, 16, 128), 32, False, [40, 7], [500, 64], 7),          # of 7: two
+    ((56, 8, 256), 16, False, [70, 4], [300, 4], 11),
+    ((64, 8, 96), 128, False, [70], [700], 3),                   # of 8: two
+    ((32, 32, 48), 8, False, [70, 2], [200, 30], 13),            # pages of fewer positions than an operand
+    ((64, 32, 64), 4, True, [60, 9, 5], [300, 9, 64], 33),
+    ((64, 16, 128), 8, False, [75, 20, 2], [400, 33, 90], 24),
+    ((64, 16, 128), 1, True, [75, 2], [300, 33], 90),
+    ((48, 16, 80), 8, True, [90], [300], 15),
+    ((64, 16, 200), 2, False, [70], [120], 21),
+    ((16, 8, 64), 16, False, [300], [320], 256),                 # lists of all that a tile holds
+]
+
+
+@pytest.mark.parametrize("order", ["ascending", "any"])
+@pytest.mark.parametrize("heads,page,int8,new,lens,n_select", TILES)
+def test_attention_of_tiles(heads, page, int8, new, lens, n_select, order):
+    """Ascending lists are merged; lists with pages twice, in any order, with -1s
+    between or places that are none are walked as they are."""
+    print(f"tiles {heads} page={page} int8={int8} new={new} lens={lens} n_select={n_select} {order}", flush=True)
+    p = ref.Paged(116, *heads, page, new, lens, int8, pad=3, lead=2, apart=page == 32)
+    lists = sel.random_lists(p, n_select, 117, odd=order == "any")
+    scale = heads[2] ** -0.5
+    check_attend(p, run_attend(p, lists, scale), lists, scale)
+
+
+def test_tiles_whose_lists_agree_differ_and_are_empty():
+    """Neighbours with the same list, with none in common, with holes, and with nothing
+    that is theirs to see."""
+    p = ref.Paged(118, 64, 16, 64, 16, [80], [400], holes=[(0, 3), (0, 9)])
+    lists = np.full((p.rows, 16, 8), -1, np.int32)
+    for t in range(80):
+        last = (320 + t) // 16
+        lists[t, :, :4] = [0, 3, 7, last] if t < 30 else [t % 4, 4 + t % 4, 9, 10 + t % 4]
+        if t % 11 == 5:
+            lists[t] = -1
+        if t % 11 == 6:
+            lists[t] = [3, 9] + [-1] * 6
+        if t % 11 == 7:
+            lists[t] = [last + 1, last + 2] + [-1] * 6
+    got = run_attend(p, lists, 0.125)
+    check_attend(p, got, lists, 0.125)
+    assert not got[5].any() and not got[6].any() and not got[7].any()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("page,int8", [(16, False), (8, False), (16, True), (4, True)])
+def test_tiles_keep_what_one_token_looks_at_from_the_others(bad, page, int8):
+    """Infinities and NaN in a page that only one token of the tile lists, and in the
+    last positions, which the tokens before do not see."""
+    p = ref.Paged(119, 64, 16, 64, page, [80], [400], int8)
+    lists = np.full((p.rows, 16, 3), -1, np.int32)
+    for t in range(80):
+        lists[t, :, 0], lists[t, :, 1] = 0, (320 + t) // page
+    lists[41, :] = [0, 2, (320 + 41) // page]
+    clean = run_attend(p, lists, 0.125).cpu()
+    check_attend(p, clean, lists, 0.125)
+    slots = p.slots(0, 400)
+    at = slots[2 * page + 1]
+    if int8:
+        p.vs.view(-1, 16)[at, 3], p.ks.view(-1, 16)[at, 5] = bad, bad
+        p.vs.view(-1, 16)[slots[399], 3] = bad
+    else:
+        p.both[1].view(-1, 16, 64)[at, 3, 7], p.both[0].view(-1, 16, 64)[at, 5, 7] = bad, bad
+        p.both[1].view(-1, 16, 64)[slots[399], 3, 7] = bad
+    got = run_attend(p, lists, 0.125).cpu()
+    rest = [t for t in range(79) if t != 41]
+    assert torch.equal(got[rest], clean[rest])
+    assert not torch.isfinite(got[41, 12:16]).all() and not torch.isfinite(got[79, 12:16]).all()
+    keep = torch.ones(64, dtype=torch.bool)
+    keep[12:16] = False
+    assert torch.equal(got[79][keep], clean[79][keep])
+    keep[20:24] = False
+    assert torch.equal(got[41][keep], clean[41][keep])
+
+
 @pytest.mark.parametrize("int8,page", [(False, 16), (True, 16), (False, 4), (True, 8)])
 def test_all_pages_listed_is_the_paged_attention(int8, page):
     """Within what two roundings of the same sums differ by: each is within its bound."""
