@@ -208,64 +208,87 @@ __device__ __forceinline__ RowsUnit tile_unit(const PagedParams &p, int &kvh) {
     return r;
 }
 
-// The pages that a tile's tokens list, each once with the tokens that do, in the order of
-// the first token's list, then what the second's adds, ..: work[k] the page of the pool,
-// work[tile * n_select + k] its place in the table | tokens << 24; how many.  Found by
-// binary search where every list ascends (rxq4_select_pages'); of others every entry stays
-// its own.  By the whole workgroup.
-__device__ __forceinline__ int merge_lists(const PagedParams &p, const RowsUnit &unit, int kvh, int *work) {
-    __shared__ int counts[2][4], out_of_order;
+// The pages that a tile's tokens list, in order, each once with the tokens that do: work[k]
+// the page of the pool, work[tile * n_select + k] its place in the table | tokens << 24; how
+// many.  A byte of `marks` (LDS of so many bytes) a page of the sequence takes the tokens'
+// bits, part after part of a long one.  Where a list has a page twice every entry of all
+// stays its own.  By the whole workgroup.
+__device__ __forceinline__ int merge_lists(const PagedParams &p, const RowsUnit &unit, int kvh, int *work,
+                                           uint32_t *marks, int bytes) {
+    __shared__ int counts[2][4], twice;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = p.n_select, total = unit.tokens * n;
     const int limit = position_limit(p.b, p.c);
-    int *const lists = work + 2 * p.tile * n;
-    constexpr int kEnd = 0x7FFFFFFF;
-    if (tid == 0) out_of_order = 0;
     const int32_t *const table = p.c.table ? p.c.table + (int64_t)unit.s * p.c.width : nullptr;
-    const auto value = [&](int t, int i) {
-        const int x = p.lists[((int64_t)(unit.span.row0 + unit.tok + t) * p.c.n_kv + kvh) * n + i];
+    const auto pages_of = [&](int t) {
         const int sees = min(limit, unit.span.pos0 + unit.tok + t + 1);
-        const int pages = sees > 0 ? ((sees - 1) >> p.c.shift) + 1 : 0;
-        return x >= 0 && x < pages ? x : kEnd;
+        return sees > 0 ? ((sees - 1) >> p.c.shift) + 1 : 0;
     };
-    for (int e = tid; e < total; e += 256) lists[e] = value(e / n, e % n);
-    __syncthreads();
-    bool wrong = false;
-    for (int e = tid; e < total; e += 256)
-        wrong |= e % n > 0 && lists[e] <= lists[e - 1] && !(lists[e] == kEnd && lists[e - 1] == kEnd);
-    if (wrong) out_of_order = 1;
-    __syncthreads();
-    const bool ascend = out_of_order == 0;
-    int found = 0;
-    for (int e0 = 0, odd = 0; e0 < total; e0 += 256, odd ^= 1) {
-        const int e = e0 + tid, t = min(e, total - 1) / n, x = e < total ? lists[e] : kEnd;
-        uint32_t tokens = 1u << t;
-        if (ascend && x != kEnd)
-            for (int o = 0; o < unit.tokens; ++o) {
-                if (o == t) continue;
-                const int *l = lists + o * n;
-                int a = 0, b = n;  // the first entry not below x
-                while (a < b) {
-                    const int m = (a + b) >> 1;
-                    if (l[m] < x) a = m + 1;
-                    else b = m;
-                }
-                if (a < n && l[a] == x) tokens |= 1u << o;
-            }
-        int page = -1;
-        if (x != kEnd && (tokens & ((1u << t) - 1u)) == 0) page = table ? table[x] : x;  // (the first that lists it)
-        const bool keep = (unsigned)page < (unsigned)p.c.n_pages;
-        const uint64_t kept = __builtin_amdgcn_ballot_w64(keep);
-        if (lane == 0) counts[odd][w] = __builtin_popcountll(kept);
+    const auto value = [&](int e, int &t) {  // -1: none that the token sees
+        t = e / n;
+        const int x = p.lists[((int64_t)(unit.span.row0 + unit.tok + t) * p.c.n_kv + kvh) * n + e % n];
+        return x >= 0 && x < pages_of(t) ? x : -1;
+    };
+    int found = 0, odd = 0;
+    // the places of the workgroup's `mine` entries a thread, behind those found
+    const auto place = [&](int mine) {
+        const int upto = wave_prefix(mine);
+        if (lane == 63) counts[odd][w] = upto;
         __syncthreads();
-        int at = found + __builtin_popcountll(kept & ((uint64_t(1) << lane) - 1));
+        int at = found + upto - mine;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             at += i < w ? counts[odd][i] : 0;
             found += counts[odd][i];
         }
-        if (keep) {
-            work[at] = page;
-            work[p.tile * n + at] = x | (int)(tokens << 24);
+        odd ^= 1;
+        return at;
+    };
+    const auto keep = [&](int at, int page, int x, uint32_t tokens) {
+        work[at] = page;
+        work[p.tile * n + at] = x | (int)(tokens << 24);
+    };
+    if (tid == 0) twice = 0;
+    const int pages = pages_of(unit.tokens - 1);
+    for (int base = 0; base < pages; base += bytes) {
+        const int words = (min(bytes, pages - base) + 3) / 4;
+        __syncthreads();  // the part before is read
+        for (int i = tid; i < words; i += 256) marks[i] = 0;
+        __syncthreads();
+        for (int e = tid; e < total; e += 256) {
+            int t;
+            const int x = value(e, t) - base;
+            if (x < 0 || x >= bytes) continue;
+            const uint32_t bit = 1u << (8 * (x & 3) + t);
+            if (atomicOr(&marks[x >> 2], bit) & bit) twice = 1;
+        }
+        __syncthreads();
+        if (twice) break;
+        for (int i0 = 0; i0 < words; i0 += 256) {
+            const uint32_t m = i0 + tid < words ? marks[i0 + tid] : 0u;
+            int page[4], mine = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int x = base + 4 * (i0 + tid) + i;
+                page[i] = m >> (8 * i) & 0xFFu ? table ? table[x] : x : -1;
+                if ((unsigned)page[i] >= (unsigned)p.c.n_pages) page[i] = -1;
+                mine += page[i] >= 0;
+            }
+            int at = place(mine);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (page[i] >= 0) keep(at++, page[i], base + 4 * (i0 + tid) + i, m >> (8 * i) & 0xFFu);
+        }
+    }
+    if (pages > 0 && twice) {  // uniform
+        __syncthreads();
+        found = 0;
+        for (int e0 = 0; e0 < total; e0 += 256) {
+            int t = 0, page = -1;
+            const int x = e0 + tid < total ? value(e0 + tid, t) : -1;
+            if (x >= 0) page = table ? table[x] : x;
+            const bool there = (unsigned)page < (unsigned)p.c.n_pages;
+            const int at = place(there);
+            if (there) keep(at, page, x, 1u << t);
         }
     }
     __syncthreads();
@@ -327,12 +350,12 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
     int kvh, head0 = 0;
     RowsUnit unit;
     int listed_pages = 0;  // TILE: pages that the tile's tokens list
-    extern __shared__ int work[];  // TILE: their pages of the pool; their places | tokens << 24; the lists
+    extern __shared__ int work[];  // TILE: their pages of the pool; their places | tokens << 24
     if constexpr (SEL) {
         unit = selected_unit(p, kvh, head0);
     } else if constexpr (TILE) {
         unit = tile_unit(p, kvh);
-        if (unit.s >= 0) listed_pages = merge_lists(p, unit, kvh, work);
+        if (unit.s >= 0) listed_pages = merge_lists(p, unit, kvh, work, reinterpret_cast<uint32_t *>(smem), sizeof(smem));
     } else {
         const int x8 = blockIdx.x / 8;
         kvh = x8 % p.c.n_kv;
@@ -1020,7 +1043,7 @@ struct SelectedPlan {
     int64_t grid;
     size_t bytes;
 };
-constexpr int kListEntries = 2048;  // of a tile's lists: 24 KB of LDS
+constexpr int kListEntries = 2048;  // of a tile's lists: 16 KB of LDS
 SelectedPlan plan_selected(PagedParams &p, int i8) {
     const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
     const int pad = p.c.hd <= 64 ? 64 : p.c.hd <= 96 ? 96 : p.c.hd <= 128 ? 128 : 256;
@@ -1056,7 +1079,7 @@ hipError_t launch_selected(PagedParams &p, const SelectedPlan &plan, float *ws, 
     p.stats = ws + (size_t)p.b.n_tokens * p.n_chunks * p.head_blocks * p.c.n_kv * p.rows_blk * HD;
     const bool big = p.c.shift >= 4;
     if (p.tile > 1) {
-        const size_t lds = (size_t)3 * p.tile * p.n_select * 4;
+        const size_t lds = (size_t)2 * p.tile * p.n_select * 4;
         if (i8 && big) attn_paged_rows_kernel<HD, true, true, kTileLists><<<grid, 256, lds, st>>>(p);
         else if (i8) attn_paged_rows_kernel<HD, true, false, kTileLists><<<grid, 256, lds, st>>>(p);
         else if (big) attn_paged_rows_kernel<HD, false, true, kTileLists><<<grid, 256, lds, st>>>(p);

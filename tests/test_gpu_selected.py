@@ -325,6 +325,7 @@ TILES = [
     ((48, 16, 80), 8, True, [90], [300], 15),
     ((64, 16, 200), 2, False, [70], [120], 21),
     ((16, 8, 64), 16, False, [300], [320], 256),                 # lists of all that a tile holds
+    ((32, 16, 16), 1, False, [140], [50000], 9),                 # more pages than are marked at a time
 ]
 
 
