@@ -152,21 +152,22 @@ __device__ __forceinline__ RowsUnit rows_unit(const PagedParams &p, int idx) {
 }
 
 // Listed pages: a token, its KV head kvh, the heads of the group from head0 on, and a chunk
-// of the places.  An XCD (workgroups are dealt to the eight in turn) takes tokens one after
-// another, which list much the same pages in a prompt, and all of a token's KV heads: their
-// rows lie beside one another, one head's alone in a part of the L2's channels.
+// of the places.  An XCD (workgroups are dealt to the eight in turn) takes the tokens of one
+// KV head one after another: the lists of two heads have no pages in common (64 sequences'
+// tokens with 1024 positions each 50.7 us; all heads of a token on one XCD 52.7).
 __device__ __forceinline__ RowsUnit selected_unit(const PagedParams &p, int &kvh, int &head0) {
     RowsUnit r{};
     r.s = -1;
     const int per = gridDim.x / 8;  // (a multiple of 8)
     const int idx = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-    kvh = idx % p.c.n_kv;
-    int at = idx / p.c.n_kv;
-    r.c = at % p.n_chunks;
-    at /= p.n_chunks;
-    const int block = at % p.head_blocks, t = at / p.head_blocks;
+    r.c = idx % p.n_chunks;
+    int at = idx / p.n_chunks;
+    const int block = at % p.head_blocks;
+    at /= p.head_blocks;
+    const int t = at % p.b.n_tokens;
+    kvh = at / p.b.n_tokens;
     head0 = block * kPagedRows;
-    if (t >= p.b.n_tokens) return r;
+    if (kvh >= p.c.n_kv) return r;
     const int s = seq_of_row(p.b, t, r.span);
     r.tok = t - r.span.row0;
     if (s >= p.b.n_seqs || r.tok < 0 || r.tok >= min(r.span.n, p.b.max_new)) return r;
