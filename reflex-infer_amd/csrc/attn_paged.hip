@@ -16,6 +16,7 @@
 // 4 KB pieces at 6.0.  So a step's loads are issued a step ahead, nothing of K passes
 // LDS, and the chunks are cut from the batch's own lengths, which only the device knows
 // (up to kSeqs sequences).
+// Attention over listed pages is the same walk over the places of a list (`Lists` below).
 // Measured, 32 / 8 heads of 128, one new token a sequence, pages of 16: 512
 // sequences of 1023 positions 372 us (5.8 TB/s), 256 of 2047 397 (5.4), 64 of 64 to
 // 8000 92 (4.7); int8 512 of 1023 231 (4.8; pages of 64 221), 256 of 2047 246 (4.5), 16
@@ -178,32 +179,19 @@ __device__ __forceinline__ RowsUnit selected_unit(const PagedParams &p, int &kvh
     return r;
 }
 
-// Listed pages: the tokens of a tile and their KV head kvh.  Unit u of the first
-// ceil(n_tokens / tile): the rows from u * tile up to the next such row that are of the
-// sequence of the first; the units behind them: a sequence's rows before its first multiple
-// of `tile`.  Every row is in one.
+// Listed pages: the tokens of a tile and their KV head kvh; an XCD takes tiles one after
+// another, with all of their KV heads.
 __device__ __forceinline__ RowsUnit tile_unit(const PagedParams &p, int &kvh) {
     RowsUnit r{};
     r.s = -1;
-    const int whole = (p.b.n_tokens + p.tile - 1) / p.tile, units = whole + p.b.n_seqs;
-    const int idx = (int)(blockIdx.x % 8) * (gridDim.x / 8) + (int)(blockIdx.x / 8), u = idx / p.c.n_kv;
+    const int idx = (int)(blockIdx.x % 8) * (gridDim.x / 8) + (int)(blockIdx.x / 8);
     kvh = idx % p.c.n_kv;
-    if (u >= units) return r;
-    int from, s;
-    if (u < whole) {
-        from = u * p.tile;
-        s = seq_of_row(p.b, from, r.span);
-        if (s >= p.b.n_seqs || from < r.span.row0) return r;
-    } else {
-        s = u - whole;
-        r.span = seq_span(p.b, s);
-        from = r.span.row0;
-        if (from % p.tile == 0) return r;
-    }
-    r.tok = from - r.span.row0;
-    r.tokens = min((from / p.tile + 1) * p.tile, r.span.row0 + min(r.span.n, p.b.max_new)) - from;
-    if (r.tokens <= 0) return r;
-    r.s = s;
+    const TileRows t = tile_rows(p.b, p.tile, idx / p.c.n_kv);
+    if (t.n == 0) return r;
+    r.span = t.span;
+    r.tok = t.row0 - t.span.row0;
+    r.tokens = t.n;
+    r.s = t.s;
     r.chunks = 1;
     r.chunk = 1 << 30;
     return r;
@@ -324,6 +312,12 @@ __device__ __forceinline__ int merge_lists(const PagedParams &p, const RowsUnit 
 // same, so the masks are the entries'.  kTileLists: several tokens of a sequence, as many as 16
 // rows hold, and the pages that any of them lists, each read once (the lists of a prompt's
 // neighbours agree on most); a row's mask is its token's bit beside the page.
+// Bound: a token's reads of the cache, in the pieces above; a tile's pages come from the L2,
+// and LDS bounds it: K and V of a step in and out, 32 KB a wave.
+// Measured, head_dim 128: 64 tokens of 32 / 8 heads, 64 pages of 16 each, 51 us (5.3 TB/s; 256
+// pages each 190, 5.65), 16 in an int8 cache, 32 pages of 64, 17 + 4 for the combine; a chunk of
+// 512 tokens of 28 / 4 heads, 64 pages of 32, 88 us (a token a workgroup 150, with K by the
+// operand's rows 134).
 enum Lists { kNoLists, kTokenLists, kTileLists };
 template <int HD, bool I8, bool BIG, Lists LISTS>
 __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, LISTS == kTileLists)) void attn_paged_rows_kernel(PagedParams p) {

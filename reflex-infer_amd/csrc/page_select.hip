@@ -209,29 +209,10 @@ __device__ __forceinline__ bool token_of(const SelectParams &p, int t, Tile &til
     tile.pos0 = span.pos0 + (t - span.row0);
     return true;
 }
-// Unit u of the first ceil(n_tokens / tokens): the rows from u * tokens up to the next such
-// row that are of the sequence of the first; the units behind them: a sequence's rows
-// before its first multiple of `tokens`.  Every row is in one.
 __device__ __forceinline__ bool tile_of(const SelectParams &p, int u, Tile &tile) {
-    const int whole = (p.b.n_tokens + p.tokens - 1) / p.tokens;
-    SeqSpan span;
-    int from;
-    if (u < whole) {
-        from = u * p.tokens;
-        tile.s = seq_of_row(p.b, from, span);
-        if (tile.s >= p.b.n_seqs || from < span.row0) return false;
-    } else {
-        tile.s = u - whole;
-        if (tile.s >= p.b.n_seqs) return false;
-        span = seq_span(p.b, tile.s);
-        from = span.row0;
-        if (from % p.tokens == 0) return false;  // a unit of the first kind
-    }
-    const int to = min((from / p.tokens + 1) * p.tokens, span.row0 + min(span.n, p.b.max_new));
-    tile.t0 = from;
-    tile.n = to - from;
-    tile.pos0 = span.pos0 + (from - span.row0);
-    return tile.n > 0;
+    const TileRows t = tile_rows(p.b, p.tokens, u);
+    tile = Tile{t.s, t.row0, t.n, t.span.pos0 + (t.row0 - t.span.row0)};
+    return t.n > 0;
 }
 
 // What the waves of a workgroup share while they score.  The queries of a tile in steps, for
@@ -511,6 +492,7 @@ struct PickShared {
     int sums[WAVES][4];
     uint32_t few[64];
     int n_few;           // 0
+    uint32_t lowest;     // 0
     int counts[kHold<WAVES> * WAVES];  // by 64 keys: those in, and of the border's key << 16
 };
 
@@ -621,8 +603,20 @@ __device__ __forceinline__ int pick_of(const uint32_t *keys, int n, int n_select
             above = tie + 1u;
             ties = need - __builtin_amdgcn_readlane(larger, at);
         } else {
-            // Many in one part, or infinities: parts of the keys' range, narrowed to one key.
+            // Many in one part, or infinities: parts of the keys' range, narrowed to one key.  From
+            // the part's own least key on: those below it are of the parts before, and not in the
+            // counts.
             uint32_t least = lo, most = high;
+            if (part >= 0) {
+                uint32_t lowest = 0;
+#pragma unroll
+                for (int c = 0; c < HOLD; ++c)
+                    if (x[c] != 0 && x[c] != kAlways && part_of(x[c]) == part) lowest = max(lowest, ~x[c]);
+                lowest = wave_max(lowest);
+                if (lane == 0) atomicMax(&sh.lowest, lowest);
+                sync_waves<WAVES>();
+                least = ~sh.lowest;
+            }
             const auto mine = [&](uint32_t key) {
                 return key >= least && key <= most && key != 0 && key != kAlways && (part < 0 || part_of(key) == part);
             };
@@ -711,7 +705,10 @@ __device__ __forceinline__ int narrow(const SelectParams &p, uint32_t *keys, int
                                       bool last, int32_t *out, PickShared<WAVES> &sh) {
     const int tid = WAVES > 1 ? threadIdx.x : threadIdx.x & 63;
     for (int i = tid; i < kBins; i += 64 * WAVES) sh.hist[0][i] = 0;
-    if (tid == 0) sh.n_few = 0;
+    if (tid == 0) {
+        sh.n_few = 0;
+        sh.lowest = 0;
+    }
     sync_waves<WAVES>();
     // (a key is kept at or before its own place, its page is that of a place as far or farther)
     const auto page = [&](int e) { return e < kept ? idx[e] : base + e - kept; };

@@ -67,6 +67,32 @@ __device__ __forceinline__ int seq_of_row(const SeqBatch &b, int t, SeqSpan &spa
     return __builtin_amdgcn_readfirstlane(base + n);
 }
 
+// Tiles of up to `tile` rows of one sequence.  Tile u of the first ceil(n_tokens / tile): the
+// rows from u * tile up to the next such row that are of the sequence of the first; the n_seqs
+// behind them: a sequence's rows before its first multiple of `tile`.  Every row is in one.
+// The same for a whole wave.
+struct TileRows {
+    int s, row0, n;  // sequence, first row, rows (none: 0)
+    SeqSpan span;
+};
+__device__ __forceinline__ TileRows tile_rows(const SeqBatch &b, int tile, int u) {
+    TileRows r{};
+    const int whole = (b.n_tokens + tile - 1) / tile;
+    if (u < whole) {
+        r.row0 = u * tile;
+        r.s = seq_of_row(b, r.row0, r.span);
+        if (r.s >= b.n_seqs || r.row0 < r.span.row0) return r;
+    } else {
+        r.s = u - whole;
+        if (r.s >= b.n_seqs) return r;
+        r.span = seq_span(b, r.s);
+        r.row0 = r.span.row0;
+        if (r.row0 % tile == 0) return r;  // one of the first kind
+    }
+    r.n = max(min((r.row0 / tile + 1) * tile, r.span.row0 + min(r.span.n, b.max_new)) - r.row0, 0);
+    return r;
+}
+
 // Positions that the batch's tokens may see or store: below the table's end.
 __device__ __forceinline__ int position_limit(const SeqBatch &b, const PagedCache &c) {
     return (int)min((int64_t)b.max_len, (int64_t)c.width << c.shift);

@@ -164,7 +164,13 @@ SELECT = [
     ((2, 1, 64), 1, [1], [14000], (4096, 5, 9)),
     ((2, 2, 64), 1, [40], [2100], (100, 1, 1)),               # sixteen tokens, several parts
     ((4, 1, 128), 1, [12], [9000], (200, 1, 1)),
-    ((64, 4, 64), 1, [20], [13000], (64, 1, 1)),              # one token a tile, several parts
+    ((64, 4, 64), 1, [20], [13000], (64, 1, 1)),              # of 16: two tokens a tile, several parts
+    ((4, 4, 256), 1, [40], [1500], (512, 1, 1)),              # the longest lists of a tile, its most LDS
+    ((8, 4, 256), 1, [40], [1500], (512, 1, 1)),
+    ((16, 4, 200), 1, [40], [1500], (511, 1, 1)),
+    ((32, 2, 256), 1, [9], [1500], (512, 1, 1)),
+    ((8, 2, 64), 1, [12], [9000], (513, 1, 1)),               # longer ones: a token a workgroup
+    ((4, 2, 256), 1, [300], [9000], (4096, 1, 1)),
 ]
 
 
@@ -204,6 +210,19 @@ def test_scores_at_their_ends():
     both[rng.random(p.pages) < 0.1] = -127
     for how in ((20, 1, 1), (70, 0, 0)):
         check_select(p, run_select(p, both, scale, *how), both, scale, *how)
+
+
+@pytest.mark.parametrize("new,length", [([300], 1500), ([1], 1500), ([1] * 140, 1500), ([40], 6000)])
+def test_scores_crowded_beside_a_few_far_ones(new, length):
+    """Most scores in one of equal parts of their range, lists that end among them: one
+    token a wave, a token a workgroup, the choice in a launch of its own."""
+    p = ref.Paged(84, 4, 2, 64, 1, new, [length] * len(new))
+    both, scale = sel.random_bounds(85, p.pages, 2, 64)
+    scale *= 1 + 1e-3 * np.random.default_rng(86).random(scale.shape).astype(np.float32)
+    for i in range(len(new)):
+        scale[p.table[i, 5], :], scale[p.table[i, 11], :] = 1e4, 1e3
+    for n in (100, 300, 500):
+        check_select(p, run_select(p, both, scale, n, 1, 1), both, scale, n, 1, 1)
 
 
 @pytest.mark.parametrize("new,page", [([1, 1], 16), ([30, 1, 9], 16), ([1], 1)])
