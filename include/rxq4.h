@@ -25,8 +25,8 @@
  *     work; no entry point but rxq4_release_workspace synchronises the
  *     device or the stream.  The one allocation is the fp32 workspace of the
  *     split launches (split-K GEMM with few output tiles, small-batch
- *     products on long rows, attention over long cached contexts) and of
- *     rxq4_sample_f32's bins: 48 MiB
+ *     products on long rows, attention over long cached contexts), of
+ *     rxq4_sample_f32's bins and rxq4_select_pages' scores: 48 MiB
  *     per (device, stream), made by the first such launch on that stream,
  *     never resized, and kept until rxq4_release_workspace(stream) frees it,
  *     so a HIP graph captured on a stream stays valid whatever runs later,
@@ -347,8 +347,10 @@ int rxq4_kv_bounds(void *bounds, float *scales, const rxq4_seq_batch *batch,
  *            rint(q / step) of the head's query (NaN as 0, infinities as 65504): up to the
  *            steps no key of the page has a larger product with the query.  The sum is
  *            exact, so the lists do not depend on how the work is cut
- * Tokens that see nothing get -1s.  Rows of no sequence are left as they are.  A few
- * tokens with many pages use the stream's workspace described above. */
+ * Bounds and scales are rxq4_kv_bounds' (a page whose scale is negative or NaN is not
+ * chosen for its score).  Tokens that see nothing get -1s.  Rows of no sequence, and of
+ * tokens past max_new, are left as they are.  A few tokens with many pages use the
+ * stream's workspace described above. */
 int rxq4_select_pages(int32_t *pages, int n_select, int n_first, int n_last, const void *q,
                       int n_heads, const void *bounds, const float *scales,
                       const rxq4_seq_batch *batch, const rxq4_paged_kv *cache, void *stream);

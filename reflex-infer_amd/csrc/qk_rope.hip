@@ -22,6 +22,9 @@
 // Bound: for many tokens the rows' bytes, in and out; for a few the chain of lengths,
 // table entry, sine and store.  So a few tokens' heads are spread over workgroups, a pass
 // each; many tokens keep all heads in one, which shares the sines.
+// With coordinates on several axes (a pair's angle from its axis's) the token's n_axes
+// values and the pairs' axes are loads beside the first rows': 3595 tokens from bf16 on three
+// axes 24.7 us, one token of 16 / 2 heads 4.5.
 // Measured, 32 / 8 heads of 128: 3595 tokens from bf16 24.4 us (3.6 TB/s; a copy of the
 // bytes 17; 31 with each row's loads after the sines), 64 tokens into int8 4.9, one token
 // of 16 / 2 heads 4.1.
