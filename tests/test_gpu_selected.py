@@ -410,6 +410,94 @@ def test_tiles_keep_what_one_token_looks_at_from_the_others(bad, page, int8):
     assert torch.equal(got[41][keep], clean[41][keep])
 
 
+def check_all(p, how, scale=0.125, seed=120, **limits):
+    """The choice against bounds of its own, and attention over its lists."""
+    both, by = sel.random_bounds(seed, p.pages, p.kv, p.hd)
+    cache, batch = p.device(capi, **limits)
+    got = run_select(p, both, by, *how, cache=cache, batch=batch)
+    check_select(p, got, both, by, *how, **limits)
+    out = run_attend(p, got, scale, cache, batch)
+    want, bound = sel.attend(p, got.cpu().numpy(), scale)
+    mine = ~torch.isnan(want)
+    for i, n in enumerate(p.new):  # new tokens past max_new are left alone
+        if limits.get("max_new") is not None and n > limits["max_new"]:
+            first = int(p.starts[i])
+            mine[first + limits["max_new"]:first + n] = False
+    out = out.cpu().double()
+    assert ((out - want).abs() <= bound)[mine].all()
+    assert (out[~mine] == 7.0).all()
+
+
+@pytest.mark.parametrize("heads", [(64, 64, 16), (32, 16, 32), (64, 16, 64), (80, 16, 16)])
+@pytest.mark.parametrize("page", [4, 16])
+def test_tiles_of_many_sequences(heads, page):
+    """Sequences that begin and end inside a tile's rows, some without new tokens, some
+    without positions, some with fewer positions than new tokens."""
+    new = [(i * 7) % 10 if i % 9 else 0 for i in range(60)]
+    lens = [0 if i % 17 == 3 else 3 + (i * 29) % 120 for i in range(60)]
+    p = ref.Paged(121, *heads, page, new, lens, pad=3, lead=1)
+    check_all(p, (5, 1, 1))
+
+
+@pytest.mark.parametrize("page,int8", [(16, False), (8, True)])
+def test_tiles_within_limits(page, int8):
+    p = ref.Paged(122, 64, 16, 64, page, [70, 25, 40], [300, 25, 12], int8, pad=2, lead=1, holes=[(0, 1), (1, 0)])
+    check_all(p, (6, 1, 2))
+    check_all(p, (6, 1, 2), max_new=24)
+    p = ref.Paged(123, 64, 16, 64, page, [70, 25], [300, 25], int8)
+    both, by = sel.random_bounds(124, p.pages, p.kv, p.hd)
+    for limits in (dict(max_len=250), dict(max_len=1 << 24)):
+        check_select(p, run_select(p, both, by, 6, 1, 2, **limits), both, by, 6, 1, 2, **limits)
+
+
+@pytest.mark.parametrize("starts", [[0, 5, 3], [-4, 2, 9], [0, 100000, 100001], [7, 2, 1], [2 ** 31 - 1] * 3, [-2 ** 31] * 3])
+@pytest.mark.parametrize("lens", [[64, 64], [2 ** 31 - 1, -2 ** 31]])
+@pytest.mark.parametrize("page", [4, 16])
+def test_tiles_with_starts_and_lengths_outside_their_limits_stay_inside(starts, lens, page):
+    p = ref.Paged(125, 64, 64, 16, page, [4, 5], [64, 64])
+    cache, batch = p.device(capi)
+    batch.tensors[0].copy_(torch.tensor(starts, dtype=torch.int32))
+    batch.tensors[1].copy_(torch.tensor(lens, dtype=torch.int32))
+    lists = torch.from_numpy(np.random.default_rng(126).integers(-2, 70 // page, (p.rows, 64, 6)).astype(np.int32)).cuda()
+    out = torch.full((p.rows + 20, 64, 16), 7.0, dtype=torch.float16, device="cuda")
+    capi.attention_selected_f16(out[10:-10], p.q.cuda(), lists, batch, cache, 0.25)
+    assert (out[:10] == 7.0).all() and (out[-10:] == 7.0).all() and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("page,int8", [(16, False), (4, True)])
+def test_tiles_captured_replayed_and_in_place(page, int8):
+    new, lens = [75, 20, 2], [500, 90, 64]
+    p = ref.Paged(127, 64, 16, 64, page, new, lens, int8)
+    cache, batch = p.device(capi, max_len=600)
+    q, n = p.q.cuda(), 7
+    out, lists = torch.empty_like(q), torch.zeros((p.rows, 16, n), dtype=torch.int32, device="cuda")
+    both, by = sel.random_bounds(128, p.pages, p.kv, p.hd)
+    bounds, scales = torch.from_numpy(both).cuda(), torch.from_numpy(by).cuda()
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        capi.select_pages(lists, q, bounds, scales, batch, cache, 1, 1, stream=s)
+        capi.attention_selected_f16(out, q, lists, batch, cache, 0.125, stream=s)
+    for step in range(3):
+        p.lens = [max(k, m - 19 * step) for k, m in zip(new, lens)]
+        p.seq_lens = torch.tensor(p.lens, dtype=torch.int32)
+        batch.tensors[1].copy_(p.seq_lens)
+        out.fill_(7.0), lists.fill_(-7)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            graph.replay()
+        torch.cuda.synchronize()
+        check_select(p, lists, both, by, n, 1, 1, max_len=600)
+        check_attend(p, out, lists.cpu().numpy(), 0.125)
+        eager, again = torch.empty_like(out), torch.zeros_like(lists)
+        capi.select_pages(again, q, bounds, scales, batch, cache, 1, 1)
+        capi.attention_selected_f16(eager, q, again, batch, cache, 0.125)
+        assert torch.equal(again, lists) and torch.equal(eager, out)
+    capi.attention_selected_f16(q, q, lists, batch, cache, 0.125)
+    assert torch.equal(q, out)
+
+
 @pytest.mark.parametrize("int8,page", [(False, 16), (True, 16), (False, 4), (True, 8)])
 def test_all_pages_listed_is_the_paged_attention(int8, page):
     """Within what two roundings of the same sums differ by: each is within its bound."""
