@@ -169,6 +169,12 @@ SELECT = [
     ((8, 4, 256), 1, [40], [1500], (512, 1, 1)),
     ((16, 4, 200), 1, [40], [1500], (511, 1, 1)),
     ((32, 2, 256), 1, [9], [1500], (512, 1, 1)),
+    ((4, 4, 256), 1, [40], [3000], (256, 1, 1)),              # several parts, pages of one token
+    ((4, 4, 256), 1, [40], [3000], (257, 1, 1)),
+    ((8, 2, 64), 1, [30], [9000], (70, 1, 69)),               # several parts; the last pages always
+    ((8, 2, 64), 1, [30], [9000], (70, 69, 1)),
+    ((2, 2, 64), 1, [50], [7000], (10, 0, 0)),
+    ((16, 1, 64), 1, [20], [9000], (200, 5, 5)),
     ((8, 2, 64), 1, [12], [9000], (513, 1, 1)),               # longer ones: a token a workgroup
     ((4, 2, 256), 1, [300], [9000], (4096, 1, 1)),
 ]
@@ -223,6 +229,21 @@ def test_scores_crowded_beside_a_few_far_ones(new, length):
         scale[p.table[i, 5], :], scale[p.table[i, 11], :] = 1e4, 1e3
     for n in (100, 300, 500):
         check_select(p, run_select(p, both, scale, n, 1, 1), both, scale, n, 1, 1)
+
+
+@pytest.mark.parametrize("kind", ["rising", "falling", "alike", "few"])
+def test_parts_whose_scores_rise_fall_or_tie(kind):
+    """Several parts of pages: every later one above the first's list, none, all the same,
+    and candidates only here and there."""
+    p = ref.Paged(87, 4, 2, 64, 1, [40], [6000], holes=[(0, j) for j in range(6000) if kind == "few" and j % 97])
+    both, scale = sel.random_bounds(88, 1, 2, 64)
+    both = np.repeat(both, p.pages, 0)
+    rank = np.empty(p.pages)
+    rank[p.table[0].numpy().clip(0, p.pages - 1)] = np.arange(6000)
+    slope = {"rising": 1 + rank / 100, "falling": 100 - rank / 100, "alike": 0 * rank + 1, "few": 1 + (rank * 7919 % 1000)}[kind]
+    scale = (scale * slope[:, None]).astype(np.float32)
+    for how in ((40, 1, 1), (100, 0, 0), (256, 2, 3)):
+        check_select(p, run_select(p, both, scale, *how), both, scale, *how)
 
 
 @pytest.mark.parametrize("new,page", [([1, 1], 16), ([30, 1, 9], 16), ([1], 1)])
