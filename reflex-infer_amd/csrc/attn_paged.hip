@@ -53,9 +53,12 @@ __device__ __forceinline__ float log2_scale(float vs) {
 // Waves per SIMD that the registers are cut to: what is in flight is what counts, and
 // an int8 step holds half the bytes of an fp16 one.  (With a list's page beside the entry,
 // small fp16 pages spill at four.)
-constexpr int rows_waves(int hd, bool i8, bool big, bool sel, bool tile) {
-    if (tile) return hd > 128 ? 1 : hd == 64 ? 4 : 3;
-    return hd > 128 ? 1 : hd == 64 ? (sel && !i8 && !big ? 3 : 4) : i8 ? 3 : 2;
+enum Lists { kNoLists, kTokenLists, kTileLists, kWideTileLists };  // (at the kernel)
+constexpr int rows_waves(int hd, bool i8, bool big, Lists lists) {
+    if (hd > 128) return 1;
+    if (lists == kWideTileLists) return hd == 64 ? 3 : 2;
+    if (lists == kTileLists) return hd == 64 ? 4 : 3;
+    return hd == 64 ? (lists == kTokenLists && !i8 && !big ? 3 : 4) : i8 ? 3 : 2;
 }
 
 // Steps of the walk over a sequence (0: not this kernel's; one where its tokens see
@@ -184,7 +187,11 @@ __device__ __forceinline__ RowsUnit selected_unit(const PagedParams &p, int &kvh
 __device__ __forceinline__ RowsUnit tile_unit(const PagedParams &p, int &kvh) {
     RowsUnit r{};
     r.s = -1;
-    const int idx = (int)(blockIdx.x % 8) * (gridDim.x / 8) + (int)(blockIdx.x / 8);
+    // the whole tiles first, as many on each XCD, then those at the sequences' starts (mostly none)
+    const int whole = (p.b.n_tokens + p.tile - 1) / p.tile, n = whole * p.c.n_kv, per = (n + 7) / 8;
+    const int x = blockIdx.x % 8, k = blockIdx.x / 8, starts = (gridDim.x / 8) - per;
+    const int idx = k < per ? x * per + k : n + x * starts + (k - per);
+    if (k < per && idx >= n) return r;
     kvh = idx % p.c.n_kv;
     const TileRows t = tile_rows(p.b, p.tile, idx / p.c.n_kv);
     if (t.n == 0) return r;
@@ -311,17 +318,20 @@ __device__ __forceinline__ int merge_lists(const PagedParams &p, const RowsUnit 
 // and one chunk of the places of its listed pages, page_size a list entry; all rows see the
 // same, so the masks are the entries'.  kTileLists: several tokens of a sequence, as many as 16
 // rows hold, and the pages that any of them lists, each read once (the lists of a prompt's
-// neighbours agree on most); a row's mask is its token's bit beside the page.
+// neighbours agree on most); a row's mask is its token's bit beside the page.  kWideTileLists:
+// of two blocks of 16 rows, which share K and V and what is done to them.
 // Bound: a token's reads of the cache, in the pieces above; a tile's pages come from the L2,
-// and LDS bounds it: K and V of a step in and out, 32 KB a wave.
+// and the chain of a step bounds it, of which 32 KB of K and V in and out of LDS are a
+// half; a wide one's step issues 270 vector instructions and 48 products for two waves a
+// SIMD, four fifths of its time.
 // Measured, head_dim 128: 64 tokens of 32 / 8 heads, 64 pages of 16 each, 51 us (5.3 TB/s; 256
 // pages each 190, 5.65), 16 in an int8 cache, 32 pages of 64, 17 + 4 for the combine; a chunk of
-// 512 tokens of 28 / 4 heads, 64 pages of 32, 88 us (a token a workgroup 150, with K by the
-// operand's rows 134).
-enum Lists { kNoLists, kTokenLists, kTileLists };
+// 512 tokens of 28 / 4 heads, 64 pages of 32, 78 us wide, 87 narrow (a token a workgroup 150,
+// with K by the operand's rows 134); of 1000 of 32 / 8, pages of 16, 99 and 117.
 template <int HD, bool I8, bool BIG, Lists LISTS>
-__global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, LISTS == kTileLists)) void attn_paged_rows_kernel(PagedParams p) {
-    constexpr bool SEL = LISTS == kTokenLists, TILE = LISTS == kTileLists;
+__global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS)) void attn_paged_rows_kernel(PagedParams p) {
+    constexpr bool SEL = LISTS == kTokenLists, TILE = LISTS == kTileLists || LISTS == kWideTileLists;
+    constexpr int RB = LISTS == kWideTileLists ? 2 : 1;  // rows, in blocks of 16
     // A chunk is 16 bytes: 8 dims of fp16, 16 of int8, which are two k steps of a
     // product (a lane's dims need only be the same in K and Q).
     constexpr int EC = I8 ? 16 : 8;                     // dims of a chunk
@@ -428,27 +438,38 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
     const int rows = SEL ? min(p.group - head0, kPagedRows) : (TILE ? unit.tokens : min(span.n, p.b.max_new)) * p.group;
     const int end_seq = TILE ? listed_pages << p.c.shift : SEL ? (limit > 0 ? p.n_select << p.c.shift : 0) : min(span.pos0 + (rows - 1) / p.group + 1, limit);
     const int end = min(end_seq, beg + unit.chunk);
-    const int row = min(r, rows - 1);  // (columns past the last row repeat it)
-    const int mine = SEL ? 0 : row / p.group;  // the row's token
-    const int tok = LISTS != kNoLists ? unit.tok + mine : mine, head = kvh * p.group + (SEL ? head0 + row : row % p.group);
-    const bool row_ok = r < rows;
     const int hd = p.c.hd, n_ch = hd / EC;
-    const int64_t orow = ((int64_t)(span.row0 + tok) * p.n_heads + head) * hd;
+    // of the lane's rows the token, its position and where the row's output is
+    int mine[RB], qpos[RB];
+    int64_t orow[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const int row = min(16 * b + r, rows - 1);  // (columns past the last row repeat it)
+        mine[b] = SEL ? 0 : row / p.group;
+        const int tok = LISTS != kNoLists ? unit.tok + mine[b] : mine[b];
+        const int head = kvh * p.group + (SEL ? head0 + row : row % p.group);
+        qpos[b] = span.pos0 + tok;
+        orow[b] = ((int64_t)(span.row0 + tok) * p.n_heads + head) * hd;
+    }
     if (end <= beg) {  // uniform
-        if (c == 0 && w == 0 && row_ok)  // the tokens see nothing
-            for (int ch = g; ch < hd / 8; ch += 4) *reinterpret_cast<u32x4 *>(p.out + orow + 8 * ch) = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+            if (c == 0 && w == 0 && 16 * b + r < rows)  // the tokens see nothing
+                for (int ch = g; ch < hd / 8; ch += 4)
+                    *reinterpret_cast<u32x4 *>(p.out + orow[b] + 8 * ch) = u32x4{0u, 0u, 0u, 0u};
         return;
     }
-    const int qpos = span.pos0 + tok;
     const int row_bytes = p.c.n_kv * hd * esz;
     const uint8_t *kb = p.c.k + (int64_t)kvh * hd * esz, *vb = p.c.v + (int64_t)kvh * hd * esz;
 
-    u32x4 qf[KS];
+    u32x4 qf[RB][KS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        const int ch = I8 ? 2 * (4 * (ks / 2) + g) + ks % 2 : 4 * ks + g;  // of 8 dims
-        qf[ks] = ch < hd / 8 ? load16(p.q + orow + 8 * ch) : u32x4{0u, 0u, 0u, 0u};
-    }
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int ch = I8 ? 2 * (4 * (ks / 2) + g) + ks % 2 : 4 * ks + g;  // of 8 dims
+            qf[b][ks] = ch < hd / 8 ? load16(p.q + orow[b] + 8 * ch) : u32x4{0u, 0u, 0u, 0u};
+        }
     // Byte offsets within a 16-row operand: K row r, dims 32 ks + 8 g; V row of the
     // lane's chunks.  Chunks past head_dim are past the operand's end (BIG), or the
     // last one again.
@@ -588,16 +609,21 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
         return u32x4{x.x, x.y, y.x, y.y};
     };
 
-    f32x4 o[DT];
+    f32x4 o[RB][DT];
+    float m[RB], l[RB];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;
+    for (int b = 0; b < RB; ++b) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[b][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m[b] = -INFINITY;
+        l[b] = 0.0f;
+    }
     bool bad = false;  // some V is not finite
     uint32_t most_vs = 0;  // int8: the lane's largest |V scale|
     auto process = [&](int j, Step &S, Rows &R, auto after_k, auto after_v) {
         if (SEL && S.seen == 0) return;  // uniform
         const int p0 = beg + kStep * j + 32 * w;
-        f32x4 acc[2];
+        f32x4 acc[RB][2];
         // (the wave's own reads of its V rows are ahead in its LDS queue, and these ahead of the next)
         constexpr int kPitch = HD * esz + 16;  // bytes of a K row
         uint8_t *const kl = reinterpret_cast<uint8_t *>(vl);
@@ -612,7 +638,8 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
         }
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-            acc[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int b = 0; b < RB; ++b) acc[b][st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             u32x4 kf[KL];
 #pragma unroll
             for (int i = 0; i < KL; ++i) {
@@ -625,7 +652,8 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
                 if constexpr (I8) k = ks % 2 ? widen(kf[ks / 2].z, kf[ks / 2].w) : widen(kf[ks / 2].x, kf[ks / 2].y);
                 else k = kf[ks];
                 if (!I8 && !BIG && 4 * ks + 4 > n_ch && 4 * ks + g >= n_ch) k = u32x4{0u, 0u, 0u, 0u};
-                acc[st] = mfma<RXQ4_DTYPE_F16>(k, qf[ks], acc[st]);
+#pragma unroll
+                for (int b = 0; b < RB; ++b) acc[b][st] = mfma<RXQ4_DTYPE_F16>(k, qf[b][ks], acc[b][st]);
             }
         }
         if constexpr (TILE) wave_lds_fence();
@@ -647,75 +675,80 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
             wave_lds_fence();
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-                acc[st] *= *reinterpret_cast<const f32x4 *>(&scl[w][0][16 * st + 4 * g]);
+                const f32x4 kx = *reinterpret_cast<const f32x4 *>(&scl[w][0][16 * st + 4 * g]);
+#pragma unroll
+                for (int b = 0; b < RB; ++b) acc[b][st] *= kx;
                 vx[st] = *reinterpret_cast<const f32x4 *>(&scl[w][1][16 * st + 4 * g]);
                 lg[st] = *reinterpret_cast<const f32x4 *>(&scl[w][2][16 * st + 4 * g]);
             }
             wave_lds_fence();
         }
         const bool part = S.seen != ~0u;
-        float sv[8], mx = -INFINITY;
+        uint32_t ph[RB][4], pl[RB][4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sv[i] = acc[i >> 2][i & 3] * p.sl2;
-        if constexpr (TILE && !BIG) {
-            if (!S.all[0]) {  // uniform
-                if (lane < 32) tokens_of[w][lane] = S.of[0];
-                wave_lds_fence();
+        for (int b = 0; b < RB; ++b) {
+            float sv[8], mx = -INFINITY;
 #pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    const i32x4 of = *reinterpret_cast<const i32x4 *>(&tokens_of[w][16 * st + 4 * g]);
+            for (int i = 0; i < 8; ++i) sv[i] = acc[b][i >> 2][i & 3] * p.sl2;
+            if constexpr (TILE && !BIG) {
+                if (!S.all[0]) {  // uniform
+                    if (b == 0 && lane < 32) tokens_of[w][lane] = S.of[0];
+                    wave_lds_fence();
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!(of[i] >> mine & 1)) sv[4 * st + i] = -INFINITY;
+                    for (int st = 0; st < 2; ++st) {
+                        const i32x4 of = *reinterpret_cast<const i32x4 *>(&tokens_of[w][16 * st + 4 * g]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (!(of[i] >> mine[b] & 1)) sv[4 * st + i] = -INFINITY;
+                    }
+                    wave_lds_fence();
                 }
-                wave_lds_fence();
+            } else if constexpr (TILE) {
+#pragma unroll
+                for (int st = 0; st < 2; ++st)
+                    if (!S.all[st]) {  // uniform
+                        // places of the operand that the row's token lists and sees
+                        const int first = ((S.of[st] & 0xFFFFFF) << p.c.shift) + ((p0 + 16 * st) & ((1 << p.c.shift) - 1));
+                        const int n = S.of[st] >> (24 + mine[b]) & 1 ? min(limit, qpos[b] + 1) - first : 0;
+                        const int here = (S.seen >> (16 * st) & 0xFFFFu) != 0 ? n : 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (4 * g + i >= here) sv[4 * st + i] = -INFINITY;
+                    }
+            } else if (part || (!SEL && p0 + 31 > span.pos0)) {  // uniform: not every row sees all of them
+                const uint32_t in = S.seen >> (4 * g);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (!((in >> (16 * (i >> 2) + (i & 3))) & 1u) || (!SEL && p0 + 16 * (i >> 2) + 4 * g + (i & 3) > qpos[b]))
+                        sv[i] = -INFINITY;
             }
-        } else if constexpr (TILE) {
 #pragma unroll
-            for (int st = 0; st < 2; ++st)
-                if (!S.all[st]) {  // uniform
-                    // places of the operand that the row's token lists and sees
-                    const int first = ((S.of[st] & 0xFFFFFF) << p.c.shift) + ((p0 + 16 * st) & ((1 << p.c.shift) - 1));
-                    const int n = S.of[st] >> (24 + mine) & 1 ? min(limit, qpos + 1) - first : 0;
-                    const int here = (S.seen >> (16 * st) & 0xFFFFu) != 0 ? n : 0;
+            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, I8 ? sv[i] + lg[i >> 2][i & 3] : sv[i]);
+            mx = max_xor_rows<16>(mx);
+            mx = max_xor_rows<32>(mx);
+            if (__builtin_amdgcn_ballot_w64(mx > m[b] + kLazy) != 0) {
+                // (each row's by its own rule: no row depends on what others see)
+                const float m_new = mx > m[b] + kLazy ? mx : m[b];
+                const float corr = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[b] - m_new);
+                m[b] = m_new;
+                l[b] *= corr;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (4 * g + i >= here) sv[4 * st + i] = -INFINITY;
+                for (int dt = 0; dt < DT; ++dt) o[b][dt] *= corr;
+            }
+            const float m_use = m[b] == -INFINITY ? 0.0f : m[b] - kShift;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                float e0 = __builtin_amdgcn_exp2f(sv[i] - m_use), e1 = __builtin_amdgcn_exp2f(sv[i + 1] - m_use);
+                l[b] += e0;
+                l[b] += e1;
+                if constexpr (I8) {
+                    // (a position that the row does not see stays 0 whatever its scale)
+                    e0 = sv[i] == -INFINITY ? 0.0f : e0 * vx[i >> 2][i & 3];
+                    e1 = sv[i + 1] == -INFINITY ? 0.0f : e1 * vx[i >> 2][(i & 3) + 1];
                 }
-        } else if (part || (!SEL && p0 + 31 > span.pos0)) {  // uniform: not every row sees all of them
-            const uint32_t in = S.seen >> (4 * g);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (!((in >> (16 * (i >> 2) + (i & 3))) & 1u) || (!SEL && p0 + 16 * (i >> 2) + 4 * g + (i & 3) > qpos))
-                    sv[i] = -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, I8 ? sv[i] + lg[i >> 2][i & 3] : sv[i]);
-        mx = max_xor_rows<16>(mx);
-        mx = max_xor_rows<32>(mx);
-        if (__builtin_amdgcn_ballot_w64(mx > m + kLazy) != 0) {
-            // (each row's by its own rule: no row depends on what others see)
-            const float m_new = mx > m + kLazy ? mx : m;
-            const float corr = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
-            m = m_new;
-            l *= corr;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o[dt] *= corr;
-        }
-        const float m_use = m == -INFINITY ? 0.0f : m - kShift;
-        uint32_t ph[4], pl[4];
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            float e0 = __builtin_amdgcn_exp2f(sv[i] - m_use), e1 = __builtin_amdgcn_exp2f(sv[i + 1] - m_use);
-            l += e0;
-            l += e1;
-            if constexpr (I8) {
-                // (a position that the row does not see stays 0 whatever its scale)
-                e0 = sv[i] == -INFINITY ? 0.0f : e0 * vx[i >> 2][i & 3];
-                e1 = sv[i + 1] == -INFINITY ? 0.0f : e1 * vx[i >> 2][(i & 3) + 1];
+                ph[b][i >> 1] = pack2<RXQ4_DTYPE_F16>(e0, e1);
+                pl[b][i >> 1] = low_halves(e0, e1, ph[b][i >> 1]);
             }
-            ph[i >> 1] = pack2<RXQ4_DTYPE_F16>(e0, e1);
-            pl[i >> 1] = low_halves(e0, e1, ph[i >> 1]);
         }
         // Rows that are not there: zeros.  An infinity or NaN in V would reach the rows
         // that do not see it as 0 times it, and the others through the low half of P: such
@@ -757,8 +790,11 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
                 u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                            (__attribute__((address_space(3))) v4i16 *)(vp + 16 * VROW)));
             const u32x4 a = u32x4{v0.x, v0.y, v1.x, v1.y};
-            o[dt] = mfma<RXQ4_DTYPE_F16>(a, u32x4{ph[0], ph[1], ph[2], ph[3]}, o[dt]);
-            o[dt] = mfma<RXQ4_DTYPE_F16>(a, u32x4{pl[0], pl[1], pl[2], pl[3]}, o[dt]);
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                o[b][dt] = mfma<RXQ4_DTYPE_F16>(a, u32x4{ph[b][0], ph[b][1], ph[b][2], ph[b][3]}, o[b][dt]);
+                o[b][dt] = mfma<RXQ4_DTYPE_F16>(a, u32x4{pl[b][0], pl[b][1], pl[b][2], pl[b][3]}, o[b][dt]);
+            }
             if (TILE && dt % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // (all reads at once: 32 registers)
         }
     };
@@ -814,91 +850,93 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS == kTokenLists, 
         }
     }
     if constexpr (I8 && !BIG) bad = __builtin_amdgcn_ballot_w64(most_vs >= 0x7F800000u) != 0;
-    l = sum_xor_rows<16>(l);
-    l = sum_xor_rows<32>(l);
-
     // Merge: lane l of every wave holds row r, dims 16 dt + 4 g + i; wave w merges
     // the dims of tiles dt = w, w + 4, ...
     float (*const mg)[NM][64] = reinterpret_cast<float (*)[NM][64]>(smem);
-    __syncthreads();  // the V rows are read
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int b = 0; b < RB; ++b) {
+        __syncthreads();  // the V rows (the block before) are read
+        l[b] = sum_xor_rows<16>(l[b]);
+        l[b] = sum_xor_rows<32>(l[b]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mg[w][4 * dt + i][lane] = o[dt][i];
-    mg[w][NM - 2][lane] = m;
-    mg[w][NM - 1][lane] = l;
-    if (bad) {  // uniform, rare: the wave's positions again (onto its part in LDS: no registers held for it)
-        for (int pos = beg; pos < end; ++pos) {
-            if (((pos - beg) / 32 & 3) != w || (LISTS == kNoLists && pos > qpos)) continue;
-            int slot;
-            if constexpr (TILE) {
-                const int k = pos >> p.c.shift, in = pos & ((1 << p.c.shift) - 1), of = work[p.tile * p.n_select + k];
-                const bool sees_it = of >> (24 + mine) & 1 && ((of & 0xFFFFFF) << p.c.shift) + in < min(limit, qpos + 1);
-                slot = sees_it ? (work[k] << p.c.shift) + in : -1;
-            } else if constexpr (SEL) {
-                const int x = listed(pos);
-                slot = x >= 0 && seen_from(x, pos) > 0 ? slot_of(p.c, s, (x << p.c.shift) + (pos & ((1 << p.c.shift) - 1))) : -1;
-            } else {
-                slot = slot_of(p.c, s, pos);
-            }
-            if (slot < 0) continue;
-            const uint8_t *v = vb + slot_bytes(p.c, slot, row_bytes);
-            const float vs = I8 ? vsp[(int64_t)slot * v_stride] : 1.0f;
-            if (I8 && fabsf(vs) < INFINITY) continue;
-            for (int dt = 0; dt < DT; ++dt) {
-                const int d = 16 * dt + 4 * g;
-                if (d >= hd) continue;
-                const u32x2 x = I8 ? u32x2{*reinterpret_cast<const uint32_t *>(v + d), 0u}
-                                   : *reinterpret_cast<const u32x2 *>(v + 2 * d);
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float y = I8 ? vs * (float)(int8_t)(x.x >> (8 * i))
-                                       : f16_bits_to_f32((i < 2 ? x.x : x.y) >> (16 * (i & 1)) & 0xFFFFu);
-                    if (!(fabsf(y) < INFINITY)) mg[w][4 * dt + i][lane] += y;
+            for (int i = 0; i < 4; ++i) mg[w][4 * dt + i][lane] = o[b][dt][i];
+        mg[w][NM - 2][lane] = m[b];
+        mg[w][NM - 1][lane] = l[b];
+        if (bad) {  // uniform, rare: the wave's positions again (onto its part in LDS: no registers held for it)
+            for (int pos = beg; pos < end; ++pos) {
+                if (((pos - beg) / 32 & 3) != w || (LISTS == kNoLists && pos > qpos[b])) continue;
+                int slot;
+                if constexpr (TILE) {
+                    const int k = pos >> p.c.shift, in = pos & ((1 << p.c.shift) - 1), of = work[p.tile * p.n_select + k];
+                    const bool sees_it = of >> (24 + mine[b]) & 1 && ((of & 0xFFFFFF) << p.c.shift) + in < min(limit, qpos[b] + 1);
+                    slot = sees_it ? (work[k] << p.c.shift) + in : -1;
+                } else if constexpr (SEL) {
+                    const int x = listed(pos);
+                    slot = x >= 0 && seen_from(x, pos) > 0 ? slot_of(p.c, s, (x << p.c.shift) + (pos & ((1 << p.c.shift) - 1))) : -1;
+                } else {
+                    slot = slot_of(p.c, s, pos);
+                }
+                if (slot < 0) continue;
+                const uint8_t *v = vb + slot_bytes(p.c, slot, row_bytes);
+                const float vs = I8 ? vsp[(int64_t)slot * v_stride] : 1.0f;
+                if (I8 && fabsf(vs) < INFINITY) continue;
+                for (int dt = 0; dt < DT; ++dt) {
+                    const int d = 16 * dt + 4 * g;
+                    if (d >= hd) continue;
+                    const u32x2 x = I8 ? u32x2{*reinterpret_cast<const uint32_t *>(v + d), 0u}
+                                       : *reinterpret_cast<const u32x2 *>(v + 2 * d);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float y = I8 ? vs * (float)(int8_t)(x.x >> (8 * i))
+                                           : f16_bits_to_f32((i < 2 ? x.x : x.y) >> (16 * (i & 1)) & 0xFFFFu);
+                        if (!(fabsf(y) < INFINITY)) mg[w][4 * dt + i][lane] += y;
+                    }
                 }
             }
         }
-    }
-    __syncthreads();
-    float mw[4], M = -INFINITY;
+        __syncthreads();
+        float mw[4], M = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        mw[v] = mg[v][NM - 2][lane];
-        M = fmaxf(M, mw[v]);
-    }
-    float cw[4], L = 0.0f;
+        for (int v = 0; v < 4; ++v) {
+            mw[v] = mg[v][NM - 2][lane];
+            M = fmaxf(M, mw[v]);
+        }
+        float cw[4], L = 0.0f;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        cw[v] = M != -INFINITY ? __builtin_amdgcn_exp2f(mw[v] - M) : 0.0f;
-        L += mg[v][NM - 1][lane] * cw[v];
-    }
-    if (!row_ok) return;
-    const bool whole = unit.chunks <= 1;  // one chunk: no partials
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    const int64_t at = (unit.slot * p.c.n_kv + kvh) * p.rows_blk + r;
+        for (int v = 0; v < 4; ++v) {
+            cw[v] = M != -INFINITY ? __builtin_amdgcn_exp2f(mw[v] - M) : 0.0f;
+            L += mg[v][NM - 1][lane] * cw[v];
+        }
+        if (16 * b + r >= rows) continue;
+        const bool whole = unit.chunks <= 1;  // one chunk: no partials
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        const int64_t at = (unit.slot * p.c.n_kv + kvh) * p.rows_blk + r;
 #pragma unroll
-    for (int dt = w; dt < DT; dt += 4) {
-        f32x4 ov{};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) ov[i] = __builtin_fmaf(cw[v], mg[v][4 * dt + i][lane], ov[i]);
-        if (!(fabsf(ov[0]) + fabsf(ov[1]) + fabsf(ov[2]) + fabsf(ov[3]) < INFINITY)) {  // rare: the same sums
-            ov = f32x4{};
+        for (int dt = w; dt < DT; dt += 4) {
+            f32x4 ov{};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int v = 0; v < 4; ++v) ov[i] = add_weighed(ov[i], cw[v], mg[v][4 * dt + i][lane]);
+                for (int v = 0; v < 4; ++v) ov[i] = __builtin_fmaf(cw[v], mg[v][4 * dt + i][lane], ov[i]);
+            if (!(fabsf(ov[0]) + fabsf(ov[1]) + fabsf(ov[2]) + fabsf(ov[3]) < INFINITY)) {  // rare: the same sums
+                ov = f32x4{};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) ov[i] = add_weighed(ov[i], cw[v], mg[v][4 * dt + i][lane]);
+            }
+            const int d = 16 * dt + 4 * g;
+            if (!whole) *reinterpret_cast<f32x4 *>(p.part + at * HD + d) = ov;
+            else if (d < hd)
+                *reinterpret_cast<u32x2 *>(p.out + orow[b] + d) = u32x2{pack2<RXQ4_DTYPE_F16>(ov[0] * inv, ov[1] * inv),
+                                                                     pack2<RXQ4_DTYPE_F16>(ov[2] * inv, ov[3] * inv)};
         }
-        const int d = 16 * dt + 4 * g;
-        if (!whole) *reinterpret_cast<f32x4 *>(p.part + at * HD + d) = ov;
-        else if (d < hd)
-            *reinterpret_cast<u32x2 *>(p.out + orow + d) = u32x2{pack2<RXQ4_DTYPE_F16>(ov[0] * inv, ov[1] * inv),
-                                                                 pack2<RXQ4_DTYPE_F16>(ov[2] * inv, ov[3] * inv)};
-    }
-    if (!whole && w == 0 && g == 0) {
-        p.stats[2 * at] = M;
-        p.stats[2 * at + 1] = L;
+        if (!whole && w == 0 && g == 0) {
+            p.stats[2 * at] = M;
+            p.stats[2 * at + 1] = L;
+        }
     }
 }
 
@@ -1045,14 +1083,24 @@ SelectedPlan plan_selected(PagedParams &p, int i8) {
     p.rows_blk = std::min(p.group, kPagedRows);
     p.head_blocks = (p.group + kPagedRows - 1) / kPagedRows;
     // Tiles where the sequences have tokens to fill them and the tiles are enough for the CUs.
-    p.tile = (int)std::min<int64_t>({(int64_t)kPagedRows / p.group, 8, kListEntries / p.n_select});
-    if (p.tile > 1 && p.b.max_new > 1 && p.b.n_tokens >= 4 * (int64_t)p.b.n_seqs) {
-        const int64_t tiles = ((p.b.n_tokens + p.tile - 1) / p.tile + p.b.n_seqs) * (int64_t)p.c.n_kv;
-        if (tiles >= cus) {
+    // Wide ones where the last of them leave few CUs idle (at 28 / 4 heads, the chip takes those of
+    // 512 tokens at a time: 384 / 448 / 600 / 900 tokens wide 74 / 76 / 115 / 137 us, narrow 67 / 86
+    // / 99 / 157).
+    if (p.b.max_new > 1 && p.b.n_tokens >= 4 * (int64_t)p.b.n_seqs)
+        for (int blocks = pad <= 128 ? 2 : 1; blocks > 0; --blocks) {
+            p.tile = (int)std::min<int64_t>({(int64_t)blocks * kPagedRows / p.group, 8, kListEntries / p.n_select});
+            if (p.tile <= 1 || (blocks == 2 && p.tile * p.group <= kPagedRows)) continue;
+            const int64_t whole = (int64_t)((p.b.n_tokens + p.tile - 1) / p.tile) * p.c.n_kv, starts = (int64_t)p.b.n_seqs * p.c.n_kv;
+            if (blocks == 2) {
+                const int64_t live = whole + starts - p.c.n_kv;  // (the first sequence starts a whole one)
+                const int64_t slots = (int64_t)rows_waves(pad, i8, p.c.shift >= 4, kWideTileLists) * cus;
+                if (4 * live <= 3 * slots * ((live + slots - 1) / slots)) continue;
+            } else if (whole + starts < cus) {
+                continue;
+            }
             p.n_chunks = 1;
-            return SelectedPlan{(tiles + 7) / 8 * 8, 0};
+            return SelectedPlan{(whole + 7) / 8 * 8 + (starts + 7) / 8 * 8, 0};
         }
-    }
     p.tile = 1;
     const int64_t units = (int64_t)p.b.n_tokens * p.c.n_kv * p.head_blocks;
     const int64_t per = units * p.rows_blk * (pad + 2) * 4;  // bytes of one chunk of every unit
@@ -1075,10 +1123,19 @@ hipError_t launch_selected(PagedParams &p, const SelectedPlan &plan, float *ws, 
     const bool big = p.c.shift >= 4;
     if (p.tile > 1) {
         const size_t lds = (size_t)2 * p.tile * p.n_select * 4;
-        if (i8 && big) attn_paged_rows_kernel<HD, true, true, kTileLists><<<grid, 256, lds, st>>>(p);
-        else if (i8) attn_paged_rows_kernel<HD, true, false, kTileLists><<<grid, 256, lds, st>>>(p);
-        else if (big) attn_paged_rows_kernel<HD, false, true, kTileLists><<<grid, 256, lds, st>>>(p);
-        else attn_paged_rows_kernel<HD, false, false, kTileLists><<<grid, 256, lds, st>>>(p);
+        const auto launch = [&](auto i8_, auto big_) {
+            constexpr bool I8 = decltype(i8_)::value, BIG = decltype(big_)::value;
+            if constexpr (HD <= 128)
+                if (p.tile * p.group > kPagedRows) {
+                    attn_paged_rows_kernel<HD, I8, BIG, kWideTileLists><<<grid, 256, lds, st>>>(p);
+                    return;
+                }
+            attn_paged_rows_kernel<HD, I8, BIG, kTileLists><<<grid, 256, lds, st>>>(p);
+        };
+        if (i8 && big) launch(std::true_type{}, std::true_type{});
+        else if (i8) launch(std::true_type{}, std::false_type{});
+        else if (big) launch(std::false_type{}, std::true_type{});
+        else launch(std::false_type{}, std::false_type{});
         return hipGetLastError();
     }
     if (i8 && big) attn_paged_rows_kernel<HD, true, true, kTokenLists><<<grid, 256, 0, st>>>(p);

@@ -431,6 +431,126 @@ def test_tiles_keep_what_one_token_looks_at_from_the_others(bad, page, int8):
     assert torch.equal(got[41][keep], clean[41][keep])
 
 
+# heads, page, int8, new, lens, n_select: 17 to 32 rows a tile, tiles for the whole chip
+WIDE_TILES = [
+    ((96, 32, 16), 16, False, [150, 7, 3], [300, 200, 3], 6),    # of 3 heads: eight tokens
+    ((64, 16, 128), 16, False, [210, 20, 2], [600, 33, 90], 12), # of 4: eight
+    ((80, 16, 64), 64, True, [240], [700], 4),                   # of 5: six
+    ((112, 16, 128), 32, False, [110, 7], [500, 64], 7),         # of 7: four
+    ((64, 8, 96), 128, False, [220], [700], 3),                  # of 8: four
+    ((72, 8, 64), 16, True, [230], [400], 9),                    # of 9: three
+    ((128, 8, 128), 16, True, [110, 3], [300, 3], 9),            # of 16: two
+    ((32, 8, 128), 16, False, [415], [420], 256),                # lists of all that a tile holds
+    ((64, 16, 128), 8, False, [210, 20, 2], [400, 33, 90], 24),  # pages of fewer positions than an operand
+    ((64, 16, 128), 1, True, [220], [300], 90),
+    ((48, 16, 80), 8, True, [220], [300], 15),
+    ((56, 8, 96), 4, False, [220], [300], 30),
+    ((64, 16, 64), 2, False, [370], [400], 21),
+]
+
+
+@pytest.mark.parametrize("order", ["ascending", "any"])
+@pytest.mark.parametrize("heads,page,int8,new,lens,n_select", WIDE_TILES)
+def test_attention_of_wide_tiles(heads, page, int8, new, lens, n_select, order):
+    print(f"wide tiles {heads} page={page} int8={int8} new={new} lens={lens} n_select={n_select} {order}", flush=True)
+    p = ref.Paged(129, *heads, page, new, lens, int8, pad=3, lead=2, apart=page == 32)
+    lists = sel.random_lists(p, n_select, 130, odd=order == "any")
+    scale = heads[2] ** -0.5
+    check_attend(p, run_attend(p, lists, scale), lists, scale)
+
+
+@pytest.mark.parametrize("page", [4, 16])
+def test_wide_tiles_whose_lists_agree_differ_and_are_empty(page):
+    p = ref.Paged(131, 64, 16, 64, page, [330], [700], holes=[(0, 3), (0, 9)])
+    lists = np.full((p.rows, 16, 8), -1, np.int32)
+    for t in range(330):
+        last = (370 + t) // page
+        lists[t, :, :4] = [0, 3, 7, last] if t < 130 else [t % 4, 4 + t % 4, 9, 10 + t % 4]
+        if t % 11 == 5 or 200 <= t < 216:
+            lists[t] = -1
+        if t % 11 == 6:
+            lists[t] = [3, 9] + [-1] * 6
+        if t % 11 == 7:
+            lists[t] = [last + 1, last + 2] + [-1] * 6
+    got = run_attend(p, lists, 0.125)
+    check_attend(p, got, lists, 0.125)
+    assert not got[5].any() and not got[6].any() and not got[7].any() and not got[200:216].any()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("page,int8", [(16, False), (8, False), (16, True), (4, True)])
+def test_wide_tiles_keep_what_one_token_looks_at_from_the_others(bad, page, int8):
+    p = ref.Paged(132, 64, 16, 64, page, [330], [700], int8)
+    lists = np.full((p.rows, 16, 3), -1, np.int32)
+    for t in range(330):
+        lists[t, :, 0], lists[t, :, 1] = 0, (370 + t) // page
+    looks = [41, 46]  # of one tile's rows the first and the second half
+    for t in looks:
+        lists[t, :] = [0, 2, (370 + t) // page]
+    clean = run_attend(p, lists, 0.125).cpu()
+    check_attend(p, clean, lists, 0.125)
+    slots = p.slots(0, 700)
+    at = slots[2 * page + 1]
+    if int8:
+        p.vs.view(-1, 16)[at, 3], p.ks.view(-1, 16)[at, 5] = bad, bad
+        p.vs.view(-1, 16)[slots[699], 3] = bad
+    else:
+        p.both[1].view(-1, 16, 64)[at, 3, 7], p.both[0].view(-1, 16, 64)[at, 5, 7] = bad, bad
+        p.both[1].view(-1, 16, 64)[slots[699], 3, 7] = bad
+    got = run_attend(p, lists, 0.125).cpu()
+    rest = [t for t in range(329) if t not in looks]
+    assert torch.equal(got[rest], clean[rest])
+    keep = torch.ones(64, dtype=torch.bool)
+    keep[12:16] = False
+    assert torch.equal(got[329][keep], clean[329][keep])
+    keep[20:24] = False
+    for t in looks + [329]:
+        assert not torch.isfinite(got[t, 12:16]).all()
+        assert torch.equal(got[t][keep], clean[t][keep])
+
+
+@pytest.mark.parametrize("starts", [[0, 5, 3], [-4, 2, 9], [0, 100000, 100001], [70, 2, 1], [2 ** 31 - 1] * 3, [-2 ** 31] * 3])
+@pytest.mark.parametrize("lens", [[64, 64], [2 ** 31 - 1, -2 ** 31]])
+@pytest.mark.parametrize("page", [4, 16])
+def test_wide_tiles_with_starts_and_lengths_outside_their_limits_stay_inside(starts, lens, page):
+    p = ref.Paged(133, 256, 64, 16, page, [36, 36], [64, 64])
+    cache, batch = p.device(capi)
+    batch.tensors[0].copy_(torch.tensor(starts, dtype=torch.int32))
+    batch.tensors[1].copy_(torch.tensor(lens, dtype=torch.int32))
+    lists = torch.from_numpy(np.random.default_rng(134).integers(-2, 70 // page, (p.rows, 64, 6)).astype(np.int32)).cuda()
+    out = torch.full((p.rows + 20, 256, 16), 7.0, dtype=torch.float16, device="cuda")
+    capi.attention_selected_f16(out[10:-10], p.q.cuda(), lists, batch, cache, 0.25)
+    assert (out[:10] == 7.0).all() and (out[-10:] == 7.0).all() and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("page,int8", [(16, False), (4, True)])
+def test_wide_tiles_of_many_sequences_replayed_and_in_place(page, int8):
+    new = [(i * 7) % 30 if i % 9 else 0 for i in range(28)]
+    lens = [0 if i % 17 == 3 else 3 + (i * 29) % 220 for i in range(28)]
+    p = ref.Paged(135, 64, 16, 64, page, new, lens, int8)
+    cache, batch = p.device(capi, max_len=300)
+    q = p.q.cuda()
+    lists = sel.random_lists(p, 9, 136)
+    ours, out = torch.from_numpy(lists).cuda(), torch.empty_like(q)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        capi.attention_selected_f16(out, q, ours, batch, cache, 0.125, stream=s)
+    eager = run_attend(p, ours, 0.125, cache, batch)
+    check_attend(p, eager, lists, 0.125)
+    mine = (eager != 7.0).flatten(1).any(1)
+    for _ in range(3):
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+    capi.attention_selected_f16(q, q, ours, batch, cache, 0.125)
+    assert torch.equal(q[mine], eager[mine])
+
+
 def check_all(p, how, scale=0.125, seed=120, **limits):
     """The choice against bounds of its own, and attention over its lists."""
     both, by = sel.random_bounds(seed, p.pages, p.kv, p.hd)
