@@ -1083,9 +1083,9 @@ SelectedPlan plan_selected(PagedParams &p, int i8) {
     p.rows_blk = std::min(p.group, kPagedRows);
     p.head_blocks = (p.group + kPagedRows - 1) / kPagedRows;
     // Tiles where the sequences have tokens to fill them and the tiles are enough for the CUs.
-    // Wide ones where the last of them leave few CUs idle (at 28 / 4 heads, the chip takes those of
-    // 512 tokens at a time: 384 / 448 / 600 / 900 tokens wide 74 / 76 / 115 / 137 us, narrow 67 / 86
-    // / 99 / 157).
+    // Wide ones where they fill more than three quarters of the rounds that they take (at 28 / 4
+    // heads a round is 512 tokens: 384 / 448 / 600 / 900 tokens wide 74 / 76 / 115 / 137 us, narrow
+    // 67 / 86 / 99 / 157).
     if (p.b.max_new > 1 && p.b.n_tokens >= 4 * (int64_t)p.b.n_seqs)
         for (int blocks = pad <= 128 ? 2 : 1; blocks > 0; --blocks) {
             p.tile = (int)std::min<int64_t>({(int64_t)blocks * kPagedRows / p.group, 8, kListEntries / p.n_select});
