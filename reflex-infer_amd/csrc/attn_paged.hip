@@ -940,6 +940,18 @@ __global__ __launch_bounds__(256, rows_waves(HD, I8, BIG, LISTS)) void attn_page
     }
 }
 
+// sum + w x of a row's chunk c.  The rounding is written out, as part of the results (left to
+// the compiler, which of the sums it fuses changes with the code around them): fused; up to
+// head_dim 64 product and sum are rounded each from the third chunk on.
+template <int HD>
+__device__ __forceinline__ float add_chunk(float sum, float w, float x, int c) {
+    if (HD > 64 || c < 2) return __builtin_fmaf(w, x, sum);
+    {
+#pragma clang fp contract(off)
+        return sum + w * x;
+    }
+}
+
 // out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over a row's n_c chunks in order,
 // partials `at` and every `step` behind.  A wave takes a row: a lane's chunk for the
 // weights, then a lane's dims.
@@ -968,7 +980,9 @@ __device__ __forceinline__ void combine_row(const PagedParams &p, int64_t at, in
             const float ec = __builtin_bit_cast(
                 float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, e), min(c0 + i, 63)));
             if (c0 + i >= n_c) continue;  // uniform
-            if (ec != 0.0f) acc += ec * x[i];
+            if (ec != 0.0f)
+#pragma unroll
+                for (int k = 0; k < VE; ++k) acc[k] = add_chunk<HD>(acc[k], ec, x[i][k], c0 + i);
             else
 #pragma unroll
                 for (int k = 0; k < VE; ++k) acc[k] = add_weighed(acc[k], 0.0f, x[i][k]);
