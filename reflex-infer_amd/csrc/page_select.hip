@@ -350,7 +350,7 @@ __device__ __forceinline__ void score_pages(const SelectParams &p, const Tile &t
     struct Operand {
         u32x4 b[NL];
     };
-    // a hole's row is the pool's first; its scale, -1, makes it no candidate
+    // a hole's row is the pool's first
     const auto in_pool = [&](int e) { return (unsigned)e < (unsigned)p.c.n_pages ? e : 0; };
     const auto load_scale = [&](int e) { return scales[(uint64_t)(uint32_t)in_pool(e) * (uint32_t)p.c.n_kv]; };
     const auto load = [&](int e, int o, Operand &S) {  // operand o of the 64 entries
@@ -399,7 +399,8 @@ __device__ __forceinline__ void score_pages(const SelectParams &p, const Tile &t
         for (; j < j1; j += step) {
             const float scale1 = load_scale(ent1);
             const int ent2 = entry(j + 2 * step + lane);
-            const float mine = (unsigned)ent < (unsigned)p.c.n_pages ? scale : -1.0f;
+            // -1: a hole, NaN: a page that is not chosen for its score
+            const float mine = (unsigned)ent < (unsigned)p.c.n_pages ? (scale >= 0.0f ? scale : __builtin_nanf("")) : -1.0f;
             float x[4][QT][PER];
 #pragma unroll
             for (int o = 0; o < 4; ++o) {
@@ -452,8 +453,9 @@ __device__ __forceinline__ void score_pages(const SelectParams &p, const Tile &t
 #pragma unroll
                         for (int d = 1; d < DUP; ++d) y = g % DUP == d ? x[k * DUP + d][t][i] : y;
                         const int n = sees[t][i];
-                        uint32_t key = ((page < p.n_first) | (page >= n - p.n_last)) ? kAlways : key_of(y * s);
-                        key = (!(s >= 0.0f) | (page >= n)) ? 0u : key;
+                        const bool always = (page < p.n_first) | (page >= n - p.n_last);
+                        uint32_t key = always ? kAlways : key_of(y * s);
+                        key = ((s < 0.0f) | (page >= n) | (!always & !(s >= 0.0f))) ? 0u : key;
                         if (n >= 0 && page < j1) {
                             if (GP == 16 && h0 > 0) key = max(key, dst[t][i][page]);  // (of the heads before, the same lane's)
                             dst[t][i][page] = key;
