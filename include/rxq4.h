@@ -348,7 +348,7 @@ int rxq4_kv_bounds(void *bounds, float *scales, const rxq4_seq_batch *batch,
  *            steps no key of the page has a larger product with the query.  The sum is
  *            exact, so the lists do not depend on how the work is cut
  * Bounds and scales are rxq4_kv_bounds' (a page whose scale is negative or NaN is not
- * chosen for its score).  Tokens that see nothing get -1s.  Rows of no sequence, and of
+ * chosen for its score; an infinite one times a sum of 0 is 0).  Tokens that see nothing get -1s.  Rows of no sequence, and of
  * tokens past max_new, are left as they are.  A few tokens with many pages use the
  * stream's workspace described above. */
 int rxq4_select_pages(int32_t *pages, int n_select, int n_first, int n_last, const void *q,

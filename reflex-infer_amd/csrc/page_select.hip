@@ -182,10 +182,11 @@ struct SelectParams {
     int parts;       // split: workgroups of a token and KV head
 };
 
-// Bits that order as the numbers do, above 0; -0 as 0.
+// Bits that order as the numbers do, above 0; -0 as 0, and NaN, which of a score is an infinite
+// scale times 0.
 __device__ __forceinline__ uint32_t key_of(float x) {
     // (not by adding 0: that becomes one rounding with the product before it, which is -0 yet)
-    const uint32_t u = x == 0.0f ? 0u : __builtin_bit_cast(uint32_t, x);
+    const uint32_t u = __builtin_islessgreater(x, 0.0f) ? __builtin_bit_cast(uint32_t, x) : 0u;
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 

@@ -1,6 +1,7 @@
-"""The choice of pages (rxq4_select_pages) where scales of bounds are no scales: negative
-ones and NaN, as arrays that were never written hold them.  The first and the last pages are
-chosen all the same; others are not."""
+"""The choice of pages (rxq4_select_pages) where scales of bounds are no scales: negative,
+NaN and infinite ones, as arrays that were never written hold them.  The first and the last
+pages are chosen all the same; others of a negative or NaN scale are not; an infinite one
+makes scores infinite, and 0 of 0."""
 from __future__ import annotations
 
 import numpy as np
@@ -31,7 +32,7 @@ def expected(p, both, scale, n_select, n_first, n_last):
             for h in range(p.kv):
                 x = scale[safe, h]
                 with np.errstate(all="ignore"):
-                    s = y[h] * x
+                    s = np.where((y[h] == 0) & np.isinf(x), np.float32(0), y[h] * x)
                     mine = there & ~always & (x >= 0)
                 best = j[mine][np.lexsort((j[mine], -s[mine]))]
                 order = np.concatenate((j[always], best))[:n_select]
@@ -41,7 +42,7 @@ def expected(p, both, scale, n_select, n_first, n_last):
 
 def spoil(scale, both, rng):
     kind = rng.integers(0, 12, scale.shape)
-    for i, x in enumerate((np.nan, -np.nan, -1.0, -1e-45, -np.inf, -0.0)):
+    for i, x in enumerate((np.nan, -np.nan, -1.0, -1e-45, -np.inf, np.inf, -0.0)):
         scale[kind == i] = x
     both[rng.random(scale.shape[0]) < 0.15] = 0  # sums of 0
 
