@@ -198,7 +198,8 @@ __device__ __forceinline__ int unit_of(const SelectParams &p, int &kvh) {
     kvh = x8 % p.c.n_kv;
     return x8 / p.c.n_kv * 8 + blockIdx.x % 8;
 }
-unsigned units_grid(int64_t units, int n_kv) { return (unsigned)((units + 7) / 8 * 8 * n_kv); }
+int64_t units_grid(int64_t units, int n_kv) { return (units + 7) / 8 * 8 * n_kv; }
+constexpr int64_t kMostWorkgroups = 0x7FFFFF;  // of a launch: of up to 512 threads each, 2^32 in all
 
 __device__ __forceinline__ float score_of(uint32_t key) {
     return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
@@ -852,18 +853,22 @@ __global__ __launch_bounds__(256) void select_tile_kernel(SelectParams p) {
 }
 
 template <int KS, int GP>
-void launch_tiles(SelectParams &p, int64_t pages, hipStream_t st) {
+hipError_t launch_tiles(SelectParams &p, int64_t pages, hipStream_t st) {
     p.tokens = 16 * kTileOperands<GP> / GP;
     p.room = (int)std::min<int64_t>(kKeys<1>, pages + p.n_select);
     const int64_t units = (p.b.n_tokens + p.tokens - 1) / p.tokens + p.b.n_seqs;
-    select_tile_kernel<KS, GP><<<units_grid(units, p.c.n_kv), 256, (size_t)p.tokens * (p.room + p.n_select) * 4, st>>>(p);
+    const int64_t grid = units_grid(units, p.c.n_kv);
+    if (grid > kMostWorkgroups) return hipErrorInvalidValue;
+    select_tile_kernel<KS, GP><<<(unsigned)grid, 256, (size_t)p.tokens * (p.room + p.n_select) * 4, st>>>(p);
+    return hipGetLastError();
 }
 
 template <int KS, int GP>
 hipError_t launch_tokens(SelectParams &p, int64_t pages, hipStream_t st) {
     const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
     const int64_t heads = (int64_t)p.b.n_tokens * p.c.n_kv;
-    const unsigned grid = units_grid(p.b.n_tokens, p.c.n_kv);
+    if (units_grid(p.b.n_tokens, p.c.n_kv) > kMostWorkgroups) return hipErrorInvalidValue;
+    const unsigned grid = (unsigned)units_grid(p.b.n_tokens, p.c.n_kv);
     // Few tokens with many pages: the scores on more workgroups than one a token and KV head.
     const int64_t parts = std::min<int64_t>((pages + kPart - 1) / kPart, 2 * cus / heads);
     if (pages >= 512 && parts > 1 && heads * pages * 4 <= (int64_t)kWorkspaceBytes) {
@@ -874,7 +879,7 @@ hipError_t launch_tokens(SelectParams &p, int64_t pages, hipStream_t st) {
         p.stride = (int)pages;
         p.parts = (int)parts;
         p.room = (int)std::min<int64_t>(kKeys<kSplitWaves>, pages + p.n_select);
-        score_pages_kernel<KS, GP><<<units_grid(p.b.n_tokens * parts, p.c.n_kv), 256, 0, st>>>(p);
+        score_pages_kernel<KS, GP><<<(unsigned)units_grid(p.b.n_tokens * parts, p.c.n_kv), 256, 0, st>>>(p);
         pick_pages_kernel<<<grid, 64 * kSplitWaves, (size_t)(p.room + p.n_select) * 4, st>>>(p);
     } else {
         p.room = (int)std::min<int64_t>(kKeys<kTokenWaves>, pages + p.n_select);
@@ -888,15 +893,13 @@ hipError_t launch_select(SelectParams p, hipStream_t st) {
     // the pages that a sequence may have
     const int64_t most = (std::min<int64_t>(p.b.max_len, (int64_t)p.c.width << p.c.shift) + (1 << p.c.shift) - 1) >> p.c.shift;
     const int64_t pages = std::max<int64_t>(128, (most + 127) / 128 * 128);
-    if (((int64_t)p.b.n_tokens + p.b.n_seqs + 16) * p.c.n_kv > 0x7FFFFF) return hipErrorInvalidValue;
     // Tiles where the sequences have tokens to fill them (and a list leaves a wave's keys room).
     if (p.b.max_new > 1 && p.b.n_tokens >= 4 * (int64_t)p.b.n_seqs && p.n_select <= kKeys<1> / 2) {
-        if (p.group == 1) launch_tiles<KS, 1>(p, pages, st);
-        else if (p.group == 2) launch_tiles<KS, 2>(p, pages, st);
-        else if (p.group <= 4) launch_tiles<KS, 4>(p, pages, st);
-        else if (p.group <= 8) launch_tiles<KS, 8>(p, pages, st);
-        else launch_tiles<KS, 16>(p, pages, st);
-        return hipGetLastError();
+        if (p.group == 1) return launch_tiles<KS, 1>(p, pages, st);
+        if (p.group == 2) return launch_tiles<KS, 2>(p, pages, st);
+        if (p.group <= 4) return launch_tiles<KS, 4>(p, pages, st);
+        if (p.group <= 8) return launch_tiles<KS, 8>(p, pages, st);
+        return launch_tiles<KS, 16>(p, pages, st);
     }
     if (p.group <= 4) return launch_tokens<KS, 4>(p, pages, st);
     if (p.group <= 8) return launch_tokens<KS, 8>(p, pages, st);
