@@ -297,7 +297,8 @@ int rxq4_attention_paged_f16(void *out, const void *q, int n_heads, float scale,
  * the position in the cache: tokens of images and video have a time, a height and a
  * width, and text behind them does not go on at the cache's position.
  *   positions  int32, device: the coordinate of token t (a row of q) on axis a is
- *              positions[a * position_stride + t], any whole number; n_axes axes, 1 to 16
+ *              positions[a * position_stride + t], any whole number; n_axes axes, 1 to 16.
+ *              position_stride: n_tokens or more (2^32 at most), or 0: one row for all axes
  *   axis_of    int32 [n_rot / 2], device: the axis whose coordinate turns pair i, times
  *              inv_freq[i]; a value outside [0, n_axes) counts as coordinate 0.  NULL:
  *              axis 0 for every pair

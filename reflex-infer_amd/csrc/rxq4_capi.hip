@@ -638,8 +638,8 @@ int rxq4_qk_norm_rope_axes(void *q_out, const void *q, const void *k, const void
     if (s != RXQ4_STATUS_SUCCESS) return s;
     if (n_axes <= 0 || n_axes > RXQ4_MAX_AXES)
         return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: n_axes=%d must be 1 to %d", fn, n_axes, RXQ4_MAX_AXES);
-    if (position_stride < batch->n_tokens || position_stride > (int64_t(1) << 32))
-        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: position_stride=%lld must hold n_tokens=%d", fn,
+    if (position_stride != 0 && (position_stride < batch->n_tokens || position_stride > (int64_t(1) << 32)))
+        return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: position_stride=%lld must be 0 or hold n_tokens=%d", fn,
                          (long long)position_stride, batch->n_tokens);
     if (batch->n_seqs > 0 && batch->n_tokens > 0 && (!positions || !aligned4(positions) || !aligned4(axis_of)))
         return set_error(RXQ4_STATUS_INVALID_ARGUMENT, "%s: positions null, or positions/axis_of not 4-byte aligned", fn);

@@ -351,8 +351,8 @@ def qk_norm_rope(q_out, q, k, v, batch, cache, inv_freq, q_weight=None, k_weight
 def qk_norm_rope_axes(q_out, q, k, v, batch, cache, inv_freq, positions, axis_of=None, q_weight=None, k_weight=None,
                       eps=1e-6, interleaved=False, stream=None):
     """qk_norm_rope with the angles from coordinates: positions int32 [n_axes,
-    n_tokens] (rows may lie apart), axis_of int32, the axis of each value of inv_freq
-    (None: axis 0)."""
+    n_tokens] (rows may lie apart, or be one row expanded), axis_of int32, the axis of
+    each value of inv_freq (None: axis 0)."""
     name = "qk_norm_rope_axes"
     args = _rope_args(name, q_out, q, k, v, batch, cache, inv_freq, q_weight, k_weight, eps, interleaved)
     n_axes, n = positions.shape
