@@ -649,7 +649,7 @@ __device__ __forceinline__ int pick_of(const uint32_t *keys, int n, int n_select
                 sync_waves<WAVES>();
                 least += (uint32_t)part_of_border(hist, count) << shift;
                 if (count == need || shift == 0) break;
-                most = min(most, least + ((1u << shift) - 1u));
+                most = least + min(most - least, (1u << shift) - 1u);  // (their sum may pass 2^32)
             }
             above = count == need ? least : least + 1u;
             tie = count == need ? 0u : least;

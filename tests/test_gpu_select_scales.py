@@ -58,6 +58,9 @@ CASES = [
     ((4, 2, 64), 1, [40], [3000], (100, 5, 9)),
     ((4, 1, 64), 1, [1], [3000], (64, 7, 9)),
     ((24, 1, 80), 1, [1, 2], [9000, 700], (300, 2, 2)),
+    ((32, 16, 64), 4, [60], [400], (20, 3, 4)),
+    ((16, 16, 64), 1, [170], [2100], (100, 5, 9)),
+    ((320, 16, 64), 4, [50], [300], (30, 1, 1)),
     ((4, 2, 96), 1, [1], [14000], (4096, 5, 9)),
 ]
 
@@ -87,3 +90,24 @@ def test_arrays_never_written_leave_the_first_and_last_pages(new, length):
     for t in range(new[0]):
         v = sel.visible(p, length - new[0] + t)
         assert got[t].tolist() == [[0, 1, v - 3, v - 2, v - 1, -1]] * 2
+
+
+@pytest.mark.parametrize("heads,new,length", [((4, 2, 64), [1], 400), ((4, 2, 64), [1], 1500), ((32, 16, 64), [80], 1500),
+                                              ((16, 16, 64), [130], 2500)])
+@pytest.mark.parametrize("low,high", [(-np.inf, np.inf), (-1e38, 3.3e38), (-1e38, np.inf), (-np.inf, 3.3e38), (-1e-38, np.inf)])
+def test_scores_at_both_ends_of_their_range(heads, new, length, low, high):
+    """Many of the largest there are beside some of the smallest: the borders of their keys'
+    range lie at the ends of 32 bits."""
+    p = ref.Paged(95, *heads, 1, new, [length])
+    p.q[:] = 1.0
+    rng = np.random.default_rng(96)
+    kind = rng.integers(0, 6, (p.pages, p.kv))
+    sign = np.where(kind <= 1, -1, 1).astype(np.int8)  # sums of 64 or -64
+    both = np.broadcast_to(sign[:, :, None, None, None], (p.pages, p.kv, 8, 2, 8)).copy()
+    scale = rng.random(kind.shape).astype(np.float32) + 1
+    scale[kind == 0], scale[kind == 5] = -low / 64, high / 64
+    cache, batch = p.device(capi)
+    for n in (9, 40, 200):
+        got = torch.full((p.rows, p.kv, n), -7, dtype=torch.int32, device="cuda")
+        capi.select_pages(got, p.q.cuda(), torch.from_numpy(both).cuda(), torch.from_numpy(scale).cuda(), batch, cache, 1, 2)
+        assert np.array_equal(got.cpu().numpy(), expected(p, both, scale, n, 1, 2)), n
