@@ -888,13 +888,31 @@ hipError_t launch_tokens(SelectParams &p, int64_t pages, hipStream_t st) {
     return hipGetLastError();
 }
 
+// Tiles where the sequences have two tokens each or more, a list leaves a wave's keys room, and
+// the tokens' KV heads are enough: 2 a CU, and 1 more for each part that a wave takes the pages in
+// (4 at most: max_len may be far above the lengths), since a token's whole workgroup then has the
+// choice and the few workgroups of the tiles the chain of the parts.  Twice as many for groups of
+// one head (16 tokens a tile); groups above 8 heads (one or two tokens) in one part alone.
+// Measured, us of tokens / tiles, pages of 16, lists of 64, one sequence of 32 / 8 heads after
+// 60000 positions: 4 new tokens 15 / 74, 32 30 / 106; after 30000, 64 28 / 55, 128 48 / 55, 256 86 / 57;
+// after 5000, 64 13 / 19, 128 22 / 20; 28 / 4 heads after 30000, 128 25 / 39, 256 44 / 39; 8 / 8 heads of
+// 64, 256 55 / 80, 512 97 / 80; 64 / 4 heads of 64, 512 54 / 73, after 1000 29 / 19.  256 sequences of
+// two new tokens 76 / 54, 32 of three 38 / 40, 32 of eight 64 / 52.  Over 342 such calls the side
+// taken is at worst 1.45 times the better one, near a border, and 1.01 in the mean.
+bool takes_tiles(const SelectParams &p, int64_t pages) {
+    const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
+    if (p.b.max_new < 2 || p.b.n_tokens < 2 * (int64_t)p.b.n_seqs || p.n_select > kKeys<1> / 2) return false;
+    const int64_t part = kKeys<1> - p.n_select, parts = std::min<int64_t>((pages + part - 1) / part, 4);
+    if (p.group > 8 && parts > 1) return false;
+    return (int64_t)p.b.n_tokens * p.c.n_kv >= (2 + parts) * cus * (p.group == 1 ? 2 : 1);
+}
+
 template <int KS>
 hipError_t launch_select(SelectParams p, hipStream_t st) {
     // the pages that a sequence may have
     const int64_t most = (std::min<int64_t>(p.b.max_len, (int64_t)p.c.width << p.c.shift) + (1 << p.c.shift) - 1) >> p.c.shift;
     const int64_t pages = std::max<int64_t>(128, (most + 127) / 128 * 128);
-    // Tiles where the sequences have tokens to fill them (and a list leaves a wave's keys room).
-    if (p.b.max_new > 1 && p.b.n_tokens >= 4 * (int64_t)p.b.n_seqs && p.n_select <= kKeys<1> / 2) {
+    if (takes_tiles(p, most)) {
         if (p.group == 1) return launch_tiles<KS, 1>(p, pages, st);
         if (p.group == 2) return launch_tiles<KS, 2>(p, pages, st);
         if (p.group <= 4) return launch_tiles<KS, 4>(p, pages, st);
