@@ -322,8 +322,9 @@ __device__ __forceinline__ int merge_lists(const PagedParams &p, const RowsUnit 
 // of two blocks of 16 rows, which share K and V and what is done to them.
 // Bound: a token's reads of the cache, in the pieces above; a tile's pages come from the L2,
 // and the chain of a step bounds it, of which 32 KB of K and V in and out of LDS are a
-// half; a wide one's step issues 270 vector instructions and 48 products for two waves a
-// SIMD, four fifths of its time.
+// half; a wide one's step issues 270 vector instructions and 48 products, which end to end
+// would be three fifths of its time (27 and 17 of 74 us at 2.4 GHz): the rest is waiting, two
+// waves a SIMD.
 // Measured, head_dim 128: 64 tokens of 32 / 8 heads, 64 pages of 16 each, 51 us (5.3 TB/s; 256
 // pages each 190, 5.65), 16 in an int8 cache, 32 pages of 64, 17 + 4 for the combine; a chunk of
 // 512 tokens of 28 / 4 heads, 64 pages of 32, 78 us wide, 87 narrow (a token a workgroup 150,
@@ -1096,7 +1097,10 @@ SelectedPlan plan_selected(PagedParams &p, int i8) {
     const int pad = p.c.hd <= 64 ? 64 : p.c.hd <= 96 ? 96 : p.c.hd <= 128 ? 128 : 256;
     p.rows_blk = std::min(p.group, kPagedRows);
     p.head_blocks = (p.group + kPagedRows - 1) / kPagedRows;
-    // Tiles where the sequences have tokens to fill them and the tiles are enough for the CUs.
+    // Tiles where the sequences have tokens to fill them and the tiles are enough for the CUs
+    // (measured, us of tokens / narrow tiles, lists of 64 pages of 16, 32 / 8 heads, one sequence:
+    // 4 new tokens 10 / 28, 32 16 / 30, 64 26 / 31, 128 45 / 32; 12 sequences of two or five 16 / 22, 25 /
+    // 26, 32 of two to four 30 / 35, 35 / 40, 46 / 37, 64 of two to four 64 / 65, 86 / 74, 110 / 73).
     // Wide ones where they fill more than three quarters of the rounds that they take (at 28 / 4
     // heads a round is 512 tokens: 384 / 448 / 600 / 900 tokens wide 74 / 76 / 115 / 137 us, narrow
     // 67 / 86 / 99 / 157).

@@ -15,11 +15,12 @@
 //   choice  the first n_first pages and the last n_last always, then the largest scores,
 //           equal ones by index, in order.  Two rounded products and comparisons: the
 //           same lists whichever way the work is cut.
-// Bound: the bytes of the bounds (272 a page and head of 128 with its scale and entry), in
+// Bound: the bytes of the bounds (264 a page and head of 128 with its scale and entry), in
 // pieces of 256: a loop that does nothing else reads those of 64 sequences of 500 to 30000
 // positions, pages of 16, in 14 us, of sequences alike in 10 (5.8 TB/s); for a prompt's chunk,
-// whose tokens share them, issuing; for a few tokens the chain of lengths, table, bounds and
-// choice.  So a row of bounds is loaded by lanes beside one another and turned in LDS (16
+// whose tokens share them, waiting (vector instructions and products are 12 of its 25 us: all
+// workgroups score first and choose then, two a CU); for a few tokens the chain of lengths,
+// table, bounds and choice.  So a row of bounds is loaded by lanes beside one another and turned in LDS (16
 // rows at a time by the operand's layout 21), a chunk's tokens share a workgroup's, and a
 // few tokens' scores and choice are two launches, the first over more workgroups.
 // Measured: those 64 sequences, 32 / 8 heads, lists of 64, 24 us (the longest sequences' steps
@@ -869,7 +870,11 @@ hipError_t launch_tokens(SelectParams &p, int64_t pages, hipStream_t st) {
     const int64_t heads = (int64_t)p.b.n_tokens * p.c.n_kv;
     if (units_grid(p.b.n_tokens, p.c.n_kv) > kMostWorkgroups) return hipErrorInvalidValue;
     const unsigned grid = (unsigned)units_grid(p.b.n_tokens, p.c.n_kv);
-    // Few tokens with many pages: the scores on more workgroups than one a token and KV head.
+    // Few tokens with many pages: the scores on more workgroups than one a token and KV head, as
+    // many as two a CU.  Measured, us of one launch / two, pages of 16, one token of 32 / 8 heads:
+    // 384 pages 9.5 / 10.8, 512 9.7 / 10.8, 768 11.1 / 10.9, 2048 18 / 12, 4096 30 / 13; 12 tokens 512
+    // 10.6 / 11.2, 1024 14 / 13, 2048 20 / 20, 4096 34 / 28, 24 tokens 2048 26 / 27, 4096 45 / 44; at
+    // head_dim 64 two launches pay later (512 7.2 / 9.3, 1024 8.5 / 9.9, 2048 11.1 / 10.6).
     const int64_t parts = std::min<int64_t>((pages + kPart - 1) / kPart, 2 * cus / heads);
     if (pages >= 512 && parts > 1 && heads * pages * 4 <= (int64_t)kWorkspaceBytes) {
         float *ws = nullptr;
