@@ -906,7 +906,9 @@ hipError_t launch_tokens(SelectParams &p, int64_t pages, hipStream_t st) {
 // taken is at worst 1.45 times the better one, near a border, and 1.01 in the mean.
 bool takes_tiles(const SelectParams &p, int64_t pages) {
     const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
-    if (p.b.max_new < 2 || p.b.n_tokens < 2 * (int64_t)p.b.n_seqs || p.n_select > kKeys<1> / 2) return false;
+    if (p.n_select > kKeys<1> / 2) return false;
+    if (units_grid(p.b.n_tokens, p.c.n_kv) > kMostWorkgroups) return true;  // (a token a workgroup is too many)
+    if (p.b.max_new < 2 || p.b.n_tokens < 2 * (int64_t)p.b.n_seqs) return false;
     const int64_t part = kKeys<1> - p.n_select, parts = std::min<int64_t>((pages + part - 1) / part, 4);
     if (p.group > 8 && parts > 1) return false;
     return (int64_t)p.b.n_tokens * p.c.n_kv >= (2 + parts) * cus * (p.group == 1 ? 2 : 1);

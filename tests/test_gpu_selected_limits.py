@@ -9,10 +9,10 @@ import rxq4
 from rxq4 import capi
 
 pytestmark = pytest.mark.gpu
-ROWS, KV, HD = 1 << 20, 8, 8
+ROWS, HD = 1 << 20, 8
 
 
-def _call(rows, max_new, width=4):
+def _call(rows, max_new, KV=8, width=4):
     """`rows` new tokens of one sequence in `width` pages of 1024, lists of the first and the last."""
     k = torch.zeros((width, 1024, KV, HD), dtype=torch.float16, device="cuda")
     cache = capi.PagedKV(k, torch.zeros_like(k), torch.arange(width, dtype=torch.int32, device="cuda")[None])
@@ -34,10 +34,20 @@ def test_the_most_rows_in_tiles():
     assert (pages[..., 1] == torch.where(last > 0, last, -1)[:, None]).all()
 
 
-def test_more_workgroups_than_a_launch_may_have():
-    """A token a workgroup (the sequences have one new token each, by the batch's limit)."""
-    with pytest.raises(rxq4.RxQ4Error):
-        _call(ROWS, 1)
-    pages = _call(ROWS - 8, 1)  # 2^23 - 64 workgroups
-    assert pages[0].tolist() == [[0, -1]] * KV
+def test_the_most_rows_with_one_new_token():
+    """A token a workgroup would be more than a launch may have."""
+    pages = _call(ROWS, 1)
+    assert pages[0].tolist() == [[0, -1]] * 8
     assert (pages[1:] == -7).all()
+
+
+def test_more_workgroups_than_a_launch_may_have():
+    """Sixteen tokens a workgroup and KV head, 1024 of them."""
+    rows = 1 << 17
+    with pytest.raises(rxq4.RxQ4Error):
+        _call(rows, rows, KV=1024)
+    rows -= 256  # 2^23 - 8192 workgroups
+    pages = _call(rows, rows, KV=1024)
+    last = (torch.arange(rows, device="cuda") // 1024).clamp(max=3)
+    assert (pages[..., 0] == 0).all()
+    assert (pages[..., 1] == torch.where(last > 0, last, -1)[:, None]).all()
