@@ -893,25 +893,27 @@ hipError_t launch_tokens(SelectParams &p, int64_t pages, hipStream_t st) {
     return hipGetLastError();
 }
 
-// Tiles where the sequences have two tokens each or more, a list leaves a wave's keys room, and
-// the tokens' KV heads are enough: 2 a CU, and 1 more for each part that a wave takes the pages in
-// (4 at most: max_len may be far above the lengths), since a token's whole workgroup then has the
-// choice and the few workgroups of the tiles the chain of the parts.  Twice as many for groups of
-// one head (16 tokens a tile); groups above 8 heads (one or two tokens) in one part alone.
+// Tiles where the tokens' KV heads are enough to fill the CUs: a token's whole workgroup scores
+// and chooses for it, a tile's wave walks a token's keys part after part.  So about one and a half
+// a CU for few pages (3/4 of the two workgroups of a CU), two more for each part of pages, three at
+// most (max_len may be far above the lengths); at head_dim above 128, where a CU holds one of the
+// tokens' workgroups, 3/4 of that, with groups of one head, of which a tile has 16, 3/2.  Groups
+// above 8 heads leave a tile one or two tokens: tiles in one part alone.
 // Measured, us of tokens / tiles, pages of 16, lists of 64, one sequence of 32 / 8 heads after
-// 60000 positions: 4 new tokens 15 / 74, 32 30 / 106; after 30000, 64 28 / 55, 128 48 / 55, 256 86 / 57;
-// after 5000, 64 13 / 19, 128 22 / 20; 28 / 4 heads after 30000, 128 25 / 39, 256 44 / 39; 8 / 8 heads of
-// 64, 256 55 / 80, 512 97 / 80; 64 / 4 heads of 64, 512 54 / 73, after 1000 29 / 19.  256 sequences of
-// two new tokens 76 / 54, 32 of three 38 / 40, 32 of eight 64 / 52.  Over 342 such calls the side
-// taken is at worst 1.45 times the better one, near a border, and 1.01 in the mean.
+// 60000 positions: 4 new tokens 15 / 74, 32 30 / 106, 256 150 / 107; after 30000, 64 28 / 55, 128 48 /
+// 55, 256 86 / 57; after 5000, 64 13 / 19, 128 22 / 20; 28 / 4 heads after 30000, 128 25 / 39, 256 44 / 39;
+// 8 / 8 heads of 64, 256 55 / 80, 512 97 / 80; 64 / 4 heads of 64, 512 54 / 73, after 1000 29 / 19.  256
+// sequences of two new tokens 76 / 54, 32 of three 38 / 40, 32 of eight 64 / 52.  Over 1042 such calls
+// the side taken is at worst 1.6 times the better one, 1.01 in the mean, in 42 more than 1.1.
 bool takes_tiles(const SelectParams &p, int64_t pages) {
-    const int cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
+    const int64_t cus = device_info().cu_count > 0 ? device_info().cu_count : 256;
     if (p.n_select > kKeys<1> / 2) return false;
     if (units_grid(p.b.n_tokens, p.c.n_kv) > kMostWorkgroups) return true;  // (a token a workgroup is too many)
     if (p.b.max_new < 2 || p.b.n_tokens < 2 * (int64_t)p.b.n_seqs) return false;
-    const int64_t part = kKeys<1> - p.n_select, parts = std::min<int64_t>((pages + part - 1) / part, 4);
-    if (p.group > 8 && parts > 1) return false;
-    return (int64_t)p.b.n_tokens * p.c.n_kv >= (2 + parts) * cus * (p.group == 1 ? 2 : 1);
+    const int64_t part = kKeys<1> - p.n_select, heads = (int64_t)p.b.n_tokens * p.c.n_kv;
+    if (p.group > 8 && pages > part) return false;
+    // heads >= (3/4 + pages / part) * 2 cus * (3/4 or 1) * (3/2 or 1)
+    return 16 * heads * part >= (3 * part + 4 * std::min(pages, 3 * part)) * cus * (p.c.hd > 128 ? 3 : 4) * (p.group == 1 ? 3 : 2);
 }
 
 template <int KS>

@@ -92,8 +92,8 @@ def test_arrays_never_written_leave_the_first_and_last_pages(new, length):
         assert got[t].tolist() == [[0, 1, v - 3, v - 2, v - 1, -1]] * 2
 
 
-@pytest.mark.parametrize("heads,new,length", [((4, 2, 64), [1], 400), ((4, 2, 64), [1], 1500), ((32, 16, 64), [80], 1500),
-                                              ((16, 16, 64), [130], 2500)])
+@pytest.mark.parametrize("heads,new,length", [((4, 2, 64), [1], 400), ((4, 2, 64), [1], 1500), ((32, 16, 64), [90], 1500),
+                                              ((16, 16, 64), [190], 2500)])
 @pytest.mark.parametrize("low,high", [(-np.inf, np.inf), (-1e38, 3.3e38), (-1e38, np.inf), (-np.inf, 3.3e38), (-1e-38, np.inf)])
 def test_scores_at_both_ends_of_their_range(heads, new, length, low, high):
     """Many of the largest there are beside some of the smallest: the borders of their keys'

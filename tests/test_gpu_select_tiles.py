@@ -31,13 +31,13 @@ TILES = [
     ((64, 64, 80), 1, [33], [300], (300, 1, 1)),                 # more than there are
     ((64, 64, 80), 1, [33], [300], (297, 1, 1)),                 # the border at the last pages
     ((32, 16, 72), 128, [200], [1000], (3, 1, 1)),
-    ((32, 16, 64), 1, [90], [2100], (100, 1, 1)),                # several parts
+    ((32, 16, 64), 1, [100], [2100], (100, 1, 1)),                # several parts
     ((16, 16, 64), 1, [170], [2100], (100, 1, 1)),
-    ((64, 8, 128), 1, [200], [4000], (64, 1, 69 - 6)),           # the last pages always
+    ((64, 8, 128), 1, [245], [4000], (64, 1, 63)),           # the last pages always
     ((16, 16, 256), 1, [165], [1500], (512, 1, 1)),              # the longest lists of a tile, its most LDS
     ((64, 16, 256), 1, [100], [1500], (512, 1, 1)),
-    ((64, 8, 200), 1, [170], [1500], (511, 1, 1)),
-    ((16, 4, 64), 1, [400], [9000], (200, 5, 5)),
+    ((64, 8, 200), 1, [180], [1500], (511, 1, 1)),
+    ((16, 4, 64), 1, [490], [9000], (200, 5, 5)),
 ]
 
 
@@ -49,7 +49,7 @@ def test_tiles(heads, page, new, lens, how):
     check_select(p, run_select(p, both, scale, *how), both, scale, *how)
 
 
-@pytest.mark.parametrize("heads,new", [((32, 8, 64), 96), ((16, 16, 64), 96), ((48, 4, 64), 192)])
+@pytest.mark.parametrize("heads,new", [((32, 8, 64), 56), ((16, 16, 64), 42), ((48, 4, 64), 112), ((32, 8, 256), 42)])
 def test_both_sides_of_the_border(heads, new):
     """A token less takes a token a workgroup on a card of 256 CUs; the lists are the same."""
     p = ref.Paged(173, *heads, 8, [new], [1000])
@@ -86,7 +86,7 @@ def test_ties_in_tiles(group, kv, new):
 
 
 def test_crowded_scores_in_tiles():
-    p = ref.Paged(180, 8, 4, 64, 1, [400], [1500])
+    p = ref.Paged(180, 8, 4, 64, 1, [480], [1500])
     both, scale = sel.random_bounds(181, p.pages, 4, 64)
     scale *= 1 + 1e-3 * np.random.default_rng(182).random(scale.shape).astype(np.float32)
     scale[p.table[0, 5], :], scale[p.table[0, 11], :] = 1e4, 1e3
@@ -96,7 +96,7 @@ def test_crowded_scores_in_tiles():
 
 @pytest.mark.parametrize("kind", ["rising", "falling", "alike", "few"])
 def test_parts_of_tiles_whose_scores_rise_fall_or_tie(kind):
-    p = ref.Paged(183, 16, 8, 64, 1, [200], [4000], holes=[(0, j) for j in range(4000) if kind == "few" and j % 97])
+    p = ref.Paged(183, 16, 8, 64, 1, [245], [4000], holes=[(0, j) for j in range(4000) if kind == "few" and j % 97])
     both, scale = sel.random_bounds(184, 1, 8, 64)
     both = np.repeat(both, p.pages, 0)
     rank = np.empty(p.pages)
